@@ -261,7 +261,10 @@ def _append_half(pool, byte, new, page, slot, head, touched, first, transposed):
     pages = pool["pages"]                                                            # the pages that new tokens fall into
     data = pool["codes"]
     was = data[pages].view(torch.float8_e4m3fn).float() * _power(old[pages])[..., None, None]
-    data[pages] = _codes(was, raised[pages][..., None, None]).view(torch.uint8)
+    earlier = (torch.arange(PAGE, device=DEV) < first[pages][:, None])[:, None]      # [pages, 1, token]
+    earlier = earlier[:, :, None] if transposed else earlier[..., None]
+    earlier = earlier & touched[pages][:, None, None, None]
+    data[pages] = torch.where(earlier, _codes(was, raised[pages][..., None, None]).view(torch.uint8), data[pages])
     byte.copy_(raised.to(torch.uint8))
     q = _codes(new, raised[page][..., None])
     if transposed:
