@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define MUSE_PROJ_ABI_VERSION 18
+#define MUSE_PROJ_ABI_VERSION 19
 
 /* Bits a kernel may OR into its status word when one of its bounded waits gives up. */
 #define MUSE_ST_PRODUCER_TIMEOUT 1
@@ -35,6 +35,10 @@ extern "C" {
 #define MUSE_ST_DRAIN_TIMEOUT 16
 #define MUSE_ST_PEER_ENTER_TIMEOUT 32
 #define MUSE_ST_PEER_DONE_TIMEOUT 64
+/* Not time-outs: what muse_rope_append and muse_cache_attention found in their index tensors (see there). */
+#define MUSE_ST_BAD_PAGE 128
+#define MUSE_ST_BAD_LENGTH 256
+#define MUSE_ST_ATTN_TIMEOUT 512
 
 /* Column-parallel output exchange (optional last-but-one argument of muse_gemv1 / muse_skinny_tc;
  * NULL or world <= 1 = single GPU). The weight is sharded by output rows over `world` GPUs of one
@@ -340,6 +344,64 @@ int muse_static_scratch_tiles(void);
 int muse_skinny_tc_noalloc(const void* tmap_w, const void* tmap_w_lo, const void* x, void* out, int* status, int m, int n,
                            int k, int ld_x, int ld_out, int ntok, int cluster, int groups, int stages, int out_is_f32,
                            void* stream);
+
+/* ---- projections in 8 bits -------------------------------------------------------------------------------------
+ * An 8-bit value is an e4m3 code times a power of two. The exponent of a block whose largest finite magnitude is a is
+ * e = max(ceil(log2(a / 448)), -64), stored as the byte e + 127; codes are rounded to nearest even; values that are not
+ * finite become the NaN code. x has one exponent per token and 128 columns ([m, ceil(K / 128)] bytes), W one per
+ * 128 x 128 block ([ceil(N / 128), ceil(K / 128)] bytes). Codes are row-major [m, K] and [N, K], K % 16 == 0, 16-byte
+ * aligned. out[m, N] (BF16) = sum over K blocks of 2^(ex + ew) * (codes of x . codes of W), sums in FP32. No counterpart
+ * in the reference, whose weights are BF16. */
+/* x BF16 [m, K] (ld_x elements between rows, ld_x % 8 == 0) to codes xq [m, K] and exponent bytes xe. */
+int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x, void* stream);
+/* 1 .. 16 tokens, K <= 8192: x in BF16, quantised on the way; one launch. */
+int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream);
+/* Any number of tokens, x already in 8 bits. */
+int muse_fp8_tile(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out,
+                  void* stream);
+
+/* ---- the 8-bit cache: rotary positions, append, attention -------------------------------------------------------
+ * What stands between the qkv_gate projection and the `o` projection of the decode layer. No counterpart in the reference's
+ * projection path. The cache is a pool of pages of MUSE_PAGE_TOKENS tokens, for `hk` KV heads of `dim` (64 or 128) values, as
+ * e4m3 codes with one power-of-two scale per page and head (number format: see the 8-bit projections):
+ *   k [pages, hk, 64, dim], v [pages, hk, dim, 64] (transposed within the page), k_exp, v_exp [pages, hk] exponent bytes.
+ * page_table [batch, width]: int32 indices into the pool, page i of a sequence holding its tokens 64 i .. 64 i + 63.
+ * seq_lens [batch]: int32, the tokens of each sequence INCLUDING its new ones. cu_q [batch + 1]: int32 first row of each
+ * sequence's new tokens in the batch of m rows, rows beyond cu_q[batch] are left as they are; NULL = one new token per
+ * sequence (m == batch, max_q == 1). max_q: at least the most new tokens of a sequence. Token j of a sequence's n new
+ * ones has position seq_lens - n + j; a new token whose position is negative (padding) or beyond the table belongs to no page.
+ * Index tensors are checked on the device: a page index outside the pool sets MUSE_ST_BAD_PAGE in `status` and that
+ * page is neither written nor read (its tokens count as masked); lengths or bounds that do not fit set
+ * MUSE_ST_BAD_LENGTH and are clamped. hq is a multiple of hk. */
+#define MUSE_PAGE_TOKENS 64
+/* qkv BF16 [m, >= (hq + 2 hk) dim], ld_qkv elements between rows, columns q | k | v. Turns the first `rot` dimensions (a
+ * multiple of 16) of every q and k head by the token's position, pairs (i, i + rot / 2), or (2 i, 2 i + 1) when
+ * `interleaved`; cos_sin FP32 [table_rows >= 64 width, rot / 2, 2]. q_out BF16 [m, hq, dim]; k and v go to the cache. The
+ * pages written must belong to one sequence of the batch each. A page's exponent never falls while the page fills:
+ * when new tokens raise it, the codes of its earlier tokens are rounded to the new scale; a page's first token
+ * starts afresh. k_val, v_val: BF16 [m, hk, dim], the values the cache then holds for the new tokens, or both NULL.
+ * Tokens that belong to no page leave zeros in q_out, k_val and v_val. */
+int muse_rope_append(const void* qkv, const void* cos_sin, const void* page_table, const void* seq_lens, const void* cu_q, void* k, void* v,
+                     void* k_exp, void* v_exp, void* q_out, void* k_val, void* v_val, void* status, long long ld_qkv, int m, int batch,
+                     int width, int pages, int max_q, int hq, int hk, int dim, int rot, int interleaved, int table_rows, void* stream);
+/* out[token, head] = softmax(scale * q . k) v over the cached tokens up to the query token's own position (the last
+ * `window` of them when window > 0), times sigmoid(gate) when gate is given; a row that sees no token is zero. q BF16
+ * [m, hq, dim], gate and out BF16 [m, hq dim] with ld_* elements between tokens. ws: muse_cache_attention_ws_bytes
+ * bytes, 16-byte aligned, contents irrelevant before and after; it belongs to the call until it completes (calls that
+ * may overlap on the GPU need one each). Two launches; bit-reproducible. */
+long long muse_cache_attention_ws_bytes(int batch, int max_q, int hq, int hk, int dim);
+int muse_cache_attention(const void* q, const void* k, const void* v, const void* k_exp, const void* v_exp, const void* page_table,
+                         const void* seq_lens, const void* cu_q, const void* gate, void* out, void* ws, void* status, long long ld_q,
+                         long long ld_gate, long long ld_out, float scale, int m, int batch, int width, int pages, int max_q, int hq,
+                         int hk, int dim, int window, void* stream);
+/* The plan of such a call, replayed on the host with host arrays (no GPU): segments[6 i ..] = worker, entry (sequence x
+ * row tiles + row tile), KV head, first page of the unit, pages, slot (-1: the worker writes the output rows itself).
+ * Returns the number of segments, at most `capacity` are stored; negative on a rejected argument. */
+long long muse_cache_attention_plan(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window,
+                                    int sms, int* segments, long long capacity);
+/* The slots that the adding-up kernel reads for unit (entry, head) of that plan, in its order; their number is returned. */
+long long muse_cache_attention_join(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window,
+                                    int sms, int entry, int head, int* slots, long long capacity);
 
 /* Launches an empty kernel on `stream`: the calibration point for the fixed cost of replaying a
  * one-kernel CUDA graph, which the benchmark reports beside every per-call time. Replaces the `nop`

@@ -65,9 +65,17 @@ SIGNATURES = {
     "muse_skinny_tc_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_void_p]),
+    "muse_fp8_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "muse_fp8_walk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "muse_fp8_tile": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "muse_rope_append": (C.c_int, [C.c_void_p] * 13 + [C.c_longlong] + [C.c_int] * 11 + [C.c_void_p]),
+    "muse_cache_attention_ws_bytes": (C.c_longlong, [C.c_int] * 5),
+    "muse_cache_attention": (C.c_int, [C.c_void_p] * 12 + [C.c_longlong] * 3 + [C.c_float] + [C.c_int] * 9 + [C.c_void_p]),
+    "muse_cache_attention_plan": (C.c_longlong, [C.c_void_p] * 2 + [C.c_int] * 8 + [C.c_void_p, C.c_longlong]),
+    "muse_cache_attention_join": (C.c_longlong, [C.c_void_p] * 2 + [C.c_int] * 10 + [C.c_void_p, C.c_longlong]),
 }
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 
 class MuseError(RuntimeError):

@@ -1,0 +1,239 @@
+"""The attention half of the decode layer over an 8-bit cache: rotary positions and the append of new keys and values
+(rope_append), and the attention that reads them (attention). They stand between the qkv_gate and the `o` projection;
+attention_half() is that whole stretch.
+
+Cache. A pool of pages of 64 tokens, held as e4m3 codes with one power-of-two scale per page and KV head (the number
+format of fp8.py): K is [pages, heads, token, dim], V [pages, heads, dim, token] (transposed within the page: what the
+attention's MMAs read without a transpose). A sequence owns the pages that its row of `page_table` names, page i holding its
+tokens 64 i .. 64 i + 63. Pages may be shared for reading (a common prefix); the pages that a call appends to must belong
+to one sequence of the batch each. A page's scale never shrinks while the page fills: when a new token raises it, the
+codes of the page's earlier tokens are rounded to the new scale; writing a page's first token starts it afresh.
+
+Batch. The new tokens of all sequences are the rows of one [m, ...] batch. cu_q [batch + 1] holds the first row of each
+sequence, None means one new token per sequence. seq_lens counts the new tokens too: token j of a sequence's n new
+ones has position seq_lens - n + j. A new token at a negative position (padding) is not appended, and its rows come back zero.
+
+The calls read page_table, seq_lens and cu_q on the device, so they can be captured in a CUDA graph and replayed with
+other lengths. What they find wrong there they report through check_status(): see its text.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _capi
+
+PAGE = 64
+HEAD_DIMS = (64, 128)
+
+_STATUS: dict[int, torch.Tensor] = {}
+
+
+class Cache8(NamedTuple):
+    """The pool: k float8_e4m3fn [pages, heads, 64, dim], v float8_e4m3fn [pages, heads, dim, 64], and their exponent
+    bytes uint8 [pages, heads] (a code stands for code * 2^(byte - 127)). All contiguous, on one device."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: torch.Tensor
+    v_exp: torch.Tensor
+
+
+def new_cache(pages: int, heads: int, dim: int, device) -> Cache8:
+    """An empty pool."""
+    if pages < 1 or heads < 1 or dim not in HEAD_DIMS:
+        raise ValueError(f"a cache has at least one page and head of {HEAD_DIMS} dimensions, got pages={pages}, heads={heads}, dim={dim}")
+    codes = lambda *shape: torch.zeros(shape, device=device, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scale = lambda: torch.full((pages, heads), 127, device=device, dtype=torch.uint8)
+    return Cache8(codes(pages, heads, PAGE, dim), codes(pages, heads, dim, PAGE), scale(), scale())
+
+
+def rotary_table(rot: int, positions: int, device, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                 trained_positions: int | None = None) -> torch.Tensor:
+    """cos and sin of every position's angles, FP32 [positions, rot / 2, 2], computed in FP64 once. Pair i of `rot`
+    dimensions turns by position * base^(-2 i / rot). For contexts longer than the trained one:
+      "linear"  positions are divided by `factor`
+      "ntk"     base * factor^(rot / (rot - 2)): the slowest pair is slowed by `factor`, the fastest not at all
+      "yarn"    pairs that make more than 32 turns over `trained_positions` keep their frequency, those that make less
+                than one are slowed by `factor`, linearly between; cos and sin grow by 0.1 ln(factor) + 1"""
+    if rot < 2 or rot % 2 or positions < 1 or factor < 1.0:
+        raise ValueError(f"rotary table of rot={rot} (even), positions={positions}, factor={factor} (at least 1)")
+    i = torch.arange(rot // 2, dtype=torch.float64, device=device)
+    inv, amplitude = base ** (-2.0 * i / rot), 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "ntk":
+        inv = (base * factor ** (rot / max(rot - 2, 1))) ** (-2.0 * i / rot)
+    elif scaling == "yarn":
+        if not trained_positions:
+            raise ValueError('scaling "yarn" needs trained_positions')
+        keep = ((trained_positions * inv / (2 * math.pi) - 1.0) / (32.0 - 1.0)).clamp(0, 1)
+        inv, amplitude = inv * (keep + (1 - keep) / factor), 0.1 * math.log(factor) + 1.0
+    elif scaling != "none":
+        raise ValueError(f"unknown scaling {scaling!r}")
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
+    return (amplitude * torch.stack([angle.cos(), angle.sin()], -1)).float().contiguous()
+
+
+def _status(device: torch.device) -> torch.Tensor:
+    word = _STATUS.get(device.index)
+    if word is None:
+        word = _STATUS[device.index] = torch.zeros(1, device=device, dtype=torch.int32)
+    return word
+
+
+def check_status(device) -> None:
+    """Synchronise and raise if a call since the last check met a page index outside the pool (the page was neither
+    read nor written), lengths or row bounds that do not fit the table, the batch or max_q (they were clamped), or gave up
+    on a bounded wait. Not for use inside a stream capture."""
+    device = torch.device(device)
+    word = _STATUS.get(torch.cuda.current_device() if device.index is None else device.index)
+    bits = 0 if word is None else int(word.item())
+    if bits:
+        word.zero_()
+        what = [text for bit, text in ((128, "a page index outside the pool"), (256, "lengths or row bounds that do not fit"),
+                                       (512, "a timed-out wait")) if bits & bit]
+        raise _capi.MuseError(f"the cache kernels reported: {', '.join(what)} (status bits {bits:#x}, see MUSE_ST_* in muse_proj.h)")
+
+
+def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
+    """The checks both operators share; returns (device, pages, heads, dim, batch, width)."""
+    k, v, ke, ve = cache
+    dev = k.device
+    if not k.is_cuda:
+        raise RuntimeError(f"the cache is on {dev}: this path runs on a CUDA device only (no CPU fallback)")
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ke.dtype != torch.uint8 or ve.dtype != torch.uint8:
+        raise TypeError(f"a cache is float8_e4m3fn codes and uint8 exponents, got {k.dtype}, {v.dtype}, {ke.dtype}, {ve.dtype}")
+    if k.dim() != 4 or k.shape[2] != PAGE or k.shape[3] not in HEAD_DIMS:
+        raise ValueError(f"k must be [pages, heads, {PAGE}, dim] with dim in {HEAD_DIMS}, got {tuple(k.shape)}")
+    pages, heads, _, dim = k.shape
+    if v.shape != (pages, heads, dim, PAGE) or ke.shape != (pages, heads) or ve.shape != (pages, heads):
+        raise ValueError(f"v {tuple(v.shape)} / exponents {tuple(ke.shape)}, {tuple(ve.shape)} do not fit k {tuple(k.shape)}")
+    if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()) or (k.data_ptr() | v.data_ptr()) % 16:
+        raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0] or not seq_lens.shape[0] or not page_table.shape[1]:
+        raise ValueError(f"page_table [batch, width] {tuple(page_table.shape)} and seq_lens [batch] {tuple(seq_lens.shape)} do not fit")
+    batch, width = page_table.shape
+    index = (page_table, seq_lens) if cu_q is None else (page_table, seq_lens, cu_q)
+    for t in index:
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
+            raise TypeError("page_table, seq_lens and cu_q must be contiguous int32 tensors on the cache's device")
+    if v.device != dev or ke.device != dev or ve.device != dev:
+        raise ValueError("the cache's tensors must be on one device")
+    if cu_q is None:
+        if m != batch or max_q != 1:
+            raise ValueError(f"without cu_q there is one new token per sequence: {m} rows for {batch} sequences, max_q={max_q}")
+    elif cu_q.shape != (batch + 1,):
+        raise ValueError(f"cu_q must be [batch + 1] = [{batch + 1}], got {tuple(cu_q.shape)}")
+    if max_q < 1 or q_heads < heads or q_heads % heads:
+        raise ValueError(f"max_q={max_q} must be positive and q_heads={q_heads} a multiple of the cache's {heads}")
+    return dev, pages, heads, dim, batch, width
+
+
+def rope_append(qkv: torch.Tensor, cache: Cache8, cos_sin: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *, q_heads: int,
+                cu_q: torch.Tensor | None = None, max_q: int = 1, interleaved: bool = False, values: bool = False):
+    """Turns q and k by their tokens' positions and appends k and v to the cache, one launch. qkv: BF16 [m, >= (q_heads +
+    2 heads) dim], unit column stride, columns q | k | v (the rows of the qkv_gate projection as they are). cos_sin:
+    rotary_table(rot, >= 64 * page_table.shape[1] positions), rot a multiple of 16 up to dim; pairs are (i, i + rot / 2),
+    or neighbours when `interleaved`. max_q: at least the most new tokens of a sequence. Returns q BF16 [m, q_heads,
+    dim]; with values=True (q, k, v), k and v BF16 [m, heads, dim]: the values that the cache then holds for the new tokens
+    (for a prompt's own attention in 16 bits to see what later tokens will see)."""
+    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[0] < 1:
+        raise TypeError(f"qkv must be BF16 [m, columns], got {qkv.dtype} {tuple(qkv.shape)}")
+    m = qkv.shape[0]
+    dev, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
+    if qkv.device != dev or cos_sin.device != dev:
+        raise ValueError("qkv and cos_sin must be on the cache's device")
+    if qkv.shape[1] < (q_heads + 2 * heads) * dim:
+        raise ValueError(f"qkv {tuple(qkv.shape)} is narrower than q | k | v = {(q_heads + 2 * heads) * dim} columns")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
+        raise TypeError(f"cos_sin must be a contiguous FP32 [positions, rot / 2, 2] table, got {cos_sin.dtype} {tuple(cos_sin.shape)}")
+    rot = 2 * cos_sin.shape[1]
+    if rot % 16 or not 16 <= rot <= dim or cos_sin.shape[0] < width * PAGE:
+        raise ValueError(f"the table turns {rot} dimensions (a multiple of 16 up to {dim}) at {cos_sin.shape[0]} positions; "
+                         f"{width} pages per sequence need {width * PAGE}")
+    if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (m > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
+        qkv = qkv[:, : (q_heads + 2 * heads) * dim].contiguous().clone()
+    lib = _capi.load()
+    with torch.cuda.device(dev):
+        q = torch.empty((m, q_heads, dim), device=dev, dtype=torch.bfloat16)
+        kv = torch.empty((2, m, heads, dim), device=dev, dtype=torch.bfloat16) if values else None
+        _capi.check(lib.muse_rope_append(qkv.data_ptr(), cos_sin.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+                                         None if cu_q is None else cu_q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+                                         cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), q.data_ptr(), kv[0].data_ptr() if values else None,
+                                         kv[1].data_ptr() if values else None, _status(dev).data_ptr(),
+                                         qkv.stride(0) if m > 1 else (q_heads + 2 * heads) * dim, m, batch, width, pages, max_q, q_heads, heads,
+                                         dim, rot, int(interleaved), cos_sin.shape[0], torch.cuda.current_stream(dev).cuda_stream),
+                    f"muse_rope_append(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
+    return (q, kv[0], kv[1]) if values else q
+
+
+def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens: torch.Tensor, *, cu_q: torch.Tensor | None = None,
+              max_q: int = 1, scale: float | None = None, window: int = 0, gate: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q K^T) V over the cached tokens up to each query token's own position (the last `window` of them
+    when window > 0), times sigmoid(gate) when gate is given: BF16 [m, q_heads * dim], ready for the `o` projection. A row
+    that sees no token is zero; rows beyond the last sequence are left as they are. q: BF16 [m, q_heads, dim]; gate: BF16
+    [m, q_heads * dim] (the gate columns of qkv_gate, any row stride); scale: 1 / sqrt(dim) by default; out (optional):
+    BF16 [m, q_heads * dim] with unit column stride. Two launches, the same bits in every run."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[0] < 1:
+        raise TypeError(f"q must be BF16 [m, heads, dim], got {q.dtype} {tuple(q.shape)}")
+    m, q_heads, d = q.shape
+    dev, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
+    if d != dim or q.device != dev or window < 0:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not fit the cache's heads of {dim} on {dev}, or window={window} is negative")
+    if q.stride(2) != 1 or q.stride(1) != dim or q.data_ptr() % 16 or (m > 1 and (q.stride(0) % 8 or q.stride(0) < q_heads * dim)):
+        q = q.contiguous().clone()
+    cols = q_heads * dim
+    for name, t in (("gate", gate), ("out", out)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != (m, cols) or t.device != dev):
+            raise TypeError(f"{name} must be BF16 [m, q_heads * dim] = [{m}, {cols}] on the cache's device, got {t.dtype} {tuple(t.shape)}")
+    if gate is not None and (gate.stride(1) != 1 or gate.data_ptr() % 4 or (m > 1 and (gate.stride(0) % 2 or gate.stride(0) < cols))):
+        gate = gate.contiguous().clone()
+    if out is not None and (out.stride(1) != 1 or out.data_ptr() % 4 or (m > 1 and (out.stride(0) % 2 or out.stride(0) < cols))):
+        raise ValueError("out must have unit column stride, an even row stride and 4-byte alignment")
+    lib = _capi.load()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty((m, cols), device=dev, dtype=torch.bfloat16)
+        # the workspace is the call's own (a captured graph keeps its own): calls may overlap on the GPU
+        ws_bytes = lib.muse_cache_attention_ws_bytes(batch, max_q, q_heads, heads, dim)
+        if ws_bytes < 0:
+            raise _capi.MuseError(f"muse_cache_attention_ws_bytes -> {ws_bytes}")
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        _capi.check(lib.muse_cache_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
+                                             page_table.data_ptr(), seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
+                                             None if gate is None else gate.data_ptr(), out.data_ptr(), ws.data_ptr(), _status(dev).data_ptr(),
+                                             q.stride(0) if m > 1 else cols, 0 if gate is None else gate.stride(0) if m > 1 else cols,
+                                             out.stride(0) if m > 1 else cols, 1.0 / math.sqrt(dim) if scale is None else scale, m, batch, width,
+                                             pages, max_q, q_heads, heads, dim, window, torch.cuda.current_stream(dev).cuda_stream),
+                    f"muse_cache_attention(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
+    return out
+
+
+def attention_half(data, state, cache: Cache8, cos_sin: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *, q_heads: int,
+                   cu_q: torch.Tensor | None = None, max_q: int = 1, window: int = 0, interleaved: bool = False, gated: bool = True,
+                   eight_bit: bool = False) -> torch.Tensor:
+    """The attention half of the decode layer: the qkv_gate projection, rope_append, attention, the `o` projection; its
+    result is what muse_bf16_proj.attn_boundary takes as attn_out. data = {"x": BF16 [m, K]}; `state` as
+    muse_bf16_proj.prepare made it, with "qkv_gate" (rows q | k | v | gate; without the gate rows when gated is False)
+    and "o". eight_bit: both projections through kernel_fn_fp8 (prepare_fp8 made their 8-bit forms). The rest as in
+    rope_append and attention."""
+    from . import muse_bf16_proj as proj
+
+    project = proj.kernel_fn_fp8 if eight_bit else proj.kernel_fn
+    x = data["x"]
+    m = x.shape[0]
+    heads, dim = cache.k.shape[1], cache.k.shape[3]
+    qkv, cols = (q_heads + 2 * heads) * dim, q_heads * dim
+    n, k = state["qkv_gate"].shape
+    if n != qkv + (cols if gated else 0) or state["o"].shape[1] != cols:
+        raise ValueError(f"qkv_gate {tuple(state['qkv_gate'].shape)} and o {tuple(state['o'].shape)} do not fit {q_heads} query heads and "
+                         f"{heads} KV heads of {dim}, {'gated' if gated else 'not gated'}")
+    rows = project({"x": x, "config": {"layer": "qkv_gate", "m": m, "n": n, "k": k}}, state)
+    q = rope_append(rows, cache, cos_sin, page_table, seq_lens, q_heads=q_heads, cu_q=cu_q, max_q=max_q, interleaved=interleaved)
+    a = attention(q, cache, page_table, seq_lens, cu_q=cu_q, max_q=max_q, window=window, gate=rows[:, qkv:] if gated else None)
+    return project({"x": a, "config": {"layer": "o", "m": m, "n": state["o"].shape[0], "k": cols}}, state)

@@ -1,0 +1,90 @@
+// How the attention over the paged cache is dealt to workers. Pure integer arithmetic, the same on host and device:
+// the kernels use it, and so does the host entry that replays a plan.
+//
+// A sequence b with n new tokens and `len` tokens in all has group * n query rows per KV head, row r = token * group +
+// head in the group, cut into tiles of `tile` rows. An ENTRY is a (sequence, row tile); its rows see the tokens from
+// `lo` to `hi` (causal, window), that is `pages` pages from `page0`; an entry with rows that see nothing counts one
+// page, so that somebody writes its zeros. A UNIT is an entry's KV head. The units' pages form one list, entry-major
+// then head then page, which is cut into equal ranges, one per worker: a unit split between workers leaves partial
+// sums that a second kernel adds up in page order.
+#pragma once
+
+namespace muse {
+
+constexpr int ATTN_PAGE = 64;   // tokens per page
+
+struct AttnEntry {
+  int first, n;      // rows of the batch that hold the sequence's new tokens
+  int pos;           // position of the first of them
+  int row0, rows;    // this tile's rows (token * group + head in group)
+  int page0, pages;  // pages its rows see; rows > 0 and nothing seen: one page that is masked whole
+  int last;          // last position its rows see (-1: none)
+};
+
+// cu0, cu1: the sequence's bounds in the batch as the caller gave them; len: its tokens, the new ones included.
+__host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m, int max_q, int capacity, int group, int tile, int rt,
+                                                int window) {
+  AttnEntry e;
+  if (len < 0) len = 0;
+  if (len > capacity) len = capacity;
+  e.first = cu0 < 0 ? 0 : cu0 > m ? m : cu0;
+  const int end = cu1 > m ? m : cu1;
+  e.n = end > e.first ? end - e.first : 0;
+  if (e.n > max_q) e.n = max_q;
+  e.pos = len - e.n;
+  const int all = e.n * group;
+  e.row0 = rt * tile;
+  e.rows = all - e.row0;
+  if (e.rows > tile) e.rows = tile;
+  e.page0 = 0;
+  e.pages = 0;
+  e.last = -1;
+  if (e.rows <= 0) {
+    e.rows = 0;
+    return e;
+  }
+  const int p_lo = e.pos + e.row0 / group, p_hi = e.pos + (e.row0 + e.rows - 1) / group;
+  if (p_hi < 0) {
+    e.pages = 1;
+    return e;
+  }
+  e.last = p_hi;
+  int lo = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
+  e.page0 = lo / ATTN_PAGE;
+  e.pages = p_hi / ATTN_PAGE - e.page0 + 1;
+  return e;
+}
+
+// First page of worker w's range when `total` pages are dealt to `workers`.
+__host__ __device__ inline long long attn_range(long long total, long long workers, long long w) { return total * w / workers; }
+// The worker whose range holds page f.
+__host__ __device__ inline long long attn_worker(long long total, long long workers, long long f) {
+  long long w = (f * workers + workers - 1) / total;   // within one of it
+  while (w > 0 && attn_range(total, workers, w) > f) --w;
+  while (w + 1 < workers && attn_range(total, workers, w + 1) <= f) ++w;
+  return w;
+}
+// Where worker w left its partial sums of the unit whose pages begin at u0 (the caller knows that w has some of them,
+// and not all): a worker has at most two partial segments, the one its range begins in (slot 0) and the one it ends in
+// (slot 1, when that is another). -1: w has no page at all (there are fewer pages than workers).
+__host__ __device__ inline long long attn_slot_of(long long total, long long workers, long long w, long long u0) {
+  const long long f = attn_range(total, workers, w);
+  if (f >= attn_range(total, workers, w + 1)) return -1;
+  return 2 * w + (f >= u0 ? 0 : 1);
+}
+// visit(slot) for the partial sums of a split unit of `pages` pages that begin at u0, in page order; nothing for a unit that
+// one worker has whole.
+template <typename F>
+__host__ __device__ inline void attn_for_slots(long long total, long long workers, long long u0, int pages, F&& visit) {
+  const long long w0 = attn_worker(total, workers, u0), w1 = attn_worker(total, workers, u0 + pages - 1);
+  if (w0 == w1) return;
+#ifdef __CUDA_ARCH__
+#pragma unroll 4
+#endif
+  for (long long w = w0; w <= w1; ++w) {
+    const long long slot = attn_slot_of(total, workers, w, u0);
+    if (slot >= 0) visit(slot);
+  }
+}
+
+}  // namespace muse

@@ -5,6 +5,7 @@
 
 #include "../../include/muse_proj.h"
 #include "boundary.cuh"
+#include "cache8.cuh"
 #include "common.cuh"
 
 namespace muse {
@@ -53,6 +54,9 @@ cudaError_t gemm_trace_set(unsigned long long* p);
 #endif
 long long skinny_static_ws_floats();
 int skinny_static_cnt_ints();
+int fp8_quantize_dispatch(const void* x, void* xq, void* xe, int m, int K, int ld_x, cudaStream_t stream);
+int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, cudaStream_t stream);
+int fp8_tile_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, cudaStream_t stream);
 
 // cuTensorMapEncodeTiled is a driver entry point; fetching it through the runtime keeps the
 // library free of a link-time dependency on libcuda (it must load on machines without a driver).
@@ -353,6 +357,54 @@ int muse_skinny_tc_noalloc(const void* tmap_w, const void* tmap_w_lo, const void
   if (tmap_w_lo) memcpy(&twlo, tmap_w_lo, sizeof(twlo));
   return muse::skinny_tc_static_dispatch(&tw, tmap_w_lo ? &twlo : nullptr, &tx, out, status, m, n, k, ld_out, ntok,
                                          cluster, groups, stages, out_is_f32, static_cast<cudaStream_t>(stream));
+}
+
+int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x, void* stream) {
+  return muse::fp8_quantize_dispatch(x, xq, xe, m, K, ld_x, static_cast<cudaStream_t>(stream));
+}
+int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream) {
+  return muse::fp8_walk_dispatch(W, we, x, out, m, N, K, ld_x, ld_out, static_cast<cudaStream_t>(stream));
+}
+int muse_fp8_tile(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, void* stream) {
+  return muse::fp8_tile_dispatch(W, we, xq, xe, out, m, N, K, ld_out, static_cast<cudaStream_t>(stream));
+}
+
+int muse_rope_append(const void* qkv, const void* cos_sin, const void* page_table, const void* seq_lens, const void* cu_q, void* k, void* v,
+                     void* k_exp, void* v_exp, void* q_out, void* k_val, void* v_val, void* status, long long ld_qkv, int m, int batch,
+                     int width, int pages, int max_q, int hq, int hk, int dim, int rot, int interleaved, int table_rows, void* stream) {
+  using bf16 = __nv_bfloat16;
+  const muse::RopeArgs a = {static_cast<const bf16*>(qkv), static_cast<const float*>(cos_sin), static_cast<const int*>(page_table),
+                            static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q), static_cast<uint8_t*>(k), static_cast<uint8_t*>(v),
+                            static_cast<uint8_t*>(k_exp), static_cast<uint8_t*>(v_exp), static_cast<bf16*>(q_out), static_cast<bf16*>(k_val),
+                            static_cast<bf16*>(v_val), static_cast<int*>(status), ld_qkv, m, batch, width, pages, max_q, hq, hk, rot, interleaved,
+                            table_rows};
+  return muse::rope_append_dispatch(a, dim, static_cast<cudaStream_t>(stream));
+}
+
+long long muse_cache_attention_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
+  return muse::cache_attn_ws_bytes(batch, max_q, hq, hk, dim);
+}
+
+int muse_cache_attention(const void* q, const void* k, const void* v, const void* k_exp, const void* v_exp, const void* page_table,
+                         const void* seq_lens, const void* cu_q, const void* gate, void* out, void* ws, void* status, long long ld_q,
+                         long long ld_gate, long long ld_out, float scale, int m, int batch, int width, int pages, int max_q, int hq,
+                         int hk, int dim, int window, void* stream) {
+  using bf16 = __nv_bfloat16;
+  const muse::AttnArgs a = {static_cast<const bf16*>(q), static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v),
+                            static_cast<const uint8_t*>(k_exp), static_cast<const uint8_t*>(v_exp), static_cast<const int*>(page_table),
+                            static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q), static_cast<const bf16*>(gate),
+                            static_cast<bf16*>(out), nullptr, nullptr, static_cast<int*>(status), ld_q, ld_gate, ld_out,
+                            scale * 1.44269504f, m, batch, width, pages, max_q, hq, hk, window, 0};
+  return muse::cache_attn_dispatch(a, dim, ws, static_cast<cudaStream_t>(stream));
+}
+
+long long muse_cache_attention_plan(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window,
+                                    int sms, int* segments, long long capacity) {
+  return muse::cache_attn_plan(seq_lens, cu_q, m, batch, width, max_q, hq, hk, window, sms, segments, capacity);
+}
+long long muse_cache_attention_join(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window,
+                                    int sms, int entry, int head, int* slots, long long capacity) {
+  return muse::cache_attn_join(seq_lens, cu_q, m, batch, width, max_q, hq, hk, window, sms, entry, head, slots, capacity);
 }
 
 }  // extern "C"

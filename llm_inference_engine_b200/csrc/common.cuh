@@ -19,6 +19,9 @@ enum : int {
   ST_EPILOGUE_TIMEOUT = 4,  // epilogue: the accumulator-ready barrier never completed
   ST_X_TIMEOUT = 8,         // GEMV: the bulk copy of x never completed
   ST_DRAIN_TIMEOUT = 16,    // teardown: an issued TMA copy did not land within the limit
+  ST_BAD_PAGE = 128,        // 8-bit cache: a page index outside the pool (the page was neither read nor written)
+  ST_BAD_LENGTH = 256,      // 8-bit cache: lengths or row bounds that do not fit the table or the batch (clamped)
+  ST_ATTN_TIMEOUT = 512,    // attention: a page's copy never landed, or a ring slot was never released
 };
 
 constexpr unsigned long long WAIT_LIMIT_NS = 500ull * 1000ull * 1000ull;  // 0.5 s

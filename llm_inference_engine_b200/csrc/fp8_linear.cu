@@ -1,0 +1,276 @@
+// out[m, N] = x[m, K] . W[N, K]^T with both operands in 8 bits and a power-of-two scale per block of 128 (fp8.cuh):
+//     out[t, n] = sum over K blocks b of 2^(ex[t, b] + ew[n / 128, b]) * sum over k in b of xq[t, k] wq[n, k]
+// BF16 out; x comes in BF16 and is quantised here (one exponent per token and 128 columns), W as codes and exponent
+// bytes. The products of codes are exact in FP32 and so is the scaling; the sums are FP32.
+//
+//   fp8_walk_kernel   up to 16 tokens: the persistent walk of fewtok_mma.cu over half the bytes. Tokens are the MMA's
+//                     M = 16, 8 weight rows its N; a lane loads 16-byte pieces of W straight into the B fragments of
+//                     two m16n8k32 MMAs (the k slots are a permutation that x follows). A warp owns whole 128-column
+//                     blocks, so its x fragments, quantised in registers from BF16 (the four lanes of a token share
+//                     the block: two shuffles give its largest magnitude), and their scales never change.
+//   fp8_tile_kernel   any number of tokens, from x quantised by fp8_quantize_kernel: 64 x 64 tiles in shared memory.
+#include "fp8.cuh"
+
+namespace muse {
+
+__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// ---------------------------------------------------------------- x to 8 bits
+// One warp per token and block of 128 columns: 4 values per lane.
+__global__ void __launch_bounds__(256) fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, uint8_t* __restrict__ xq,
+                                                           uint8_t* __restrict__ xe, int m, int K, int ld_x, int kblocks) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const long long item = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (item >= static_cast<long long>(m) * kblocks) return;
+  const int t = static_cast<int>(item / kblocks), b = static_cast<int>(item % kblocks), lane = threadIdx.x & 31;
+  const int k = b * FP8_BLOCK + lane * 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (k < K) {   // K % 16 == 0: a lane's four columns are in or out together
+    const uint2 w = __ldcg(reinterpret_cast<const uint2*>(x + static_cast<size_t>(t) * ld_x + k));
+    v[0] = bf16lo_f32(w.x); v[1] = bf16hi_f32(w.x); v[2] = bf16lo_f32(w.y); v[3] = bf16hi_f32(w.y);
+  }
+  float a = fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])));
+#pragma unroll
+  for (int s = 16; s; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
+  const int e = fp8_exponent_byte(a);
+  const float inv = exp2_byte_inv(e);
+  if (k < K) *reinterpret_cast<uint32_t*>(xq + static_cast<size_t>(t) * K + k) = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  if (lane == 0) xe[static_cast<size_t>(t) * kblocks + b] = static_cast<uint8_t>(e);
+}
+
+// ---------------------------------------------------------------- up to 16 tokens
+// NW warps; BPW blocks of K per warp (K <= 128 * NW * BPW); D row groups in flight per warp; HI: tokens 8..15 exist.
+// The warps are wk (a power of two) slices of K times NW / wk neighbouring row groups.
+template <int NW, int BPW, int D, bool HI>
+__global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ we,
+                                                           const __nv_bfloat16* __restrict__ x, __nv_bfloat16* __restrict__ out, int m,
+                                                           int N, int K, int ld_x, int ld_out, int wk) {
+  constexpr int OUTS = HI ? 128 : 64;   // 8 or 16 tokens x 8 rows
+  __shared__ __align__(16) float red[2][NW][OUTS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  const int ks = warp & (wk - 1), rs = warp / wk, rslots = NW / wk;   // this warp's K slice and row slot
+  const int groups = (N + 7) >> 3;
+  const int sets = (groups + rslots - 1) / rslots;                    // a CTA step walks rslots groups
+  const int my_sets = static_cast<int>(blockIdx.x) < sets ? (sets - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+  auto group_of = [&](int i) { return (static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x)) * rslots + rs; };
+
+  uint4 w[D][BPW][2];
+  uint32_t se[D][BPW];
+  auto load = [&](uint4 (&d)[BPW][2], uint32_t (&s)[BPW], int i) {
+    const int grp = group_of(i);
+    const int row = min(grp * 8 + g, N - 1);
+#pragma unroll
+    for (int j = 0; j < BPW; ++j) {
+      const int kb = ks + j * wk;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int k = kb * FP8_BLOCK + 64 * p + 16 * t;
+        d[j][p] = k < K && grp < groups ? ldg_stream16(W + static_cast<size_t>(row) * K + k) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      s[j] = kb < kblocks ? __ldg(we + static_cast<size_t>(min(grp * 8, N - 1) >> 7) * kblocks + kb) : 0u;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < my_sets) load(w[d], se[d], d);
+  griddep_launch_dependents();
+  griddep_wait();   // x and out belong to the stream: only the weights were touched so far
+
+  // x fragments: the lane's 32 columns of each of its blocks, for token g (and g + 8), in BF16 -> codes in registers.
+  uint32_t xa[BPW][8], xb[HI ? BPW : 1][8];
+  float sa[BPW], sb[HI ? BPW : 1];
+  auto quantise = [&](int tok, int kb, uint32_t (&q)[8], float& scale) {
+    uint4 v[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int k = kb * FP8_BLOCK + 64 * (p >> 1) + 16 * t + 8 * (p & 1);
+      v[p] = tok < m && k < K ? __ldcg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(tok) * ld_x + k)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    float a = 0.f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t u[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a = fmaxf(a, fmaxf(finite_abs(bf16lo_f32(u[c])), finite_abs(bf16hi_f32(u[c]))));
+    }
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const int e = fp8_exponent_byte(a);
+    const float inv = exp2_byte_inv(e);
+    scale = exp2_byte(e);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t u[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        q[2 * p + c] = fp8_pack4(bf16lo_f32(u[2 * c]) * inv, bf16hi_f32(u[2 * c]) * inv, bf16lo_f32(u[2 * c + 1]) * inv, bf16hi_f32(u[2 * c + 1]) * inv);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < BPW; ++j) {
+    quantise(g, ks + j * wk, xa[j], sa[j]);
+    if constexpr (HI) quantise(g + 8, ks + j * wk, xb[j], sb[j]);
+  }
+
+  for (int i0 = 0; i0 < my_sets; i0 += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int i = i0 + d;
+      if (i < my_sets) {   // CTA-uniform
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < BPW; ++j) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const uint4 u = w[d][j][p];
+            mma_e4m3_16832(c, xa[j][4 * p], HI ? xb[HI ? j : 0][4 * p] : 0u, xa[j][4 * p + 1], HI ? xb[HI ? j : 0][4 * p + 1] : 0u, u.x, u.y);
+            mma_e4m3_16832(c, xa[j][4 * p + 2], HI ? xb[HI ? j : 0][4 * p + 2] : 0u, xa[j][4 * p + 3], HI ? xb[HI ? j : 0][4 * p + 3] : 0u, u.z, u.w);
+          }
+          const float s = exp2_byte(static_cast<int>(se[d][j]));
+          acc[0] = fmaf(c[0], s * sa[j], acc[0]);
+          acc[1] = fmaf(c[1], s * sa[j], acc[1]);
+          if constexpr (HI) {
+            acc[2] = fmaf(c[2], s * sb[j], acc[2]);
+            acc[3] = fmaf(c[3], s * sb[j], acc[3]);
+          }
+        }
+        if (i + D < my_sets) load(w[d], se[d], i + D);   // into the registers just read: in flight across the reduction
+        float* mine = red[i & 1][warp];
+        *reinterpret_cast<float2*>(mine + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
+        if constexpr (HI) *reinterpret_cast<float2*>(mine + (g + 8) * 8 + 2 * t) = make_float2(acc[2], acc[3]);
+        __syncthreads();   // the buffer written two steps ago is free again once every warp passed this
+        for (int o = threadIdx.x; o < rslots * OUTS; o += NW * 32) {
+          const int slot = o / OUTS, v = o % OUTS;
+          float sum = 0.f;
+#pragma unroll 8
+          for (int s = 0; s < wk; ++s) sum += red[i & 1][slot * wk + s][v];
+          const int tok = v >> 3, row = ((static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x)) * rslots + slot) * 8 + (v & 7);
+          if (tok < m && row < N) out[static_cast<size_t>(tok) * ld_out + row] = __float2bfloat16_rn(sum);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- any number of tokens
+constexpr int FT_T = 64, FT_R = 64, FT_LD = FP8_BLOCK + 16;   // tokens, rows, padded bytes of a tile row
+
+__global__ void __launch_bounds__(256) fp8_tile_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ we,
+                                                       const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xe,
+                                                       __nv_bfloat16* __restrict__ out, int m, int N, int K, int kblocks, int ld_out) {
+  __shared__ __align__(16) uint8_t sx[FT_T][FT_LD], sw[FT_R][FT_LD];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = blockIdx.x * FT_R, t0 = blockIdx.y * FT_T;
+  const int wt = (warp & 3) * 16, wr = (warp >> 2) * 32;   // this warp's 16 tokens and 32 rows of the tile
+  float acc[4][4] = {};
+  for (int kb = 0; kb < kblocks; ++kb) {
+    for (int i = threadIdx.x; i < (FT_T + FT_R) * 8; i += 256) {
+      const int row = i >> 3, k = kb * FP8_BLOCK + (i & 7) * 16;
+      const bool is_x = row < FT_T;
+      const int at = is_x ? t0 + row : r0 + row - FT_T;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (k < K && at < (is_x ? m : N)) v = __ldcg(reinterpret_cast<const uint4*>((is_x ? xq : W) + static_cast<size_t>(at) * K + k));
+      *reinterpret_cast<uint4*>(is_x ? &sx[row][(i & 7) * 16] : &sw[row - FT_T][(i & 7) * 16]) = v;
+    }
+    __syncthreads();
+    float c[4][4] = {};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      auto word = [&](const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); };
+      const uint32_t a0 = word(&sx[wt + g][32 * s + 4 * t]), a1 = word(&sx[wt + g + 8][32 * s + 4 * t]);
+      const uint32_t a2 = word(&sx[wt + g][32 * s + 16 + 4 * t]), a3 = word(&sx[wt + g + 8][32 * s + 16 + 4 * t]);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        mma_e4m3_16832(c[n], a0, a1, a2, a3, word(&sw[wr + 8 * n + g][32 * s + 4 * t]), word(&sw[wr + 8 * n + g][32 * s + 16 + 4 * t]));
+    }
+    const float e0 = t0 + wt + g < m ? exp2_byte(__ldcg(xe + static_cast<size_t>(t0 + wt + g) * kblocks + kb)) : 0.f;
+    const float e1 = t0 + wt + g + 8 < m ? exp2_byte(__ldcg(xe + static_cast<size_t>(t0 + wt + g + 8) * kblocks + kb)) : 0.f;
+    const float s = exp2_byte(__ldg(we + static_cast<size_t>(r0 >> 7) * kblocks + kb));
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      acc[n][0] = fmaf(c[n][0], s * e0, acc[n][0]);
+      acc[n][1] = fmaf(c[n][1], s * e0, acc[n][1]);
+      acc[n][2] = fmaf(c[n][2], s * e1, acc[n][2]);
+      acc[n][3] = fmaf(c[n][3], s * e1, acc[n][3]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = t0 + wt + g + 8 * (i >> 1), row = r0 + wr + 8 * n + 2 * t + (i & 1);
+      if (tok < m && row < N) out[static_cast<size_t>(tok) * ld_out + row] = __float2bfloat16_rn(acc[n][i]);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+static int sm_count() {
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return v;
+}
+
+int fp8_quantize_dispatch(const void* x, void* xq, void* xe, int m, int K, int ld_x, cudaStream_t stream) {
+  if (!x || !xq || !xe || m < 1 || K < 16 || K % 16) return -1;
+  if (ld_x < K || ld_x % 8 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xq)) & 15)) return -2;
+  const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  const long long blocks = (static_cast<long long>(m) * kblocks + 7) / 8;
+  if (blocks > 0x7fffffffll) return -3;
+  return static_cast<int>(launch_dependent(fp8_quantize_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+                                           static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(xq), static_cast<uint8_t*>(xe), m, K, ld_x, kblocks));
+}
+
+template <int NW, int BPW, int D, bool HI>
+static cudaError_t fp8_walk_launch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out,
+                                   int sms, cudaStream_t stream) {
+  const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  int wk = 1;
+  while (wk < NW && wk < kblocks) wk *= 2;
+  const int sets = ((N + 7) / 8 + NW / wk - 1) / (NW / wk);
+  return launch_dependent(fp8_walk_kernel<NW, BPW, D, HI>, dim3(sets < sms ? sets : sms), dim3(NW * 32), 0, stream,
+                          static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(we), static_cast<const __nv_bfloat16*>(x),
+                          static_cast<__nv_bfloat16*>(out), m, N, K, ld_x, ld_out, wk);
+}
+
+int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, cudaStream_t stream) {
+  if (!W || !we || !x || !out || m < 1 || m > 16 || N < 1 || K < 16 || K % 16 || K > 8192) return -1;
+  if (ld_x < K || ld_x % 8 || ld_out < N || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
+  const int sms = sm_count();
+  if (sms < 1) return -4;
+  cudaError_t e;
+  // 32 warps of 64 registers hold 16 bytes x 4 of W and up to 16 words of x per lane; longer rows of more tokens
+  // take 16 warps of 128.
+  if (K <= 4096)
+    e = m <= 8 ? fp8_walk_launch<32, 1, 2, false>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
+               : fp8_walk_launch<32, 1, 2, true>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream);
+  else
+    e = m <= 8 ? fp8_walk_launch<32, 2, 1, false>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
+               : fp8_walk_launch<16, 4, 1, true>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream);
+  return static_cast<int>(e);
+}
+
+int fp8_tile_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, cudaStream_t stream) {
+  if (!W || !we || !xq || !xe || !out || m < 1 || N < 1 || K < 16 || K % 16) return -1;
+  if (ld_out < N || ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
+  const long long ty = (m + FT_T - 1) / FT_T;
+  if (ty > 65535) return -3;
+  return static_cast<int>(launch_dependent(fp8_tile_kernel, dim3((N + FT_R - 1) / FT_R, static_cast<unsigned>(ty)), dim3(256), 0, stream,
+                                           static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(we), static_cast<const uint8_t*>(xq),
+                                           static_cast<const uint8_t*>(xe), static_cast<__nv_bfloat16*>(out), m, N, K,
+                                           (K + FP8_BLOCK - 1) / FP8_BLOCK, ld_out));
+}
+
+}  // namespace muse

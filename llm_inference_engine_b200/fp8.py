@@ -1,0 +1,127 @@
+"""Projections with both operands in 8 bits: out = x @ W.T from e4m3 codes with a power-of-two scale per block.
+
+An 8-bit value is an e4m3 code times 2^e. The exponent of a block whose largest finite magnitude is a is
+e = max(ceil(log2(a / 448)), -64); it is held as the byte e + 127. Codes are rounded to nearest even, values that are not
+finite become NaN. W has one exponent per 128 x 128 block, x one per token and 128 columns. Sums are FP32, the result is
+BF16: the format costs a relative rounding of 2^-4 per code and nothing for the scale.
+
+quantize_weight() makes the codes of a BF16 (or FP32) weight once; linear() is the product, quantising x on the way;
+quantize() gives x's codes for callers that share them between several products. kernel_fn_fp8() of muse_bf16_proj is the
+same behind the layer names of prepare().
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _capi
+
+BLOCK = 128
+E_MIN = -64
+WALK_MAX_TOKENS = 16   # csrc/fp8_linear.cu: more tokens take the tiled kernel, fewer and K <= WALK_MAX_K the walk
+WALK_MAX_K = 8192
+
+
+def _require(t: torch.Tensor, what: str, dtype: torch.dtype, dims: int) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} is on {t.device}: this path runs on a CUDA device only (no CPU fallback)")
+    if t.dtype != dtype or t.dim() != dims:
+        raise TypeError(f"{what} must be {dtype} with {dims} dimensions, got {t.dtype} {tuple(t.shape)}")
+
+
+def exponent_byte(amax: torch.Tensor) -> torch.Tensor:
+    """e + 127 of blocks with these largest magnitudes (int32): 448 = 0.875 * 2^9."""
+    m, e = torch.frexp(amax.float())
+    e = torch.where(m <= 0.875, e - 9, e - 8)
+    return torch.where(amax > 0, e, torch.full_like(e, E_MIN)).clamp(min=E_MIN) + 127
+
+
+def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """W [N, K] (BF16 or FP32, any device) as codes (float8_e4m3fn [N, K]) and exponent bytes (uint8
+    [ceil(N / 128), ceil(K / 128)]). Done once; in torch."""
+    if w.dim() != 2 or not w.is_floating_point():
+        raise TypeError(f"a weight is a floating-point [N, K] tensor, got {w.dtype} {tuple(w.shape)}")
+    n, k = w.shape
+    f = w.float()
+    a = torch.where(f.isfinite(), f.abs(), torch.zeros_like(f))
+    a = torch.nn.functional.pad(a, (0, -k % BLOCK, 0, -n % BLOCK)).view(-(-n // BLOCK), BLOCK, -(-k // BLOCK), BLOCK).amax((1, 3))
+    byte = exponent_byte(a)
+    inv = ((254 - byte) << 23).to(torch.int32).view(torch.float32)
+    y = (f * inv.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]).clamp(-448.0, 448.0)
+    y = torch.where(f.isfinite(), y, torch.full_like(y, float("nan")))
+    return y.to(torch.float8_e4m3fn).contiguous(), byte.to(torch.uint8).contiguous()
+
+
+def dequantize_weight(w8: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor:
+    """The FP32 values that quantize_weight()'s codes stand for."""
+    n, k = w8.shape
+    scale = (exponents.to(torch.int32) << 23).view(torch.float32)
+    return w8.float() * scale.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x itself where its rows can be read in 16-byte vectors, else a copy."""
+    m, k = x.shape
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
+        return x.contiguous().clone()
+    return x
+
+
+def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x BF16 [m, K], K a multiple of 16, as codes (float8_e4m3fn [m, K]) and exponent bytes (uint8 [m, ceil(K / 128)])."""
+    _require(x, "x", torch.bfloat16, 2)
+    m, k = x.shape
+    if m < 1 or k < 16 or k % 16:
+        raise ValueError(f"x must have at least one row and a multiple of 16 columns, got {tuple(x.shape)}")
+    with torch.cuda.device(x.device):
+        x = _rows(x)
+        xq = torch.empty((m, k), device=x.device, dtype=torch.float8_e4m3fn)
+        xe = torch.empty((m, -(-k // BLOCK)), device=x.device, dtype=torch.uint8)
+        _capi.check(_capi.load().muse_fp8_quantize(x.data_ptr(), xq.data_ptr(), xe.data_ptr(), m, k, x.stride(0) if m > 1 else k,
+                                                   torch.cuda.current_stream(x.device).cuda_stream), f"muse_fp8_quantize(m={m}, k={k})")
+    return xq, xe
+
+
+def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x @ W.T in BF16. `x`: BF16 [m, K] (any strides), or the pair that quantize() returns. `w8`, `w_exp`: the codes
+    [N, K] and exponent bytes of W, contiguous; K a multiple of 16. `out` (optional): BF16 [m, >= N] with unit column
+    stride, of which the first N columns are written."""
+    pair = isinstance(x, (tuple, list))
+    if pair:
+        xq, xe = x
+        _require(xq, "x's codes", torch.float8_e4m3fn, 2)
+        _require(xe, "x's exponents", torch.uint8, 2)
+        m, k = xq.shape
+        if xe.shape != (m, -(-k // BLOCK)) or not xq.is_contiguous() or not xe.is_contiguous() or xq.data_ptr() % 16:
+            raise ValueError(f"x's codes {tuple(xq.shape)} and exponents {tuple(xe.shape)} must be contiguous, one exponent per 128 columns")
+    else:
+        _require(x, "x", torch.bfloat16, 2)
+        m, k = x.shape
+    _require(w8, "w8", torch.float8_e4m3fn, 2)
+    _require(w_exp, "w_exp", torch.uint8, 2)
+    n = w8.shape[0]
+    dev = w8.device
+    if w8.shape[1] != k or m < 1 or n < 1 or k < 16 or k % 16:
+        raise ValueError(f"x [{m}, {k}] and W {tuple(w8.shape)} do not fit, or K is not a multiple of 16")
+    if w_exp.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not w8.is_contiguous() or not w_exp.is_contiguous() or w8.data_ptr() % 16:
+        raise ValueError(f"w8 {tuple(w8.shape)} and w_exp {tuple(w_exp.shape)} must be contiguous, one exponent per 128 x 128 block")
+    if w_exp.device != dev or (x[0] if pair else x).device != dev:
+        raise ValueError("x, w8 and w_exp must be on the same device")
+    if out is not None and (out.device != dev or out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n
+                            or out.stride(1) != 1 or (m > 1 and out.stride(0) < n)):
+        raise ValueError("out must be BF16 [m, >= N] with unit column stride on W's device")
+    lib = _capi.load()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty((m, n), device=dev, dtype=torch.bfloat16)
+        ld_out = out.stride(0) if m > 1 else n
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if not pair and m <= WALK_MAX_TOKENS and k <= WALK_MAX_K:
+            x = _rows(x)
+            _capi.check(lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k, x.stride(0) if m > 1 else k,
+                                          ld_out, stream), f"muse_fp8_walk(m={m}, n={n}, k={k})")
+            return out
+        xq, xe = x if pair else quantize(x)
+        _capi.check(lib.muse_fp8_tile(w8.data_ptr(), w_exp.data_ptr(), xq.data_ptr(), xe.data_ptr(), out.data_ptr(), m, n, k, ld_out, stream),
+                    f"muse_fp8_tile(m={m}, n={n}, k={k})")
+    return out

@@ -543,6 +543,41 @@ def kernel_fn_zip12(data, state) -> torch.Tensor:
     return out
 
 
+def prepare_fp8(state, layers=None) -> None:
+    """The 8-bit form (fp8.quantize_weight: e4m3 codes, a power-of-two scale per 128 x 128 block) of the BF16 weights
+    named in `layers` (default: all of them), kept in `state` beside the weights for kernel_fn_fp8(). K must be a multiple
+    of 16. The router stays in FP32: its logits decide between experts."""
+    from . import fp8
+
+    for name in (layers if layers is not None else [k for k in state if not k.startswith("_") and k not in FP32_LAYERS]):
+        if name not in state or name.startswith("_"):
+            raise KeyError(f"unknown layer {name!r}")
+        w = state[name]
+        if w.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: the 8-bit form is for BF16 weights")
+        if w.shape[1] % 16:
+            raise ValueError(f"{name}: K = {w.shape[1]} is not a multiple of 16")
+        state.setdefault("_fp8", {})[name] = fp8.quantize_weight(w)
+        torch.cuda.synchronize(w.device)   # codes are weights: complete before the first call
+
+
+def kernel_fn_fp8(data: Inputs, state, out: torch.Tensor | None = None) -> torch.Tensor:
+    """kernel_fn with both operands in 8 bits (fp8.linear): x is quantised per token and 128 columns on the way, the
+    weight's codes are those of prepare_fp8(). Same arguments, same slice rule, BF16 result; half the weight bytes. The
+    values differ from kernel_fn's by the rounding of 2^-4 per code (about 4 % of the result's norm at random data)."""
+    from . import fp8
+
+    x, cfg = data["x"], data["config"]
+    layer, n = cfg["layer"], int(cfg["n"])
+    form = state.get("_fp8", _EMPTY).get(layer)
+    if form is None:
+        raise KeyError(f"{layer}: prepare_fp8() has not made an 8-bit form of this layer")
+    w8, w_exp = form
+    if not 0 < n <= w8.shape[0]:
+        raise ValueError(f"{layer}: n={n} does not fit W {tuple(w8.shape)}")
+    return fp8.linear(x, w8[:n], w_exp[: -(-n // fp8.BLOCK)], out)
+
+
 FETCH_X_BY_KERNEL = True
 STORE_OUT_BY_KERNEL = True   # the copy-out of the larger calls by the same small kernel (786 KB: 5 us less than the copy engine)
 FETCH_MAX_TOKENS = 32       # x up to 256 KB: the fetch kernel beats the copy engine at every size measured
