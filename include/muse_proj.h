@@ -356,9 +356,12 @@ int muse_skinny_tc_noalloc(const void* tmap_w, const void* tmap_w_lo, const void
 int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x, void* stream);
 /* 1 .. 16 tokens, K <= 8192: x in BF16, quantised on the way; one launch. */
 int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream);
-/* Any number of tokens, x already in 8 bits. */
-int muse_fp8_tile(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out,
-                  void* stream);
+
+/* Any number of tokens, x already in 8 bits: TMA and block-scaled tcgen05 MMAs. ws: muse_fp8_gemm_ws_bytes bytes (0: may be NULL), 16-byte aligned,
+ * contents irrelevant; it belongs to the call until it completes. status: as for muse_gemm_tc. */
+long long muse_fp8_gemm_ws_bytes(int m, int N, int K);
+int muse_fp8_gemm(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int N, int K,
+                  int ld_out, void* stream);
 
 /* ---- the 8-bit cache: rotary positions, append, attention -------------------------------------------------------
  * What stands between the qkv_gate projection and the `o` projection of the decode layer. No counterpart in the reference's

@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 from pathlib import Path
 
+import torch
+
 from . import build as _build
 
 _LIB = None
@@ -67,7 +69,8 @@ SIGNATURES = {
                                          C.c_void_p]),
     "muse_fp8_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "muse_fp8_walk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
-    "muse_fp8_tile": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "muse_fp8_gemm_ws_bytes": (C.c_longlong, [C.c_int] * 3),
+    "muse_fp8_gemm": (C.c_int, [C.c_void_p] * 7 + [C.c_int] * 4 + [C.c_void_p]),
     "muse_rope_append": (C.c_int, [C.c_void_p] * 13 + [C.c_longlong] + [C.c_int] * 11 + [C.c_void_p]),
     "muse_cache_attention_ws_bytes": (C.c_longlong, [C.c_int] * 5),
     "muse_cache_attention": (C.c_int, [C.c_void_p] * 12 + [C.c_longlong] * 3 + [C.c_float] + [C.c_int] * 9 + [C.c_void_p]),
@@ -111,6 +114,54 @@ def check(rc: int, what: str) -> None:
     if rc != 0:
         kind = "rejected argument" if rc < 0 else "CUDA error"
         raise MuseError(f"{what}: {kind} {rc}")
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device `index` as the C ABI takes it (torch.cuda.current_stream() without building the
+    Python object: 2 us of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class on_device:
+    """torch.cuda.device for the calls that nearly always find their device current."""
+
+    __slots__ = ("index", "was")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.was != self.index:
+            torch.cuda.set_device(self.was)
+
+
+_STATUS: dict[int, torch.Tensor] = {}
+STATUS_TEXT = ((128, "a page index outside the pool"), (256, "lengths or row bounds that do not fit"))
+
+
+def status_word(device: torch.device) -> torch.Tensor:
+    """The status word that the 8-bit operators of a device share (the projections of prepare() have one per state)."""
+    word = _STATUS.get(device.index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():   # it must outlive the graph
+            raise MuseError("the first call of the 8-bit operators on a device makes their status word: make it outside stream capture")
+        word = _STATUS[device.index] = torch.zeros(1, device=device, dtype=torch.int32)
+    return word
+
+
+def check_status_word(device) -> None:
+    device = torch.device(device)
+    word = _STATUS.get(torch.cuda.current_device() if device.index is None else device.index)
+    bits = 0 if word is None else int(word.item())
+    if bits:
+        word.zero_()
+        what = [text for bit, text in STATUS_TEXT if bits & bit] + (["a timed-out wait"] if bits & ~384 else [])
+        raise MuseError(f"the 8-bit operators reported: {', '.join(what)} (status bits {bits:#x}, see MUSE_ST_* in muse_proj.h)")
 
 
 MAX_WORLD = 8

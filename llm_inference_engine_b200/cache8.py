@@ -19,6 +19,7 @@ other lengths. What they find wrong there they report through check_status(): se
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -28,8 +29,6 @@ from . import _capi
 
 PAGE = 64
 HEAD_DIMS = (64, 128)
-
-_STATUS: dict[int, torch.Tensor] = {}
 
 
 class Cache8(NamedTuple):
@@ -78,25 +77,11 @@ def rotary_table(rot: int, positions: int, device, base: float = 10000.0, scalin
     return (amplitude * torch.stack([angle.cos(), angle.sin()], -1)).float().contiguous()
 
 
-def _status(device: torch.device) -> torch.Tensor:
-    word = _STATUS.get(device.index)
-    if word is None:
-        word = _STATUS[device.index] = torch.zeros(1, device=device, dtype=torch.int32)
-    return word
-
-
 def check_status(device) -> None:
     """Synchronise and raise if a call since the last check met a page index outside the pool (the page was neither
     read nor written), lengths or row bounds that do not fit the table, the batch or max_q (they were clamped), or gave up
-    on a bounded wait. Not for use inside a stream capture."""
-    device = torch.device(device)
-    word = _STATUS.get(torch.cuda.current_device() if device.index is None else device.index)
-    bits = 0 if word is None else int(word.item())
-    if bits:
-        word.zero_()
-        what = [text for bit, text in ((128, "a page index outside the pool"), (256, "lengths or row bounds that do not fit"),
-                                       (512, "a timed-out wait")) if bits & bit]
-        raise _capi.MuseError(f"the cache kernels reported: {', '.join(what)} (status bits {bits:#x}, see MUSE_ST_* in muse_proj.h)")
+    on a bounded wait. Not for use inside a stream capture. (One word per device for the 8-bit operators, fp8's among them.)"""
+    _capi.check_status_word(device)
 
 
 def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
@@ -151,24 +136,26 @@ def rope_append(qkv: torch.Tensor, cache: Cache8, cos_sin: torch.Tensor, page_ta
         raise ValueError(f"qkv {tuple(qkv.shape)} is narrower than q | k | v = {(q_heads + 2 * heads) * dim} columns")
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
         raise TypeError(f"cos_sin must be a contiguous FP32 [positions, rot / 2, 2] table, got {cos_sin.dtype} {tuple(cos_sin.shape)}")
-    rot = 2 * cos_sin.shape[1]
-    if rot % 16 or not 16 <= rot <= dim or cos_sin.shape[0] < width * PAGE:
-        raise ValueError(f"the table turns {rot} dimensions (a multiple of 16 up to {dim}) at {cos_sin.shape[0]} positions; "
+    positions, rot = cos_sin.shape[0], 2 * cos_sin.shape[1]
+    if rot % 16 or not 16 <= rot <= dim or positions < width * PAGE:
+        raise ValueError(f"the table turns {rot} dimensions (a multiple of 16 up to {dim}) at {positions} positions; "
                          f"{width} pages per sequence need {width * PAGE}")
     if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (m > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
         qkv = qkv[:, : (q_heads + 2 * heads) * dim].contiguous().clone()
-    lib = _capi.load()
-    with torch.cuda.device(dev):
+    lib, index = _capi.load(), dev.index
+    with _capi.on_device(index):
         q = torch.empty((m, q_heads, dim), device=dev, dtype=torch.bfloat16)
-        kv = torch.empty((2, m, heads, dim), device=dev, dtype=torch.bfloat16) if values else None
+        k_val = v_val = None
+        if values:
+            k_val = torch.empty((m, heads, dim), device=dev, dtype=torch.bfloat16)
+            v_val = torch.empty((m, heads, dim), device=dev, dtype=torch.bfloat16)
         _capi.check(lib.muse_rope_append(qkv.data_ptr(), cos_sin.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
-                                         None if cu_q is None else cu_q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
-                                         cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), q.data_ptr(), kv[0].data_ptr() if values else None,
-                                         kv[1].data_ptr() if values else None, _status(dev).data_ptr(),
+                                         None if cu_q is None else cu_q.data_ptr(), cache[0].data_ptr(), cache[1].data_ptr(),
+                                         cache[2].data_ptr(), cache[3].data_ptr(), q.data_ptr(), k_val.data_ptr() if values else None,
+                                         v_val.data_ptr() if values else None, _capi.status_word(dev).data_ptr(),
                                          qkv.stride(0) if m > 1 else (q_heads + 2 * heads) * dim, m, batch, width, pages, max_q, q_heads, heads,
-                                         dim, rot, int(interleaved), cos_sin.shape[0], torch.cuda.current_stream(dev).cuda_stream),
-                    f"muse_rope_append(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
-    return (q, kv[0], kv[1]) if values else q
+                                         dim, rot, int(interleaved), positions, _capi.raw_stream(index)), "muse_rope_append")
+    return (q, k_val, v_val) if values else q
 
 
 def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens: torch.Tensor, *, cu_q: torch.Tensor | None = None,
@@ -195,23 +182,28 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
         gate = gate.contiguous().clone()
     if out is not None and (out.stride(1) != 1 or out.data_ptr() % 4 or (m > 1 and (out.stride(0) % 2 or out.stride(0) < cols))):
         raise ValueError("out must have unit column stride, an even row stride and 4-byte alignment")
-    lib = _capi.load()
-    with torch.cuda.device(dev):
+    lib, index = _capi.load(), dev.index
+    with _capi.on_device(index):
         if out is None:
             out = torch.empty((m, cols), device=dev, dtype=torch.bfloat16)
         # the workspace is the call's own (a captured graph keeps its own): calls may overlap on the GPU
-        ws_bytes = lib.muse_cache_attention_ws_bytes(batch, max_q, q_heads, heads, dim)
-        if ws_bytes < 0:
-            raise _capi.MuseError(f"muse_cache_attention_ws_bytes -> {ws_bytes}")
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        _capi.check(lib.muse_cache_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
+        ws = torch.empty(_ws_bytes(index, batch, max_q, q_heads, heads, dim), device=dev, dtype=torch.uint8)
+        _capi.check(lib.muse_cache_attention(q.data_ptr(), cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(),
                                              page_table.data_ptr(), seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
-                                             None if gate is None else gate.data_ptr(), out.data_ptr(), ws.data_ptr(), _status(dev).data_ptr(),
-                                             q.stride(0) if m > 1 else cols, 0 if gate is None else gate.stride(0) if m > 1 else cols,
-                                             out.stride(0) if m > 1 else cols, 1.0 / math.sqrt(dim) if scale is None else scale, m, batch, width,
-                                             pages, max_q, q_heads, heads, dim, window, torch.cuda.current_stream(dev).cuda_stream),
-                    f"muse_cache_attention(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
+                                             None if gate is None else gate.data_ptr(), out.data_ptr(), ws.data_ptr(),
+                                             _capi.status_word(dev).data_ptr(), q.stride(0) if m > 1 else cols,
+                                             0 if gate is None else gate.stride(0) if m > 1 else cols, out.stride(0) if m > 1 else cols,
+                                             1.0 / math.sqrt(dim) if scale is None else scale, m, batch, width, pages, max_q, q_heads, heads,
+                                             dim, window, _capi.raw_stream(index)), "muse_cache_attention")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(index: int, batch: int, max_q: int, q_heads: int, heads: int, dim: int) -> int:
+    size = _capi.load().muse_cache_attention_ws_bytes(batch, max_q, q_heads, heads, dim)
+    if size < 0:
+        raise _capi.MuseError(f"muse_cache_attention_ws_bytes -> {size}")
+    return size
 
 
 def attention_half(data, state, cache: Cache8, cos_sin: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *, q_heads: int,

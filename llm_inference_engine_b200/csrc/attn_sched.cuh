@@ -55,36 +55,30 @@ __host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m
   return e;
 }
 
-// First page of worker w's range when `total` pages are dealt to `workers`.
-__host__ __device__ inline long long attn_range(long long total, long long workers, long long w) { return total * w / workers; }
+// `total` pages dealt to `workers` in equal ranges: the first `rem` workers get one page more. With fewer pages than
+// workers only `total` workers take part, with one page each.
+struct AttnDeal {
+  long long total, base, rem;
+  int workers;   // those that take part
+};
+__host__ __device__ inline AttnDeal attn_deal(long long total, int workers) {
+  AttnDeal d;
+  d.total = total;
+  d.workers = total < workers ? static_cast<int>(total) : workers;
+  d.base = d.workers > 0 ? total / d.workers : 0;
+  d.rem = total - d.base * d.workers;
+  return d;
+}
+// First page of worker w's range (w = workers: the end).
+__host__ __device__ inline long long attn_range(const AttnDeal& d, int w) { return d.base * w + (w < d.rem ? w : d.rem); }
 // The worker whose range holds page f.
-__host__ __device__ inline long long attn_worker(long long total, long long workers, long long f) {
-  long long w = (f * workers + workers - 1) / total;   // within one of it
-  while (w > 0 && attn_range(total, workers, w) > f) --w;
-  while (w + 1 < workers && attn_range(total, workers, w + 1) <= f) ++w;
-  return w;
+__host__ __device__ inline int attn_worker(const AttnDeal& d, long long f) {
+  const long long big = d.rem * (d.base + 1);
+  return static_cast<int>(f < big ? f / (d.base + 1) : d.rem + (f - big) / d.base);
 }
 // Where worker w left its partial sums of the unit whose pages begin at u0 (the caller knows that w has some of them,
 // and not all): a worker has at most two partial segments, the one its range begins in (slot 0) and the one it ends in
-// (slot 1, when that is another). -1: w has no page at all (there are fewer pages than workers).
-__host__ __device__ inline long long attn_slot_of(long long total, long long workers, long long w, long long u0) {
-  const long long f = attn_range(total, workers, w);
-  if (f >= attn_range(total, workers, w + 1)) return -1;
-  return 2 * w + (f >= u0 ? 0 : 1);
-}
-// visit(slot) for the partial sums of a split unit of `pages` pages that begin at u0, in page order; nothing for a unit that
-// one worker has whole.
-template <typename F>
-__host__ __device__ inline void attn_for_slots(long long total, long long workers, long long u0, int pages, F&& visit) {
-  const long long w0 = attn_worker(total, workers, u0), w1 = attn_worker(total, workers, u0 + pages - 1);
-  if (w0 == w1) return;
-#ifdef __CUDA_ARCH__
-#pragma unroll 4
-#endif
-  for (long long w = w0; w <= w1; ++w) {
-    const long long slot = attn_slot_of(total, workers, w, u0);
-    if (slot >= 0) visit(slot);
-  }
-}
+// (slot 1, when that is another).
+__host__ __device__ inline int attn_slot_of(const AttnDeal& d, int w, long long u0) { return 2 * w + (attn_range(d, w) >= u0 ? 0 : 1); }
 
 }  // namespace muse

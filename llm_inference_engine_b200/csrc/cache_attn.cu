@@ -60,10 +60,10 @@ __device__ __forceinline__ AttnEntry attn_entry_of(const AttnArgs& a, int e, int
   return attn_entry(c0, c1, __ldcg(a.seq_lens + b), a.m, a.max_q, a.width * ATTN_PAGE, group, tile, rt, a.window);
 }
 
-// A place in the list of pages: entry, head, page of the unit.
+// A place in the list of pages: entry, head, i-th page of the unit.
 struct Cursor {
   AttnEntry en;
-  int e, h, i;   // i-th page of the unit
+  int e, h, i;
 };
 
 // The rows' state of one 16-row tile in a warp: lane (g, t) holds rows g and g + 8.
@@ -172,15 +172,14 @@ __device__ __forceinline__ void page_pv(TileState<D>& st, const uint32_t (&p)[4]
 }
 
 // lim[2], low[2]: first and last token of the page that rows g and g + 8 see; any_lo, any_hi: of any row of the tile,
-// all_lo, all_hi: of all of them.
+// all_lo, all_hi: of all of them. `s`: the page's raw scores; they become the weights `p`, and (a0, a1) what the rows' sums so
+// far are to be scaled by. Returns whether some row does not see some token.
 template <int D>
-__device__ __forceinline__ void page_step(TileState<D>& st, const uint32_t (&qf)[D / 16][4], const float (&qs)[2], uint32_t ks, uint32_t vs, float kscale,
-                                          float vscale, const int (&low)[2], const int (&lim)[2], int any_lo, int any_hi, int all_lo, int all_hi) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float s[8][4];
-  page_scores<D>(s, qf, ks);
+__device__ __forceinline__ bool page_softmax(TileState<D>& st, float (&s)[8][4], uint32_t (&p)[4][4], float& a0, float& a1, const float (&qs)[2], float kscale,
+                                             const int (&low)[2], const int (&lim)[2], int all_lo, int all_hi) {
+  const int t = threadIdx.x & 3;
   const float f0 = qs[0] * kscale, f1 = qs[1] * kscale;
-  const bool edge = all_lo > 0 || all_hi < ATTN_PAGE - 1;   // warp-uniform: some row does not see some token
+  const bool edge = all_lo > 0 || all_hi < ATTN_PAGE - 1;   // warp-uniform
   float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -204,11 +203,11 @@ __device__ __forceinline__ void page_step(TileState<D>& st, const uint32_t (&qf)
   m0 = fmaxf(m0, st.mx[0]);
   m1 = fmaxf(m1, st.mx[1]);
   const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;   // nothing seen yet: every weight is 2^-inf = 0
-  const float a0 = exp2_fast(st.mx[0] - b0), a1 = exp2_fast(st.mx[1] - b1);
+  a0 = exp2_fast(st.mx[0] - b0);
+  a1 = exp2_fast(st.mx[1] - b1);
   st.mx[0] = m0;
   st.mx[1] = m1;
   float l0 = 0.f, l1 = 0.f;
-  uint32_t p[4][4];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float e0 = exp2_fast(s[j][0] - b0), e1 = exp2_fast(s[j][1] - b0), e2 = exp2_fast(s[j][2] - b1), e3 = exp2_fast(s[j][3] - b1);
@@ -219,15 +218,18 @@ __device__ __forceinline__ void page_step(TileState<D>& st, const uint32_t (&qf)
   }
   st.l[0] = st.l[0] * a0 + l0;
   st.l[1] = st.l[1] * a1 + l1;
-  if (!edge) {
-    page_pv<D, false>(st, p, vs, a0, a1, vscale, 0, ATTN_PAGE - 1);
-    return;
-  }
-  // Tokens that no row sees (behind the sequence, or left of the window) may hold anything: their codes count as zero.
-  // A token that only some rows see and that holds NaN must not reach the others through 0 * NaN: those rows' pages
-  // are then multiplied once per distinct bound (rare: looked for in the codes).
+  return edge;
+}
+
+// A page that some row does not see all of. Tokens that no row sees (behind the sequence, or left of the window) may hold
+// anything: their codes count as zero. A token that only some rows see and that holds NaN must not reach the others
+// through 0 * NaN: such a page is multiplied once per distinct bound (rare: looked for in the codes).
+template <int D>
+__device__ __forceinline__ void page_pv_edge(TileState<D>& st, const uint32_t (&p)[4][4], uint32_t vs, float a0, float a1, float vscale, const int (&low)[2],
+                                          const int (&lim)[2], int any_lo, int any_hi) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   bool nan = false;
-#pragma unroll 1
+#pragma unroll 4
   for (int n = 0; n < D / 8; ++n) {
     const uint4 w = lds16(vs + static_cast<uint32_t>(8 * n + g) * ATTN_PAGE + 16 * t);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -245,7 +247,6 @@ __device__ __forceinline__ void page_step(TileState<D>& st, const uint32_t (&qf)
     st.o[n][2] *= a1;
     st.o[n][3] *= a1;
   }
-  // every row on its own: the rows whose (low, lim) the warp's row r has are multiplied with r's tokens only
 #pragma unroll 1
   for (int r = 0; r < ATTN_TILE; ++r) {
     const int rl = __shfl_sync(0xffffffffu, r < 8 ? low[0] : low[1], (r & 7) * 4), rh = __shfl_sync(0xffffffffu, r < 8 ? lim[0] : lim[1], (r & 7) * 4);
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   __shared__ long long s_sum[ATTN_WARPS + 1];
   __shared__ int s_entry[ATTN_WARPS];
   __shared__ long long s_start[ATTN_WARPS];
+  __shared__ int2 s_rec[ATTN_WARPS][64];   // looked-up pages: tile index in the pool, exponents (k | v << 8)
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.hq / a.hk, entries = a.batch * a.tiles;
@@ -378,10 +380,13 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     total += s_sum[w];
   }
   const long long begin = base + incl - mine, end = base + incl;   // this thread's share of the list
-  const long long workers = SHARED ? gridDim.x : static_cast<long long>(gridDim.x) * ATTN_WARPS;
+  const AttnDeal deal = attn_deal(total, static_cast<int>(SHARED ? gridDim.x : gridDim.x * ATTN_WARPS));
+  // Neighbouring workers sit on different SMs, so that a list with fewer pages than warps is spread over all of them.
+  auto worker_of = [&](int w) { return static_cast<int>(SHARED ? blockIdx.x : w * gridDim.x + blockIdx.x); };
   if (total > 0) {
     for (int w = 0; w < (SHARED ? 1 : ATTN_WARPS); ++w) {
-      const long long f = attn_range(total, workers, SHARED ? blockIdx.x : static_cast<long long>(blockIdx.x) * ATTN_WARPS + w);
+      if (worker_of(w) >= deal.workers) break;
+      const long long f = attn_range(deal, worker_of(w));
       if (f >= begin && f < end) {
         long long at = begin;
         for (int e = e0; e < e1; ++e) {
@@ -405,111 +410,130 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   }
   if (blockIdx.x == 0 && tid == 0) a.prefix[entries] = total;
   __syncthreads();
-  if (total == 0) return;
-  const long long worker = SHARED ? blockIdx.x : static_cast<long long>(blockIdx.x) * ATTN_WARPS + warp;
-  long long f = attn_range(total, workers, worker);
-  const long long f1 = attn_range(total, workers, worker + 1);
-  if (f >= f1) return;   // SHARED: CTA-uniform; else this warp has no page, and nobody waits for it
+  const int worker = worker_of(warp);
+  if (worker >= deal.workers) return;   // SHARED: CTA-uniform; else this warp has no page, and nobody waits for it
+  const long long f0 = attn_range(deal, worker);
+  const int count = static_cast<int>(attn_range(deal, worker + 1) - f0);   // this worker's pages
 
-  auto place = [&](Cursor& c, int e, long long start) {   // at page f of the list
-    c.e = e;
-    c.en = attn_entry_of(a, e, group, TILE);
-    const int off = static_cast<int>(f - start);
-    c.h = off / c.en.pages;
-    c.i = off % c.en.pages;
-  };
-  auto advance = [&](Cursor& c) {
-    if (++c.i < c.en.pages) return;
+  Cursor rd, fill;   // where the warp computes, and up to where it has looked up pages
+  {
+    const int w = SHARED ? 0 : warp;
+    rd.e = s_entry[w];
+    rd.en = attn_entry_of(a, rd.e, group, TILE);
+    const int off = static_cast<int>(f0 - s_start[w]);
+    rd.h = off / rd.en.pages;
+    rd.i = off % rd.en.pages;
+    fill = rd;
+  }
+  auto next_unit = [&](Cursor& c) {   // false behind the last entry
     c.i = 0;
-    if (++c.h < a.hk) return;
+    if (++c.h < a.hk) return true;
     c.h = 0;
     do {
-      ++c.e;
-      if (c.e >= entries) return;
+      if (++c.e >= entries) return false;
       c.en = attn_entry_of(a, c.e, group, TILE);
     } while (c.en.pages == 0);
+    return true;
   };
-  // The page a cursor stands at: its index in the pool, or -1 (not a page of the pool, or nothing is seen).
-  auto page_of = [&](const Cursor& c) {
-    if (c.en.last < 0) return -1;
-    const int p = __ldcg(a.page_table + static_cast<size_t>(c.e / a.tiles) * a.width + c.en.page0 + c.i);
-    if (p >= 0 && p < a.pages) return p;
-    if (lane == 0) atomicOr(a.status, ST_BAD_PAGE);
-    return -1;
+  // Looks up the next 32 pages of the worker's list, a page per lane: the tile's index in the pool (page * hk + head; -1:
+  // not a page of the pool, or nothing is seen) and its two exponents, into the warp's ring of records.
+  int filled = 0;
+  auto look_up = [&]() {
+    int b = -1, h = 0, i = 0, off = 0;
+    while (off < 32 && filled + off < count) {
+      const int left = fill.en.pages - fill.i, take = min(left, 32 - off);
+      if (lane >= off && lane < off + take) {
+        b = fill.en.last < 0 ? -1 : fill.e / a.tiles;
+        h = fill.h;
+        i = fill.en.page0 + fill.i + lane - off;
+      }
+      off += take;
+      fill.i += take;
+      if (fill.i == fill.en.pages && !next_unit(fill)) break;
+    }
+    int2 rec = make_int2(-1, 127 | 127 << 8);
+    if (b >= 0 && filled + lane < count) {
+      const int p = __ldcg(a.page_table + static_cast<size_t>(b) * a.width + i);
+      if (p >= 0 && p < a.pages) {
+        rec.x = p * a.hk + h;
+        rec.y = __ldcg(a.k_exp + rec.x) | __ldcg(a.v_exp + rec.x) << 8;
+      } else {
+        atomicOr(a.status, ST_BAD_PAGE);
+      }
+    }
+    s_rec[warp][(filled + lane) & 63] = rec;
+    filled += 32;
+    __syncwarp();
   };
+  look_up();
 
-  Cursor rd, wr;   // where the warp computes, and where it has requested up to
-  place(wr, s_entry[SHARED ? 0 : warp], s_start[SHARED ? 0 : warp]);
-  rd = wr;
-  long long fw = f;
-  uint32_t issued = 0, used = 0;          // halves (K, then V of a page) requested and consumed by this worker
-  const uint32_t halves = static_cast<uint32_t>(2 * (f1 - f));
+  int issued = 0, used = 0;               // halves (K, then V of a page) requested and consumed by this worker
+  const int halves = 2 * count;
   const bool issuer = !SHARED || warp == 0;
-  int wr_page = -1;
   // Requests the next half; every lane of the issuing warp runs it.
   auto request = [&]() {
-    const uint32_t slot = issued % SLOTS, turn = issued / SLOTS;
-    if (SHARED && turn > 0 && !mbar_wait(smem_u32(&empty[slot]), (turn - 1) & 1u)) {
+    const int slot = issued % SLOTS, turn = issued / SLOTS;
+    if (SHARED && turn > 0 && !mbar_wait(smem_u32(&empty[slot]), (turn - 1) & 1)) {
       if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
       s_abort = 1;
       return;
     }
-    if ((issued & 1u) == 0) wr_page = page_of(wr);
     if (lane == 0) {
       const uint32_t bar = smem_u32(&full[slot]);
-      if (wr_page >= 0) {
-        const size_t off = (static_cast<size_t>(wr_page) * a.hk + wr.h) * SLOT_BYTES;
+      const int tile = s_rec[warp][(issued >> 1) & 63].x;
+      if (tile >= 0) {
         mbar_expect_tx(bar, SLOT_BYTES);
-        bulk_load_1d(ring_base + slot * SLOT_BYTES, ((issued & 1u) ? a.v : a.k) + off, SLOT_BYTES, bar);
+        bulk_load_1d(ring_base + static_cast<uint32_t>(slot) * SLOT_BYTES, ((issued & 1) ? a.v : a.k) + static_cast<size_t>(tile) * SLOT_BYTES, SLOT_BYTES, bar);
       } else {
         mbar_arrive(bar);   // nothing to bring: the page is masked whole
       }
     }
-    if (issued & 1u) {
-      ++fw;
-      if (fw < f1) advance(wr);
-    }
     ++issued;
   };
+  // The warp has read a half: its slot may be filled again.
+  auto release = [&]() {
+    __syncwarp();
+    if (SHARED && lane == 0) mbar_arrive(smem_u32(&empty[used % SLOTS]));
+    ++used;
+    if (issuer)
+      while (issued < halves && issued < used + SLOTS && (issued >> 1) < filled && !(SHARED && s_abort)) request();
+  };
   if (issuer)
-    while (issued < halves && issued < SLOTS) request();
+    while (issued < halves && issued < SLOTS && (issued >> 1) < filled) request();
 
   TileState<D> st;
   uint32_t qf[D / 16][4];
   float qs[2];
   const int wrow = SHARED ? warp * ATTN_TILE : 0;   // this warp's first row in the worker's tile
-  bool fresh = true;
-  int seg_first = 0;                                // first page of the segment
-  bool first_segment = true;
-  for (; f < f1; ++f) {
-    const int my_rows = max(0, min(ATTN_TILE, rd.en.rows - wrow));
+  bool fresh = true, first_segment = true;
+  int seg_first = 0, my_rows = 0;                   // first page of the segment; rows of this warp
+  for (int n = 0; n < count; ++n) {
     if (fresh) {
+      my_rows = max(0, min(ATTN_TILE, rd.en.rows - wrow));
       tile_reset(st);
       load_q<D>(a, rd.en, rd.h, rd.en.row0 + wrow, my_rows, group, qf, qs);
       fresh = false;
       seg_first = rd.i;
     }
-    const int page = page_of(rd);
-    float kscale = 1.f, vscale = 1.f;
-    if (page >= 0) {
-      kscale = exp2_byte(__ldcg(a.k_exp + static_cast<size_t>(page) * a.hk + rd.h));
-      vscale = exp2_byte(__ldcg(a.v_exp + static_cast<size_t>(page) * a.hk + rd.h));
-    }
-    const uint32_t ks = used % SLOTS, kt = used / SLOTS, vsl = (used + 1) % SLOTS, vt = (used + 1) / SLOTS;
-    const bool ok = mbar_wait(smem_u32(&full[ks]), kt & 1u) && mbar_wait(smem_u32(&full[vsl]), vt & 1u);
-    if (!ok || (SHARED && s_abort)) {
-      if (lane == 0 && !ok) atomicOr(a.status, ST_ATTN_TIMEOUT);
-      s_abort = 1;
-      break;
-    }
-    if (page >= 0 && my_rows > 0) {
+    // records: looked up 32 at a time, while those of the pages under way stay (the ring of records holds 64)
+    if (filled < count && filled - n <= SLOTS / 2 + 2) look_up();
+    const int2 rec = s_rec[warp][n & 63];
+    const bool live = rec.x >= 0 && my_rows > 0;
+    const int ks = used % SLOTS, vsl = (used + 1) % SLOTS, vt = (used + 1) / SLOTS;
+    bool ok = mbar_wait(smem_u32(&full[ks]), (used / SLOTS) & 1);
+    float s[8][4], a0, a1;
+    uint32_t p[4][4];
+    int low[2], lim[2], any_lo, any_hi, all_lo, all_hi;   // positions grow with the row
+    bool edge = false;
+    if (ok && live) page_scores<D>(s, qf, ring_base + static_cast<uint32_t>(ks) * SLOT_BYTES);
+    release();
+    if (ok && live) {
       const int p0 = (rd.en.page0 + rd.i) * ATTN_PAGE, g = lane >> 2;
       auto bounds = [&](int r, int& lo, int& hi) {   // tokens of the page that row r of the warp's tile sees
         const int pos = rd.en.pos + (rd.en.row0 + wrow + r) / group;
         hi = pos - p0;
         lo = a.window > 0 ? pos - a.window + 1 - p0 : 0;
       };
-      int low[2], lim[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         bounds(g + 8 * half, low[half], lim[half]);
@@ -518,44 +542,49 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
           lim[half] = -1;
         }
       }
-      int any_lo, any_hi, all_lo, all_hi;   // positions grow with the row
       bounds(0, any_lo, all_hi);
       bounds(my_rows - 1, all_lo, any_hi);
-      page_step<D>(st, qf, qs, ring_base + ks * SLOT_BYTES, ring_base + vsl * SLOT_BYTES, kscale, vscale, low, lim, any_lo, any_hi, all_lo, all_hi);
+      edge = page_softmax<D>(st, s, p, a0, a1, qs, exp2_byte(rec.y & 255), low, lim, all_lo, all_hi);
     }
-    used += 2;
-    __syncwarp();
-    if (SHARED) {
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&empty[ks]));
-        mbar_arrive(smem_u32(&empty[vsl]));
-      }
+    ok = ok && mbar_wait(smem_u32(&full[vsl]), vt & 1);
+    if (!ok || (SHARED && s_abort)) {
+      if (lane == 0 && !ok) atomicOr(a.status, ST_ATTN_TIMEOUT);
+      s_abort = 1;
+      break;
     }
-    if (issuer)
-      while (issued < halves && issued < used + SLOTS && !(SHARED && s_abort)) request();
+    if (live) {
+      const uint32_t vs = ring_base + static_cast<uint32_t>(vsl) * SLOT_BYTES;
+      const float vscale = exp2_byte(rec.y >> 8);
+      if (edge) page_pv_edge<D>(st, p, vs, a0, a1, vscale, low, lim, any_lo, any_hi);
+      else page_pv<D, false>(st, p, vs, a0, a1, vscale, 0, ATTN_PAGE - 1);
+    }
+    release();
     // end of the unit or of the range: the segment [seg_first, rd.i] is done
-    const bool unit_end = rd.i == rd.en.pages - 1, range_end = f + 1 == f1;
-    if (unit_end || range_end) {
+    const bool unit_end = rd.i == rd.en.pages - 1;
+    if (unit_end || n + 1 == count) {
       const bool whole = unit_end && seg_first == 0;
       // a worker has at most two partial segments: the one it begins inside a unit, and the one it ends inside one
-      float* slot = a.part + (2 * worker + (first_segment ? 0 : 1)) * attn_slot_floats(D, TILE);
+      float* slot = a.part + (2ll * worker + (first_segment ? 0 : 1)) * attn_slot_floats(D, TILE);
       tile_store<D>(st, a, rd.en, rd.h, rd.en.row0 + wrow, my_rows, group, whole, slot, TILE, wrow);
       fresh = true;
       first_segment = false;
     }
-    if (!range_end) advance(rd);
+    if (n + 1 < count) {
+      if (unit_end) next_unit(rd);
+      else ++rd.i;
+    }
   }
   if (s_abort) {
     // leave no copy in flight behind: each slot's last request is waited for (bounded)
     if (issuer)
-      for (uint32_t i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(smem_u32(&full[i % SLOTS]), (i / SLOTS) & 1u);
+      for (int i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(smem_u32(&full[i % SLOTS]), (i / SLOTS) & 1);
   }
 }
 
 // Adds up the partial sums of the units that were split between workers: one warp per row, a unit's segments in page
 // order (the same bits in every run).
 template <int D, bool SHARED>
-__global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnArgs a, long long workers) {
+__global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnArgs a, int workers) {
   constexpr int TILE = SHARED ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
   constexpr int V = D / 32;   // dimensions per lane
   griddep_launch_dependents();
@@ -563,24 +592,27 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
   const int entries = a.batch * a.tiles, group = a.hq / a.hk;
   const int e = static_cast<int>(blockIdx.x) / a.hk, h = static_cast<int>(blockIdx.x) % a.hk;
   const int r = static_cast<int>(blockIdx.y) * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
   const AttnEntry en = attn_entry_of(a, e, group, TILE);
   if (r >= en.rows) return;
-  const long long total = __ldcg(a.prefix + entries);
-  const long long u0 = __ldcg(a.prefix + e) + static_cast<long long>(h) * en.pages, u1 = u0 + en.pages;
-  const long long w0 = attn_worker(total, workers, u0), w1 = attn_worker(total, workers, u1 - 1);
+  const AttnDeal deal = attn_deal(total, workers);
+  const long long u0 = start + static_cast<long long>(h) * en.pages;
+  const int w0 = attn_worker(deal, u0), w1 = attn_worker(deal, u0 + en.pages - 1);
   if (w0 == w1) return;   // one worker had the whole unit and has written it
-  auto at = [&](long long slot) { return a.part + slot * attn_slot_floats(D, TILE); };
+  // all but the first worker's segments are that worker's first
+  const size_t stride = 2ull * attn_slot_floats(D, TILE);
+  const float* const first = a.part + static_cast<size_t>(attn_slot_of(deal, w0, u0)) * attn_slot_floats(D, TILE);
+  const float* const rest = a.part + static_cast<size_t>(w0) * stride;   // worker w0 + i's first slot, i > 0: rest + i stride
+  const int parts = w1 - w0 + 1;
   float mx = -INFINITY;
-  for (long long w = w0 + lane; w <= w1; w += 32) {
-    const long long slot = attn_slot_of(total, workers, w, u0);
-    if (slot >= 0) mx = fmaxf(mx, __ldcg(at(slot) + r));
-  }
+  for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, __ldcg((i ? rest + i * stride : first) + r));
 #pragma unroll
   for (int s = 16; s; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
   const float b = mx == -INFINITY ? 0.f : mx;
   float l = 0.f, o[V] = {};
-  attn_for_slots(total, workers, u0, en.pages, [&](long long slot) {
-    const float* s = at(slot);
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float* s = i ? rest + i * stride : first;
     const float f = exp2_fast(__ldcg(s + r) - b);
     l = fmaf(__ldcg(s + TILE + r), f, l);
     const float* src = s + 2 * TILE + static_cast<size_t>(r) * D + lane * V;
@@ -591,7 +623,7 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
       const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
       o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]);
     }
-  });
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int rr = en.row0 + r;
   const size_t tok = en.first + rr / group;
@@ -640,7 +672,7 @@ static cudaError_t attn_launch(const AttnArgs& a, int sms, cudaStream_t stream) 
   const int rows = a.max_q * (a.hq / a.hk) < tile ? a.max_q * (a.hq / a.hk) : tile;
   const long long workers = SHARED ? sms : static_cast<long long>(sms) * ATTN_WARPS;
   const long long units = static_cast<long long>(a.batch) * a.tiles * a.hk;
-  return launch_dependent(cache_attn_join_kernel<D, SHARED>, dim3(static_cast<unsigned>(units), (rows + 3) / 4), dim3(128), 0, stream, a, workers);
+  return launch_dependent(cache_attn_join_kernel<D, SHARED>, dim3(static_cast<unsigned>(units), (rows + 3) / 4), dim3(128), 0, stream, a, static_cast<int>(workers));
 }
 
 int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
@@ -655,7 +687,7 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   const int sms = attn_sms();
   if (sms < 1) return -7;
   a.tiles = attn_tiles(a.max_q, a.hq, a.hk);
-  if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll) return -3;
+  if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
   const bool sh = attn_shared(a.max_q, a.hq, a.hk);
   const long long workers = sh ? sms : static_cast<long long>(sms) * ATTN_WARPS;
   a.part = static_cast<float*>(ws);
@@ -698,12 +730,13 @@ long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch
   if (!p.ok || !segments) return -1;
   for (int e = 0; e < p.entries; ++e) p.total += static_cast<long long>(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e).pages) * hk;
   if (p.total == 0) return 0;
+  const AttnDeal deal = attn_deal(p.total, static_cast<int>(p.workers));
   long long count = 0, start = 0;
   int e = 0;
   AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, 0);
-  for (long long w = 0; w < p.workers; ++w) {
+  for (int w = 0; w < deal.workers; ++w) {
     bool first = true;
-    for (long long f = attn_range(p.total, p.workers, w), f1 = attn_range(p.total, p.workers, w + 1); f < f1;) {
+    for (long long f = attn_range(deal, w), f1 = attn_range(deal, w + 1); f < f1;) {
       while (f >= start + static_cast<long long>(en.pages) * hk) {
         start += static_cast<long long>(en.pages) * hk;
         en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, ++e);
@@ -712,8 +745,8 @@ long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch
       const int n = static_cast<int>(f1 - f < en.pages - i ? f1 - f : en.pages - i);
       if (count < capacity) {
         int* s = segments + 6 * count;
-        s[0] = static_cast<int>(w); s[1] = e; s[2] = h; s[3] = en.page0 + i; s[4] = n;
-        s[5] = n == en.pages ? -1 : static_cast<int>(2 * w + (first ? 0 : 1));
+        s[0] = w; s[1] = e; s[2] = h; s[3] = en.page0 + i; s[4] = n;
+        s[5] = n == en.pages ? -1 : 2 * w + (first ? 0 : 1);
       }
       ++count;
       first = false;
@@ -734,12 +767,13 @@ long long cache_attn_join(const int* seq_lens, const int* cu_q, int m, int batch
   }
   const AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, entry);
   if (en.rows == 0) return 0;
-  long long count = 0;
-  attn_for_slots(p.total, p.workers, before + static_cast<long long>(head) * en.pages, en.pages, [&](long long slot) {
-    if (count < capacity) slots[count] = static_cast<int>(slot);
-    ++count;
-  });
-  return count;
+  const AttnDeal deal = attn_deal(p.total, static_cast<int>(p.workers));
+  const long long u0 = before + static_cast<long long>(head) * en.pages;
+  const int w0 = attn_worker(deal, u0), w1 = attn_worker(deal, u0 + en.pages - 1);
+  if (w0 == w1) return 0;
+  for (int w = w0; w <= w1; ++w)
+    if (w - w0 < capacity) slots[w - w0] = attn_slot_of(deal, w, u0);
+  return w1 - w0 + 1;
 }
 
 }  // namespace muse

@@ -56,7 +56,9 @@ long long skinny_static_ws_floats();
 int skinny_static_cnt_ints();
 int fp8_quantize_dispatch(const void* x, void* xq, void* xe, int m, int K, int ld_x, cudaStream_t stream);
 int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, cudaStream_t stream);
-int fp8_tile_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, cudaStream_t stream);
+int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int n, int k, int ld_out,
+                      cudaStream_t stream);
+long long fp8_gemm_ws_bytes(int m, int n, int k);
 
 // cuTensorMapEncodeTiled is a driver entry point; fetching it through the runtime keeps the
 // library free of a link-time dependency on libcuda (it must load on machines without a driver).
@@ -86,6 +88,19 @@ static int encode_2d(CUtensorMap* tm, const void* base, long long rows, long lon
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return static_cast<int>(r);
+}
+// The same for a row-major matrix of bytes (contiguous rows): boxes of [box_rows, 128 columns].
+int encode_2d_u8(CUtensorMap* tm, const void* base, long long rows, long long cols, int box_rows) {
+  if (!tm || !base || rows <= 0 || cols <= 0 || box_rows <= 0 || box_rows > 256) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (cols & 15)) return -2;
+  PFN_cuTensorMapEncodeTiled fn = encode_fn();
+  if (!fn) return -8;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return static_cast<int>(fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
 }
 __global__ void nop_kernel() {}
 
@@ -365,8 +380,11 @@ int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x,
 int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream) {
   return muse::fp8_walk_dispatch(W, we, x, out, m, N, K, ld_x, ld_out, static_cast<cudaStream_t>(stream));
 }
-int muse_fp8_tile(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, void* stream) {
-  return muse::fp8_tile_dispatch(W, we, xq, xe, out, m, N, K, ld_out, static_cast<cudaStream_t>(stream));
+
+long long muse_fp8_gemm_ws_bytes(int m, int N, int K) { return muse::fp8_gemm_ws_bytes(m, N, K); }
+int muse_fp8_gemm(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int N, int K, int ld_out,
+                  void* stream) {
+  return muse::fp8_gemm_dispatch(W, we, xq, xe, out, ws, status, m, N, K, ld_out, static_cast<cudaStream_t>(stream));
 }
 
 int muse_rope_append(const void* qkv, const void* cos_sin, const void* page_table, const void* seq_lens, const void* cu_q, void* k, void* v,

@@ -1,0 +1,452 @@
+// out[m, N] = x[m, K] . W[N, K]^T, both in 8 bits with a power-of-two scale per block of 128 (fp8.cuh), for more tokens than
+// the walk of fp8_linear.cu takes: TMA -> shared-memory ring -> block-scaled tcgen05.mma -> tensor memory.
+//
+// The scales are powers of two, so the tensor core applies them itself (kind::mxf8f6f4, one exponent byte per row and 32
+// columns; four neighbouring 32-column pieces share ours): the accumulator holds the scaled sum in FP32 and nothing is
+// read back between blocks. A = up to MT x 128 tokens (lanes of tensor memory), B = nt rows of W (columns). The exponents
+// live in tensor memory too, as the instruction wants them: row r of 128 in lane r % 32 of every quarter, 32-bit column
+// r / 32, the bytes of a word being four successive blocks of 128 columns, which the instruction descriptor
+// selects; so one store serves 512 columns of K.
+//
+// What bounds it at many tokens is traffic from L2 into shared memory, (256 + nt) x 128 bytes per 256 x nt x 128
+// products with MT = 2, hence the widest tile that tensor memory holds beside the scales (2 x 224 + 2 x 16 columns);
+// at 17..256 tokens it is the weight's own bytes, for which K is cut so that all SMs load.
+//
+// Roles: warp 0 TMA, warp 1 tensor memory and MMA issue, warps 2..5 scales (registers one group ahead) and epilogue, a
+// warp per quarter of the lanes. The grid is persistent: a CTA walks tiles of (K slice, row tile, token tile), and the
+// loads of its next tile start while the epilogue drains the accumulators. K slices leave FP32 sums in a workspace that a
+// second kernel adds up in slice order (same bits in every run).
+#include "fp8.cuh"
+
+namespace muse {
+
+constexpr int G8_TOK = 128;             // rows of one MMA
+constexpr int G8_MAX_STAGES = 12;
+constexpr int G8_SF_COL = 448;          // first tensor-memory column of the scales
+constexpr int G8_SF_STRIDE = 16;        // columns of one group of scales: 4 per token tile, 8 for W's rows
+constexpr int G8_THREADS = 192;
+constexpr int G8_MIN_SMEM = 116 * 1024;  // one CTA per SM: it takes all of tensor memory
+
+struct G8Args {
+  const uint8_t* xe;   // [m, kblocks]
+  const uint8_t* we;   // [ceil(N / 128), kblocks]
+  __nv_bfloat16* out;
+  float* ws;           // [split, m, N] when split > 1
+  int* status;
+  int m, n, k, kblocks, ld_out;
+  int nt, a_rows;      // rows of W per tile; token rows a TMA box brings
+  int row_tiles, tok_tiles, split, stages;
+};
+
+__device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: e4m3 x e4m3 -> FP32, K-major, power-of-two scales; which byte of a scale word counts.
+__host__ __device__ constexpr uint32_t g8_idesc(int N, int sf_byte) {
+  return (static_cast<uint32_t>(sf_byte) << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(G8_TOK >> 7) << 27) |
+         (static_cast<uint32_t>(sf_byte) << 29);
+}
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int MT>
+__global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                                                                 const __grid_constant__ G8Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[G8_MAX_STAGES], bar_empty[G8_MAX_STAGES];
+  __shared__ __align__(8) uint64_t bar_sf_full[2], bar_sf_empty[2], bar_acc_full, bar_acc_empty;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // the 128-byte swizzle repeats every 1024 bytes
+  const uint32_t a_tile = G8_TOK * FP8_BLOCK;                          // a token tile's place in a stage (its box may be shorter)
+  const uint32_t b_bytes = static_cast<uint32_t>(a.nt) * FP8_BLOCK;
+  const uint32_t stage_bytes = MT * a_tile + b_bytes;
+  const uint32_t tx_bytes = MT * static_cast<uint32_t>(a.a_rows) * FP8_BLOCK + b_bytes;
+  const int tiles = a.row_tiles * a.tok_tiles * a.split;
+  // Tile t: token tiles innermost (neighbouring CTAs share W's rows through L2), then row tiles, then K slices.
+  auto slice = [&](int t, int& tok, int& row, int& kb0, int& kb1) {
+    tok = t % a.tok_tiles;
+    row = t / a.tok_tiles % a.row_tiles;
+    const int s = t / (a.tok_tiles * a.row_tiles);
+    kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * s / a.split);
+    kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (s + 1) / a.split);
+    return s;
+  };
+
+  if (tid == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_sf_full[i]), 4);
+      mbar_init(smem_u32(&bar_sf_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&bar_acc_full), 1);
+    mbar_init(smem_u32(&bar_acc_empty), 4);
+    fence_mbar_init();
+    s_abort = 0;
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  griddep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = l2_policy_evict_last();
+      int s = 0;
+      uint32_t phase = 0, issued = 0;
+      bool ok = true, waited = false;
+      auto load_x = [&](int st, int kb, int tok) {
+        const uint32_t bar = smem_u32(&bar_full[st]), at = smem_base + static_cast<uint32_t>(st) * stage_bytes;
+        for (int h = 0; h < MT; ++h) tma_load_2d(at + static_cast<uint32_t>(h) * a_tile, &tm_x, kb * FP8_BLOCK, (tok * MT + h) * G8_TOK, bar, pol);
+      };
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int tok, row, kb0, kb1;
+        slice(t, tok, row, kb0, kb1);
+        int held = 0;   // stages whose weights are under way while x may still be being written by the kernel ahead
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (issued >= static_cast<uint32_t>(a.stages) && !mbar_wait(smem_u32(&bar_empty[s]), phase ^ 1u)) {
+            atomicOr(a.status, ST_PRODUCER_TIMEOUT);
+            s_abort = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&bar_full[s]), at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
+          mbar_expect_tx(bar, tx_bytes);
+          tma_load_2d(at + MT * a_tile, &tm_w, kb * FP8_BLOCK, row * a.nt, bar, pol);
+          ++issued;
+          if (waited) {
+            load_x(s, kb, tok);
+          } else if (++held == a.stages || kb + 1 == kb1) {
+            griddep_wait();
+            waited = true;
+            for (int i = 0; i < held; ++i) load_x(i, kb0 + i, tok);
+          }
+          if (++s == a.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok)   // leave no copy in flight: the stages issued last (bounded)
+        for (int i = 0; i < a.stages && i < static_cast<int>(issued); ++i) {
+          const uint32_t j = issued - 1 - static_cast<uint32_t>(i);
+          if (!mbar_wait(smem_u32(&bar_full[j % static_cast<uint32_t>(a.stages)]), (j / static_cast<uint32_t>(a.stages)) & 1u)) atomicOr(a.status, ST_DRAIN_TIMEOUT);
+        }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0, sf = 0;
+      uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int tok, row, kb0, kb1;
+        slice(t, tok, row, kb0, kb1);
+        // the accumulators are free once the epilogue has read the tile before
+        if (t != static_cast<int>(blockIdx.x) && !mbar_wait(smem_u32(&bar_acc_empty), acc_phase ^ 1u)) ok = false;
+        tc_fence_after_sync();
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          const int j = (kb - kb0) & 3;
+          if (j == 0 && !mbar_wait(smem_u32(&bar_sf_full[sf]), sf_phase)) ok = false;
+          if (ok && !mbar_wait(smem_u32(&bar_full[s]), phase)) ok = false;
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
+          const uint64_t bd = umma_desc_k_sw128(at + MT * a_tile);
+          const uint32_t sfa = tmem + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE, sfb = sfa + 4 * MT;
+          const uint32_t idesc = g8_idesc(a.nt, j);
+#pragma unroll
+          for (int k = 0; k < FP8_BLOCK / 32; ++k)   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
+#pragma unroll
+            for (int h = 0; h < MT; ++h)
+              umma_mxf8(tmem + static_cast<uint32_t>(h * a.nt), umma_desc_k_sw128(at + static_cast<uint32_t>(h) * a_tile) + 2 * k, bd + 2 * k, idesc,
+                        sfa + 4u * static_cast<uint32_t>(h), sfb, (kb > kb0 || k > 0) ? 1u : 0u);
+          umma_commit(smem_u32(&bar_empty[s]));
+          if (j == 3 || kb + 1 == kb1) {
+            umma_commit(smem_u32(&bar_sf_empty[sf]));
+            if (++sf == 2) {
+              sf = 0;
+              sf_phase ^= 1u;
+            }
+          }
+          if (++s == a.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+        umma_commit(smem_u32(&bar_acc_full));   // also on the way out, so that the epilogue is released
+        acc_phase ^= 1u;
+      }
+      if (!ok) {
+        atomicOr(a.status, ST_MMA_TIMEOUT);
+        s_abort = 1;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- scales and epilogue: this warp's quarter of the tensor memory lanes
+    const int quarter = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    int sf = 0;
+    uint32_t sf_phase = 0, acc_phase = 0, groups = 0;
+    bool ok = true;
+    griddep_wait();   // x's exponents come from the kernel ahead, and out may still be being read
+    auto word = [&](const uint8_t* row, int kb, int kb1) {   // four successive exponents of a row
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (kb + i < kb1) w |= static_cast<uint32_t>(__ldcg(row + kb + i)) << (8 * i);
+      return w;
+    };
+    const bool words = (a.kblocks & 3) == 0 && (reinterpret_cast<uintptr_t>(a.xe) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.we) & 3) == 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      int tok, row, kb0, kb1;
+      const int s = slice(t, tok, row, kb0, kb1);
+      const bool fast = words && (kb0 & 3) == 0;
+      auto fetch = [&](int kb, uint32_t (&wa)[MT][4], uint32_t (&wb)[8]) {
+        auto get = [&](const uint8_t* r) { return fast && kb + 4 <= kb1 ? __ldcg(reinterpret_cast<const uint32_t*>(r + kb)) : word(r, kb, kb1); };
+#pragma unroll
+        for (int h = 0; h < MT; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = (tok * MT + h) * G8_TOK + 32 * c + lane;
+            wa[h][c] = r < a.m ? get(a.xe + static_cast<size_t>(r) * a.kblocks) : 0u;
+          }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int r = row * a.nt + 32 * c + lane;
+          wb[c] = 32 * c < a.nt && r < a.n ? get(a.we + static_cast<size_t>(r >> 7) * a.kblocks) : 0u;
+        }
+      };
+      uint32_t wa[MT][4], wb[8];
+      fetch(kb0, wa, wb);
+      for (int kb = kb0; kb < kb1 && ok; kb += 4) {
+        if (groups >= 2 && !mbar_wait(smem_u32(&bar_sf_empty[sf]), sf_phase ^ 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t at = tmem + lanes + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE;
+#pragma unroll
+        for (int h = 0; h < MT; ++h) tmem_st4(at + 4u * static_cast<uint32_t>(h), wa[h]);
+        tmem_st8(at + 4 * MT, wb);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_sf_full[sf]));
+        ++groups;
+        if (++sf == 2) {
+          sf = 0;
+          sf_phase ^= 1u;
+        }
+        if (kb + 4 < kb1) fetch(kb + 4, wa, wb);
+      }
+      if (ok && !mbar_wait(smem_u32(&bar_acc_full), acc_phase)) ok = false;
+      if (!ok || s_abort) {
+        if (!ok && lane == 0) atomicOr(a.status, ST_EPILOGUE_TIMEOUT);
+        s_abort = 1;
+        break;
+      }
+      acc_phase ^= 1u;
+      tc_fence_after_sync();
+      const bool vec = (a.ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.nt & 7) == 0;
+#pragma unroll 1
+      for (int h = 0; h < MT; ++h) {
+        const int token = (tok * MT + h) * G8_TOK + quarter * 32 + lane;
+#pragma unroll 1
+        for (int c = 0; c < a.nt; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c), v);
+          tmem_ld_wait();
+          const int n0 = row * a.nt + c;
+          if (token >= a.m || n0 >= a.n) continue;
+          if (a.split > 1) {
+            float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
+            if ((a.n & 3) == 0 && n0 + 16 <= a.n) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (n0 + i < a.n) o[i] = __uint_as_float(v[i]);
+            }
+          } else {
+            __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
+            if (vec && n0 + 16 <= a.n) {
+#pragma unroll
+              for (int i = 0; i < 16; i += 8) {
+                uint32_t p[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[i + 2 * q]), __uint_as_float(v[i + 2 * q + 1]));
+                  p[q] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                *reinterpret_cast<uint4*>(o + i) = make_uint4(p[0], p[1], p[2], p[3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (n0 + i < a.n) o[i] = __float2bfloat16_rn(__uint_as_float(v[i]));
+            }
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_acc_empty));
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Adds up the K slices' sums, in slice order.
+__global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ ws, __nv_bfloat16* __restrict__ out, int m, int n, int split, int ld_out) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const long long total = static_cast<long long>(m) * n;
+  const bool vec = (n & 3) == 0 && (ld_out & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  if (vec) {
+    for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < total; i += static_cast<long long>(gridDim.x) * 1024) {
+      float4 v = __ldcg(reinterpret_cast<const float4*>(ws + i));
+      for (int s = 1; s < split; ++s) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(ws + static_cast<size_t>(s) * total + i));
+        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+      }
+      const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y), q = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(out + i / n * ld_out + i % n) = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+    }
+  } else {
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256) {
+      float v = __ldcg(ws + i);
+      for (int s = 1; s < split; ++s) v += __ldcg(ws + static_cast<size_t>(s) * total + i);
+      out[i / n * ld_out + i % n] = __float2bfloat16_rn(v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct G8Plan {
+  int mt, nt, split, stages;
+};
+
+static int g8_sms() {
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return v;
+}
+
+// The tile and the K slices that make the longest CTA's traffic smallest: bytes it brings into shared memory, at
+// about 60 bytes per ns, against its MMAs, plus what a tile and a join cost.
+static G8Plan g8_plan(int m, int n, int k, int sms) {
+  const int kblocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
+  G8Plan best = {};
+  double best_ns = 1e30;
+  for (int mt = 1; mt <= 2; ++mt) {
+    if (mt == 2 && m <= G8_TOK) continue;
+    const int tok_tiles = (m + mt * G8_TOK - 1) / (mt * G8_TOK);
+    const double a_rows = mt == 1 && m < G8_TOK ? (m + 7) / 8 * 8 : mt * G8_TOK;
+    for (int nt = 32; nt <= (mt == 2 ? 224 : 256); nt += 16) {
+      const int row_tiles = (n + nt - 1) / nt;
+      for (int split = 1; split <= 16 && split <= kblocks; ++split) {
+        const long long tiles = static_cast<long long>(tok_tiles) * row_tiles * split;
+        const long long waves = (tiles + sms - 1) / sms;
+        const int kb = (kblocks + split - 1) / split;
+        const double load = kb * (a_rows + nt) * FP8_BLOCK / 60.0, mma = kb * 4.0 * mt * nt / 2.0 / 1.8;
+        double ns = waves * ((load > mma ? load : mma) + 1500.0 + 8.0 * mt * nt / 2) + 3000.0;
+        if (split > 1) ns += 2000.0 + static_cast<double>(m) * n * split * 8 / 5000.0;
+        if (ns < best_ns) {
+          best_ns = ns;
+          best = {mt, nt, split, 0};
+        }
+      }
+    }
+  }
+  const int stage = best.mt * G8_TOK * FP8_BLOCK + best.nt * FP8_BLOCK;
+  best.stages = (225 * 1024 - 1024) / stage;
+  if (best.stages > G8_MAX_STAGES) best.stages = G8_MAX_STAGES;
+  return best;
+}
+
+long long fp8_gemm_ws_bytes(int m, int n, int k) {
+  if (m < 1 || n < 1 || k < 16 || k % 16) return -1;
+  const int sms = g8_sms();
+  if (sms < 1) return -2;
+  const G8Plan p = g8_plan(m, n, k, sms);
+  return p.split > 1 ? static_cast<long long>(p.split) * m * n * 4 : 0;
+}
+
+template <int MT>
+static cudaError_t g8_launch(const CUtensorMap& tx, const CUtensorMap& tw, const G8Args& a, int grid, size_t smem, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  return launch_dependent(fp8_gemm_kernel<MT>, dim3(grid), dim3(G8_THREADS), smem, stream, tx, tw, a);
+}
+
+int encode_2d_u8(CUtensorMap* tm, const void* base, long long rows, long long cols, int box_rows);   // capi.cu
+
+int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int n, int k, int ld_out,
+                      cudaStream_t stream) {
+  if (!W || !we || !xq || !xe || !out || !status || m < 1 || n < 1 || k < 16 || k % 16) return -1;
+  if (ld_out < n || ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
+  const int sms = g8_sms();
+  if (sms < 1) return -4;
+  const G8Plan p = g8_plan(m, n, k, sms);
+  if (p.split > 1 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15))) return -3;
+  G8Args a = {};
+  a.xe = static_cast<const uint8_t*>(xe);
+  a.we = static_cast<const uint8_t*>(we);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ws = static_cast<float*>(ws);
+  a.status = status;
+  a.m = m; a.n = n; a.k = k;
+  a.kblocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
+  a.ld_out = ld_out;
+  a.nt = p.nt;
+  a.a_rows = p.mt == 1 && m < G8_TOK ? (m + 7) / 8 * 8 : G8_TOK;
+  a.tok_tiles = (m + p.mt * G8_TOK - 1) / (p.mt * G8_TOK);
+  a.row_tiles = (n + p.nt - 1) / p.nt;
+  a.split = p.split;
+  a.stages = p.stages;
+  CUtensorMap tx, tw;
+  int r = encode_2d_u8(&tx, xq, m, k, a.a_rows);
+  if (r == 0) r = encode_2d_u8(&tw, W, n, k, p.nt);
+  if (r != 0) return r;
+  const long long tiles = static_cast<long long>(a.row_tiles) * a.tok_tiles * a.split;
+  if (tiles > 0x7fffffffll) return -3;
+  const int grid = static_cast<int>(tiles < sms ? tiles : sms);
+  size_t smem = static_cast<size_t>(p.stages) * (p.mt * G8_TOK + p.nt) * FP8_BLOCK + 1024;
+  if (smem < G8_MIN_SMEM) smem = G8_MIN_SMEM;
+  cudaError_t e = p.mt == 2 ? g8_launch<2>(tx, tw, a, grid, smem, stream) : g8_launch<1>(tx, tw, a, grid, smem, stream);
+  if (e == cudaSuccess && p.split > 1) {
+    const long long quads = (static_cast<long long>(m) * n + 1023) / 1024;
+    e = launch_dependent(fp8_join_kernel, dim3(static_cast<unsigned>(quads < 4ll * sms ? quads : 4ll * sms)), dim3(256), 0, stream, a.ws, a.out, m, n, p.split, ld_out);
+  }
+  return static_cast<int>(e);
+}
+
+}  // namespace muse

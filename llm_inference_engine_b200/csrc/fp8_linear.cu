@@ -3,12 +3,12 @@
 // BF16 out; x comes in BF16 and is quantised here (one exponent per token and 128 columns), W as codes and exponent
 // bytes. The products of codes are exact in FP32 and so is the scaling; the sums are FP32.
 //
-//   fp8_walk_kernel   up to 16 tokens: the persistent walk of fewtok_mma.cu over half the bytes. Tokens are the MMA's
+//   fp8_walk_kernel       up to 16 tokens: the persistent walk of fewtok_mma.cu over half the bytes. Tokens are the MMA's
 //                     M = 16, 8 weight rows its N; a lane loads 16-byte pieces of W straight into the B fragments of
 //                     two m16n8k32 MMAs (the k slots are a permutation that x follows). A warp owns whole 128-column
 //                     blocks, so its x fragments, quantised in registers from BF16 (the four lanes of a token share
 //                     the block: two shuffles give its largest magnitude), and their scales never change.
-//   fp8_tile_kernel   any number of tokens, from x quantised by fp8_quantize_kernel: 64 x 64 tiles in shared memory.
+//   fp8_quantize_kernel   x to codes and exponents, for the many-token kernel (fp8_gemm.cu) and for callers.
 #include "fp8.cuh"
 
 namespace muse {
@@ -162,60 +162,6 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
   }
 }
 
-// ---------------------------------------------------------------- any number of tokens
-constexpr int FT_T = 64, FT_R = 64, FT_LD = FP8_BLOCK + 16;   // tokens, rows, padded bytes of a tile row
-
-__global__ void __launch_bounds__(256) fp8_tile_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ we,
-                                                       const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xe,
-                                                       __nv_bfloat16* __restrict__ out, int m, int N, int K, int kblocks, int ld_out) {
-  __shared__ __align__(16) uint8_t sx[FT_T][FT_LD], sw[FT_R][FT_LD];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int r0 = blockIdx.x * FT_R, t0 = blockIdx.y * FT_T;
-  const int wt = (warp & 3) * 16, wr = (warp >> 2) * 32;   // this warp's 16 tokens and 32 rows of the tile
-  float acc[4][4] = {};
-  for (int kb = 0; kb < kblocks; ++kb) {
-    for (int i = threadIdx.x; i < (FT_T + FT_R) * 8; i += 256) {
-      const int row = i >> 3, k = kb * FP8_BLOCK + (i & 7) * 16;
-      const bool is_x = row < FT_T;
-      const int at = is_x ? t0 + row : r0 + row - FT_T;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (k < K && at < (is_x ? m : N)) v = __ldcg(reinterpret_cast<const uint4*>((is_x ? xq : W) + static_cast<size_t>(at) * K + k));
-      *reinterpret_cast<uint4*>(is_x ? &sx[row][(i & 7) * 16] : &sw[row - FT_T][(i & 7) * 16]) = v;
-    }
-    __syncthreads();
-    float c[4][4] = {};
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      auto word = [&](const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); };
-      const uint32_t a0 = word(&sx[wt + g][32 * s + 4 * t]), a1 = word(&sx[wt + g + 8][32 * s + 4 * t]);
-      const uint32_t a2 = word(&sx[wt + g][32 * s + 16 + 4 * t]), a3 = word(&sx[wt + g + 8][32 * s + 16 + 4 * t]);
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        mma_e4m3_16832(c[n], a0, a1, a2, a3, word(&sw[wr + 8 * n + g][32 * s + 4 * t]), word(&sw[wr + 8 * n + g][32 * s + 16 + 4 * t]));
-    }
-    const float e0 = t0 + wt + g < m ? exp2_byte(__ldcg(xe + static_cast<size_t>(t0 + wt + g) * kblocks + kb)) : 0.f;
-    const float e1 = t0 + wt + g + 8 < m ? exp2_byte(__ldcg(xe + static_cast<size_t>(t0 + wt + g + 8) * kblocks + kb)) : 0.f;
-    const float s = exp2_byte(__ldg(we + static_cast<size_t>(r0 >> 7) * kblocks + kb));
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      acc[n][0] = fmaf(c[n][0], s * e0, acc[n][0]);
-      acc[n][1] = fmaf(c[n][1], s * e0, acc[n][1]);
-      acc[n][2] = fmaf(c[n][2], s * e1, acc[n][2]);
-      acc[n][3] = fmaf(c[n][3], s * e1, acc[n][3]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = t0 + wt + g + 8 * (i >> 1), row = r0 + wr + 8 * n + 2 * t + (i & 1);
-      if (tok < m && row < N) out[static_cast<size_t>(tok) * ld_out + row] = __float2bfloat16_rn(acc[n][i]);
-    }
-}
-
 // ---------------------------------------------------------------- host side
 static int sm_count() {
   int dev = 0, v = 0;
@@ -260,17 +206,6 @@ int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, i
     e = m <= 8 ? fp8_walk_launch<32, 2, 1, false>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
                : fp8_walk_launch<16, 4, 1, true>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream);
   return static_cast<int>(e);
-}
-
-int fp8_tile_dispatch(const void* W, const void* we, const void* xq, const void* xe, void* out, int m, int N, int K, int ld_out, cudaStream_t stream) {
-  if (!W || !we || !xq || !xe || !out || m < 1 || N < 1 || K < 16 || K % 16) return -1;
-  if (ld_out < N || ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
-  const long long ty = (m + FT_T - 1) / FT_T;
-  if (ty > 65535) return -3;
-  return static_cast<int>(launch_dependent(fp8_tile_kernel, dim3((N + FT_R - 1) / FT_R, static_cast<unsigned>(ty)), dim3(256), 0, stream,
-                                           static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(we), static_cast<const uint8_t*>(xq),
-                                           static_cast<const uint8_t*>(xe), static_cast<__nv_bfloat16*>(out), m, N, K,
-                                           (K + FP8_BLOCK - 1) / FP8_BLOCK, ld_out));
 }
 
 }  // namespace muse

@@ -12,13 +12,15 @@ same behind the layer names of prepare().
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _capi
 
 BLOCK = 128
 E_MIN = -64
-WALK_MAX_TOKENS = 16   # csrc/fp8_linear.cu: more tokens take the tiled kernel, fewer and K <= WALK_MAX_K the walk
+WALK_MAX_TOKENS = 16   # csrc/fp8_linear.cu; more tokens or a longer K take csrc/fp8_gemm.cu
 WALK_MAX_K = 8192
 
 
@@ -59,12 +61,26 @@ def dequantize_weight(w8: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor
     return w8.float() * scale.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
+def _rows(x: torch.Tensor, m: int, k: int) -> torch.Tensor:
     """x itself where its rows can be read in 16-byte vectors, else a copy."""
-    m, k = x.shape
     if x.stride(1) != 1 or x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
         return x.contiguous().clone()
     return x
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(index: int, m: int, n: int, k: int) -> int:
+    """Workspace of the many-token kernel's plan for a shape (the plan goes by sizes and the device's SM count)."""
+    size = _capi.load().muse_fp8_gemm_ws_bytes(m, n, k)
+    if size < 0:
+        raise _capi.MuseError(f"muse_fp8_gemm_ws_bytes(m={m}, n={n}, k={k}) -> {size}")
+    return size
+
+
+def check_status(device) -> None:
+    """Synchronise and raise if a kernel since the last check gave up on one of its bounded waits. Not for use inside a
+    stream capture. (One word per device for the 8-bit operators, cache8's among them.)"""
+    _capi.check_status_word(device)
 
 
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -73,19 +89,24 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     if m < 1 or k < 16 or k % 16:
         raise ValueError(f"x must have at least one row and a multiple of 16 columns, got {tuple(x.shape)}")
-    with torch.cuda.device(x.device):
-        x = _rows(x)
-        xq = torch.empty((m, k), device=x.device, dtype=torch.float8_e4m3fn)
-        xe = torch.empty((m, -(-k // BLOCK)), device=x.device, dtype=torch.uint8)
-        _capi.check(_capi.load().muse_fp8_quantize(x.data_ptr(), xq.data_ptr(), xe.data_ptr(), m, k, x.stride(0) if m > 1 else k,
-                                                   torch.cuda.current_stream(x.device).cuda_stream), f"muse_fp8_quantize(m={m}, k={k})")
+    dev = x.device
+    with _capi.on_device(dev.index):
+        return _quantize(_rows(x, m, k), m, k, dev)
+
+
+def _quantize(x, m, k, dev):
+    xq = torch.empty((m, k), device=dev, dtype=torch.float8_e4m3fn)
+    xe = torch.empty((m, -(-k // BLOCK)), device=dev, dtype=torch.uint8)
+    _capi.check(_capi.load().muse_fp8_quantize(x.data_ptr(), xq.data_ptr(), xe.data_ptr(), m, k, x.stride(0) if m > 1 else k,
+                                               _capi.raw_stream(dev.index)), "muse_fp8_quantize")
     return xq, xe
 
 
 def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """x @ W.T in BF16. `x`: BF16 [m, K] (any strides), or the pair that quantize() returns. `w8`, `w_exp`: the codes
     [N, K] and exponent bytes of W, contiguous; K a multiple of 16. `out` (optional): BF16 [m, >= N] with unit column
-    stride, of which the first N columns are written."""
+    stride, of which the first N columns are written. Weights are static: what made them must be complete before the first
+    call (kernels may read them ahead of the work before them in the stream)."""
     pair = isinstance(x, (tuple, list))
     if pair:
         xq, xe = x
@@ -94,34 +115,43 @@ def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = 
         m, k = xq.shape
         if xe.shape != (m, -(-k // BLOCK)) or not xq.is_contiguous() or not xe.is_contiguous() or xq.data_ptr() % 16:
             raise ValueError(f"x's codes {tuple(xq.shape)} and exponents {tuple(xe.shape)} must be contiguous, one exponent per 128 columns")
+        x_dev = xq.device
+        if xe.device != x_dev:
+            raise ValueError("x's codes and exponents must be on the same device")
     else:
         _require(x, "x", torch.bfloat16, 2)
         m, k = x.shape
+        x_dev = x.device
     _require(w8, "w8", torch.float8_e4m3fn, 2)
     _require(w_exp, "w_exp", torch.uint8, 2)
-    n = w8.shape[0]
+    n, kw = w8.shape
     dev = w8.device
-    if w8.shape[1] != k or m < 1 or n < 1 or k < 16 or k % 16:
+    if kw != k or m < 1 or n < 1 or k < 16 or k % 16:
         raise ValueError(f"x [{m}, {k}] and W {tuple(w8.shape)} do not fit, or K is not a multiple of 16")
     if w_exp.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not w8.is_contiguous() or not w_exp.is_contiguous() or w8.data_ptr() % 16:
         raise ValueError(f"w8 {tuple(w8.shape)} and w_exp {tuple(w_exp.shape)} must be contiguous, one exponent per 128 x 128 block")
-    if w_exp.device != dev or (x[0] if pair else x).device != dev:
+    if w_exp.device != dev or x_dev != dev:
         raise ValueError("x, w8 and w_exp must be on the same device")
     if out is not None and (out.device != dev or out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n
                             or out.stride(1) != 1 or (m > 1 and out.stride(0) < n)):
         raise ValueError("out must be BF16 [m, >= N] with unit column stride on W's device")
-    lib = _capi.load()
-    with torch.cuda.device(dev):
+    lib, index = _capi.load(), dev.index
+    with _capi.on_device(index):
         if out is None:
             out = torch.empty((m, n), device=dev, dtype=torch.bfloat16)
-        ld_out = out.stride(0) if m > 1 else n
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if not pair and m <= WALK_MAX_TOKENS and k <= WALK_MAX_K:
-            x = _rows(x)
-            _capi.check(lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k, x.stride(0) if m > 1 else k,
-                                          ld_out, stream), f"muse_fp8_walk(m={m}, n={n}, k={k})")
-            return out
-        xq, xe = x if pair else quantize(x)
-        _capi.check(lib.muse_fp8_tile(w8.data_ptr(), w_exp.data_ptr(), xq.data_ptr(), xe.data_ptr(), out.data_ptr(), m, n, k, ld_out, stream),
-                    f"muse_fp8_tile(m={m}, n={n}, k={k})")
+            ld_out = n
+        else:
+            ld_out = out.stride(0) if m > 1 else n
+        if not pair:
+            x = _rows(x, m, k)
+            if m <= WALK_MAX_TOKENS and k <= WALK_MAX_K:
+                _capi.check(lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k,
+                                              x.stride(0) if m > 1 else k, ld_out, _capi.raw_stream(index)), "muse_fp8_walk")
+                return out
+            xq, xe = _quantize(x, m, k, dev)
+        size = _ws_bytes(index, m, n, k)
+        ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None   # the call's own: calls may overlap on the GPU
+        _capi.check(lib.muse_fp8_gemm(w8.data_ptr(), w_exp.data_ptr(), xq.data_ptr(), xe.data_ptr(), out.data_ptr(),
+                                      ws.data_ptr() if size else None, _capi.status_word(dev).data_ptr(), m, n, k, ld_out,
+                                      _capi.raw_stream(index)), "muse_fp8_gemm")
     return out

@@ -527,3 +527,25 @@ def test_attention_half_of_a_layer_over_a_prompt_and_steps(c8, eight_bit):
         assert bool(((got.double() - want).abs() <= allow).all())
     c8.check_status(DEV)
     proj.check_status(state)
+
+
+def test_first_call_of_a_device_inside_a_capture_is_refused(c8):
+    """The status word is made by the first call and has to outlive every graph."""
+    from llm_inference_engine_b200 import _capi
+
+    cache = filled_cache(c8, 2, 1, 64, 81)
+    q = torch.randn((1, 1, 64), device=DEV).bfloat16()
+    table, lens = i32([[0]]), i32([5])
+    torch.cuda.synchronize(DEV)
+    kept = _capi._STATUS.pop(DEV.index, None)
+    try:
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(_capi.MuseError, match="outside stream capture"):
+            with torch.cuda.graph(g):
+                c8.attention(q, cache, table, lens)
+    finally:
+        if kept is not None:
+            _capi._STATUS[DEV.index] = kept
+    torch.cuda.synchronize(DEV)
+    c8.attention(q, cache, table, lens)
+    c8.check_status(DEV)
