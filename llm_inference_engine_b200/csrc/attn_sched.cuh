@@ -4,9 +4,10 @@
 // A sequence b with n new tokens and `len` tokens in all has group * n query rows per KV head, row r = token * group +
 // head in the group, cut into tiles of `tile` rows. An ENTRY is a (sequence, row tile); its rows see the tokens from
 // `lo` to `hi` (causal, window), that is `pages` pages from `page0`; an entry with rows that see nothing counts one
-// page, so that somebody writes its zeros. A UNIT is an entry's KV head. The units' pages form one list, entry-major
-// then head then page, which is cut into equal ranges, one per worker: a unit split between workers leaves partial
-// sums that a second kernel adds up in page order.
+// page, so that somebody writes its zeros. A UNIT is an entry's KV head. The units form one list, entry-major, then
+// head, of ITEMS: a head item, which stands for what a unit costs beside its pages (bringing in q, storing the
+// rows: about a page's time), and the unit's pages. The list is cut into equal ranges, one per worker; a unit whose pages
+// are split between workers leaves partial sums that a second kernel adds up in page order.
 #pragma once
 
 namespace muse {
@@ -20,6 +21,8 @@ struct AttnEntry {
   int page0, pages;  // pages its rows see; rows > 0 and nothing seen: one page that is masked whole
   int last;          // last position its rows see (-1: none)
 };
+// Items of a unit of the entry.
+__host__ __device__ inline int attn_items(const AttnEntry& e) { return e.pages > 0 ? e.pages + 1 : 0; }
 
 // cu0, cu1: the sequence's bounds in the batch as the caller gave them; len: its tokens, the new ones included.
 __host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m, int max_q, int capacity, int group, int tile, int rt,
@@ -55,8 +58,8 @@ __host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m
   return e;
 }
 
-// `total` pages dealt to `workers` in equal ranges: the first `rem` workers get one page more. With fewer pages than
-// workers only `total` workers take part, with one page each.
+// `total` items dealt to `workers` in equal ranges: the first `rem` workers get one more. With fewer items than workers
+// only `total` workers take part, with one item each.
 struct AttnDeal {
   long long total, base, rem;
   int workers;   // those that take part
@@ -69,16 +72,53 @@ __host__ __device__ inline AttnDeal attn_deal(long long total, int workers) {
   d.rem = total - d.base * d.workers;
   return d;
 }
-// First page of worker w's range (w = workers: the end).
+// First item of worker w's range (w = workers: the end).
 __host__ __device__ inline long long attn_range(const AttnDeal& d, int w) { return d.base * w + (w < d.rem ? w : d.rem); }
-// The worker whose range holds page f.
+// The worker whose range holds item f.
 __host__ __device__ inline int attn_worker(const AttnDeal& d, long long f) {
   const long long big = d.rem * (d.base + 1);
   return static_cast<int>(f < big ? f / (d.base + 1) : d.rem + (f - big) / d.base);
 }
-// Where worker w left its partial sums of the unit whose pages begin at u0 (the caller knows that w has some of them,
-// and not all): a worker has at most two partial segments, the one its range begins in (slot 0) and the one it ends in
-// (slot 1, when that is another).
+// Where worker w left its partial sums of the unit whose first page is item u0 (the caller knows that w has some of its
+// pages, and not all): a worker has at most two partial segments, one of a unit whose first page lies at or before its
+// range (slot 0) and one of a unit that begins inside it (slot 1).
 __host__ __device__ inline int attn_slot_of(const AttnDeal& d, int w, long long u0) { return 2 * w + (attn_range(d, w) >= u0 ? 0 : 1); }
+// Workers that are the warps of a CTA, `per` of them from w on (a multiple of per), add their sums up on chip when
+// nothing but this one unit's pages [u0, u1) is theirs; the sums are then in the first one's slot 0.
+__host__ __device__ inline bool attn_merged(const AttnDeal& d, int w, int per, long long u0, long long u1) {
+  return per > 1 && w + per <= d.workers && attn_range(d, w) >= u0 && attn_range(d, w + per) <= u1;
+}
+// The partial sums of a split unit, in page order: slot(i) for i = 0 .. parts - 1. Workers w0 .. w1 have the unit's
+// pages; whole groups of `per` in between count once.
+struct AttnParts {
+  int w0, w1, per;
+  int head, groups, parts;   // single workers in front, groups behind them; the rest is single again
+  int first_slot;
+};
+__host__ __device__ inline AttnParts attn_parts(const AttnDeal& d, int per, long long u0, int pages) {
+  AttnParts p;
+  p.per = per;
+  p.w0 = attn_worker(d, u0);
+  p.w1 = attn_worker(d, u0 + pages - 1);
+  p.first_slot = attn_slot_of(d, p.w0, u0);
+  const int n = p.w1 - p.w0 + 1;
+  p.head = (per - p.w0 % per) % per;   // to the first group boundary
+  if (p.head == 0 && !attn_merged(d, p.w0, per, u0, u0 + pages)) p.head = per;   // w0's CTA begins ahead of the unit
+  if (p.head > n) p.head = n;
+  p.groups = 0;
+  if (per > 1 && n > p.head) {
+    p.groups = (n - p.head) / per;
+    // the last group may reach beyond the unit
+    if (p.groups > 0 && !attn_merged(d, p.w0 + p.head + (p.groups - 1) * per, per, u0, u0 + pages)) --p.groups;
+  }
+  p.parts = n - p.groups * (per - 1);
+  return p;
+}
+__host__ __device__ inline int attn_part_slot(const AttnParts& p, int i) {
+  if (i == 0 && p.head > 0) return p.first_slot;
+  if (i < p.head) return 2 * (p.w0 + i);
+  const int g = i - p.head;
+  return g < p.groups ? 2 * (p.w0 + p.head + g * p.per) : 2 * (p.w0 + p.head + p.groups * p.per + g - p.groups);
+}
 
 }  // namespace muse

@@ -4,32 +4,34 @@
 // position, the last `window` of them where a window is given; a row that sees none is zero.
 //
 // What bounds it is reading the cache: 2 D bytes per token and KV head, for all query heads that share the head (and a
-// sequence's few new tokens) at once: they are the rows of one 16-row MMA tile. The pages of all sequences and heads
-// form one list that is cut into equal ranges (attn_sched.cuh), one per warp, whatever the sequences' lengths, so
-// that a batch of any shape keeps every SM's loads in flight; a warp brings its pages in with bulk copies (K and V of
-// a page and head are 64 D contiguous bytes each) into a ring of its own and waits for nobody else. More than 16
-// rows (a chunk of a prompt) take 16 rows per warp and one ring and range per CTA.
+// sequence's few new tokens) at once: they are the rows. The pages of all sequences and heads form one list that is
+// cut into equal ranges (attn_sched.cuh), one per warp, whatever the sequences' lengths, so that a batch of any shape
+// keeps every SM's loads in flight; a warp brings its pages in with bulk copies (K and V of a page and head are 64 D
+// contiguous bytes each) into a ring of its own and waits for nobody else. More than 16 rows (a chunk of a prompt) take
+// 16 rows per warp and one ring and range per CTA.
 //
-// Codes become FP16 in registers (exact, as e4m3 is a subset), q becomes FP16 under a power of two per row (exact down
-// to 2^-34 of the row's largest value), the scores take both powers in FP32. A lane's 16 bytes of k are 4 k-slots of 4 MMAs; the
-// order of slots is free as long as q follows it. The n-index of the score MMAs is a token order of our choosing too:
-// lane (g, t) gets tokens 16 t .. 16 t + 15 of the page for row g, which is what the second product wants as its A
-// fragment beside V kept [dim, token], so neither operand passes through shared memory again. The probabilities are
-// rounded to FP16 (2^-11, values below 2^-14 of the running maximum to 2^-25 of it), a page's sum is scaled by its V
-// exponent in FP32.
+// The cache is the MMAs' M operand and the rows their N = 8 (or two such tiles): the work per page then follows the
+// rows there are, and a page's codes are converted once for all of them. Codes become FP16 in registers (exact, as e4m3
+// is a subset), q becomes FP16 under a power of two per row (exact down to 2^-34 of the row's largest value), the scores take
+// both powers in FP32. Scores S^T[token][row]: a lane's 16 bytes of k are 4 k-slots of 4 MMAs; the order of slots is free as
+// long as q follows it. O^T[dim][row] += V^T[dim][token] P^T[token][row]: V is kept [dim, token], so a lane's 16 bytes are
+// tokens 16 t .. 16 t + 15 of a dimension, and the token order of the score tiles is chosen so that, after one 8 x 8
+// transpose in registers (movmatrix), the lane holds the same tokens' weights. Neither operand passes through
+// shared memory a second time. The weights are rounded to FP16 (2^-11, values below 2^-14 of the running maximum to 2^-25
+// of it), a page's sum is scaled by its V exponent in FP32.
 #include "attn_sched.cuh"
 #include "cache8.cuh"
 #include "fp8.cuh"
 
 namespace muse {
 
-constexpr int ATTN_TILE = 16;   // rows of one warp's MMA tile
 constexpr int ATTN_WARPS = 8;
 constexpr int ATTN_THREADS = ATTN_WARPS * 32;
 
 __host__ __device__ constexpr int attn_slots(int D) { return D == 128 ? 3 : 6; }              // ring slots per warp
 __host__ __device__ constexpr int attn_ring_bytes(int D) { return ATTN_WARPS * attn_slots(D) * ATTN_PAGE * D; }
-// Floats of one partial slot of a tile of `rows` rows: (max, sum) per row, then the rows.
+// Floats of one partial slot of `rows` rows: max and sum per row, then the accumulators as the lanes hold them,
+// [8 rows][D / 16][lane] float4.
 __host__ __device__ constexpr int attn_slot_floats(int D, int rows) { return rows * (D + 2); }
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -54,50 +56,93 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return r;
 }
 
+// Lists of up to so many items are spread over the SMs (a warp each) instead of filling CTA after CTA.
+__host__ __device__ constexpr int attn_spread_below(int sms) { return 2 * sms; }
+
+// 8 x 8 16-bit matrix, a row per quad of lanes: transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
 __device__ __forceinline__ AttnEntry attn_entry_of(const AttnArgs& a, int e, int group, int tile) {
   const int b = e / a.tiles, rt = e % a.tiles;
   const int c0 = a.cu_q ? __ldcg(a.cu_q + b) : b, c1 = a.cu_q ? __ldcg(a.cu_q + b + 1) : b + 1;
   return attn_entry(c0, c1, __ldcg(a.seq_lens + b), a.m, a.max_q, a.width * ATTN_PAGE, group, tile, rt, a.window);
 }
 
-// A place in the list of pages: entry, head, i-th page of the unit.
+// Entries as a warp walks them: 32 at a time, one per lane, so that a walk over short sequences pays one round trip
+// per 32 of them.
+struct EntryCache {
+  int base, c0, c1, len;
+};
+__device__ __forceinline__ AttnEntry attn_entry_cached(const AttnArgs& a, EntryCache& c, int e, int entries, int group, int tile) {
+  if (e < c.base || e >= c.base + 32) {   // warp-uniform
+    c.base = e;
+    const int b = min(e + static_cast<int>(threadIdx.x & 31), entries - 1) / a.tiles;
+    c.c0 = a.cu_q ? __ldcg(a.cu_q + b) : b;
+    c.c1 = a.cu_q ? __ldcg(a.cu_q + b + 1) : b + 1;
+    c.len = __ldcg(a.seq_lens + b);
+  }
+  const int l = e - c.base;
+  return attn_entry(__shfl_sync(0xffffffffu, c.c0, l), __shfl_sync(0xffffffffu, c.c1, l), __shfl_sync(0xffffffffu, c.len, l), a.m, a.max_q,
+                    a.width * ATTN_PAGE, group, tile, e % a.tiles, a.window);
+}
+
+// A place in the list: entry, head, i-th page of the unit (-1: the unit's head item).
 struct Cursor {
   AttnEntry en;
   int e, h, i;
 };
 
-// The rows' state of one 16-row tile in a warp: lane (g, t) holds rows g and g + 8.
-template <int D>
+// The state of a warp's 8 NT rows. Lane (g, t) holds rows 8 n + 2 t and + 1 of dimensions 16 d + g and + 8.
+template <int D, int NT>
 struct TileState {
-  float o[D / 8][4];
-  float mx[2], l[2];   // running maximum (log2 units) and the lane's share of the running sum
+  float o[D / 16][NT][4];
+  float mx[NT][2], l[NT][2];   // running maximum (log2 units) and the lane's share of the running sum
 };
 
-template <int D>
-__device__ __forceinline__ void tile_reset(TileState<D>& s) {
+template <int D, int NT>
+__device__ __forceinline__ void tile_reset(TileState<D, NT>& s) {
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n) s.o[n][0] = s.o[n][1] = s.o[n][2] = s.o[n][3] = 0.f;
-  s.mx[0] = s.mx[1] = -INFINITY;
-  s.l[0] = s.l[1] = 0.f;
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) s.o[d][n][0] = s.o[d][n][1] = s.o[d][n][2] = s.o[d][n][3] = 0.f;
+    s.mx[n][0] = s.mx[n][1] = -INFINITY;
+    s.l[n][0] = s.l[n][1] = 0.f;
+  }
 }
 
-// q fragments of 16 rows (row0 .. of the unit's rows) as FP16 under a power of two per row; qs = the row's factor for
-// the scores in log2 units.
-template <int D>
-__device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, int h, int row0, int rows, int group, uint32_t (&qf)[D / 16][4], float (&qs)[2]) {
+// What a warp knows of its rows: positions of the lane's rows, of the first and of the last row.
+template <int NT>
+struct RowInfo {
+  int pos[NT][2];
+  bool there[NT][2];
+  int first, last;
+};
+
+// q fragments of 8 NT rows (from row0 of the unit's rows) as FP16 under a power of two per row; qs = the factor of the
+// lane's rows 2 t, 2 t + 1 for the scores in log2 units.
+template <int D, int NT>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, int h, int row0, int rows, int group, uint32_t (&qf)[NT][D / 16][2],
+                                       float (&qs)[NT][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint4 w[NT][D / 32];   // 16 dimensions (two vectors) per 64
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = g + 8 * half;
-    uint4 w[D / 32];   // 16 dimensions (two vectors) per 64
+  for (int n = 0; n < NT; ++n) {
+    const int r = g + 8 * n, tok = (row0 + r) / group, hd = (row0 + r) - tok * group;
+    const __nv_bfloat16* src = a.q + static_cast<size_t>(en.first + tok) * a.ld_q + static_cast<size_t>(h * group + hd) * D;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+      w[n][c] = r < rows ? __ldcg(reinterpret_cast<const uint4*>(src + 64 * (c >> 1) + 16 * t + 8 * (c & 1))) : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     float amax = 0.f;
-    const bool live = r < rows;
-    const int rr = row0 + r;
-    const __nv_bfloat16* src = a.q + static_cast<size_t>(en.first + (live ? rr / group : 0)) * a.ld_q + static_cast<size_t>(h * group + (live ? rr % group : 0)) * D;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      w[c] = live ? __ldcg(reinterpret_cast<const uint4*>(src + 64 * (c >> 1) + 16 * t + 8 * (c & 1))) : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+      const uint32_t u[4] = {w[n][c].x, w[n][c].y, w[n][c].z, w[n][c].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(bf16lo_f32(u[i])), finite_abs(bf16hi_f32(u[i]))));
     }
@@ -105,38 +150,40 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, i
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     // largest value to [2^9, 2^10): FP16's smallest step, 2^-24, is then 2^-34 of it
     const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 9, 100), -100);
-    const float down = exp2_byte(127 - e);
-    qs[half] = a.scale_log2 * exp2_byte(127 + e);
+    const float down = exp2_byte(127 - e), up = a.scale_log2 * exp2_byte(127 + e);
+    qs[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+    qs[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+      const uint32_t u[4] = {w[n][c].x, w[n][c].y, w[n][c].z, w[n][c].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // word i of vector c holds dimensions 8 (c & 1) + 2 i, + 1 of the lane's 16: MMA 4 (c >> 1) + 2 (c & 1) + (i >> 1)
-        const uint32_t hv = pack_half2(bf16lo_f32(u[i]) * down, bf16hi_f32(u[i]) * down);
-        qf[4 * (c >> 1) + 2 * (c & 1) + (i >> 1)][2 * (i & 1) + half] = hv;
-      }
+      for (int i = 0; i < 4; ++i)   // word i holds dimensions 8 (c & 1) + 2 i, + 1 of the lane's 16: k-step 4 (c >> 1) + 2 (c & 1) + (i >> 1)
+        qf[n][4 * (c >> 1) + 2 * (c & 1) + (i >> 1)][i & 1] = pack_half2(bf16lo_f32(u[i]) * down, bf16hi_f32(u[i]) * down);
     }
   }
 }
 
-// One page: scores, softmax step, P V. `ks`, `vs`: shared-memory addresses of the page's k [64][D] and v [D][64].
-// lim / low: last and first position each of the lane's rows sees, relative to the page's first token.
-template <int D>
-__device__ __forceinline__ void page_scores(float (&s)[8][4], const uint32_t (&qf)[D / 16][4], uint32_t ks) {
+// Raw scores of a page: s[i][n] holds tokens 16 (g >> 1) + 4 i + (g & 1) (values 0, 1: rows 2 t, 2 t + 1) and the token two
+// further (values 2, 3). ks: the page's k [64][D] in shared memory.
+template <int D, int NT>
+__device__ __forceinline__ void page_scores(float (&s)[4][NT][4], const uint32_t (&qf)[NT][D / 16][2], uint32_t ks) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t base = ks + static_cast<uint32_t>(16 * (g >> 1) + (g & 1)) * D + 16 * t;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-    const uint32_t row = ks + static_cast<uint32_t>(16 * (g >> 1) + 2 * j + (g & 1)) * D + 16 * t;
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-      const uint4 w = lds16(row + 64 * c);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      const uint4 x = lds16(base + static_cast<uint32_t>(4 * i) * D + 64 * c), y = lds16(base + static_cast<uint32_t>(4 * i + 2) * D + 64 * c);
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mma_f16_16816(s[j], qf[4 * c + i][0], qf[4 * c + i][1], qf[4 * c + i][2], qf[4 * c + i][3], fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu)),
-                      fp8_to_half2(static_cast<uint16_t>(u[i] >> 16)));
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t a0 = fp8_to_half2(static_cast<uint16_t>(u[k] & 0xffffu)), a2 = fp8_to_half2(static_cast<uint16_t>(u[k] >> 16));
+        const uint32_t a1 = fp8_to_half2(static_cast<uint16_t>(v[k] & 0xffffu)), a3 = fp8_to_half2(static_cast<uint16_t>(v[k] >> 16));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(s[i][n], a0, a1, a2, a3, qf[n][4 * c + k][0], qf[n][4 * c + k][1]);
+      }
     }
   }
 }
@@ -150,194 +197,292 @@ __device__ __forceinline__ uint32_t keep_tokens(uint32_t w, int tok, int lo, int
 }
 __device__ __forceinline__ bool has_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
 
-// o = o * alpha + vscale * P V. Tokens outside [lo, hi] of the page have P = 0, but their codes may stand for NaN.
-template <int D, bool EDGE>
-__device__ __forceinline__ void page_pv(TileState<D>& st, const uint32_t (&p)[4][4], uint32_t vs, float a0, float a1, float vscale, int lo, int hi) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// Scores to weights: p[i][n] = the weights of the lane's two tokens of tile i, packed over rows (2 t, 2 t + 1), before the
+// transpose; `a`: what the rows' sums so far are to be scaled by (`moved`: not all of the warp's are 1).
+template <int D, int NT>
+__device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4][NT][4], uint32_t (&p)[4][NT][2], float (&a)[NT][2], bool& moved,
+                                             const float (&qs)[NT][2], float kscale, const RowInfo<NT>& ri, int p0, int window, bool edge) {
+  const int lane = threadIdx.x & 31, g = lane >> 2;
+  bool same = true;
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n) {
-    const uint4 w = lds16(vs + static_cast<uint32_t>(8 * n + g) * ATTN_PAGE + 16 * t);
-    uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NT; ++n) {
+    const float f[2] = {qs[n][0] * kscale, qs[n][1] * kscale};
+    if (edge) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (EDGE) u[i] = keep_tokens(u[i], 16 * t + 4 * i, lo, hi);
-      mma_f16_16816(c, p[i][0], p[i][1], p[i][2], p[i][3], fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu)), fp8_to_half2(static_cast<uint16_t>(u[i] >> 16)));
+      for (int c = 0; c < 2; ++c) {
+        const int lim = ri.there[n][c] ? ri.pos[n][c] - p0 : -1, low = window > 0 ? ri.pos[n][c] - window + 1 - p0 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int tok = 16 * (g >> 1) + (g & 1) + 4 * i + 2 * x;
+            if (tok < low || tok > lim) s[i][n][2 * x + c] = -INFINITY;
+          }
+      }
     }
-    st.o[n][0] = fmaf(c[0], vscale, st.o[n][0] * a0);
-    st.o[n][1] = fmaf(c[1], vscale, st.o[n][1] * a0);
-    st.o[n][2] = fmaf(c[2], vscale, st.o[n][2] * a1);
-    st.o[n][3] = fmaf(c[3], vscale, st.o[n][3] * a1);
-  }
-}
-
-// lim[2], low[2]: first and last token of the page that rows g and g + 8 see; any_lo, any_hi: of any row of the tile,
-// all_lo, all_hi: of all of them. `s`: the page's raw scores; they become the weights `p`, and (a0, a1) what the rows' sums so
-// far are to be scaled by. Returns whether some row does not see some token.
-template <int D>
-__device__ __forceinline__ bool page_softmax(TileState<D>& st, float (&s)[8][4], uint32_t (&p)[4][4], float& a0, float& a1, const float (&qs)[2], float kscale,
-                                             const int (&low)[2], const int (&lim)[2], int all_lo, int all_hi) {
-  const int t = threadIdx.x & 3;
-  const float f0 = qs[0] * kscale, f1 = qs[1] * kscale;
-  const bool edge = all_lo > 0 || all_hi < ATTN_PAGE - 1;   // warp-uniform
-  float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      s[j][c] *= f0;
-      s[j][2 + c] *= f1;
-      if (edge) {
-        const int tok = 16 * t + 2 * j + c;
-        if (tok < low[0] || tok > lim[0]) s[j][c] = -INFINITY;
-        if (tok < low[1] || tok > lim[1]) s[j][2 + c] = -INFINITY;
-      }
-      m0 = fmaxf(m0, s[j][c]);
-      m1 = fmaxf(m1, s[j][2 + c]);
+      float m = s[0][n][c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(s[i][n][c], s[i][n][2 + c]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      m = fmaxf(m * f[c], st.mx[n][c]);                  // the factor is positive
+      const float b = m == -INFINITY ? 0.f : m;          // nothing seen yet: every weight is 2^-inf = 0
+      a[n][c] = exp2_fast(st.mx[n][c] - b);
+      same &= st.mx[n][c] == m;
+      st.mx[n][c] = m;
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float e = exp2_fast(fmaf(s[i][n][2 * x + c], f[c], -b));
+          s[i][n][2 * x + c] = e;
+          l += e;
+        }
+      st.l[n][c] = fmaf(st.l[n][c], a[n][c], l);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i][n][0] = pack_half2(s[i][n][0], s[i][n][1]);
+      p[i][n][1] = pack_half2(s[i][n][2], s[i][n][3]);
     }
   }
-  m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-  m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-  m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-  m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-  m0 = fmaxf(m0, st.mx[0]);
-  m1 = fmaxf(m1, st.mx[1]);
-  const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;   // nothing seen yet: every weight is 2^-inf = 0
-  a0 = exp2_fast(st.mx[0] - b0);
-  a1 = exp2_fast(st.mx[1] - b1);
-  st.mx[0] = m0;
-  st.mx[1] = m1;
-  float l0 = 0.f, l1 = 0.f;
+  moved = !__all_sync(0xffffffffu, same);
+}
+
+// o = o * a + vscale * V^T P^T; vs: the page's v [D][64] in shared memory. EDGE: tokens outside [lo, hi] have weight 0, but
+// their codes may stand for NaN.
+template <int D, int NT, bool EDGE>
+__device__ __forceinline__ void page_pv(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
+                                        int lo, int hi) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t b[4][NT][2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float e0 = exp2_fast(s[j][0] - b0), e1 = exp2_fast(s[j][1] - b0), e2 = exp2_fast(s[j][2] - b1), e3 = exp2_fast(s[j][3] - b1);
-    l0 += e0 + e1;
-    l1 += e2 + e3;
-    p[j >> 1][2 * (j & 1)] = pack_half2(e0, e1);
-    p[j >> 1][2 * (j & 1) + 1] = pack_half2(e2, e3);
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      b[i][n][0] = transpose_8x8(p[i][n][0]);
+      b[i][n][1] = transpose_8x8(p[i][n][1]);
+    }
+  if (moved) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        st.o[d][n][0] *= a[n][0];
+        st.o[d][n][1] *= a[n][1];
+        st.o[d][n][2] *= a[n][0];
+        st.o[d][n][3] *= a[n][1];
+      }
   }
-  st.l[0] = st.l[0] * a0 + l0;
-  st.l[1] = st.l[1] * a1 + l1;
-  return edge;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    const uint4 x = lds16(vs + static_cast<uint32_t>(16 * d + g) * ATTN_PAGE + 16 * t), y = lds16(vs + static_cast<uint32_t>(16 * d + 8 + g) * ATTN_PAGE + 16 * t);
+    uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+    float c[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (EDGE) {
+        u[i] = keep_tokens(u[i], 16 * t + 4 * i, lo, hi);
+        v[i] = keep_tokens(v[i], 16 * t + 4 * i, lo, hi);
+      }
+      const uint32_t a0 = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu)), a2 = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
+      const uint32_t a1 = fp8_to_half2(static_cast<uint16_t>(v[i] & 0xffffu)), a3 = fp8_to_half2(static_cast<uint16_t>(v[i] >> 16));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16_16816(c[n], a0, a1, a2, a3, b[i][n][0], b[i][n][1]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) st.o[d][n][k] = fmaf(c[n][k], vscale, st.o[d][n][k]);
+  }
 }
 
 // A page that some row does not see all of. Tokens that no row sees (behind the sequence, or left of the window) may hold
 // anything: their codes count as zero. A token that only some rows see and that holds NaN must not reach the others
 // through 0 * NaN: such a page is multiplied once per distinct bound (rare: looked for in the codes).
-template <int D>
-__device__ __forceinline__ void page_pv_edge(TileState<D>& st, const uint32_t (&p)[4][4], uint32_t vs, float a0, float a1, float vscale, const int (&low)[2],
-                                          const int (&lim)[2], int any_lo, int any_hi) {
+template <int D, int NT>
+__device__ __forceinline__ void page_pv_edge(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
+                                             const RowInfo<NT>& ri, int p0, int window) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int lo = window > 0 ? ri.first - window + 1 - p0 : 0, hi = ri.last - p0;   // what any row sees
   bool nan = false;
 #pragma unroll 4
   for (int n = 0; n < D / 8; ++n) {
     const uint4 w = lds16(vs + static_cast<uint32_t>(8 * n + g) * ATTN_PAGE + 16 * t);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) nan |= has_nan_code(keep_tokens(u[i], 16 * t + 4 * i, any_lo, any_hi));
+    for (int i = 0; i < 4; ++i) nan |= has_nan_code(keep_tokens(u[i], 16 * t + 4 * i, lo, hi));
   }
   if (!__any_sync(0xffffffffu, nan)) {
-    page_pv<D, true>(st, p, vs, a0, a1, vscale, any_lo, any_hi);
+    page_pv<D, NT, true>(st, p, vs, a, moved, vscale, lo, hi);
     return;
   }
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n) {
-    st.o[n][0] *= a0;
-    st.o[n][1] *= a0;
-    st.o[n][2] *= a1;
-    st.o[n][3] *= a1;
-  }
 #pragma unroll 1
-  for (int r = 0; r < ATTN_TILE; ++r) {
-    const int rl = __shfl_sync(0xffffffffu, r < 8 ? low[0] : low[1], (r & 7) * 4), rh = __shfl_sync(0xffffffffu, r < 8 ? lim[0] : lim[1], (r & 7) * 4);
-    bool seen_before = false;
-    for (int x = 0; x < r; ++x) {
-      const int xl = __shfl_sync(0xffffffffu, x < 8 ? low[0] : low[1], (x & 7) * 4), xh = __shfl_sync(0xffffffffu, x < 8 ? lim[0] : lim[1], (x & 7) * 4);
-      seen_before |= xl == rl && xh == rh;
-    }
-    if (seen_before || rl > rh) continue;   // warp-uniform
-    const bool u0 = low[0] == rl && lim[0] == rh, u1 = low[1] == rl && lim[1] == rh;
-    uint32_t pr[4][4];
+  for (int pos = ri.first; pos <= ri.last; ++pos) {   // rows at one position see the same tokens
+    uint32_t pr[4][NT][2];
+    float ar[NT][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pr[i][0] = u0 ? p[i][0] : 0u;
-      pr[i][1] = u1 ? p[i][1] : 0u;
-      pr[i][2] = u0 ? p[i][2] : 0u;
-      pr[i][3] = u1 ? p[i][3] : 0u;
-    }
-    TileState<D> one;
-    tile_reset(one);
-    page_pv<D, true>(one, pr, vs, 0.f, 0.f, vscale, max(rl, 0), min(rh, ATTN_PAGE - 1));
+    for (int n = 0; n < NT; ++n) {
+      const uint32_t keep = (ri.there[n][0] && ri.pos[n][0] == pos ? 0xffffu : 0u) | (ri.there[n][1] && ri.pos[n][1] == pos ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      if (u0) { st.o[n][0] += one.o[n][0]; st.o[n][1] += one.o[n][1]; }
-      if (u1) { st.o[n][2] += one.o[n][2]; st.o[n][3] += one.o[n][3]; }
+      for (int i = 0; i < 4; ++i) {
+        pr[i][n][0] = p[i][n][0] & keep;
+        pr[i][n][1] = p[i][n][1] & keep;
+      }
+      ar[n][0] = pos == ri.first ? a[n][0] : 1.f;
+      ar[n][1] = pos == ri.first ? a[n][1] : 1.f;
     }
+    // the other rows' weights are 0 here: NaN codes must not meet them either, so their sums are put back
+    const TileState<D, NT> was = st;
+    page_pv<D, NT, true>(st, pr, vs, ar, true, vscale, window > 0 ? pos - window + 1 - p0 : 0, pos - p0);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (!ri.there[n][k & 1] || ri.pos[n][k & 1] != pos) st.o[d][n][k] = was.o[d][n][k] * ar[n][k & 1];
   }
 }
 
 __device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + __expf(-x)); }
 
-// A finished segment of a unit: the output rows themselves when the segment is the whole unit, else a partial slot.
-template <int D>
-__device__ __forceinline__ void tile_store(TileState<D>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, int rows, int group, bool whole, float* slot,
-                                           int slot_rows, int slot_row0) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// Output values of accumulator quads o[d] (rows row, row + 1 of the entry's tile, dimensions 16 d + g and + 8 of a head).
+template <int N>
+__device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& en, int h, int group, int row, int d0, const float (&o)[N][4], const float (&inv)[2],
+                                            int D) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float l = st.l[half];
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const int r = g + 8 * half;
-    if (r >= rows) continue;
-    if (whole) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;   // no token seen: the row is zero
-      const int rr = row0 + r;
-      const size_t tok = en.first + rr / group;
-      const int col = (h * group + rr % group) * D;
-      __nv_bfloat16* o = a.out + tok * a.ld_out + col;
-      const __nv_bfloat16* gt = a.gate ? a.gate + tok * a.ld_gate + col : nullptr;
+  for (int c = 0; c < 2; ++c) {
+    if (row + c >= en.rows) continue;
+    const int rr = en.row0 + row + c, tk = rr / group;
+    const size_t tok = en.first + tk;
+    const int col = (h * group + rr - tk * group) * D + d0;
+    __nv_bfloat16* dst = a.out + tok * a.ld_out + col;
+    unsigned short gt[N][2];
+    if (a.gate) {   // all in flight before the first is used
+      const unsigned short* g = reinterpret_cast<const unsigned short*>(a.gate + tok * a.ld_gate + col);
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        float x = st.o[n][2 * half] * inv, y = st.o[n][2 * half + 1] * inv;
-        if (gt) {
-          const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(gt + 8 * n + 2 * t));
-          x *= sigmoid_f32(bf16lo_f32(w));
-          y *= sigmoid_f32(bf16hi_f32(w));
-        }
-        *reinterpret_cast<__nv_bfloat162*>(o + 8 * n + 2 * t) = __floats2bfloat162_rn(x, y);
+      for (int d = 0; d < N; ++d) {
+        gt[d][0] = __ldcg(g + 16 * d);
+        gt[d][1] = __ldcg(g + 16 * d + 8);
       }
-    } else {
-      if (t == 0) {
-        slot[slot_row0 + r] = st.mx[half];
-        slot[slot_rows + slot_row0 + r] = l;
-      }
-      float* o = slot + 2 * slot_rows + static_cast<size_t>(slot_row0 + r) * D;
+    }
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(o + 8 * n + 2 * t) = make_float2(st.o[n][2 * half], st.o[n][2 * half + 1]);
+    for (int d = 0; d < N; ++d) {
+      float x = o[d][c] * inv[c], y = o[d][2 + c] * inv[c];
+      if (a.gate) {
+        x *= sigmoid_f32(bf16lo_f32(gt[d][0]));
+        y *= sigmoid_f32(bf16lo_f32(gt[d][1]));
+      }
+      dst[16 * d] = __float2bfloat16_rn(x);
+      dst[16 * d + 8] = __float2bfloat16_rn(y);
     }
   }
 }
 
-// SHARED: the CTA is one worker of 128 rows, all warps on the same pages; else every warp is a worker of 16 rows.
-template <int D, bool SHARED>
+// A finished segment of a unit: the output rows themselves when it is the whole unit, else a partial slot. row0: the
+// warp's first row in the entry's tile of `rows` rows.
+template <int D, int NT>
+__device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, int group, bool whole, float* slot,
+                                           int slot_rows) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float l[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[c] = st.l[n][c];
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
+    }
+    const int row = row0 + 8 * n + 2 * t;
+    if (row0 + 8 * n >= en.rows) continue;   // warp-uniform
+    if (whole) {
+      const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};   // no token seen: the row is zero
+      float o[D / 16][4];
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[d][k] = st.o[d][n][k];
+      store_quads<D / 16>(a, en, h, group, row, g, o, inv, D);
+    } else {
+      if (g == 0) {
+        *reinterpret_cast<float2*>(slot + row) = make_float2(st.mx[n][0], st.mx[n][1]);
+        *reinterpret_cast<float2*>(slot + slot_rows + row) = make_float2(l[0], l[1]);
+      }
+      float4* o = reinterpret_cast<float4*>(slot + 2 * slot_rows) + static_cast<size_t>(row0 / 8 + n) * (D / 16) * 32 + lane;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[d * 32] = make_float4(st.o[d][n][0], st.o[d][n][1], st.o[d][n][2], st.o[d][n][3]);
+    }
+  }
+}
+
+// Adds up the slots of a CTA's warps (`stride` floats apart in shared memory) into one: a warp per 16 dimensions (D = 64:
+// half the warps) and 8 rows at a time, lanes as the accumulators lie.
+template <int D, int NT>
+__device__ __forceinline__ void merge_slots(const float* slots, int stride, float* out) {
+  constexpr int TILE = 8 * NT;
+  const int d = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (d >= D / 16) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = 8 * n + 2 * t;
+    float2 mx = make_float2(-INFINITY, -INFINITY), m[ATTN_WARPS];
+#pragma unroll
+    for (int w = 0; w < ATTN_WARPS; ++w) {
+      m[w] = *reinterpret_cast<const float2*>(slots + static_cast<size_t>(w) * stride + row);
+      mx.x = fmaxf(mx.x, m[w].x);
+      mx.y = fmaxf(mx.y, m[w].y);
+    }
+    const float b0 = mx.x == -INFINITY ? 0.f : mx.x, b1 = mx.y == -INFINITY ? 0.f : mx.y;
+    float2 l = make_float2(0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < ATTN_WARPS; ++w) {
+      const float* s = slots + static_cast<size_t>(w) * stride;
+      const float2 k = *reinterpret_cast<const float2*>(s + TILE + row);
+      const float4 x = reinterpret_cast<const float4*>(s + 2 * TILE)[(n * (D / 16) + d) * 32 + lane];
+      const float f0 = exp2_fast(m[w].x - b0), f1 = exp2_fast(m[w].y - b1);
+      l.x = fmaf(k.x, f0, l.x);
+      l.y = fmaf(k.y, f1, l.y);
+      o.x = fmaf(x.x, f0, o.x);
+      o.y = fmaf(x.y, f1, o.y);
+      o.z = fmaf(x.z, f0, o.z);
+      o.w = fmaf(x.w, f1, o.w);
+    }
+    if (d == 0 && g == 0) {
+      *reinterpret_cast<float2*>(out + row) = mx;
+      *reinterpret_cast<float2*>(out + TILE + row) = l;
+    }
+    reinterpret_cast<float4*>(out + 2 * TILE)[(n * (D / 16) + d) * 32 + lane] = o;
+  }
+}
+
+// SHARED: the CTA is one worker, all its warps on the same pages, 8 NT rows each; else every warp is a worker of 8 NT rows.
+template <int D, int NT, bool SHARED>
 __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int TILE = SHARED ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
+  constexpr int WARP_ROWS = 8 * NT, TILE = SHARED ? WARP_ROWS * ATTN_WARPS : WARP_ROWS;
   constexpr int SLOTS = SHARED ? attn_slots(D) * ATTN_WARPS : attn_slots(D);   // ring slots of one worker
   constexpr uint32_t SLOT_BYTES = ATTN_PAGE * D;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bar_full[attn_slots(D) * ATTN_WARPS], bar_empty[attn_slots(D) * ATTN_WARPS];
-  __shared__ long long s_sum[ATTN_WARPS + 1];
+  __shared__ long long s_sum[ATTN_WARPS];
   __shared__ int s_entry[ATTN_WARPS];
   __shared__ long long s_start[ATTN_WARPS];
   __shared__ int2 s_rec[ATTN_WARPS][64];   // looked-up pages: tile index in the pool, exponents (k | v << 8)
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.hq / a.hk, entries = a.batch * a.tiles;
-  const int ring = SHARED ? 0 : warp;   // this warp's ring
   uint64_t* const full = bar_full + (SHARED ? 0 : warp * attn_slots(D));
   uint64_t* const empty = bar_empty + (SHARED ? 0 : warp * attn_slots(D));
-  const uint32_t ring_base = smem_u32(smem) + static_cast<uint32_t>(ring) * attn_slots(D) * SLOT_BYTES;
+  const uint32_t ring_base = smem_u32(smem) + static_cast<uint32_t>(SHARED ? 0 : warp) * attn_slots(D) * SLOT_BYTES;
   if (tid < attn_slots(D) * ATTN_WARPS) {
     mbar_init(smem_u32(&bar_full[tid]), 1);
     mbar_init(smem_u32(&bar_empty[tid]), ATTN_WARPS);   // used by the shared ring only
@@ -347,17 +492,16 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   griddep_launch_dependents();
   griddep_wait();
 
-  // The list of pages: every thread adds up the entries of its share, a scan over the CTA gives the total and where
-  // each share begins; the thread whose share holds a worker's first page finds the entry.
+  // The list: every thread adds up the items of its share of the entries, a scan over the CTA gives the total and where
+  // each share begins; the thread whose share holds a worker's first item finds the entry.
   const int per = (entries + ATTN_THREADS - 1) / ATTN_THREADS;
   const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
   long long mine = 0;
+  auto items_of = [&](int e) { return static_cast<long long>(attn_items(attn_entry_of(a, e, group, TILE))) * a.hk; };
   for (int e = e0; e < e1; ++e) {
-    const AttnEntry en = attn_entry_of(a, e, group, TILE);
-    mine += static_cast<long long>(en.pages) * a.hk;
+    mine += items_of(e);
     if (blockIdx.x == 0) {
-      const int b = e / a.tiles;
-      const int len = __ldcg(a.seq_lens + b);
+      const int b = e / a.tiles, len = __ldcg(a.seq_lens + b);
       bool bad = len < 0 || len > a.width * ATTN_PAGE;
       if (a.cu_q) {
         const int c0 = __ldcg(a.cu_q + b), c1 = __ldcg(a.cu_q + b + 1);
@@ -381,67 +525,79 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   }
   const long long begin = base + incl - mine, end = base + incl;   // this thread's share of the list
   const AttnDeal deal = attn_deal(total, static_cast<int>(SHARED ? gridDim.x : gridDim.x * ATTN_WARPS));
-  // Neighbouring workers sit on different SMs, so that a list with fewer pages than warps is spread over all of them.
-  auto worker_of = [&](int w) { return static_cast<int>(SHARED ? blockIdx.x : w * gridDim.x + blockIdx.x); };
+  // Neighbouring workers are a CTA's warps, so that sums of a long unit meet on chip; a list with few items is spread over
+  // the SMs instead.
+  const bool spread = !SHARED && total <= attn_spread_below(static_cast<int>(gridDim.x));
+  auto worker_of = [&](int w) { return static_cast<int>(SHARED ? blockIdx.x : spread ? w * gridDim.x + blockIdx.x : blockIdx.x * ATTN_WARPS + w); };
   if (total > 0) {
     for (int w = 0; w < (SHARED ? 1 : ATTN_WARPS); ++w) {
       if (worker_of(w) >= deal.workers) break;
       const long long f = attn_range(deal, worker_of(w));
       if (f >= begin && f < end) {
         long long at = begin;
-        for (int e = e0; e < e1; ++e) {
-          const long long next = at + static_cast<long long>(attn_entry_of(a, e, group, TILE).pages) * a.hk;
-          if (f < next) {
-            s_entry[w] = e;
-            s_start[w] = at;
-            break;
-          }
+        int e = e0;
+        for (; e + 1 < e1; ++e) {
+          const long long next = at + items_of(e);
+          if (f < next) break;
           at = next;
         }
+        s_entry[w] = e;
+        s_start[w] = at;
       }
     }
     if (blockIdx.x == 0) {   // for the kernel that adds up the partial sums
       long long at = begin;
       for (int e = e0; e < e1; ++e) {
         a.prefix[e] = at;
-        at += static_cast<long long>(attn_entry_of(a, e, group, TILE).pages) * a.hk;
+        if (e + 1 < e1) at += items_of(e);
       }
     }
   }
   if (blockIdx.x == 0 && tid == 0) a.prefix[entries] = total;
   __syncthreads();
   const int worker = worker_of(warp);
-  if (worker >= deal.workers) return;   // SHARED: CTA-uniform; else this warp has no page, and nobody waits for it
+  if (worker >= deal.workers) return;   // SHARED: CTA-uniform; else this warp has no item, and no warp waits for it (a merging CTA's have)
   const long long f0 = attn_range(deal, worker);
-  const int count = static_cast<int>(attn_range(deal, worker + 1) - f0);   // this worker's pages
+  const int items = static_cast<int>(attn_range(deal, worker + 1) - f0);
 
+  EntryCache rd_cache, fill_cache;
+  rd_cache.base = fill_cache.base = -64;
   Cursor rd, fill;   // where the warp computes, and up to where it has looked up pages
+  long long unit0;   // first item of the unit that rd stands in
   {
     const int w = SHARED ? 0 : warp;
-    rd.e = s_entry[w];
-    rd.en = attn_entry_of(a, rd.e, group, TILE);
-    const int off = static_cast<int>(f0 - s_start[w]);
-    rd.h = off / rd.en.pages;
-    rd.i = off % rd.en.pages;
-    fill = rd;
+    fill.e = s_entry[w];
+    fill.en = attn_entry_cached(a, fill_cache, fill.e, entries, group, TILE);
+    const int off = static_cast<int>(f0 - s_start[w]), per_unit = attn_items(fill.en);
+    fill.h = off / per_unit;
+    fill.i = off % per_unit - 1;
+    unit0 = s_start[w] + static_cast<long long>(fill.h) * per_unit;
+    rd_cache = fill_cache;
+    rd = fill;
   }
-  auto next_unit = [&](Cursor& c) {   // false behind the last entry
-    c.i = 0;
+  auto next_unit = [&](Cursor& c, EntryCache& ec) {   // false behind the last entry
+    c.i = -1;
     if (++c.h < a.hk) return true;
     c.h = 0;
     do {
       if (++c.e >= entries) return false;
-      c.en = attn_entry_of(a, c.e, group, TILE);
+      c.en = attn_entry_cached(a, ec, c.e, entries, group, TILE);
     } while (c.en.pages == 0);
     return true;
   };
-  // Looks up the next 32 pages of the worker's list, a page per lane: the tile's index in the pool (page * hk + head; -1:
-  // not a page of the pool, or nothing is seen) and its two exponents, into the warp's ring of records.
-  int filled = 0;
+  // Looks up the next pages of the worker's range, up to 32, a page per lane: the tile's index in the pool (page * hk +
+  // head; -1: not a page of the pool, or nothing is seen) and its two exponents, into the warp's ring of records.
+  int filled = 0, fill_left = items;   // pages looked up; items of the range not yet walked
+  int pend_at = 0, pend_tile = -2;     // the lane's page of the last look-up
   auto look_up = [&]() {
     int b = -1, h = 0, i = 0, off = 0;
-    while (off < 32 && filled + off < count) {
-      const int left = fill.en.pages - fill.i, take = min(left, 32 - off);
+    while (off < 32 && fill_left > 0) {
+      if (fill.i < 0) {   // the unit's head item
+        fill.i = 0;
+        --fill_left;
+        continue;
+      }
+      const int take = min(min(fill.en.pages - fill.i, 32 - off), fill_left);
       if (lane >= off && lane < off + take) {
         b = fill.en.last < 0 ? -1 : fill.e / a.tiles;
         h = fill.h;
@@ -449,26 +605,31 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       }
       off += take;
       fill.i += take;
-      if (fill.i == fill.en.pages && !next_unit(fill)) break;
+      fill_left -= take;
+      if (fill.i == fill.en.pages && !next_unit(fill, fill_cache)) break;
     }
-    int2 rec = make_int2(-1, 127 | 127 << 8);
-    if (b >= 0 && filled + lane < count) {
+    int tile = -1;
+    if (b >= 0) {
       const int p = __ldcg(a.page_table + static_cast<size_t>(b) * a.width + i);
-      if (p >= 0 && p < a.pages) {
-        rec.x = p * a.hk + h;
-        rec.y = __ldcg(a.k_exp + rec.x) | __ldcg(a.v_exp + rec.x) << 8;
-      } else {
-        atomicOr(a.status, ST_BAD_PAGE);
-      }
+      if (p >= 0 && p < a.pages) tile = p * a.hk + h;
+      else atomicOr(a.status, ST_BAD_PAGE);
     }
-    s_rec[warp][(filled + lane) & 63] = rec;
-    filled += 32;
+    if (lane < off) s_rec[warp][(filled + lane) & 63].x = tile;
+    __syncwarp();
+    pend_at = filled + lane;
+    pend_tile = lane < off ? tile : -2;
+    filled += off;
+  };
+  // The second half of a look-up: the exponents, needed only once the page's copy has landed.
+  auto look_up_exponents = [&]() {
+    int e = 127 | 127 << 8;
+    if (pend_tile >= 0) e = __ldcg(a.k_exp + pend_tile) | __ldcg(a.v_exp + pend_tile) << 8;
+    if (pend_tile > -2) s_rec[warp][pend_at & 63].y = e;
     __syncwarp();
   };
   look_up();
 
   int issued = 0, used = 0;               // halves (K, then V of a page) requested and consumed by this worker
-  const int halves = 2 * count;
   const bool issuer = !SHARED || warp == 0;
   // Requests the next half; every lane of the issuing warp runs it.
   auto request = [&]() {
@@ -496,56 +657,62 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (SHARED && lane == 0) mbar_arrive(smem_u32(&empty[used % SLOTS]));
     ++used;
     if (issuer)
-      while (issued < halves && issued < used + SLOTS && (issued >> 1) < filled && !(SHARED && s_abort)) request();
+      while (issued < used + SLOTS && (issued >> 1) < filled && !(SHARED && s_abort)) request();
   };
   if (issuer)
-    while (issued < halves && issued < SLOTS && (issued >> 1) < filled) request();
+    while (issued < SLOTS && (issued >> 1) < filled) request();
+  look_up_exponents();
 
-  TileState<D> st;
-  uint32_t qf[D / 16][4];
-  float qs[2];
-  const int wrow = SHARED ? warp * ATTN_TILE : 0;   // this warp's first row in the worker's tile
-  bool fresh = true, first_segment = true;
-  int seg_first = 0, my_rows = 0;                   // first page of the segment; rows of this warp
-  for (int n = 0; n < count; ++n) {
+  TileState<D, NT> st;
+  uint32_t qf[NT][D / 16][2];
+  float qs[NT][2];
+  RowInfo<NT> ri;
+  const int wrow = SHARED ? warp * WARP_ROWS : 0;   // this warp's first row in the worker's tile
+  // All eight warps inside one unit: their sums meet in shared memory, and one slot leaves the CTA.
+  const int w_first = worker - warp;
+  const bool merge = !SHARED && !spread && attn_merged(deal, w_first, ATTN_WARPS, unit0 + 1, unit0 + attn_items(rd.en));   // CTA-uniform
+  bool fresh = true;
+  int seg_first = 0, left = items, n = 0;           // first page of the segment; items to go; pages done
+  while (left > 0) {
+    if (rd.i < 0) {   // the unit's head item
+      rd.i = 0;
+      --left;
+      continue;
+    }
+    const int my_rows = max(0, min(WARP_ROWS, rd.en.rows - wrow));
     if (fresh) {
-      my_rows = max(0, min(ATTN_TILE, rd.en.rows - wrow));
       tile_reset(st);
-      load_q<D>(a, rd.en, rd.h, rd.en.row0 + wrow, my_rows, group, qf, qs);
+      const int r0 = rd.en.row0 + wrow, t = lane & 3;
+      load_q<D, NT>(a, rd.en, rd.h, r0, my_rows, group, qf, qs);
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          ri.there[k][c] = 8 * k + 2 * t + c < my_rows;
+          ri.pos[k][c] = rd.en.pos + (r0 + 8 * k + 2 * t + c) / group;
+        }
+      ri.first = rd.en.pos + r0 / group;
+      ri.last = rd.en.pos + (r0 + my_rows - 1) / group;
       fresh = false;
       seg_first = rd.i;
     }
     // records: looked up 32 at a time, while those of the pages under way stay (the ring of records holds 64)
-    if (filled < count && filled - n <= SLOTS / 2 + 2) look_up();
+    if (fill_left > 0 && filled - n <= SLOTS / 2 + 2) {
+      look_up();
+      look_up_exponents();
+    }
     const int2 rec = s_rec[warp][n & 63];
     const bool live = rec.x >= 0 && my_rows > 0;
+    const int p0 = (rd.en.page0 + rd.i) * ATTN_PAGE;
+    // some row does not see some token of the page (positions grow with the row)
+    const bool edge = ri.first < p0 + ATTN_PAGE - 1 || (a.window > 0 && ri.last - a.window + 1 > p0);
     const int ks = used % SLOTS, vsl = (used + 1) % SLOTS, vt = (used + 1) / SLOTS;
-    bool ok = mbar_wait(smem_u32(&full[ks]), (used / SLOTS) & 1);
-    float s[8][4], a0, a1;
-    uint32_t p[4][4];
-    int low[2], lim[2], any_lo, any_hi, all_lo, all_hi;   // positions grow with the row
-    bool edge = false;
-    if (ok && live) page_scores<D>(s, qf, ring_base + static_cast<uint32_t>(ks) * SLOT_BYTES);
+    bool ok = mbar_wait(smem_u32(&full[ks]), (used / SLOTS) & 1), moved = false;
+    float s[4][NT][4], al[NT][2];
+    uint32_t p[4][NT][2];
+    if (ok && live) page_scores<D, NT>(s, qf, ring_base + static_cast<uint32_t>(ks) * SLOT_BYTES);
     release();
-    if (ok && live) {
-      const int p0 = (rd.en.page0 + rd.i) * ATTN_PAGE, g = lane >> 2;
-      auto bounds = [&](int r, int& lo, int& hi) {   // tokens of the page that row r of the warp's tile sees
-        const int pos = rd.en.pos + (rd.en.row0 + wrow + r) / group;
-        hi = pos - p0;
-        lo = a.window > 0 ? pos - a.window + 1 - p0 : 0;
-      };
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        bounds(g + 8 * half, low[half], lim[half]);
-        if (g + 8 * half >= my_rows) {   // rows that are not there see nothing
-          low[half] = ATTN_PAGE;
-          lim[half] = -1;
-        }
-      }
-      bounds(0, any_lo, all_hi);
-      bounds(my_rows - 1, all_lo, any_hi);
-      edge = page_softmax<D>(st, s, p, a0, a1, qs, exp2_byte(rec.y & 255), low, lim, all_lo, all_hi);
-    }
+    if (ok && live) page_softmax<D, NT>(st, s, p, al, moved, qs, exp2_byte(rec.y & 255), ri, p0, a.window, edge);
     ok = ok && mbar_wait(smem_u32(&full[vsl]), vt & 1);
     if (!ok || (SHARED && s_abort)) {
       if (lane == 0 && !ok) atomicOr(a.status, ST_ATTN_TIMEOUT);
@@ -555,23 +722,35 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (live) {
       const uint32_t vs = ring_base + static_cast<uint32_t>(vsl) * SLOT_BYTES;
       const float vscale = exp2_byte(rec.y >> 8);
-      if (edge) page_pv_edge<D>(st, p, vs, a0, a1, vscale, low, lim, any_lo, any_hi);
-      else page_pv<D, false>(st, p, vs, a0, a1, vscale, 0, ATTN_PAGE - 1);
+      if (edge) page_pv_edge<D, NT>(st, p, vs, al, moved, vscale, ri, p0, a.window);
+      else page_pv<D, NT, false>(st, p, vs, al, moved, vscale, 0, ATTN_PAGE - 1);
     }
     release();
+    ++n;
+    --left;
     // end of the unit or of the range: the segment [seg_first, rd.i] is done
     const bool unit_end = rd.i == rd.en.pages - 1;
-    if (unit_end || n + 1 == count) {
+    if (unit_end || left == 0) {
       const bool whole = unit_end && seg_first == 0;
-      // a worker has at most two partial segments: the one it begins inside a unit, and the one it ends inside one
-      float* slot = a.part + (2ll * worker + (first_segment ? 0 : 1)) * attn_slot_floats(D, TILE);
-      tile_store<D>(st, a, rd.en, rd.h, rd.en.row0 + wrow, my_rows, group, whole, slot, TILE, wrow);
+      // (a warp's ring is idle by now when it merges: its range ends with this segment)
+      float* slot = merge ? reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * attn_slots(D) * SLOT_BYTES / 4
+                          : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + 1)) * attn_slot_floats(D, TILE);
+      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, group, whole && !merge, slot, TILE);
       fresh = true;
-      first_segment = false;
     }
-    if (n + 1 < count) {
-      if (unit_end) next_unit(rd);
-      else ++rd.i;
+    if (left > 0) {
+      if (unit_end) {
+        unit0 += attn_items(rd.en);
+        next_unit(rd, rd_cache);
+      } else {
+        ++rd.i;
+      }
+    }
+  }
+  if constexpr (!SHARED) {
+    if (merge) {
+      __syncthreads();   // every warp of the CTA comes here, also one that gave up
+      merge_slots<D, NT>(reinterpret_cast<const float*>(smem), attn_slots(D) * SLOT_BYTES / 4, a.part + static_cast<size_t>(2 * w_first) * attn_slot_floats(D, TILE));
     }
   }
   if (s_abort) {
@@ -581,63 +760,75 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   }
 }
 
-// Adds up the partial sums of the units that were split between workers: one warp per row, a unit's segments in page
-// order (the same bits in every run).
-template <int D, bool SHARED>
-__global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnArgs a, int workers) {
-  constexpr int TILE = SHARED ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
-  constexpr int V = D / 32;   // dimensions per lane
+// Adds up the partial sums of the units that were split between workers, in a fixed order (the same bits in every run).
+// Lanes as the accumulators lie: a warp has 8 rows and 16 dimensions of a unit. DEEP (few units, many parts each): a CTA's
+// eight warps take every eighth part of the same 16 dimensions and meet in shared memory; else a warp takes all parts.
+template <int D, int TILE, bool DEEP>
+__global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(const __grid_constant__ AttnArgs a, int workers, int spread_below) {
+  constexpr int STEP = DEEP ? 8 : 1, FLOATS = attn_slot_floats(D, TILE);
+  __shared__ float s_m[STEP][8], s_l[STEP][8];
+  __shared__ float4 s_o[STEP][32];
   griddep_launch_dependents();
   griddep_wait();
   const int entries = a.batch * a.tiles, group = a.hq / a.hk;
   const int e = static_cast<int>(blockIdx.x) / a.hk, h = static_cast<int>(blockIdx.x) % a.hk;
-  const int r = static_cast<int>(blockIdx.y) * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = static_cast<int>(blockIdx.y) * 8, d = DEEP ? static_cast<int>(blockIdx.z) : warp;
   const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
   const AttnEntry en = attn_entry_of(a, e, group, TILE);
-  if (r >= en.rows) return;
+  if (r0 >= en.rows) return;
   const AttnDeal deal = attn_deal(total, workers);
-  const long long u0 = start + static_cast<long long>(h) * en.pages;
-  const int w0 = attn_worker(deal, u0), w1 = attn_worker(deal, u0 + en.pages - 1);
-  if (w0 == w1) return;   // one worker had the whole unit and has written it
-  // all but the first worker's segments are that worker's first
-  const size_t stride = 2ull * attn_slot_floats(D, TILE);
-  const float* const first = a.part + static_cast<size_t>(attn_slot_of(deal, w0, u0)) * attn_slot_floats(D, TILE);
-  const float* const rest = a.part + static_cast<size_t>(w0) * stride;   // worker w0 + i's first slot, i > 0: rest + i stride
-  const int parts = w1 - w0 + 1;
-  float mx = -INFINITY;
-  for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, __ldcg((i ? rest + i * stride : first) + r));
+  const long long u0 = start + static_cast<long long>(h) * attn_items(en) + 1;
+  if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;   // one worker had all of the unit's pages and has written it
+  const AttnParts ps = attn_parts(deal, TILE > 16 || total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
+  const int row = r0 + 2 * t;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float2& pm, const float2& pl, const float4& po) {   // one more part, or a warp's sums
+    const float m0 = fmaxf(m[0], pm.x), m1 = fmaxf(m[1], pm.y);
+    const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+    const float f0 = exp2_fast(m[0] - b0), f1 = exp2_fast(m[1] - b1), k0 = exp2_fast(pm.x - b0), k1 = exp2_fast(pm.y - b1);
+    l[0] = fmaf(l[0], f0, pl.x * k0);
+    l[1] = fmaf(l[1], f1, pl.y * k1);
+    o[0] = fmaf(o[0], f0, po.x * k0);
+    o[1] = fmaf(o[1], f1, po.y * k1);
+    o[2] = fmaf(o[2], f0, po.z * k0);
+    o[3] = fmaf(o[3], f1, po.w * k1);
+    m[0] = m0;
+    m[1] = m1;
+  };
+  constexpr int AHEAD = 4;
+  for (int i = DEEP ? warp : 0; i < ps.parts; i += STEP * AHEAD) {
+    float2 pm[AHEAD], pl[AHEAD];
+    float4 po[AHEAD];
 #pragma unroll
-  for (int s = 16; s; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-  const float b = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, o[V] = {};
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float* s = i ? rest + i * stride : first;
-    const float f = exp2_fast(__ldcg(s + r) - b);
-    l = fmaf(__ldcg(s + TILE + r), f, l);
-    const float* src = s + 2 * TILE + static_cast<size_t>(r) * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-      o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]); o[2] = fmaf(x.z, f, o[2]); o[3] = fmaf(x.w, f, o[3]);
-    } else {
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-      o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]);
+    for (int k = 0; k < AHEAD; ++k) {
+      const int j = i + k * STEP;
+      if (j < ps.parts) {
+        const float* s = a.part + static_cast<size_t>(attn_part_slot(ps, j)) * FLOATS;
+        pm[k] = __ldcg(reinterpret_cast<const float2*>(s + row));
+        pl[k] = __ldcg(reinterpret_cast<const float2*>(s + TILE + row));
+        po[k] = __ldcg(reinterpret_cast<const float4*>(s + 2 * TILE) + static_cast<size_t>((r0 / 8) * (D / 16) + d) * 32 + lane);
+      }
     }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int rr = en.row0 + r;
-  const size_t tok = en.first + rr / group;
-  const int col = (h * group + rr % group) * D + lane * V;
 #pragma unroll
-  for (int c = 0; c < V; c += 2) {
-    float x = o[c] * inv, y = o[c + 1] * inv;
-    if (a.gate) {
-      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(a.gate + tok * a.ld_gate + col + c));
-      x *= sigmoid_f32(bf16lo_f32(w));
-      y *= sigmoid_f32(bf16hi_f32(w));
-    }
-    *reinterpret_cast<__nv_bfloat162*>(a.out + tok * a.ld_out + col + c) = __floats2bfloat162_rn(x, y);
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + k * STEP < ps.parts) add(pm[k], pl[k], po[k]);
   }
+  if constexpr (DEEP) {
+    if (g == 0) {
+      s_m[warp][2 * t] = m[0]; s_m[warp][2 * t + 1] = m[1];
+      s_l[warp][2 * t] = l[0]; s_l[warp][2 * t + 1] = l[1];
+    }
+    s_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+      add(make_float2(s_m[w][2 * t], s_m[w][2 * t + 1]), make_float2(s_l[w][2 * t], s_l[w][2 * t + 1]), s_o[w][lane]);
+  }
+  const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
+  const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
+  store_quads<1>(a, en, h, group, row, 16 * d + g, quad, inv, D);
 }
 
 // ---------------------------------------------------------------- host side
@@ -646,63 +837,75 @@ static int attn_sms() {
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
   return v;
 }
-static bool attn_shared(int max_q, int hq, int hk) { return static_cast<long long>(max_q) * (hq / hk) > ATTN_TILE; }
-static int attn_tiles(int max_q, int hq, int hk) {
-  const int tile = attn_shared(max_q, hq, hk) ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
-  return (max_q * (hq / hk) + tile - 1) / tile;
+// The form a call takes goes by the rows a KV head has at most: 8 or 16 per warp, or 128 per CTA.
+struct AttnForm {
+  bool shared;
+  int tile, tiles;
+  int workers(int sms) const { return shared ? sms : sms * ATTN_WARPS; }
+};
+static AttnForm attn_form(int max_q, int hq, int hk) {
+  const long long rows = static_cast<long long>(max_q) * (hq / hk);
+  AttnForm f;
+  f.shared = rows > 16;
+  f.tile = f.shared ? 16 * ATTN_WARPS : rows > 8 ? 16 : 8;
+  f.tiles = static_cast<int>((rows + f.tile - 1) / f.tile);
+  return f;
 }
 
 long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
   const int sms = attn_sms();
   if (batch < 1 || max_q < 1 || hk < 1 || hq < hk || hq % hk || (dim != 64 && dim != 128) || sms < 1) return -1;
-  const bool sh = attn_shared(max_q, hq, hk);
-  const long long workers = sh ? sms : static_cast<long long>(sms) * ATTN_WARPS;
-  const long long part = 2 * workers * attn_slot_floats(dim, sh ? ATTN_TILE * ATTN_WARPS : ATTN_TILE) * 4;
-  return part + (static_cast<long long>(batch) * attn_tiles(max_q, hq, hk) + 1) * 8;
+  const AttnForm f = attn_form(max_q, hq, hk);
+  return 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile) * 4 + (static_cast<long long>(batch) * f.tiles + 1) * 8;
 }
 
-template <int D, bool SHARED>
-static cudaError_t attn_launch(const AttnArgs& a, int sms, cudaStream_t stream) {
+template <int D, int NT, bool SHARED>
+static cudaError_t attn_launch(const AttnArgs& a, const AttnForm& f, int sms, cudaStream_t stream) {
   const size_t smem = attn_ring_bytes(D);
-  cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  e = launch_dependent(cache_attn_kernel<D, SHARED>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
+  e = launch_dependent(cache_attn_kernel<D, NT, SHARED>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
   if (e != cudaSuccess) return e;
-  const int tile = SHARED ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
-  const int rows = a.max_q * (a.hq / a.hk) < tile ? a.max_q * (a.hq / a.hk) : tile;
-  const long long workers = SHARED ? sms : static_cast<long long>(sms) * ATTN_WARPS;
-  const long long units = static_cast<long long>(a.batch) * a.tiles * a.hk;
-  return launch_dependent(cache_attn_join_kernel<D, SHARED>, dim3(static_cast<unsigned>(units), (rows + 3) / 4), dim3(128), 0, stream, a, static_cast<int>(workers));
+  const int all = a.max_q * (a.hq / a.hk), rows = all < f.tile ? all : f.tile;
+  const unsigned units = static_cast<unsigned>(a.batch) * a.tiles * a.hk;
+  constexpr int TILE = SHARED ? 16 * ATTN_WARPS : 8 * NT;
+  const unsigned groups = (rows + 7) / 8;
+  // Few units may have many parts each; many units have few (there are two partial segments per worker in all).
+  if (static_cast<long long>(units) * groups < 2ll * sms)
+    return launch_dependent(cache_attn_join_kernel<D, TILE, true>, dim3(units, groups, D / 16), dim3(256), 0, stream, a, f.workers(sms), attn_spread_below(sms));
+  return launch_dependent(cache_attn_join_kernel<D, TILE, false>, dim3(units, groups), dim3(D * 2), 0, stream, a, f.workers(sms), attn_spread_below(sms));
 }
 
 int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   if (!a.q || !a.k || !a.v || !a.k_exp || !a.v_exp || !a.page_table || !a.seq_lens || !a.out || !a.status || !ws) return -1;
   if (a.m < 1 || a.batch < 1 || a.width < 1 || a.pages < 1 || a.max_q < 1 || a.hk < 1 || a.hq < a.hk || a.hq % a.hk || (dim != 64 && dim != 128)) return -2;
   if (a.width > 0x7fffffff / ATTN_PAGE || a.window < 0 || static_cast<long long>(a.max_q) * (a.hq / a.hk) > 0x3fffffff) return -3;
-  if (a.ld_q % 8 || a.ld_q < static_cast<long long>(a.hq) * dim || a.ld_out % 2 || a.ld_out < static_cast<long long>(a.hq) * dim) return -4;
-  if (a.gate && (a.ld_gate % 2 || a.ld_gate < static_cast<long long>(a.hq) * dim || (reinterpret_cast<uintptr_t>(a.gate) & 3))) return -4;
+  if (a.ld_q % 8 || a.ld_q < static_cast<long long>(a.hq) * dim || a.ld_out < static_cast<long long>(a.hq) * dim) return -4;
+  if (a.gate && a.ld_gate < static_cast<long long>(a.hq) * dim) return -4;
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(ws)) & 15) return -5;
-  if (reinterpret_cast<uintptr_t>(a.out) & 3) return -5;
+  if ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 1) return -5;
   if (!a.cu_q && a.max_q != 1) return -6;
   const int sms = attn_sms();
   if (sms < 1) return -7;
-  a.tiles = attn_tiles(a.max_q, a.hq, a.hk);
+  const AttnForm f = attn_form(a.max_q, a.hq, a.hk);
+  a.tiles = f.tiles;
   if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
-  const bool sh = attn_shared(a.max_q, a.hq, a.hk);
-  const long long workers = sh ? sms : static_cast<long long>(sms) * ATTN_WARPS;
   a.part = static_cast<float*>(ws);
-  a.prefix = reinterpret_cast<long long*>(a.part + 2 * workers * attn_slot_floats(dim, sh ? ATTN_TILE * ATTN_WARPS : ATTN_TILE));
+  a.prefix = reinterpret_cast<long long*>(a.part + 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile));
   cudaError_t e;
-  if (dim == 128) e = sh ? attn_launch<128, true>(a, sms, stream) : attn_launch<128, false>(a, sms, stream);
-  else e = sh ? attn_launch<64, true>(a, sms, stream) : attn_launch<64, false>(a, sms, stream);
+  if (dim == 128)
+    e = f.shared ? attn_launch<128, 2, true>(a, f, sms, stream) : f.tile == 16 ? attn_launch<128, 2, false>(a, f, sms, stream) : attn_launch<128, 1, false>(a, f, sms, stream);
+  else
+    e = f.shared ? attn_launch<64, 2, true>(a, f, sms, stream) : f.tile == 16 ? attn_launch<64, 2, false>(a, f, sms, stream) : attn_launch<64, 1, false>(a, f, sms, stream);
   return static_cast<int>(e);
 }
 
 // ---- the same plan on the host
 namespace {
 struct HostPlan {
-  int group, tile, tiles, entries;
-  long long workers, total;
+  AttnForm form;
+  int group, entries;
+  long long total;
   bool ok;
 };
 }  // namespace
@@ -711,45 +914,46 @@ static HostPlan host_plan(const int* seq_lens, int m, int batch, int width, int 
   p.ok = seq_lens && m >= 1 && batch >= 1 && width >= 1 && width <= 0x7fffffff / ATTN_PAGE && max_q >= 1 && hk >= 1 && hq >= hk && hq % hk == 0 &&
          window >= 0 && sms >= 1;
   if (!p.ok) return p;
-  const bool sh = attn_shared(max_q, hq, hk);
+  p.form = attn_form(max_q, hq, hk);
   p.group = hq / hk;
-  p.tile = sh ? ATTN_TILE * ATTN_WARPS : ATTN_TILE;
-  p.tiles = attn_tiles(max_q, hq, hk);
-  p.entries = batch * p.tiles;
-  p.workers = sh ? sms : static_cast<long long>(sms) * ATTN_WARPS;
+  p.entries = batch * p.form.tiles;
   return p;
 }
 static AttnEntry host_entry(const HostPlan& p, const int* seq_lens, const int* cu_q, int m, int width, int max_q, int window, int e) {
-  const int b = e / p.tiles;
-  return attn_entry(cu_q ? cu_q[b] : b, cu_q ? cu_q[b + 1] : b + 1, seq_lens[b], m, max_q, width * ATTN_PAGE, p.group, p.tile, e % p.tiles, window);
+  const int b = e / p.form.tiles;
+  return attn_entry(cu_q ? cu_q[b] : b, cu_q ? cu_q[b + 1] : b + 1, seq_lens[b], m, max_q, width * ATTN_PAGE, p.group, p.form.tile, e % p.form.tiles, window);
 }
 
 long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window, int sms,
                           int* segments, long long capacity) {
   HostPlan p = host_plan(seq_lens, m, batch, width, max_q, hq, hk, window, sms);
   if (!p.ok || !segments) return -1;
-  for (int e = 0; e < p.entries; ++e) p.total += static_cast<long long>(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e).pages) * hk;
+  for (int e = 0; e < p.entries; ++e) p.total += static_cast<long long>(attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e))) * hk;
   if (p.total == 0) return 0;
-  const AttnDeal deal = attn_deal(p.total, static_cast<int>(p.workers));
+  const AttnDeal deal = attn_deal(p.total, p.form.workers(sms));
   long long count = 0, start = 0;
   int e = 0;
   AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, 0);
   for (int w = 0; w < deal.workers; ++w) {
-    bool first = true;
     for (long long f = attn_range(deal, w), f1 = attn_range(deal, w + 1); f < f1;) {
-      while (f >= start + static_cast<long long>(en.pages) * hk) {
-        start += static_cast<long long>(en.pages) * hk;
+      while (f >= start + static_cast<long long>(attn_items(en)) * hk) {
+        start += static_cast<long long>(attn_items(en)) * hk;
         en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, ++e);
       }
-      const int off = static_cast<int>(f - start), h = off / en.pages, i = off % en.pages;
+      const int off = static_cast<int>(f - start), h = off / attn_items(en), i = off % attn_items(en) - 1;
+      if (i < 0) {
+        ++f;
+        continue;
+      }
       const int n = static_cast<int>(f1 - f < en.pages - i ? f1 - f : en.pages - i);
       if (count < capacity) {
         int* s = segments + 6 * count;
         s[0] = w; s[1] = e; s[2] = h; s[3] = en.page0 + i; s[4] = n;
-        s[5] = n == en.pages ? -1 : 2 * w + (first ? 0 : 1);
+        const long long u0 = start + static_cast<long long>(h) * attn_items(en) + 1;
+        const int per = p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, first = w - w % per;
+        s[5] = n == en.pages ? -1 : attn_merged(deal, first, per, u0, u0 + en.pages) ? 2 * first : attn_slot_of(deal, w, u0);
       }
       ++count;
-      first = false;
       f += n;
     }
   }
@@ -763,17 +967,16 @@ long long cache_attn_join(const int* seq_lens, const int* cu_q, int m, int batch
   long long before = 0;
   for (int e = 0; e < p.entries; ++e) {
     if (e == entry) before = p.total;
-    p.total += static_cast<long long>(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e).pages) * hk;
+    p.total += static_cast<long long>(attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e))) * hk;
   }
   const AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, entry);
   if (en.rows == 0) return 0;
-  const AttnDeal deal = attn_deal(p.total, static_cast<int>(p.workers));
-  const long long u0 = before + static_cast<long long>(head) * en.pages;
-  const int w0 = attn_worker(deal, u0), w1 = attn_worker(deal, u0 + en.pages - 1);
-  if (w0 == w1) return 0;
-  for (int w = w0; w <= w1; ++w)
-    if (w - w0 < capacity) slots[w - w0] = attn_slot_of(deal, w, u0);
-  return w1 - w0 + 1;
+  const AttnDeal deal = attn_deal(p.total, p.form.workers(sms));
+  const long long u0 = before + static_cast<long long>(head) * attn_items(en) + 1;
+  if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return 0;
+  const AttnParts ps = attn_parts(deal, p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, u0, en.pages);
+  for (int i = 0; i < ps.parts && i < capacity; ++i) slots[i] = attn_part_slot(ps, i);
+  return ps.parts;
 }
 
 }  // namespace muse

@@ -8,7 +8,7 @@ import ctypes as C
 
 import pytest
 
-PAGE, TILE, WARPS = 64, 16, 8
+PAGE, WARPS = 64, 8
 
 
 def plan(lens, cu, m, width, max_q, hq, hk, window, sms):
@@ -53,6 +53,9 @@ CASES = [
     ([4096, 4096], [512, 512], 64, 32, 8, 0, 148),
     ([700, 50, 1300], [129, 50, 1], 21, 8, 1, 200, 5),
     ([3, 0], [5, 2], 1, 8, 8, 0, 4),          # more new tokens than tokens: padding rows
+    ([64 * 1184 * 3], None, 1184 * 3, 4, 1, 0, 148),
+    ([64 * 500, 64 * 37, 64 * 900 + 1], None, 1000, 16, 1, 0, 9),
+    ([64 * 700 + i for i in range(5)], None, 1000, 8, 2, 0, 16),
 ]
 
 
@@ -63,14 +66,23 @@ def test_every_page_is_read_once_and_joined_in_order(case):
     n = [1] * len(lens) if new is None else new
     m, max_q, group = sum(n), max(n), hq // hk
     segs, join = plan(lens, cu, m, width, max_q, hq, hk, window, sms)
-    tile = TILE if max_q * group <= TILE else TILE * WARPS
+    rows = max_q * group
+    tile = 8 if rows <= 8 else 16 if rows <= 16 else 128
     tiles = -(-max_q * group // tile)
     units = {}
     for worker, entry, head, first, count, slot in segs:
         units.setdefault((entry, head), []).append((first, count, worker, slot))
-    slots = [s[5] for s in segs if s[5] >= 0]
-    assert len(slots) == len(set(slots)), "two segments share a partial slot"
-    workers = sms if tile > TILE else sms * WARPS
+    # a slot holds one segment, or the segments of a CTA's eight warps inside one unit, which are added up on chip
+    slots = {}
+    for i, s in enumerate(segs):
+        if s[5] >= 0:
+            slots.setdefault(s[5], []).append(i)
+    for slot, where in slots.items():
+        if len(where) > 1:
+            same = [segs[i] for i in where]
+            assert where == list(range(where[0], where[0] + WARPS)) and len({s[1:3] for s in same}) == 1
+            assert [s[0] for s in same] == list(range(slot // 2, slot // 2 + WARPS)) and slot // 2 % WARPS == 0
+    workers = sms if tile == 128 else sms * WARPS
     assert all(0 <= s[0] < workers for s in segs) and all(s < 2 * workers for s in slots)
     want = {}
     for b, (length, k) in enumerate(zip(lens, n)):
@@ -89,10 +101,14 @@ def test_every_page_is_read_once_and_joined_in_order(case):
         if len(parts) == 1:
             assert parts[0][3] == -1 and join(*key) == []
         else:
-            assert [p[3] for p in parts] == join(*key) and all(p[3] >= 0 for p in parts)
+            in_order = [p[3] for i, p in enumerate(parts) if i == 0 or parts[i - 1][3] != p[3]]
+            assert in_order == join(*key) and all(s >= 0 for s in in_order)
         for _, count, w, _ in parts:
             share[w] += count
-    assert max(share) - min(share) <= 1, "the pages are dealt evenly"
+    # equal shares of pages plus one head item per unit: no worker has more than its share, a segment's head item counted
+    items = sum(len(pages) + 1 for pages in want.values())
+    assert all(share[w] <= -(-items // workers) for w in range(workers))
+    assert sum(share) == sum(len(pages) for pages in want.values())
 
 
 def test_bad_lengths_and_bounds_stay_inside():
