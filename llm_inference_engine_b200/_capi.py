@@ -116,10 +116,10 @@ def check(rc: int, what: str) -> None:
         raise MuseError(f"{what}: {kind} {rc}")
 
 
-def raw_stream(index: int) -> int:
-    """The current stream of CUDA device `index` as the C ABI takes it (torch.cuda.current_stream() without building the
-    Python object: 2 us of a small call)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+# Small calls are bound by what the host does for them: the two helpers below are torch.cuda.current_stream(i).cuda_stream
+# and torch.cuda.device(i) without the objects those build (2 us and 1 us a call).
+raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 class on_device:
@@ -131,7 +131,7 @@ class on_device:
         self.index = index
 
     def __enter__(self):
-        self.was = torch.cuda.current_device()
+        self.was = _current_device()
         if self.was != self.index:
             torch.cuda.set_device(self.index)
 
@@ -140,18 +140,24 @@ class on_device:
             torch.cuda.set_device(self.was)
 
 
+def new_tensor(shape, strides, dtype, device) -> torch.Tensor:
+    """torch.empty of known strides (1.5 us against 2.3)."""
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
 _STATUS: dict[int, torch.Tensor] = {}
 STATUS_TEXT = ((128, "a page index outside the pool"), (256, "lengths or row bounds that do not fit"))
 
 
-def status_word(device: torch.device) -> torch.Tensor:
-    """The status word that the 8-bit operators of a device share (the projections of prepare() have one per state)."""
-    word = _STATUS.get(device.index)
+def status_ptr(index: int) -> int:
+    """Address of the status word that the 8-bit operators of a device share (the projections of prepare() have one per
+    state)."""
+    word = _STATUS.get(index)
     if word is None:
         if torch.cuda.is_current_stream_capturing():   # it must outlive the graph
             raise MuseError("the first call of the 8-bit operators on a device makes their status word: make it outside stream capture")
-        word = _STATUS[device.index] = torch.zeros(1, device=device, dtype=torch.int32)
-    return word
+        word = _STATUS[index] = torch.zeros(1, device=torch.device("cuda", index), dtype=torch.int32)
+    return word.data_ptr()
 
 
 def check_status_word(device) -> None:

@@ -84,13 +84,16 @@ def check_status(device) -> None:
     _capi.check_status_word(device)
 
 
-def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
-    """The checks both operators share; returns (device, pages, heads, dim, batch, width)."""
+_F8, _BF16, _U8, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.uint8, torch.int32
+
+
+def _refuse_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
+    """Says what is wrong with a batch that _check_batch() does not take."""
     k, v, ke, ve = cache
     dev = k.device
     if not k.is_cuda:
         raise RuntimeError(f"the cache is on {dev}: this path runs on a CUDA device only (no CPU fallback)")
-    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ke.dtype != torch.uint8 or ve.dtype != torch.uint8:
+    if k.dtype != _F8 or v.dtype != _F8 or ke.dtype != _U8 or ve.dtype != _U8:
         raise TypeError(f"a cache is float8_e4m3fn codes and uint8 exponents, got {k.dtype}, {v.dtype}, {ke.dtype}, {ve.dtype}")
     if k.dim() != 4 or k.shape[2] != PAGE or k.shape[3] not in HEAD_DIMS:
         raise ValueError(f"k must be [pages, heads, {PAGE}, dim] with dim in {HEAD_DIMS}, got {tuple(k.shape)}")
@@ -99,62 +102,88 @@ def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, 
         raise ValueError(f"v {tuple(v.shape)} / exponents {tuple(ke.shape)}, {tuple(ve.shape)} do not fit k {tuple(k.shape)}")
     if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()) or (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("the cache's tensors must be contiguous and 16-byte aligned")
-    if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0] or not seq_lens.shape[0] or not page_table.shape[1]:
-        raise ValueError(f"page_table [batch, width] {tuple(page_table.shape)} and seq_lens [batch] {tuple(seq_lens.shape)} do not fit")
-    batch, width = page_table.shape
-    index = (page_table, seq_lens) if cu_q is None else (page_table, seq_lens, cu_q)
-    for t in index:
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
-            raise TypeError("page_table, seq_lens and cu_q must be contiguous int32 tensors on the cache's device")
     if v.device != dev or ke.device != dev or ve.device != dev:
         raise ValueError("the cache's tensors must be on one device")
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or page_table.shape[0] != seq_lens.shape[0] or not seq_lens.shape[0] or not page_table.shape[1]:
+        raise ValueError(f"page_table [batch, width] {tuple(page_table.shape)} and seq_lens [batch] {tuple(seq_lens.shape)} do not fit")
+    batch = page_table.shape[0]
+    for t in (page_table, seq_lens) if cu_q is None else (page_table, seq_lens, cu_q):
+        if t.dtype != _I32 or not t.is_contiguous() or t.device != dev:
+            raise TypeError("page_table, seq_lens and cu_q must be contiguous int32 tensors on the cache's device")
     if cu_q is None:
         if m != batch or max_q != 1:
             raise ValueError(f"without cu_q there is one new token per sequence: {m} rows for {batch} sequences, max_q={max_q}")
     elif cu_q.shape != (batch + 1,):
         raise ValueError(f"cu_q must be [batch + 1] = [{batch + 1}], got {tuple(cu_q.shape)}")
-    if max_q < 1 or q_heads < heads or q_heads % heads:
-        raise ValueError(f"max_q={max_q} must be positive and q_heads={q_heads} a multiple of the cache's {heads}")
-    return dev, pages, heads, dim, batch, width
+    raise ValueError(f"max_q={max_q} must be positive and q_heads={q_heads} a multiple of the cache's {heads}")
+
+
+def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
+    """The checks both operators share, in one expression (they are a good part of a small call's time); returns (device
+    index, addresses of k, v, k_exp, v_exp, page_table, seq_lens, cu_q, pages, heads, dim, batch, width)."""
+    k, v, ke, ve = cache
+    shape, index = k.shape, k.get_device()
+    if len(shape) == 4 and index >= 0:
+        pages, heads, page, dim = shape
+        kp, vp = k.data_ptr(), v.data_ptr()
+        batch, width = page_table.shape if page_table.dim() == 2 else (0, 0)
+        if (page == PAGE and (dim == 128 or dim == 64) and k.dtype is _F8 and v.dtype is _F8 and ke.dtype is _U8 and ve.dtype is _U8
+                and v.shape == (pages, heads, dim, PAGE) and ke.shape == (pages, heads) and ve.shape == (pages, heads)
+                and k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous() and not (kp | vp) & 15
+                and v.get_device() == index and ke.get_device() == index and ve.get_device() == index
+                and batch and width and seq_lens.shape == (batch,) and page_table.dtype is _I32 and seq_lens.dtype is _I32
+                and page_table.is_contiguous() and seq_lens.is_contiguous() and page_table.get_device() == index
+                and seq_lens.get_device() == index and max_q >= 1 and q_heads >= heads and not q_heads % heads):
+            if cu_q is None:
+                if m == batch and max_q == 1:
+                    return index, kp, vp, ke.data_ptr(), ve.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), None, pages, heads, dim, batch, width
+            elif cu_q.shape == (batch + 1,) and cu_q.dtype is _I32 and cu_q.is_contiguous() and cu_q.get_device() == index:
+                return (index, kp, vp, ke.data_ptr(), ve.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(), pages, heads, dim,
+                        batch, width)
+    _refuse_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
 
 
 def rope_append(qkv: torch.Tensor, cache: Cache8, cos_sin: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *, q_heads: int,
                 cu_q: torch.Tensor | None = None, max_q: int = 1, interleaved: bool = False, values: bool = False):
     """Turns q and k by their tokens' positions and appends k and v to the cache, one launch. qkv: BF16 [m, >= (q_heads +
-    2 heads) dim], unit column stride, columns q | k | v (the rows of the qkv_gate projection as they are). cos_sin:
-    rotary_table(rot, >= 64 * page_table.shape[1] positions), rot a multiple of 16 up to dim; pairs are (i, i + rot / 2),
-    or neighbours when `interleaved`. max_q: at least the most new tokens of a sequence. Returns q BF16 [m, q_heads,
-    dim]; with values=True (q, k, v), k and v BF16 [m, heads, dim]: the values that the cache then holds for the new tokens
-    (for a prompt's own attention in 16 bits to see what later tokens will see)."""
-    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[0] < 1:
+    2 heads) dim], columns q | k | v (the rows of the qkv_gate projection as they are). cos_sin: rotary_table(rot, >= 64 *
+    page_table.shape[1] positions), rot a multiple of 16 up to dim; pairs are (i, i + rot / 2), or neighbours when
+    `interleaved`. max_q: at least the most new tokens of a sequence. Returns q BF16 [m, q_heads, dim]; with values=True
+    (q, k, v), k and v BF16 [m, heads, dim]: the values that the cache then holds for the new tokens (for a prompt's own
+    attention in 16 bits to see what later tokens will see)."""
+    if qkv.dtype is not _BF16 or qkv.dim() != 2 or not qkv.shape[0]:
         raise TypeError(f"qkv must be BF16 [m, columns], got {qkv.dtype} {tuple(qkv.shape)}")
-    m = qkv.shape[0]
-    dev, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
-    if qkv.device != dev or cos_sin.device != dev:
+    m, width_in = qkv.shape
+    index, kp, vp, kep, vep, tp, lp, cp, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
+    cols = (q_heads + 2 * heads) * dim
+    if qkv.get_device() != index or cos_sin.get_device() != index:
         raise ValueError("qkv and cos_sin must be on the cache's device")
-    if qkv.shape[1] < (q_heads + 2 * heads) * dim:
-        raise ValueError(f"qkv {tuple(qkv.shape)} is narrower than q | k | v = {(q_heads + 2 * heads) * dim} columns")
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
+    if width_in < cols:
+        raise ValueError(f"qkv {tuple(qkv.shape)} is narrower than q | k | v = {cols} columns")
+    if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 3 or not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15 or cos_sin.shape[2] != 2:
         raise TypeError(f"cos_sin must be a contiguous FP32 [positions, rot / 2, 2] table, got {cos_sin.dtype} {tuple(cos_sin.shape)}")
-    positions, rot = cos_sin.shape[0], 2 * cos_sin.shape[1]
+    positions, rot, _ = cos_sin.shape
+    rot *= 2
     if rot % 16 or not 16 <= rot <= dim or positions < width * PAGE:
         raise ValueError(f"the table turns {rot} dimensions (a multiple of 16 up to {dim}) at {positions} positions; "
                          f"{width} pages per sequence need {width * PAGE}")
-    if qkv.stride(1) != 1 or qkv.data_ptr() % 16 or (m > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1])):
-        qkv = qkv[:, : (q_heads + 2 * heads) * dim].contiguous().clone()
-    lib, index = _capi.load(), dev.index
+    ld, unit = qkv.stride()
+    if unit != 1 or qkv.data_ptr() & 15 or (m > 1 and (ld & 7 or ld < width_in)):
+        qkv = qkv[:, :cols].contiguous().clone()
+        ld = cols
+    dev = qkv.device
     with _capi.on_device(index):
-        q = torch.empty((m, q_heads, dim), device=dev, dtype=torch.bfloat16)
-        k_val = v_val = None
+        q = _capi.new_tensor((m, q_heads, dim), (q_heads * dim, dim, 1), _BF16, dev)
+        k_val = v_val = kvp = vvp = None
         if values:
-            k_val = torch.empty((m, heads, dim), device=dev, dtype=torch.bfloat16)
-            v_val = torch.empty((m, heads, dim), device=dev, dtype=torch.bfloat16)
-        _capi.check(lib.muse_rope_append(qkv.data_ptr(), cos_sin.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
-                                         None if cu_q is None else cu_q.data_ptr(), cache[0].data_ptr(), cache[1].data_ptr(),
-                                         cache[2].data_ptr(), cache[3].data_ptr(), q.data_ptr(), k_val.data_ptr() if values else None,
-                                         v_val.data_ptr() if values else None, _capi.status_word(dev).data_ptr(),
-                                         qkv.stride(0) if m > 1 else (q_heads + 2 * heads) * dim, m, batch, width, pages, max_q, q_heads, heads,
-                                         dim, rot, int(interleaved), positions, _capi.raw_stream(index)), "muse_rope_append")
+            k_val = _capi.new_tensor((m, heads, dim), (heads * dim, dim, 1), _BF16, dev)
+            v_val = _capi.new_tensor((m, heads, dim), (heads * dim, dim, 1), _BF16, dev)
+            kvp, vvp = k_val.data_ptr(), v_val.data_ptr()
+        rc = _capi.load().muse_rope_append(qkv.data_ptr(), cos_sin.data_ptr(), tp, lp, cp, kp, vp, kep, vep, q.data_ptr(), kvp, vvp,
+                                           _capi.status_ptr(index), ld if m > 1 else cols, m, batch, width, pages, max_q, q_heads, heads, dim,
+                                           rot, 1 if interleaved else 0, positions, _capi.raw_stream(index))
+    if rc:
+        _capi.check(rc, f"muse_rope_append(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
     return (q, k_val, v_val) if values else q
 
 
@@ -164,37 +193,50 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
     """softmax(scale q K^T) V over the cached tokens up to each query token's own position (the last `window` of them
     when window > 0), times sigmoid(gate) when gate is given: BF16 [m, q_heads * dim], ready for the `o` projection. A row
     that sees no token is zero; rows beyond the last sequence are left as they are. q: BF16 [m, q_heads, dim]; gate: BF16
-    [m, q_heads * dim] (the gate columns of qkv_gate, any row stride); scale: 1 / sqrt(dim) by default; out (optional):
-    BF16 [m, q_heads * dim] with unit column stride. Two launches, the same bits in every run."""
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[0] < 1:
+    [m, q_heads * dim] (the gate columns of qkv_gate, any row stride); scale: positive, 1 / sqrt(dim) by default; out
+    (optional): BF16 [m, q_heads * dim] with unit column stride. Two launches, the same bits in every run."""
+    if q.dtype is not _BF16 or q.dim() != 3 or not q.shape[0]:
         raise TypeError(f"q must be BF16 [m, heads, dim], got {q.dtype} {tuple(q.shape)}")
     m, q_heads, d = q.shape
-    dev, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
-    if d != dim or q.device != dev or window < 0:
-        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not fit the cache's heads of {dim} on {dev}, or window={window} is negative")
-    if q.stride(2) != 1 or q.stride(1) != dim or q.data_ptr() % 16 or (m > 1 and (q.stride(0) % 8 or q.stride(0) < q_heads * dim)):
-        q = q.contiguous().clone()
+    index, kp, vp, kep, vep, tp, lp, cp, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
+    if d != dim or q.get_device() != index or window < 0:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not fit the cache's heads of {dim}, or window={window} is negative")
+    if scale is None:
+        scale = 0.08838834764831845 if dim == 128 else 0.125
+    elif not 0.0 < scale < math.inf:
+        raise ValueError(f"scale={scale} must be positive")
     cols = q_heads * dim
-    for name, t in (("gate", gate), ("out", out)):
-        if t is not None and (t.dtype != torch.bfloat16 or t.shape != (m, cols) or t.device != dev):
-            raise TypeError(f"{name} must be BF16 [m, q_heads * dim] = [{m}, {cols}] on the cache's device, got {t.dtype} {tuple(t.shape)}")
-    if gate is not None and (gate.stride(1) != 1 or gate.data_ptr() % 4 or (m > 1 and (gate.stride(0) % 2 or gate.stride(0) < cols))):
-        gate = gate.contiguous().clone()
-    if out is not None and (out.stride(1) != 1 or out.data_ptr() % 4 or (m > 1 and (out.stride(0) % 2 or out.stride(0) < cols))):
-        raise ValueError("out must have unit column stride, an even row stride and 4-byte alignment")
-    lib, index = _capi.load(), dev.index
+    ld_q, head, unit = q.stride()
+    if unit != 1 or head != dim or q.data_ptr() & 15 or (m > 1 and (ld_q & 7 or ld_q < cols)):
+        q = q.contiguous().clone()
+        ld_q = cols
+    gp, ld_gate = None, 0
+    if gate is not None:
+        if gate.dtype is not _BF16 or gate.shape != (m, cols) or gate.get_device() != index:
+            raise TypeError(f"gate must be BF16 [m, q_heads * dim] = [{m}, {cols}] on the cache's device, got {gate.dtype} {tuple(gate.shape)}")
+        ld_gate, unit = gate.stride()
+        if unit != 1 or (m > 1 and ld_gate < cols):
+            gate = gate.contiguous().clone()
+            ld_gate = cols
+        gp = gate.data_ptr()
+    ld_out = cols
+    if out is not None:
+        if out.dtype is not _BF16 or out.shape != (m, cols) or out.get_device() != index:
+            raise TypeError(f"out must be BF16 [m, q_heads * dim] = [{m}, {cols}] on the cache's device, got {out.dtype} {tuple(out.shape)}")
+        ld_out, unit = out.stride()
+        if unit != 1 or (m > 1 and ld_out < cols):
+            raise ValueError("out must have unit column stride and rows that do not overlap")
+    dev = q.device
     with _capi.on_device(index):
         if out is None:
-            out = torch.empty((m, cols), device=dev, dtype=torch.bfloat16)
+            out = _capi.new_tensor((m, cols), (cols, 1), _BF16, dev)
         # the workspace is the call's own (a captured graph keeps its own): calls may overlap on the GPU
-        ws = torch.empty(_ws_bytes(index, batch, max_q, q_heads, heads, dim), device=dev, dtype=torch.uint8)
-        _capi.check(lib.muse_cache_attention(q.data_ptr(), cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(),
-                                             page_table.data_ptr(), seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
-                                             None if gate is None else gate.data_ptr(), out.data_ptr(), ws.data_ptr(),
-                                             _capi.status_word(dev).data_ptr(), q.stride(0) if m > 1 else cols,
-                                             0 if gate is None else gate.stride(0) if m > 1 else cols, out.stride(0) if m > 1 else cols,
-                                             1.0 / math.sqrt(dim) if scale is None else scale, m, batch, width, pages, max_q, q_heads, heads,
-                                             dim, window, _capi.raw_stream(index)), "muse_cache_attention")
+        ws = _capi.new_tensor((_ws_bytes(index, batch, max_q, q_heads, heads, dim),), (1,), _U8, dev)
+        rc = _capi.load().muse_cache_attention(q.data_ptr(), kp, vp, kep, vep, tp, lp, cp, gp, out.data_ptr(), ws.data_ptr(), _capi.status_ptr(index),
+                                               ld_q if m > 1 else cols, ld_gate if m > 1 else cols, ld_out if m > 1 else cols, scale, m, batch,
+                                               width, pages, max_q, q_heads, heads, dim, window, _capi.raw_stream(index))
+    if rc:
+        _capi.check(rc, f"muse_cache_attention(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
     return out
 
 

@@ -44,6 +44,8 @@ struct AttnArgs {
   long long ld_q, ld_gate, ld_out;
   float scale_log2;            // softmax scale * log2(e)
   int m, batch, width, pages, max_q, hq, hk, window, tiles;   // tiles: row tiles per sequence
+  int group;                   // hq / hk
+  uint32_t group_magic;        // 2^32 / group + 1: a row's token without a division
 };
 
 int rope_append_dispatch(const RopeArgs& a, int dim, cudaStream_t stream);

@@ -56,6 +56,9 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return r;
 }
 
+// Row to token: n / group, for n * group < 2^32 (the host sees to it).
+__device__ __forceinline__ int div_group(const AttnArgs& a, int n) { return a.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), a.group_magic)); }
+
 // Lists of up to so many items are spread over the SMs (a warp each) instead of filling CTA after CTA.
 __host__ __device__ constexpr int attn_spread_below(int sms) { return 2 * sms; }
 
@@ -67,7 +70,7 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 
 __device__ __forceinline__ AttnEntry attn_entry_of(const AttnArgs& a, int e, int group, int tile) {
-  const int b = e / a.tiles, rt = e % a.tiles;
+  const int b = a.tiles == 1 ? e : e / a.tiles, rt = e - b * a.tiles;
   const int c0 = a.cu_q ? __ldcg(a.cu_q + b) : b, c1 = a.cu_q ? __ldcg(a.cu_q + b + 1) : b + 1;
   return attn_entry(c0, c1, __ldcg(a.seq_lens + b), a.m, a.max_q, a.width * ATTN_PAGE, group, tile, rt, a.window);
 }
@@ -125,14 +128,14 @@ struct RowInfo {
 // q fragments of 8 NT rows (from row0 of the unit's rows) as FP16 under a power of two per row; qs = the factor of the
 // lane's rows 2 t, 2 t + 1 for the scores in log2 units.
 template <int D, int NT>
-__device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, int h, int row0, int rows, int group, uint32_t (&qf)[NT][D / 16][2],
+__device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, int h, int row0, int rows, uint32_t (&qf)[NT][D / 16][2],
                                        float (&qs)[NT][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint4 w[NT][D / 32];   // 16 dimensions (two vectors) per 64
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = g + 8 * n, tok = (row0 + r) / group, hd = (row0 + r) - tok * group;
-    const __nv_bfloat16* src = a.q + static_cast<size_t>(en.first + tok) * a.ld_q + static_cast<size_t>(h * group + hd) * D;
+    const int r = g + 8 * n, tok = div_group(a, row0 + r), hd = (row0 + r) - tok * a.group;
+    const __nv_bfloat16* src = a.q + static_cast<size_t>(en.first + tok) * a.ld_q + static_cast<size_t>(h * a.group + hd) * D;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
       w[n][c] = r < rows ? __ldcg(reinterpret_cast<const uint4*>(src + 64 * (c >> 1) + 16 * t + 8 * (c & 1))) : make_uint4(0u, 0u, 0u, 0u);
@@ -187,15 +190,6 @@ __device__ __forceinline__ void page_scores(float (&s)[4][NT][4], const uint32_t
     }
   }
 }
-
-// Bytes of `w` (four tokens from `tok`) outside [lo, hi] become zero.
-__device__ __forceinline__ uint32_t keep_tokens(uint32_t w, int tok, int lo, int hi) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m |= (tok + i >= lo && tok + i <= hi) ? 0xffu << (8 * i) : 0u;
-  return w & m;
-}
-__device__ __forceinline__ bool has_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
 
 // Scores to weights: p[i][n] = the weights of the lane's two tokens of tile i, packed over rows (2 t, 2 t + 1), before the
 // transpose; `a`: what the rows' sums so far are to be scaled by (`moved`: not all of the warp's are 1).
@@ -253,13 +247,14 @@ __device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4]
   moved = !__all_sync(0xffffffffu, same);
 }
 
-// o = o * a + vscale * V^T P^T; vs: the page's v [D][64] in shared memory. EDGE: tokens outside [lo, hi] have weight 0, but
-// their codes may stand for NaN.
+// o = o * a + vscale * V^T P^T; vs: the page's v [D][64] in shared memory. EDGE: some row does not see some token. Tokens
+// outside [lo, hi], what any row sees, may hold anything: their codes count as zero. Inside, a token that only some rows
+// see may hold NaN, which must not reach the others through 0 * NaN: its code counts as zero too, and true is returned.
 template <int D, int NT, bool EDGE>
-__device__ __forceinline__ void page_pv(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
+__device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
                                         int lo, int hi) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint32_t b[4][NT][2];
+  uint32_t b[4][NT][2], nan = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -267,6 +262,15 @@ __device__ __forceinline__ void page_pv(TileState<D, NT>& st, const uint32_t (&p
       b[i][n][0] = transpose_8x8(p[i][n][0]);
       b[i][n][1] = transpose_8x8(p[i][n][1]);
     }
+  uint32_t keep[4];   // bytes of the lane's tokens that some row sees
+  if (EDGE) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      keep[i] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) keep[i] |= (16 * t + 4 * i + k >= lo && 16 * t + 4 * i + k <= hi) ? 0xffu << (8 * k) : 0u;
+    }
+  }
   if (moved) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
@@ -288,8 +292,14 @@ __device__ __forceinline__ void page_pv(TileState<D, NT>& st, const uint32_t (&p
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (EDGE) {
-        u[i] = keep_tokens(u[i], 16 * t + 4 * i, lo, hi);
-        v[i] = keep_tokens(v[i], 16 * t + 4 * i, lo, hi);
+        auto tame = [&](uint32_t w) {   // code 0x7f or 0xff: NaN
+          w &= keep[i];
+          const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          nan |= bad;
+          return w & ~((bad >> 7) * 0xffu);
+        };
+        u[i] = tame(u[i]);
+        v[i] = tame(v[i]);
       }
       const uint32_t a0 = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu)), a2 = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
       const uint32_t a1 = fp8_to_half2(static_cast<uint16_t>(v[i] & 0xffffu)), a3 = fp8_to_half2(static_cast<uint16_t>(v[i] >> 16));
@@ -301,53 +311,35 @@ __device__ __forceinline__ void page_pv(TileState<D, NT>& st, const uint32_t (&p
 #pragma unroll
       for (int k = 0; k < 4; ++k) st.o[d][n][k] = fmaf(c[n][k], vscale, st.o[d][n][k]);
   }
+  return EDGE && __any_sync(0xffffffffu, nan != 0);
 }
 
-// A page that some row does not see all of. Tokens that no row sees (behind the sequence, or left of the window) may hold
-// anything: their codes count as zero. A token that only some rows see and that holds NaN must not reach the others
-// through 0 * NaN: such a page is multiplied once per distinct bound (rare: looked for in the codes).
+// The rows that see a NaN token of an edge page become NaN in its dimension.
 template <int D, int NT>
-__device__ __forceinline__ void page_pv_edge(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
-                                             const RowInfo<NT>& ri, int p0, int window) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int lo = window > 0 ? ri.first - window + 1 - p0 : 0, hi = ri.last - p0;   // what any row sees
-  bool nan = false;
-#pragma unroll 4
-  for (int n = 0; n < D / 8; ++n) {
-    const uint4 w = lds16(vs + static_cast<uint32_t>(8 * n + g) * ATTN_PAGE + 16 * t);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) nan |= has_nan_code(keep_tokens(u[i], 16 * t + 4 * i, lo, hi));
-  }
-  if (!__any_sync(0xffffffffu, nan)) {
-    page_pv<D, NT, true>(st, p, vs, a, moved, vscale, lo, hi);
-    return;
-  }
+__device__ __forceinline__ void page_nan(TileState<D, NT>& st, uint32_t vs, const RowInfo<NT>& ri, int p0, int window) {
+  const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll 1
-  for (int pos = ri.first; pos <= ri.last; ++pos) {   // rows at one position see the same tokens
-    uint32_t pr[4][NT][2];
-    float ar[NT][2];
+  for (int tok = 0; tok < ATTN_PAGE; ++tok) {
+    bool sees[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint32_t keep = (ri.there[n][0] && ri.pos[n][0] == pos ? 0xffffu : 0u) | (ri.there[n][1] && ri.pos[n][1] == pos ? 0xffff0000u : 0u);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pr[i][n][0] = p[i][n][0] & keep;
-        pr[i][n][1] = p[i][n][1] & keep;
-      }
-      ar[n][0] = pos == ri.first ? a[n][0] : 1.f;
-      ar[n][1] = pos == ri.first ? a[n][1] : 1.f;
-    }
-    // the other rows' weights are 0 here: NaN codes must not meet them either, so their sums are put back
-    const TileState<D, NT> was = st;
-    page_pv<D, NT, true>(st, pr, vs, ar, true, vscale, window > 0 ? pos - window + 1 - p0 : 0, pos - p0);
+      for (int c = 0; c < 2; ++c)
+        sees[n][c] = ri.there[n][c] && p0 + tok <= ri.pos[n][c] && (window <= 0 || p0 + tok > ri.pos[n][c] - window);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int x = 0; x < 2; ++x) {
+        uint32_t code;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(vs + static_cast<uint32_t>(16 * d + 8 * x + g) * ATTN_PAGE + tok));
+        if ((code & 0x7fu) == 0x7fu) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (!ri.there[n][k & 1] || ri.pos[n][k & 1] != pos) st.o[d][n][k] = was.o[d][n][k] * ar[n][k & 1];
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (sees[n][c]) st.o[d][n][2 * x + c] = __uint_as_float(0x7fffffffu);
+        }
+      }
   }
 }
 
@@ -355,14 +347,14 @@ __device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + __ex
 
 // Output values of accumulator quads o[d] (rows row, row + 1 of the entry's tile, dimensions 16 d + g and + 8 of a head).
 template <int N>
-__device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& en, int h, int group, int row, int d0, const float (&o)[N][4], const float (&inv)[2],
+__device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& en, int h, int row, int d0, const float (&o)[N][4], const float (&inv)[2],
                                             int D) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (row + c >= en.rows) continue;
-    const int rr = en.row0 + row + c, tk = rr / group;
+    const int rr = en.row0 + row + c, tk = div_group(a, rr);
     const size_t tok = en.first + tk;
-    const int col = (h * group + rr - tk * group) * D + d0;
+    const int col = (h * a.group + rr - tk * a.group) * D + d0;
     __nv_bfloat16* dst = a.out + tok * a.ld_out + col;
     unsigned short gt[N][2];
     if (a.gate) {   // all in flight before the first is used
@@ -389,7 +381,7 @@ __device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& 
 // A finished segment of a unit: the output rows themselves when it is the whole unit, else a partial slot. row0: the
 // warp's first row in the entry's tile of `rows` rows.
 template <int D, int NT>
-__device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, int group, bool whole, float* slot,
+__device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, bool whole, float* slot,
                                            int slot_rows) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -411,7 +403,7 @@ __device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs&
       for (int d = 0; d < D / 16; ++d)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[d][k] = st.o[d][n][k];
-      store_quads<D / 16>(a, en, h, group, row, g, o, inv, D);
+      store_quads<D / 16>(a, en, h, row, g, o, inv, D);
     } else {
       if (g == 0) {
         *reinterpret_cast<float2*>(slot + row) = make_float2(st.mx[n][0], st.mx[n][1]);
@@ -489,8 +481,9 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     fence_mbar_init();
   }
   if (tid == 0) s_abort = 0;
-  griddep_launch_dependents();
   griddep_wait();
+  // Only now: the kernel that adds up, when it comes in, may then take what was ready before this one as ready.
+  griddep_launch_dependents();
 
   // The list: every thread adds up the items of its share of the entries, a scan over the CTA gives the total and where
   // each share begins; the thread whose share holds a worker's first item finds the entry.
@@ -683,16 +676,16 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (fresh) {
       tile_reset(st);
       const int r0 = rd.en.row0 + wrow, t = lane & 3;
-      load_q<D, NT>(a, rd.en, rd.h, r0, my_rows, group, qf, qs);
+      load_q<D, NT>(a, rd.en, rd.h, r0, my_rows, qf, qs);
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           ri.there[k][c] = 8 * k + 2 * t + c < my_rows;
-          ri.pos[k][c] = rd.en.pos + (r0 + 8 * k + 2 * t + c) / group;
+          ri.pos[k][c] = rd.en.pos + div_group(a, r0 + 8 * k + 2 * t + c);
         }
-      ri.first = rd.en.pos + r0 / group;
-      ri.last = rd.en.pos + (r0 + my_rows - 1) / group;
+      ri.first = rd.en.pos + div_group(a, r0);
+      ri.last = rd.en.pos + div_group(a, r0 + max(my_rows, 1) - 1);
       fresh = false;
       seg_first = rd.i;
     }
@@ -722,8 +715,12 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (live) {
       const uint32_t vs = ring_base + static_cast<uint32_t>(vsl) * SLOT_BYTES;
       const float vscale = exp2_byte(rec.y >> 8);
-      if (edge) page_pv_edge<D, NT>(st, p, vs, al, moved, vscale, ri, p0, a.window);
-      else page_pv<D, NT, false>(st, p, vs, al, moved, vscale, 0, ATTN_PAGE - 1);
+      if (edge) {
+        if (page_pv<D, NT, true>(st, p, vs, al, moved, vscale, a.window > 0 ? ri.first - a.window + 1 - p0 : 0, ri.last - p0))
+          page_nan<D, NT>(st, vs, ri, p0, a.window);
+      } else {
+        page_pv<D, NT, false>(st, p, vs, al, moved, vscale, 0, ATTN_PAGE - 1);
+      }
     }
     release();
     ++n;
@@ -735,7 +732,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       // (a warp's ring is idle by now when it merges: its range ends with this segment)
       float* slot = merge ? reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * attn_slots(D) * SLOT_BYTES / 4
                           : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + 1)) * attn_slot_floats(D, TILE);
-      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, group, whole && !merge, slot, TILE);
+      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, whole && !merge, slot, TILE);
       fresh = true;
     }
     if (left > 0) {
@@ -768,14 +765,15 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   constexpr int STEP = DEEP ? 8 : 1, FLOATS = attn_slot_floats(D, TILE);
   __shared__ float s_m[STEP][8], s_l[STEP][8];
   __shared__ float4 s_o[STEP][32];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int entries = a.batch * a.tiles, group = a.hq / a.hk;
+  const int entries = a.batch * a.tiles, group = a.group;
   const int e = static_cast<int>(blockIdx.x) / a.hk, h = static_cast<int>(blockIdx.x) % a.hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int r0 = static_cast<int>(blockIdx.y) * 8, d = DEEP ? static_cast<int>(blockIdx.z) : warp;
-  const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
+  // Ready before the kernel ahead began to launch this one: the index tensors (and the gate).
   const AttnEntry en = attn_entry_of(a, e, group, TILE);
+  griddep_launch_dependents();
+  griddep_wait();
+  const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
   if (r0 >= en.rows) return;
   const AttnDeal deal = attn_deal(total, workers);
   const long long u0 = start + static_cast<long long>(h) * attn_items(en) + 1;
@@ -828,15 +826,10 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   }
   const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
   const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
-  store_quads<1>(a, en, h, group, row, 16 * d + g, quad, inv, D);
+  store_quads<1>(a, en, h, row, 16 * d + g, quad, inv, D);
 }
 
 // ---------------------------------------------------------------- host side
-static int attn_sms() {
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return v;
-}
 // The form a call takes goes by the rows a KV head has at most: 8 or 16 per warp, or 128 per CTA.
 struct AttnForm {
   bool shared;
@@ -853,7 +846,7 @@ static AttnForm attn_form(int max_q, int hq, int hk) {
 }
 
 long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
-  const int sms = attn_sms();
+  const int sms = device_sms();
   if (batch < 1 || max_q < 1 || hk < 1 || hq < hk || hq % hk || (dim != 64 && dim != 128) || sms < 1) return -1;
   const AttnForm f = attn_form(max_q, hq, hk);
   return 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile) * 4 + (static_cast<long long>(batch) * f.tiles + 1) * 8;
@@ -862,8 +855,11 @@ long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
 template <int D, int NT, bool SHARED>
 static cudaError_t attn_launch(const AttnArgs& a, const AttnForm& f, int sms, cudaStream_t stream) {
   const size_t smem = attn_ring_bytes(D);
-  cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static DeviceOnce once;
+  cudaError_t e = cudaSuccess;
+  if (once.first()) e = cudaFuncSetAttribute(cache_attn_kernel<D, NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
+  once.done();
   e = launch_dependent(cache_attn_kernel<D, NT, SHARED>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
   if (e != cudaSuccess) return e;
   const int all = a.max_q * (a.hq / a.hk), rows = all < f.tile ? all : f.tile;
@@ -885,10 +881,13 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(ws)) & 15) return -5;
   if ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 1) return -5;
   if (!a.cu_q && a.max_q != 1) return -6;
-  const int sms = attn_sms();
+  const int sms = device_sms();
   if (sms < 1) return -7;
   const AttnForm f = attn_form(a.max_q, a.hq, a.hk);
   a.tiles = f.tiles;
+  a.group = a.hq / a.hk;
+  a.group_magic = static_cast<uint32_t>((1ull << 32) / static_cast<unsigned>(a.group) + 1);
+  if (static_cast<long long>(f.tiles) * f.tile * a.group >= 1ll << 32) return -3;
   if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
   a.part = static_cast<float*>(ws);
   a.prefix = reinterpret_cast<long long*>(a.part + 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile));

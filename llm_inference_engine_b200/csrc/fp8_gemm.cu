@@ -354,15 +354,9 @@ struct G8Plan {
   int mt, nt, split, stages;
 };
 
-static int g8_sms() {
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return v;
-}
-
 // The tile and the K slices that make the longest CTA's traffic smallest: bytes it brings into shared memory, at
 // about 60 bytes per ns, against its MMAs, plus what a tile and a join cost.
-static G8Plan g8_plan(int m, int n, int k, int sms) {
+static G8Plan g8_search(int m, int n, int k, int sms) {
   const int kblocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
   G8Plan best = {};
   double best_ns = 1e30;
@@ -392,9 +386,21 @@ static G8Plan g8_plan(int m, int n, int k, int sms) {
   return best;
 }
 
+// The search takes microseconds; a thread's last shapes are kept.
+static G8Plan g8_plan(int m, int n, int k, int sms) {
+  struct Kept {
+    int m, n, k, sms;
+    G8Plan plan;
+  };
+  static thread_local Kept kept[64];
+  Kept& c = kept[(static_cast<unsigned>(m) * 31u + static_cast<unsigned>(n) * 7u + static_cast<unsigned>(k)) & 63u];
+  if (c.m != m || c.n != n || c.k != k || c.sms != sms) c = {m, n, k, sms, g8_search(m, n, k, sms)};
+  return c.plan;
+}
+
 long long fp8_gemm_ws_bytes(int m, int n, int k) {
   if (m < 1 || n < 1 || k < 16 || k % 16) return -1;
-  const int sms = g8_sms();
+  const int sms = device_sms();
   if (sms < 1) return -2;
   const G8Plan p = g8_plan(m, n, k, sms);
   return p.split > 1 ? static_cast<long long>(p.split) * m * n * 4 : 0;
@@ -402,8 +408,11 @@ long long fp8_gemm_ws_bytes(int m, int n, int k) {
 
 template <int MT>
 static cudaError_t g8_launch(const CUtensorMap& tx, const CUtensorMap& tw, const G8Args& a, int grid, size_t smem, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static DeviceOnce once;   // the largest any plan asks for, once
+  cudaError_t e = cudaSuccess;
+  if (once.first()) e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
   if (e != cudaSuccess) return e;
+  once.done();
   return launch_dependent(fp8_gemm_kernel<MT>, dim3(grid), dim3(G8_THREADS), smem, stream, tx, tw, a);
 }
 
@@ -413,7 +422,7 @@ int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void*
                       cudaStream_t stream) {
   if (!W || !we || !xq || !xe || !out || !status || m < 1 || n < 1 || k < 16 || k % 16) return -1;
   if (ld_out < n || ((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
-  const int sms = g8_sms();
+  const int sms = device_sms();
   if (sms < 1) return -4;
   const G8Plan p = g8_plan(m, n, k, sms);
   if (p.split > 1 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15))) return -3;

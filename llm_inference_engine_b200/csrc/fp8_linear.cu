@@ -163,12 +163,6 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
 }
 
 // ---------------------------------------------------------------- host side
-static int sm_count() {
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return v;
-}
-
 int fp8_quantize_dispatch(const void* x, void* xq, void* xe, int m, int K, int ld_x, cudaStream_t stream) {
   if (!x || !xq || !xe || m < 1 || K < 16 || K % 16) return -1;
   if (ld_x < K || ld_x % 8 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xq)) & 15)) return -2;
@@ -194,7 +188,7 @@ static cudaError_t fp8_walk_launch(const void* W, const void* we, const void* x,
 int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, cudaStream_t stream) {
   if (!W || !we || !x || !out || m < 1 || m > 16 || N < 1 || K < 16 || K % 16 || K > 8192) return -1;
   if (ld_x < K || ld_x % 8 || ld_out < N || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
-  const int sms = sm_count();
+  const int sms = device_sms();
   if (sms < 1) return -4;
   cudaError_t e;
   // 32 warps of 64 registers hold 16 bytes x 4 of W and up to 16 words of x per lane; longer rows of more tokens

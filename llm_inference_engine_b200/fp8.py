@@ -91,15 +91,44 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"x must have at least one row and a multiple of 16 columns, got {tuple(x.shape)}")
     dev = x.device
     with _capi.on_device(dev.index):
-        return _quantize(_rows(x, m, k), m, k, dev)
+        return _quantize(_rows(x, m, k), m, k, dev, dev.index)
 
 
-def _quantize(x, m, k, dev):
-    xq = torch.empty((m, k), device=dev, dtype=torch.float8_e4m3fn)
-    xe = torch.empty((m, -(-k // BLOCK)), device=dev, dtype=torch.uint8)
+def _quantize(x, m, k, dev, index):
+    kb = -(-k // BLOCK)
+    xq = _capi.new_tensor((m, k), (k, 1), torch.float8_e4m3fn, dev)
+    xe = _capi.new_tensor((m, kb), (kb, 1), torch.uint8, dev)
     _capi.check(_capi.load().muse_fp8_quantize(x.data_ptr(), xq.data_ptr(), xe.data_ptr(), m, k, x.stride(0) if m > 1 else k,
-                                               _capi.raw_stream(dev.index)), "muse_fp8_quantize")
+                                               _capi.raw_stream(index)), "muse_fp8_quantize")
     return xq, xe
+
+
+def _refuse_linear(x, w8, w_exp, out):
+    """Says what is wrong with the arguments that linear() does not take."""
+    if isinstance(x, (tuple, list)):
+        xq, xe = x
+        _require(xq, "x's codes", torch.float8_e4m3fn, 2)
+        _require(xe, "x's exponents", torch.uint8, 2)
+        m, k = xq.shape
+        if xe.shape != (m, -(-k // BLOCK)) or not xq.is_contiguous() or not xe.is_contiguous() or xq.data_ptr() % 16:
+            raise ValueError(f"x's codes {tuple(xq.shape)} and exponents {tuple(xe.shape)} must be contiguous, one exponent per 128 columns")
+    else:
+        _require(x, "x", torch.bfloat16, 2)
+        m, k = x.shape
+    _require(w8, "w8", torch.float8_e4m3fn, 2)
+    _require(w_exp, "w_exp", torch.uint8, 2)
+    n = w8.shape[0]
+    if w8.shape[1] != k or m < 1 or n < 1 or k < 16 or k % 16:
+        raise ValueError(f"x [{m}, {k}] and W {tuple(w8.shape)} do not fit, or K is not a multiple of 16")
+    if w_exp.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not w8.is_contiguous() or not w_exp.is_contiguous() or w8.data_ptr() % 16:
+        raise ValueError(f"w8 {tuple(w8.shape)} and w_exp {tuple(w_exp.shape)} must be contiguous, one exponent per 128 x 128 block")
+    if out is not None and (out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n or out.stride(1) != 1
+                            or (m > 1 and out.stride(0) < n)):
+        raise ValueError("out must be BF16 [m, >= N] with unit column stride")
+    raise ValueError("x, w8, w_exp and out must be on the same CUDA device")
+
+
+_F8, _BF16, _U8 = torch.float8_e4m3fn, torch.bfloat16, torch.uint8
 
 
 def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -107,51 +136,49 @@ def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = 
     [N, K] and exponent bytes of W, contiguous; K a multiple of 16. `out` (optional): BF16 [m, >= N] with unit column
     stride, of which the first N columns are written. Weights are static: what made them must be complete before the first
     call (kernels may read them ahead of the work before them in the stream)."""
+    # One expression takes what is right (the checks are a good part of a small call's time); what it does not take is
+    # looked at again to say why.
     pair = isinstance(x, (tuple, list))
-    if pair:
-        xq, xe = x
-        _require(xq, "x's codes", torch.float8_e4m3fn, 2)
-        _require(xe, "x's exponents", torch.uint8, 2)
-        m, k = xq.shape
-        if xe.shape != (m, -(-k // BLOCK)) or not xq.is_contiguous() or not xe.is_contiguous() or xq.data_ptr() % 16:
-            raise ValueError(f"x's codes {tuple(xq.shape)} and exponents {tuple(xe.shape)} must be contiguous, one exponent per 128 columns")
-        x_dev = xq.device
-        if xe.device != x_dev:
-            raise ValueError("x's codes and exponents must be on the same device")
-    else:
-        _require(x, "x", torch.bfloat16, 2)
-        m, k = x.shape
-        x_dev = x.device
-    _require(w8, "w8", torch.float8_e4m3fn, 2)
-    _require(w_exp, "w_exp", torch.uint8, 2)
-    n, kw = w8.shape
-    dev = w8.device
-    if kw != k or m < 1 or n < 1 or k < 16 or k % 16:
-        raise ValueError(f"x [{m}, {k}] and W {tuple(w8.shape)} do not fit, or K is not a multiple of 16")
-    if w_exp.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not w8.is_contiguous() or not w_exp.is_contiguous() or w8.data_ptr() % 16:
-        raise ValueError(f"w8 {tuple(w8.shape)} and w_exp {tuple(w_exp.shape)} must be contiguous, one exponent per 128 x 128 block")
-    if w_exp.device != dev or x_dev != dev:
-        raise ValueError("x, w8 and w_exp must be on the same device")
-    if out is not None and (out.device != dev or out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n
-                            or out.stride(1) != 1 or (m > 1 and out.stride(0) < n)):
-        raise ValueError("out must be BF16 [m, >= N] with unit column stride on W's device")
-    lib, index = _capi.load(), dev.index
+    xt = x[0] if pair else x
+    shape, w_shape, index = xt.shape, w8.shape, w8.get_device()
+    if len(shape) != 2 or len(w_shape) != 2:
+        _refuse_linear(x, w8, w_exp, out)
+    m, k = shape
+    n = w_shape[0]
+    kb = (k + 127) // 128
+    if not (m >= 1 and n >= 1 and k >= 16 and not k & 15 and w_shape[1] == k and index >= 0 and xt.get_device() == index
+            and w_exp.get_device() == index and w8.dtype is _F8 and w_exp.dtype is _U8 and w_exp.shape == ((n + 127) // 128, kb)
+            and w8.is_contiguous() and w_exp.is_contiguous() and not w8.data_ptr() & 15
+            and (xt.dtype is _BF16 if not pair else
+                 xt.dtype is _F8 and x[1].dtype is _U8 and x[1].shape == (m, kb) and xt.is_contiguous() and x[1].is_contiguous()
+                 and x[1].get_device() == index and not xt.data_ptr() & 15)):
+        _refuse_linear(x, w8, w_exp, out)
+    ld_out = n
+    if out is not None:
+        if (out.dtype is not _BF16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n or out.get_device() != index or out.stride(1) != 1
+                or (m > 1 and out.stride(0) < n)):
+            _refuse_linear(x, w8, w_exp, out)
+        if m > 1:
+            ld_out = out.stride(0)
+    lib, dev = _capi.load(), w8.device
     with _capi.on_device(index):
         if out is None:
-            out = torch.empty((m, n), device=dev, dtype=torch.bfloat16)
-            ld_out = n
-        else:
-            ld_out = out.stride(0) if m > 1 else n
+            out = _capi.new_tensor((m, n), (n, 1), _BF16, dev)
         if not pair:
             x = _rows(x, m, k)
             if m <= WALK_MAX_TOKENS and k <= WALK_MAX_K:
-                _capi.check(lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k,
-                                              x.stride(0) if m > 1 else k, ld_out, _capi.raw_stream(index)), "muse_fp8_walk")
+                rc = lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k, x.stride(0) if m > 1 else k, ld_out,
+                                       _capi.raw_stream(index))
+                if rc:
+                    _capi.check(rc, f"muse_fp8_walk(m={m}, n={n}, k={k})")
                 return out
-            xq, xe = _quantize(x, m, k, dev)
+            xq, xe = _quantize(x, m, k, dev, index)
+        else:
+            xq, xe = x
         size = _ws_bytes(index, m, n, k)
-        ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None   # the call's own: calls may overlap on the GPU
-        _capi.check(lib.muse_fp8_gemm(w8.data_ptr(), w_exp.data_ptr(), xq.data_ptr(), xe.data_ptr(), out.data_ptr(),
-                                      ws.data_ptr() if size else None, _capi.status_word(dev).data_ptr(), m, n, k, ld_out,
-                                      _capi.raw_stream(index)), "muse_fp8_gemm")
+        ws = _capi.new_tensor((size,), (1,), _U8, dev) if size else None   # the call's own: calls may overlap on the GPU
+        rc = lib.muse_fp8_gemm(w8.data_ptr(), w_exp.data_ptr(), xq.data_ptr(), xe.data_ptr(), out.data_ptr(), ws.data_ptr() if size else None,
+                               _capi.status_ptr(index), m, n, k, ld_out, _capi.raw_stream(index))
+    if rc:
+        _capi.check(rc, f"muse_fp8_gemm(m={m}, n={n}, k={k})")
     return out

@@ -455,7 +455,7 @@ def test_refusals(c8):
         (TypeError, dict(q=q.float())), (TypeError, dict(q=q[0])), (ValueError, dict(q=torch.zeros((2, 4, 128), device=DEV, dtype=torch.bfloat16))),
         (ValueError, dict(q=q[:, :3])), (ValueError, dict(q=q[:1])), (TypeError, dict(page_table=table.long())), (ValueError, dict(seq_lens=lens[:1])),
         (TypeError, dict(seq_lens=lens.cpu())), (ValueError, dict(cu_q=i32([0, 1]))), (ValueError, dict(max_q=2)), (ValueError, dict(max_q=0, cu_q=i32([0, 1, 2]))),
-        (ValueError, dict(window=-1)), (TypeError, dict(gate=q.flatten(1).float())), (TypeError, dict(gate=q.flatten(1)[:, :8])),
+        (ValueError, dict(window=-1)), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (TypeError, dict(gate=q.flatten(1).float())), (TypeError, dict(gate=q.flatten(1)[:, :8])),
         (ValueError, dict(out=torch.empty((256, 2), device=DEV, dtype=torch.bfloat16).T)),
         (ValueError, dict(cache=cache._replace(v=cache.v[:3]))), (TypeError, dict(cache=cache._replace(k=cache.k.view(torch.uint8)))),
         (ValueError, dict(cache=cache._replace(k_exp=cache.k_exp[:3]))),
