@@ -5,14 +5,15 @@
 // head in the group, cut into tiles of `tile` rows. An ENTRY is a (sequence, row tile); its rows see the tokens from
 // `lo` to `hi` (causal, window), that is `pages` pages from `page0`; an entry with rows that see nothing counts one
 // page, so that somebody writes its zeros. A UNIT is an entry's KV head. The units form one list, entry-major, then
-// head, of ITEMS: a head item, which stands for what a unit costs beside its pages (bringing in q, storing the
-// rows: about a page's time), and the unit's pages. The list is cut into equal ranges, one per worker; a unit whose pages
+// head, of ITEMS: ATTN_HEAD head items, which stand for what a unit costs beside its pages (bringing in q, the masked
+// last page, gate and output rows: two pages' time in a busy batch), and the unit's pages. The list is cut into equal ranges, one per worker; a unit whose pages
 // are split between workers leaves partial sums that a second kernel adds up in page order.
 #pragma once
 
 namespace muse {
 
 constexpr int ATTN_PAGE = 64;   // tokens per page
+constexpr int ATTN_HEAD = 2;    // head items of a unit
 
 struct AttnEntry {
   int first, n;      // rows of the batch that hold the sequence's new tokens
@@ -22,7 +23,7 @@ struct AttnEntry {
   int last;          // last position its rows see (-1: none)
 };
 // Items of a unit of the entry.
-__host__ __device__ inline int attn_items(const AttnEntry& e) { return e.pages > 0 ? e.pages + 1 : 0; }
+__host__ __device__ inline int attn_items(const AttnEntry& e) { return e.pages > 0 ? e.pages + ATTN_HEAD : 0; }
 
 // cu0, cu1: the sequence's bounds in the batch as the caller gave them; len: its tokens, the new ones included.
 __host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m, int max_q, int capacity, int group, int tile, int rt,

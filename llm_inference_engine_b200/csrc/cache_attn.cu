@@ -93,7 +93,7 @@ __device__ __forceinline__ AttnEntry attn_entry_cached(const AttnArgs& a, EntryC
                     a.width * ATTN_PAGE, group, tile, e % a.tiles, a.window);
 }
 
-// A place in the list: entry, head, i-th page of the unit (-1: the unit's head item).
+// A place in the list: entry, head, i-th page of the unit (below zero: the unit's head items).
 struct Cursor {
   AttnEntry en;
   int e, h, i;
@@ -563,13 +563,13 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     fill.en = attn_entry_cached(a, fill_cache, fill.e, entries, group, TILE);
     const int off = static_cast<int>(f0 - s_start[w]), per_unit = attn_items(fill.en);
     fill.h = off / per_unit;
-    fill.i = off % per_unit - 1;
+    fill.i = off % per_unit - ATTN_HEAD;
     unit0 = s_start[w] + static_cast<long long>(fill.h) * per_unit;
     rd_cache = fill_cache;
     rd = fill;
   }
   auto next_unit = [&](Cursor& c, EntryCache& ec) {   // false behind the last entry
-    c.i = -1;
+    c.i = -ATTN_HEAD;
     if (++c.h < a.hk) return true;
     c.h = 0;
     do {
@@ -585,8 +585,8 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   auto look_up = [&]() {
     int b = -1, h = 0, i = 0, off = 0;
     while (off < 32 && fill_left > 0) {
-      if (fill.i < 0) {   // the unit's head item
-        fill.i = 0;
+      if (fill.i < 0) {   // the unit's head items
+        ++fill.i;
         --fill_left;
         continue;
       }
@@ -663,12 +663,12 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   const int wrow = SHARED ? warp * WARP_ROWS : 0;   // this warp's first row in the worker's tile
   // All eight warps inside one unit: their sums meet in shared memory, and one slot leaves the CTA.
   const int w_first = worker - warp;
-  const bool merge = !SHARED && !spread && attn_merged(deal, w_first, ATTN_WARPS, unit0 + 1, unit0 + attn_items(rd.en));   // CTA-uniform
+  const bool merge = !SHARED && !spread && attn_merged(deal, w_first, ATTN_WARPS, unit0 + ATTN_HEAD, unit0 + attn_items(rd.en));   // CTA-uniform
   bool fresh = true;
   int seg_first = 0, left = items, n = 0;           // first page of the segment; items to go; pages done
   while (left > 0) {
-    if (rd.i < 0) {   // the unit's head item
-      rd.i = 0;
+    if (rd.i < 0) {   // the unit's head items
+      ++rd.i;
       --left;
       continue;
     }
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       const bool whole = unit_end && seg_first == 0;
       // (a warp's ring is idle by now when it merges: its range ends with this segment)
       float* slot = merge ? reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * attn_slots(D) * SLOT_BYTES / 4
-                          : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + 1)) * attn_slot_floats(D, TILE);
+                          : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + ATTN_HEAD)) * attn_slot_floats(D, TILE);
       tile_store<D, NT>(st, a, rd.en, rd.h, wrow, whole && !merge, slot, TILE);
       fresh = true;
     }
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
   if (r0 >= en.rows) return;
   const AttnDeal deal = attn_deal(total, workers);
-  const long long u0 = start + static_cast<long long>(h) * attn_items(en) + 1;
+  const long long u0 = start + static_cast<long long>(h) * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;   // one worker had all of the unit's pages and has written it
   const AttnParts ps = attn_parts(deal, TILE > 16 || total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
   const int row = r0 + 2 * t;
@@ -939,7 +939,7 @@ long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch
         start += static_cast<long long>(attn_items(en)) * hk;
         en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, ++e);
       }
-      const int off = static_cast<int>(f - start), h = off / attn_items(en), i = off % attn_items(en) - 1;
+      const int off = static_cast<int>(f - start), h = off / attn_items(en), i = off % attn_items(en) - ATTN_HEAD;
       if (i < 0) {
         ++f;
         continue;
@@ -948,7 +948,7 @@ long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch
       if (count < capacity) {
         int* s = segments + 6 * count;
         s[0] = w; s[1] = e; s[2] = h; s[3] = en.page0 + i; s[4] = n;
-        const long long u0 = start + static_cast<long long>(h) * attn_items(en) + 1;
+        const long long u0 = start + static_cast<long long>(h) * attn_items(en) + ATTN_HEAD;
         const int per = p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, first = w - w % per;
         s[5] = n == en.pages ? -1 : attn_merged(deal, first, per, u0, u0 + en.pages) ? 2 * first : attn_slot_of(deal, w, u0);
       }
@@ -971,7 +971,7 @@ long long cache_attn_join(const int* seq_lens, const int* cu_q, int m, int batch
   const AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, entry);
   if (en.rows == 0) return 0;
   const AttnDeal deal = attn_deal(p.total, p.form.workers(sms));
-  const long long u0 = before + static_cast<long long>(head) * attn_items(en) + 1;
+  const long long u0 = before + static_cast<long long>(head) * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return 0;
   const AttnParts ps = attn_parts(deal, p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, u0, en.pages);
   for (int i = 0; i < ps.parts && i < capacity; ++i) slots[i] = attn_part_slot(ps, i);

@@ -65,24 +65,31 @@ __device__ __forceinline__ Unit unit_of(int u, int rot, int interleaved) {
   d.hi = d.turns && !interleaved ? rot / 2 + 8 * u : 16 * u + 8;
   return d;
 }
-__device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const float* cs, int u, int interleaved) {
-  const float4* t = reinterpret_cast<const float4*>(cs + 16 * u);   // 8 pairs of (cos, sin)
+// cos and sin of a unit's 8 pairs.
+struct Turn {
+  float4 w[4];
+  __device__ __forceinline__ void load(const float* cs, int u) {
+    const float4* t = reinterpret_cast<const float4*>(cs + 16 * u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 w = __ldg(t + i);   // the table is as static as a weight
-    const float c[2] = {w.x, w.z}, n[2] = {w.y, w.w};
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(t + i);   // the table is as static as a weight
+  }
+  __device__ __forceinline__ void apply(float (&a)[8], float (&b)[8], int interleaved) const {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int p = 2 * i + j;   // pair p of the unit
-      float& x = interleaved ? (p < 4 ? a[(2 * p) & 7] : b[(2 * p) & 7]) : a[p];
-      float& y = interleaved ? (p < 4 ? a[(2 * p + 1) & 7] : b[(2 * p + 1) & 7]) : b[p];
-      const float x1 = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, n[j]));
-      const float y1 = __fadd_rn(__fmul_rn(y, c[j]), __fmul_rn(x, n[j]));
-      x = x1;
-      y = y1;
+    for (int i = 0; i < 4; ++i) {
+      const float c[2] = {w[i].x, w[i].z}, n[2] = {w[i].y, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int p = 2 * i + j;   // pair p of the unit
+        float& x = interleaved ? (p < 4 ? a[(2 * p) & 7] : b[(2 * p) & 7]) : a[p];
+        float& y = interleaved ? (p < 4 ? a[(2 * p + 1) & 7] : b[(2 * p + 1) & 7]) : b[p];
+        const float x1 = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, n[j]));
+        const float y1 = __fadd_rn(__fmul_rn(y, c[j]), __fmul_rn(x, n[j]));
+        x = x1;
+        y = y1;
+      }
     }
   }
-}
+};
 
 __device__ __forceinline__ float block_max(float v, float* s, int threads) {
 #pragma unroll
@@ -113,28 +120,47 @@ __global__ void __launch_bounds__(THREADS) rope_append_kernel(const __grid_const
   const int tid = threadIdx.x;
   const int capacity = a.width * PAGE_TOKENS;
   if (static_cast<int>(blockIdx.x) >= kv_ctas) {   // ---- q
+    // A thread turns one unit of up to QH heads of a token, with the unit's 8 pairs of cos and sin in registers.
+    constexpr int QH = THREADS > 64 ? 4 : 1;
     const int i = static_cast<int>(blockIdx.x) - kv_ctas, b = i / q_ctas_per_seq;
     const SeqSpan s = seq_span(a.cu_q, a.seq_lens, b, a.m, a.max_q, capacity, a.status);
-    const long long items = static_cast<long long>(s.n) * a.hq * UPR;
-    for (long long it = static_cast<long long>(i % q_ctas_per_seq) * THREADS + tid; it < items; it += static_cast<long long>(q_ctas_per_seq) * THREADS) {
-      const int u = static_cast<int>(it % UPR), h = static_cast<int>(it / UPR % a.hq), j = static_cast<int>(it / (UPR * a.hq));
-      const int pos = s.pos + j;
+    const uint32_t hgroups = static_cast<uint32_t>((a.hq + QH - 1) / QH), items = static_cast<uint32_t>(s.n) * hgroups * UPR;
+    for (uint32_t it = static_cast<uint32_t>(i % q_ctas_per_seq) * THREADS + tid; it < items; it += static_cast<uint32_t>(q_ctas_per_seq) * THREADS) {
+      const uint32_t u = it % UPR, row_g = it / UPR, j = row_g / hgroups, hg = row_g - j * hgroups;
+      const int pos = s.pos + static_cast<int>(j), h0 = static_cast<int>(hg) * QH;
       const size_t row = s.first + j;
-      const Unit d = unit_of(u, a.rot, a.interleaved);
-      __nv_bfloat16* o = a.q_out + (row * a.hq + h) * D;
+      const Unit d = unit_of(static_cast<int>(u), a.rot, a.interleaved);
       const bool in = pos >= 0 && pos < capacity;   // a token that is in no page leaves zeros
-      float x[8] = {}, y[8] = {};
-      if (in) {
-        const __nv_bfloat16* src = a.qkv + row * a.ld_qkv + static_cast<size_t>(h) * D;
-        unpack8(__ldcg(reinterpret_cast<const uint4*>(src + d.lo)), x);
-        unpack8(__ldcg(reinterpret_cast<const uint4*>(src + d.hi)), y);
-        if (d.turns) rotate(x, y, a.cos_sin + static_cast<size_t>(pos) * a.rot, u, a.interleaved);
+      const __nv_bfloat16* src = a.qkv + row * a.ld_qkv + static_cast<size_t>(h0) * D;
+      __nv_bfloat16* o = a.q_out + (row * a.hq + h0) * D;
+      uint4 r0[QH], r1[QH];
+#pragma unroll
+      for (int h = 0; h < QH; ++h)
+        if (in && h0 + h < a.hq) {
+          r0[h] = __ldcg(reinterpret_cast<const uint4*>(src + h * D + d.lo));
+          r1[h] = __ldcg(reinterpret_cast<const uint4*>(src + h * D + d.hi));
+        } else {
+          r0[h] = r1[h] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      Turn turn;
+      if (in && d.turns) turn.load(a.cos_sin + static_cast<size_t>(pos) * a.rot, static_cast<int>(u));
+#pragma unroll
+      for (int h = 0; h < QH; ++h) {
+        if (h0 + h >= a.hq) break;
+        if (in && d.turns) {
+          float x[8], y[8];
+          unpack8(r0[h], x);
+          unpack8(r1[h], y);
+          turn.apply(x, y, a.interleaved);
+          r0[h] = pack8(x);
+          r1[h] = pack8(y);
+        }
+        *reinterpret_cast<uint4*>(o + h * D + d.lo) = r0[h];
+        *reinterpret_cast<uint4*>(o + h * D + d.hi) = r1[h];
       }
-      *reinterpret_cast<uint4*>(o + d.lo) = pack8(x);
-      *reinterpret_cast<uint4*>(o + d.hi) = pack8(y);
       if (!in && a.k_val) {
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        for (int kh = h; kh < a.hk; kh += a.hq) {
+        for (int kh = static_cast<int>(hg); kh < a.hk; kh += static_cast<int>(hgroups)) {
           const size_t at = (row * a.hk + kh) * D;
           *reinterpret_cast<uint4*>(a.k_val + at + d.lo) = zero;
           *reinterpret_cast<uint4*>(a.k_val + at + d.hi) = zero;
@@ -147,7 +173,7 @@ __global__ void __launch_bounds__(THREADS) rope_append_kernel(const __grid_const
   }
   // ---- one page of one sequence, one head: k and v
   __shared__ float s_red[2][THREADS / 32];
-  __shared__ __align__(16) uint8_t s_t[D][PAGE_TOKENS];   // a full page of v, turned
+  __shared__ uint32_t s_t[D][PAGE_TOKENS / 4];   // a full page of v, turned
   const int h = static_cast<int>(blockIdx.x) % a.hk, i = static_cast<int>(blockIdx.x) / a.hk, b = i / reach;
   const SeqSpan s = seq_span(a.cu_q, a.seq_lens, b, a.m, a.max_q, capacity, a.status);
   const int first_pos = max(s.pos, 0), end_pos = min(s.pos + s.n, capacity);
@@ -179,7 +205,11 @@ __global__ void __launch_bounds__(THREADS) rope_append_kernel(const __grid_const
       const uint4 r0 = __ldcg(reinterpret_cast<const uint4*>(src + d.lo)), r1 = __ldcg(reinterpret_cast<const uint4*>(src + d.hi));
       const uint4 r2 = __ldcg(reinterpret_cast<const uint4*>(vsrc)), r3 = __ldcg(reinterpret_cast<const uint4*>(vsrc + 8));
       unpack8(r0, kx[w]); unpack8(r1, ky[w]); unpack8(r2, vx[w]); unpack8(r3, vy[w]);
-      if (d.turns) rotate(kx[w], ky[w], a.cos_sin + static_cast<size_t>(pos) * a.rot, u, a.interleaved);
+      if (d.turns) {
+        Turn turn;
+        turn.load(a.cos_sin + static_cast<size_t>(pos) * a.rot, u);
+        turn.apply(kx[w], ky[w], a.interleaved);
+      }
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         kmax = fmaxf(kmax, fmaxf(finite_abs(kx[w][c]), finite_abs(ky[w][c])));
@@ -239,11 +269,32 @@ __global__ void __launch_bounds__(THREADS) rope_append_kernel(const __grid_const
       uint8_t* kr = kp + static_cast<size_t>(slot0 + r) * D;
       *reinterpret_cast<uint2*>(kr + d.lo) = make_uint2(q[0], q[1]);
       *reinterpret_cast<uint2*>(kr + d.hi) = make_uint2(q[2], q[3]);
+      if (!full) {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint8_t code = static_cast<uint8_t>(q[4 + c / 4] >> (8 * (c & 3)));
-        if (full) s_t[16 * u + c][r] = code;
-        else vp[(16 * u + c) * PAGE_TOKENS + slot0 + r] = code;
+        for (int c = 0; c < 16; ++c) vp[(16 * u + c) * PAGE_TOKENS + slot0 + r] = static_cast<uint8_t>(q[4 + c / 4] >> (8 * (c & 3)));
+      } else {
+        // A full page fills every thread's units (n UPR = THREADS U or a divisor): the four lanes that hold four
+        // neighbouring tokens of the same 16 dimensions swap words, so that each then has four tokens of four dimensions.
+        uint32_t m[4];
+        const int me = (tid / UPR) & 3;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {   // step c: send the word of lane me ^ c, take mine from it
+          const int other = me ^ c;
+          const uint32_t send = other == 0 ? q[4] : other == 1 ? q[5] : other == 2 ? q[6] : q[7];
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, send, c * UPR);
+          if (other == 0) m[0] = got;
+          if (other == 1) m[1] = got;
+          if (other == 2) m[2] = got;
+          if (other == 3) m[3] = got;
+        }
+        const uint32_t a01 = __byte_perm(m[0], m[1], 0x5140), a23 = __byte_perm(m[2], m[3], 0x5140);   // dimensions 0, 1 of tokens 0, 1 / 2, 3
+        const uint32_t b01 = __byte_perm(m[0], m[1], 0x7362), b23 = __byte_perm(m[2], m[3], 0x7362);   // dimensions 2, 3
+        const uint32_t t4[4] = {__byte_perm(a01, a23, 0x5410), __byte_perm(a01, a23, 0x7632), __byte_perm(b01, b23, 0x5410), __byte_perm(b01, b23, 0x7632)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int dim = 16 * u + 4 * me + c;
+          s_t[dim][(r / 4) ^ ((dim >> 2) & 15)] = t4[c];   // words of a row swizzled: two lanes per bank
+        }
       }
       if (a.k_val) {
         const size_t at = (static_cast<size_t>(s.first + p0 - s.pos + r) * a.hk + h) * D;
@@ -264,8 +315,10 @@ __global__ void __launch_bounds__(THREADS) rope_append_kernel(const __grid_const
   }
   if (full) {
     __syncthreads();
-    for (int it = tid; it < D * PAGE_TOKENS / 16; it += THREADS)
-      reinterpret_cast<uint4*>(vp)[it] = reinterpret_cast<const uint4*>(&s_t[0][0])[it];
+    for (int it = tid; it < D * PAGE_TOKENS / 4; it += THREADS) {
+      const int dim = it / (PAGE_TOKENS / 4), w = it % (PAGE_TOKENS / 4);
+      reinterpret_cast<uint32_t*>(vp)[it] = s_t[dim][w ^ ((dim >> 2) & 15)];
+    }
   }
 }
 
@@ -273,8 +326,9 @@ template <int D, int THREADS, int U>
 static cudaError_t rope_launch(const RopeArgs& a, cudaStream_t stream) {
   const int reach = (a.max_q + PAGE_TOKENS - 2) / PAGE_TOKENS + 1;   // pages that max_q neighbouring tokens can touch
   const long long kv = static_cast<long long>(a.batch) * reach * a.hk;
-  const long long per = (static_cast<long long>(a.max_q) * a.hq * (D / 16) + THREADS - 1) / THREADS;
-  if (kv + per * a.batch > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  const int qh = THREADS > 64 ? 4 : 1;
+  const long long items = static_cast<long long>(a.max_q) * ((a.hq + qh - 1) / qh) * (D / 16), per = (items + THREADS - 1) / THREADS;
+  if (kv + per * a.batch > 0x7fffffffll || items > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   return launch_dependent(rope_append_kernel<D, THREADS, U>, dim3(static_cast<unsigned>(kv + per * a.batch)), dim3(THREADS), 0, stream, a,
                           static_cast<int>(kv), reach, static_cast<int>(per));
 }

@@ -105,8 +105,8 @@ def test_every_page_is_read_once_and_joined_in_order(case):
             assert in_order == join(*key) and all(s >= 0 for s in in_order)
         for _, count, w, _ in parts:
             share[w] += count
-    # equal shares of pages plus one head item per unit: no worker has more than its share, a segment's head item counted
-    items = sum(len(pages) + 1 for pages in want.values())
+    # equal shares of items, a unit's pages and its two head items: no worker has more pages than its share of items
+    items = sum(len(pages) + 2 for pages in want.values())
     assert all(share[w] <= -(-items // workers) for w in range(workers))
     assert sum(share) == sum(len(pages) for pages in want.values())
 
