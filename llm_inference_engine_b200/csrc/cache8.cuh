@@ -45,6 +45,7 @@ struct AttnArgs {
   float scale_log2;            // softmax scale * log2(e)
   int m, batch, width, pages, max_q, hq, hk, window, tiles;   // tiles: row tiles per sequence
   int group;                   // hq / hk
+  int vec_gate, vec_out;       // 16-byte vectors of gate and out are aligned
   uint32_t group_magic;        // 2^32 / group + 1: a row's token without a division
 };
 

@@ -247,12 +247,13 @@ __device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4]
   moved = !__all_sync(0xffffffffu, same);
 }
 
-// o = o * a + vscale * V^T P^T; vs: the page's v [D][64] in shared memory. EDGE: some row does not see some token. Tokens
+// o = o * a + vscale * V^T P^T; vs: the page's v [D][64] in shared memory. edge: some row does not see some token. Tokens
 // outside [lo, hi], what any row sees, may hold anything: their codes count as zero. Inside, a token that only some rows
 // see may hold NaN, which must not reach the others through 0 * NaN: its code counts as zero too, and true is returned.
-template <int D, int NT, bool EDGE>
+// One body for both kinds of page: a second one would have to come through the instruction cache at every unit's end.
+template <int D, int NT>
 __device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p)[4][NT][2], uint32_t vs, const float (&a)[NT][2], bool moved, float vscale,
-                                        int lo, int hi) {
+                                        bool edge, int lo, int hi) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint32_t b[4][NT][2], nan = 0;
 #pragma unroll
@@ -263,12 +264,12 @@ __device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p
       b[i][n][1] = transpose_8x8(p[i][n][1]);
     }
   uint32_t keep[4];   // bytes of the lane's tokens that some row sees
-  if (EDGE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      keep[i] = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) keep[i] |= (16 * t + 4 * i + k >= lo && 16 * t + 4 * i + k <= hi) ? 0xffu << (8 * k) : 0u;
+  for (int i = 0; i < 4; ++i) {
+    keep[i] = 0xffffffffu;
+    if (edge) {
+      const int from = max(lo - (16 * t + 4 * i), 0), to = min(hi - (16 * t + 4 * i), 3);
+      keep[i] = from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
     }
   }
   if (moved) {
@@ -289,9 +290,9 @@ __device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p
     float c[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+    if (edge) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (EDGE) {
+      for (int i = 0; i < 4; ++i) {
         auto tame = [&](uint32_t w) {   // code 0x7f or 0xff: NaN
           w &= keep[i];
           const uint32_t bad = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -301,6 +302,9 @@ __device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p
         u[i] = tame(u[i]);
         v[i] = tame(v[i]);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       const uint32_t a0 = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu)), a2 = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
       const uint32_t a1 = fp8_to_half2(static_cast<uint16_t>(v[i] & 0xffffu)), a3 = fp8_to_half2(static_cast<uint16_t>(v[i] >> 16));
 #pragma unroll
@@ -311,7 +315,7 @@ __device__ __forceinline__ bool page_pv(TileState<D, NT>& st, const uint32_t (&p
 #pragma unroll
       for (int k = 0; k < 4; ++k) st.o[d][n][k] = fmaf(c[n][k], vscale, st.o[d][n][k]);
   }
-  return EDGE && __any_sync(0xffffffffu, nan != 0);
+  return edge && __any_sync(0xffffffffu, nan != 0);
 }
 
 // The rows that see a NaN token of an edge page become NaN in its dimension.
@@ -349,28 +353,33 @@ __device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + __ex
 template <int N>
 __device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& en, int h, int row, int d0, const float (&o)[N][4], const float (&inv)[2],
                                             int D) {
+  size_t tok[2];
+  int col[2];
+  unsigned short gt[2][N][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {   // the gates of both rows are in flight before the first is used
+    const int rr = en.row0 + min(row + c, en.rows - 1), tk = div_group(a, rr);
+    tok[c] = en.first + tk;
+    col[c] = (h * a.group + rr - tk * a.group) * D + d0;
+    if (a.gate) {
+      const unsigned short* g = reinterpret_cast<const unsigned short*>(a.gate + tok[c] * a.ld_gate + col[c]);
+#pragma unroll
+      for (int d = 0; d < N; ++d) {
+        gt[c][d][0] = __ldcg(g + 16 * d);
+        gt[c][d][1] = __ldcg(g + 16 * d + 8);
+      }
+    }
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (row + c >= en.rows) continue;
-    const int rr = en.row0 + row + c, tk = div_group(a, rr);
-    const size_t tok = en.first + tk;
-    const int col = (h * a.group + rr - tk * a.group) * D + d0;
-    __nv_bfloat16* dst = a.out + tok * a.ld_out + col;
-    unsigned short gt[N][2];
-    if (a.gate) {   // all in flight before the first is used
-      const unsigned short* g = reinterpret_cast<const unsigned short*>(a.gate + tok * a.ld_gate + col);
-#pragma unroll
-      for (int d = 0; d < N; ++d) {
-        gt[d][0] = __ldcg(g + 16 * d);
-        gt[d][1] = __ldcg(g + 16 * d + 8);
-      }
-    }
+    __nv_bfloat16* dst = a.out + tok[c] * a.ld_out + col[c];
 #pragma unroll
     for (int d = 0; d < N; ++d) {
       float x = o[d][c] * inv[c], y = o[d][2 + c] * inv[c];
       if (a.gate) {
-        x *= sigmoid_f32(bf16lo_f32(gt[d][0]));
-        y *= sigmoid_f32(bf16lo_f32(gt[d][1]));
+        x *= sigmoid_f32(bf16lo_f32(gt[c][d][0]));
+        y *= sigmoid_f32(bf16lo_f32(gt[c][d][1]));
       }
       dst[16 * d] = __float2bfloat16_rn(x);
       dst[16 * d + 8] = __float2bfloat16_rn(y);
@@ -378,11 +387,52 @@ __device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& 
   }
 }
 
+constexpr int STAGE_LD = 68;   // floats of a staged row of 64 dimensions: rows four banks apart
+// Eight neighbouring output values from shared memory, gated.
+__device__ __forceinline__ void store8(const AttnArgs& a, size_t tok, int col, const float* s) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(s + i);
+    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+  }
+  if (a.gate) {
+    const __nv_bfloat16* g = a.gate + tok * a.ld_gate + col;
+    uint32_t w[4];
+    if (a.vec_gate) {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(g));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __ldcg(p + 2 * i) | static_cast<uint32_t>(__ldcg(p + 2 * i + 1)) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] *= sigmoid_f32(bf16lo_f32(w[i]));
+      x[2 * i + 1] *= sigmoid_f32(bf16hi_f32(w[i]));
+    }
+  }
+  __nv_bfloat16* o = a.out + tok * a.ld_out + col;
+  if (a.vec_out) {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      p[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(o) = make_uint4(p[0], p[1], p[2], p[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(x[i]);
+  }
+}
+
 // A finished segment of a unit: the output rows themselves when it is the whole unit, else a partial slot. row0: the
 // warp's first row in the entry's tile of `rows` rows.
 template <int D, int NT>
 __device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, bool whole, float* slot,
-                                           int slot_rows) {
+                                           int slot_rows, float* stage) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -398,12 +448,26 @@ __device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs&
     if (row0 + 8 * n >= en.rows) continue;   // warp-uniform
     if (whole) {
       const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};   // no token seen: the row is zero
-      float o[D / 16][4];
+      // Through shared memory, 64 dimensions at a time, and out in a loop: written out for every accumulator these lines
+      // were 10 KB of code that each unit's end had to bring in (6 us of a busy batch; this is 1).
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d)
+      for (int half = 0; half < D / 64; ++half) {
+        __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[d][k] = st.o[d][n][k];
-      store_quads<D / 16>(a, en, h, row, g, o, inv, D);
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            stage[(2 * t + (k & 1)) * STAGE_LD + 16 * d + 8 * (k >> 1) + g] = st.o[4 * half + d][n][k] * inv[k & 1];
+        __syncwarp();
+        const int here = min(8, en.rows - (row0 + 8 * n));
+#pragma unroll 1
+        for (int it = lane; it < here * 8; it += 32) {
+          const int r = it >> 3, c = (it & 7) * 8, rr = en.row0 + row0 + 8 * n + r, tk = div_group(a, rr);
+          const size_t tok = en.first + tk;
+          const int col = (h * a.group + rr - tk * a.group) * D + 64 * half + c;
+          store8(a, tok, col, stage + r * STAGE_LD + c);
+        }
+      }
     } else {
       if (g == 0) {
         *reinterpret_cast<float2*>(slot + row) = make_float2(st.mx[n][0], st.mx[n][1]);
@@ -468,6 +532,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   __shared__ long long s_sum[ATTN_WARPS];
   __shared__ int s_entry[ATTN_WARPS];
   __shared__ long long s_start[ATTN_WARPS];
+  __shared__ __align__(16) float s_stage[ATTN_WARPS][8 * STAGE_LD];   // rows on their way out
   __shared__ int2 s_rec[ATTN_WARPS][64];   // looked-up pages: tile index in the pool, exponents (k | v << 8)
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -660,6 +725,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   uint32_t qf[NT][D / 16][2];
   float qs[NT][2];
   RowInfo<NT> ri;
+  float* const stage = s_stage[warp];
   const int wrow = SHARED ? warp * WARP_ROWS : 0;   // this warp's first row in the worker's tile
   // All eight warps inside one unit: their sums meet in shared memory, and one slot leaves the CTA.
   const int w_first = worker - warp;
@@ -677,6 +743,14 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       tile_reset(st);
       const int r0 = rd.en.row0 + wrow, t = lane & 3;
       load_q<D, NT>(a, rd.en, rd.h, r0, my_rows, qf, qs);
+      if (a.gate && (lane & 3) == 0 && (lane >> 2) < my_rows) {   // on its way to L2 while the pages are worked on
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          const int rr = r0 + 8 * k + (lane >> 2), tk = div_group(a, rr);
+          if (8 * k + (lane >> 2) < my_rows)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a.gate + (rd.en.first + tk) * a.ld_gate + static_cast<size_t>(rd.h * a.group + rr - tk * a.group) * D));
+        }
+      }
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
@@ -715,12 +789,8 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (live) {
       const uint32_t vs = ring_base + static_cast<uint32_t>(vsl) * SLOT_BYTES;
       const float vscale = exp2_byte(rec.y >> 8);
-      if (edge) {
-        if (page_pv<D, NT, true>(st, p, vs, al, moved, vscale, a.window > 0 ? ri.first - a.window + 1 - p0 : 0, ri.last - p0))
-          page_nan<D, NT>(st, vs, ri, p0, a.window);
-      } else {
-        page_pv<D, NT, false>(st, p, vs, al, moved, vscale, 0, ATTN_PAGE - 1);
-      }
+      if (page_pv<D, NT>(st, p, vs, al, moved, vscale, edge, a.window > 0 ? ri.first - a.window + 1 - p0 : 0, ri.last - p0))
+        page_nan<D, NT>(st, vs, ri, p0, a.window);
     }
     release();
     ++n;
@@ -732,7 +802,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       // (a warp's ring is idle by now when it merges: its range ends with this segment)
       float* slot = merge ? reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * attn_slots(D) * SLOT_BYTES / 4
                           : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + ATTN_HEAD)) * attn_slot_floats(D, TILE);
-      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, whole && !merge, slot, TILE);
+      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, whole && !merge, slot, TILE, stage);
       fresh = true;
     }
     if (left > 0) {
@@ -886,6 +956,8 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   const AttnForm f = attn_form(a.max_q, a.hq, a.hk);
   a.tiles = f.tiles;
   a.group = a.hq / a.hk;
+  a.vec_gate = a.ld_gate % 8 == 0 && (reinterpret_cast<uintptr_t>(a.gate) & 15) == 0;
+  a.vec_out = a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   a.group_magic = static_cast<uint32_t>((1ull << 32) / static_cast<unsigned>(a.group) + 1);
   if (static_cast<long long>(f.tiles) * f.tile * a.group >= 1ll << 32) return -3;
   if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;

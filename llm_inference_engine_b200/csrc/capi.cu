@@ -412,7 +412,7 @@ int muse_cache_attention(const void* q, const void* k, const void* v, const void
                             static_cast<const uint8_t*>(k_exp), static_cast<const uint8_t*>(v_exp), static_cast<const int*>(page_table),
                             static_cast<const int*>(seq_lens), static_cast<const int*>(cu_q), static_cast<const bf16*>(gate),
                             static_cast<bf16*>(out), nullptr, nullptr, static_cast<int*>(status), ld_q, ld_gate, ld_out,
-                            scale * 1.44269504f, m, batch, width, pages, max_q, hq, hk, window, 0, 0, 0};
+                            scale * 1.44269504f, m, batch, width, pages, max_q, hq, hk, window, 0, 0, 0, 0, 0};
   return muse::cache_attn_dispatch(a, dim, ws, static_cast<cudaStream_t>(stream));
 }
 
