@@ -354,7 +354,9 @@ int muse_skinny_tc_noalloc(const void* tmap_w, const void* tmap_w_lo, const void
  * in the reference, whose weights are BF16. */
 /* x BF16 [m, K] (ld_x elements between rows, ld_x % 8 == 0) to codes xq [m, K] and exponent bytes xe. */
 int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x, void* stream);
-/* 1 .. 16 tokens, K <= 8192: x in BF16, quantised on the way; one launch. */
+#define MUSE_FP8_WALK_TOKENS 16
+#define MUSE_FP8_WALK_K 8192
+/* 1 .. MUSE_FP8_WALK_TOKENS tokens, K <= MUSE_FP8_WALK_K: x in BF16, quantised on the way; one launch. */
 int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream);
 
 /* Any number of tokens, x already in 8 bits: TMA and block-scaled tcgen05 MMAs. ws: muse_fp8_gemm_ws_bytes bytes (0: may be NULL), 16-byte aligned,

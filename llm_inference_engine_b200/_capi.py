@@ -110,6 +110,31 @@ def load(build_if_missing: bool = True):
     return lib
 
 
+_BIND = None
+
+
+def bind():
+    """The torch-side binding of the 8-bit operators (csrc/bind.cpp): their ordinary calls in one step. Built with the
+    library; like it, loading raises where it is missing and cannot be built."""
+    global _BIND
+    if _BIND is None:
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_loader
+
+        lib = load()
+        path = str(_build.build_bind() if not _build.BIND_PATH.exists() else _build.BIND_PATH)
+        loader = ExtensionFileLoader("_bind", path)
+        module = module_from_spec(spec_from_loader("_bind", loader))
+        loader.exec_module(module)
+        module.set_entries(*[C.cast(getattr(lib, f"muse_{name}"), C.c_void_p).value
+                             for name in ("fp8_walk", "fp8_quantize", "fp8_gemm", "fp8_gemm_ws_bytes", "rope_append", "cache_attention",
+                                          "cache_attention_ws_bytes")])
+        for index, word in _STATUS.items():
+            module.set_status(index, word.data_ptr())
+        _BIND = module
+    return _BIND
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         kind = "rejected argument" if rc < 0 else "CUDA error"
@@ -157,6 +182,7 @@ def status_ptr(index: int) -> int:
         if torch.cuda.is_current_stream_capturing():   # it must outlive the graph
             raise MuseError("the first call of the 8-bit operators on a device makes their status word: make it outside stream capture")
         word = _STATUS[index] = torch.zeros(1, device=torch.device("cuda", index), dtype=torch.int32)
+        bind().set_status(index, word.data_ptr())
     return word.data_ptr()
 
 

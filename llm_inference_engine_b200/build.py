@@ -21,6 +21,9 @@ CSRC = PKG_DIR / "csrc"
 TRACE = bool(os.environ.get("MUSE_TRACE"))
 LIB_PATH = PKG_DIR / ("libmuse_proj_trace.so" if TRACE else "libmuse_proj.so")
 SOURCES = ["gemv1.cu", "fewtok_mma.cu", "fewtok_zip.cu", "ffn_boundary.cu", "skinny_tc.cu", "gemm_tc.cu", "fp8_linear.cu", "fp8_gemm.cu", "rope_append.cu", "cache_attn.cu", "capi.cu"]
+# The torch-side binding of the 8-bit operators (a host-only extension module), beside the library.
+BIND_SOURCE = CSRC / "bind.cpp"
+BIND_PATH = PKG_DIR / "_bind.so"
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -43,9 +46,36 @@ def _stale() -> bool:
     return any(d.stat().st_mtime > built for d in deps)
 
 
+def _bind_stale() -> bool:
+    deps = [BIND_SOURCE, PKG_DIR.parent / "include" / "muse_proj.h"]
+    return not BIND_PATH.exists() or any(d.stat().st_mtime > BIND_PATH.stat().st_mtime for d in deps)
+
+
+def build_bind(force: bool = False) -> Path:
+    """Compile the binding if it is missing or older than its source; return its path."""
+    if not force and not _bind_stale():
+        return BIND_PATH
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    nvcc = Path(_nvcc()).resolve()
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], nvcc.parent.parent / "include"]
+    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in include], str(BIND_SOURCE), "-o", str(BIND_PATH), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError(f"g++ failed ({proc.returncode}) on {BIND_SOURCE.name}")
+    return BIND_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if it is missing or older than its sources; return its path."""
+    """Compile the library and the binding where they are missing or older than their sources; return the library's path."""
     if not force and not _stale():
+        build_bind()
         return LIB_PATH
     nvcc = _nvcc()
     compile_flags = ([f for f in NVCC_FLAGS if f != "--shared"] + (["-Xptxas", "-v"] if verbose else [])
@@ -58,8 +88,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
     from concurrent.futures import ThreadPoolExecutor
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:   # one nvcc per translation unit, side by side
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as pool:   # one nvcc per translation unit, side by side
+        bind = pool.submit(build_bind, force)
         results = list(pool.map(compile_one, zip(SOURCES, objs)))
+    bind.result()
     for src, proc in zip(SOURCES, results):
         if verbose or proc.returncode != 0:
             sys.stderr.write(proc.stdout + proc.stderr)

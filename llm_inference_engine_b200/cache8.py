@@ -119,7 +119,7 @@ def _refuse_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int,
 
 
 def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
-    """The checks both operators share, in one expression (they are a good part of a small call's time); returns (device
+    """The checks both operators share, in one expression; returns (device
     index, addresses of k, v, k_exp, v_exp, page_table, seq_lens, cu_q, pages, heads, dim, batch, width)."""
     k, v, ke, ve = cache
     shape, index = k.shape, k.get_device()
@@ -151,6 +151,9 @@ def rope_append(qkv: torch.Tensor, cache: Cache8, cos_sin: torch.Tensor, page_ta
     `interleaved`. max_q: at least the most new tokens of a sequence. Returns q BF16 [m, q_heads, dim]; with values=True
     (q, k, v), k and v BF16 [m, heads, dim]: the values that the cache then holds for the new tokens (for a prompt's own
     attention in 16 bits to see what later tokens will see)."""
+    r = (_capi._BIND or _capi.bind()).rope_append(qkv, cache, cos_sin, page_table, seq_lens, cu_q, q_heads, max_q, interleaved, values)
+    if r is not None:   # an ordinary call is done
+        return r
     if qkv.dtype is not _BF16 or qkv.dim() != 2 or not qkv.shape[0]:
         raise TypeError(f"qkv must be BF16 [m, columns], got {qkv.dtype} {tuple(qkv.shape)}")
     m, width_in = qkv.shape
@@ -195,6 +198,10 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
     that sees no token is zero; rows beyond the last sequence are left as they are. q: BF16 [m, q_heads, dim]; gate: BF16
     [m, q_heads * dim] (the gate columns of qkv_gate, any row stride); scale: positive, 1 / sqrt(dim) by default; out
     (optional): BF16 [m, q_heads * dim] with unit column stride. Two launches, the same bits in every run."""
+    if out is None:
+        r = (_capi._BIND or _capi.bind()).attention(q, cache, page_table, seq_lens, cu_q, max_q, scale, window, gate)
+        if r is not None:   # an ordinary call is done
+            return r
     if q.dtype is not _BF16 or q.dim() != 3 or not q.shape[0]:
         raise TypeError(f"q must be BF16 [m, heads, dim], got {q.dtype} {tuple(q.shape)}")
     m, q_heads, d = q.shape

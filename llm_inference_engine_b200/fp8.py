@@ -136,8 +136,11 @@ def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = 
     [N, K] and exponent bytes of W, contiguous; K a multiple of 16. `out` (optional): BF16 [m, >= N] with unit column
     stride, of which the first N columns are written. Weights are static: what made them must be complete before the first
     call (kernels may read them ahead of the work before them in the stream)."""
-    # One expression takes what is right (the checks are a good part of a small call's time); what it does not take is
-    # looked at again to say why.
+    if out is None:
+        r = (_capi._BIND or _capi.bind()).linear(x, w8, w_exp)
+        if r is not None:   # an ordinary call is done
+            return r
+    # One expression takes what is right; what it does not take is looked at again to say why.
     pair = isinstance(x, (tuple, list))
     xt = x[0] if pair else x
     shape, w_shape, index = xt.shape, w8.shape, w8.get_device()

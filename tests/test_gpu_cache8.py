@@ -538,6 +538,7 @@ def test_first_call_of_a_device_inside_a_capture_is_refused(c8):
     table, lens = i32([[0]]), i32([5])
     torch.cuda.synchronize(DEV)
     kept = _capi._STATUS.pop(DEV.index, None)
+    _capi.bind().set_status(DEV.index, 0)
     try:
         g = torch.cuda.CUDAGraph()
         with pytest.raises(_capi.MuseError, match="outside stream capture"):
@@ -546,6 +547,47 @@ def test_first_call_of_a_device_inside_a_capture_is_refused(c8):
     finally:
         if kept is not None:
             _capi._STATUS[DEV.index] = kept
+            _capi.bind().set_status(DEV.index, kept.data_ptr())
     torch.cuda.synchronize(DEV)
     c8.attention(q, cache, table, lens)
+    c8.check_status(DEV)
+
+
+def test_ordinary_calls_take_the_short_way_and_give_the_same_bits(c8, monkeypatch):
+    """What csrc/bind.cpp takes and what the Python code does with the same arguments: equal results, equal cache."""
+    from llm_inference_engine_b200 import _capi, fp8
+
+    class Never:
+        linear = rope_append = attention = staticmethod(lambda *a: None)
+        set_status = staticmethod(lambda *a: None)
+
+    hq, hk, d = 8, 2, 64
+    cos_sin = c8.rotary_table(64, 4 * PAGE, DEV)
+    table = torch.arange(12, dtype=torch.int32, device=DEV).view(3, 4)
+    x = torch.randn((3, 512), device=DEV).bfloat16()
+    w8, we = fp8.quantize_weight(torch.randn(((2 * hq + 2 * hk) * d, 512), device=DEV))
+    start = filled_cache(c8, 12, hk, d, 91)
+
+    def run(cache):
+        rows = fp8.linear(x, w8, we)
+        many = fp8.linear(x.repeat(30, 1), w8, we)
+        q, kv, vv = c8.rope_append(rows, cache, cos_sin, table, i32([3, 70, 128]), q_heads=hq, values=True)
+        q2 = c8.rope_append(rows, cache, cos_sin, table, i32([3, 70, 0]), q_heads=hq, cu_q=i32([0, 2, 3, 3]), max_q=2, interleaved=True)
+        a = c8.attention(q, cache, table, i32([3, 70, 128]), gate=rows[:, (hq + 2 * hk) * d :], window=50, scale=0.2)
+        return [rows, many, q, kv, vv, q2, a, *[t.view(torch.uint8) for t in cache]]
+
+    run(clone(start))
+    b = _capi.bind()
+    q = torch.randn((3, hq, d), device=DEV).bfloat16()
+    assert b.attention(q, start, table, i32([3, 70, 128]), None, 1, None, 0, None) is not None
+    assert b.linear(x, w8, we) is not None
+    for args in ((q.float(), start, table, i32([3, 70, 128]), None, 1, None, 0, None), (q, start, table, i32([3, 70]), None, 1, None, 0, None),
+                 (q, start, table, i32([3, 70, 128]), None, 2, None, 0, None), (q, start, table, i32([3, 70, 128]), None, 1, -1.0, 0, None),
+                 (q, start, table, i32([3, 70, 128]), None, 1, None, -1, None), (q, list(start), table, i32([3, 70, 128]), None, 1, None, 0, None),
+                 (None, start, table, i32([3, 70, 128]), None, 1, None, 0, None), (q, start)):
+        assert b.attention(*args) is None, "not an ordinary call"
+    short = run(clone(start))
+    monkeypatch.setattr(_capi, "_BIND", Never)
+    long_way = run(clone(start))
+    assert all(torch.equal(u, w) for u, w in zip(short, long_way))
     c8.check_status(DEV)
