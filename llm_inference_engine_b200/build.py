@@ -20,7 +20,7 @@ CSRC = PKG_DIR / "csrc"
 # stamp their phases; the ordinary library carries none of that code.
 TRACE = bool(os.environ.get("MUSE_TRACE"))
 LIB_PATH = PKG_DIR / ("libmuse_proj_trace.so" if TRACE else "libmuse_proj.so")
-SOURCES = ["gemv1.cu", "fewtok_mma.cu", "fewtok_zip.cu", "ffn_boundary.cu", "skinny_tc.cu", "gemm_tc.cu", "fp8_linear.cu", "fp8_gemm.cu", "rope_append.cu", "cache_attn.cu", "capi.cu"]
+SOURCES = ["gemv1.cu", "fewtok_mma.cu", "fewtok_zip.cu", "ffn_boundary.cu", "skinny_tc.cu", "gemm_tc.cu", "fp8_linear.cu", "fp8_gemm.cu", "rope_append.cu", "cache_attn.cu", "cache_attn_tc.cu", "capi.cu"]
 # The torch-side binding of the 8-bit operators (a host-only extension module), beside the library.
 BIND_SOURCE = CSRC / "bind.cpp"
 BIND_PATH = PKG_DIR / "_bind.so"

@@ -8,7 +8,7 @@
 // cut into equal ranges (attn_sched.cuh), one per warp, whatever the sequences' lengths, so that a batch of any shape
 // keeps every SM's loads in flight; a warp brings its pages in with bulk copies (K and V of a page and head are 64 D
 // contiguous bytes each) into a ring of its own and waits for nobody else. More than 16 rows (a chunk of a prompt) take
-// 16 rows per warp and one ring and range per CTA.
+// the kernel of cache_attn_tc.cu, with a range per CTA.
 //
 // The cache is the MMAs' M operand and the rows their N = 8 (or two such tiles): the work per page then follows the
 // rows there are, and a page's codes are converted once for all of them. Codes become FP16 in registers (exact, as e4m3
@@ -19,9 +19,7 @@
 // transpose in registers (movmatrix), the lane holds the same tokens' weights. Neither operand passes through
 // shared memory a second time. The weights are rounded to FP16 (2^-11, values below 2^-14 of the running maximum to 2^-25
 // of it), a page's sum is scaled by its V exponent in FP32.
-#include "attn_sched.cuh"
-#include "cache8.cuh"
-#include "fp8.cuh"
+#include "cache_attn.cuh"
 
 namespace muse {
 
@@ -30,35 +28,12 @@ constexpr int ATTN_THREADS = ATTN_WARPS * 32;
 
 __host__ __device__ constexpr int attn_slots(int D) { return D == 128 ? 3 : 6; }              // ring slots per warp
 __host__ __device__ constexpr int attn_ring_bytes(int D) { return ATTN_WARPS * attn_slots(D) * ATTN_PAGE * D; }
-// Floats of one partial slot of `rows` rows: max and sum per row, then the accumulators as the lanes hold them,
-// [8 rows][D / 16][lane] float4.
-__host__ __device__ constexpr int attn_slot_floats(int D, int rows) { return rows * (D + 2); }
-
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
-}
-
-// Row to token: n / group, for n * group < 2^32 (the host sees to it).
-__device__ __forceinline__ int div_group(const AttnArgs& a, int n) { return a.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), a.group_magic)); }
-
 // Lists of up to so many items are spread over the SMs (a warp each) instead of filling CTA after CTA.
 __host__ __device__ constexpr int attn_spread_below(int sms) { return 2 * sms; }
 
@@ -68,36 +43,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-
-__device__ __forceinline__ AttnEntry attn_entry_of(const AttnArgs& a, int e, int group, int tile) {
-  const int b = a.tiles == 1 ? e : e / a.tiles, rt = e - b * a.tiles;
-  const int c0 = a.cu_q ? __ldcg(a.cu_q + b) : b, c1 = a.cu_q ? __ldcg(a.cu_q + b + 1) : b + 1;
-  return attn_entry(c0, c1, __ldcg(a.seq_lens + b), a.m, a.max_q, a.width * ATTN_PAGE, group, tile, rt, a.window);
-}
-
-// Entries as a warp walks them: 32 at a time, one per lane, so that a walk over short sequences pays one round trip
-// per 32 of them.
-struct EntryCache {
-  int base, c0, c1, len;
-};
-__device__ __forceinline__ AttnEntry attn_entry_cached(const AttnArgs& a, EntryCache& c, int e, int entries, int group, int tile) {
-  if (e < c.base || e >= c.base + 32) {   // warp-uniform
-    c.base = e;
-    const int b = min(e + static_cast<int>(threadIdx.x & 31), entries - 1) / a.tiles;
-    c.c0 = a.cu_q ? __ldcg(a.cu_q + b) : b;
-    c.c1 = a.cu_q ? __ldcg(a.cu_q + b + 1) : b + 1;
-    c.len = __ldcg(a.seq_lens + b);
-  }
-  const int l = e - c.base;
-  return attn_entry(__shfl_sync(0xffffffffu, c.c0, l), __shfl_sync(0xffffffffu, c.c1, l), __shfl_sync(0xffffffffu, c.len, l), a.m, a.max_q,
-                    a.width * ATTN_PAGE, group, tile, e % a.tiles, a.window);
-}
-
-// A place in the list: entry, head, i-th page of the unit (below zero: the unit's head items).
-struct Cursor {
-  AttnEntry en;
-  int e, h, i;
-};
 
 // The state of a warp's 8 NT rows. Lane (g, t) holds rows 8 n + 2 t and + 1 of dimensions 16 d + g and + 8.
 template <int D, int NT>
@@ -347,8 +292,6 @@ __device__ __forceinline__ void page_nan(TileState<D, NT>& st, uint32_t vs, cons
   }
 }
 
-__device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + __expf(-x)); }
-
 // Output values of accumulator quads o[d] (rows row, row + 1 of the entry's tile, dimensions 16 d + g and + 8 of a head).
 template <int N>
 __device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& en, int h, int row, int d0, const float (&o)[N][4], const float (&inv)[2],
@@ -388,51 +331,10 @@ __device__ __forceinline__ void store_quads(const AttnArgs& a, const AttnEntry& 
 }
 
 constexpr int STAGE_LD = 68;   // floats of a staged row of 64 dimensions: rows four banks apart
-// Eight neighbouring output values from shared memory, gated.
-__device__ __forceinline__ void store8(const AttnArgs& a, size_t tok, int col, const float* s) {
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(s + i);
-    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-  }
-  if (a.gate) {
-    const __nv_bfloat16* g = a.gate + tok * a.ld_gate + col;
-    uint32_t w[4];
-    if (a.vec_gate) {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(g));
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
-      const unsigned short* p = reinterpret_cast<const unsigned short*>(g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __ldcg(p + 2 * i) | static_cast<uint32_t>(__ldcg(p + 2 * i + 1)) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] *= sigmoid_f32(bf16lo_f32(w[i]));
-      x[2 * i + 1] *= sigmoid_f32(bf16hi_f32(w[i]));
-    }
-  }
-  __nv_bfloat16* o = a.out + tok * a.ld_out + col;
-  if (a.vec_out) {
-    uint32_t p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      p[i] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    *reinterpret_cast<uint4*>(o) = make_uint4(p[0], p[1], p[2], p[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(x[i]);
-  }
-}
-
-// A finished segment of a unit: the output rows themselves when it is the whole unit, else a partial slot. row0: the
-// warp's first row in the entry's tile of `rows` rows.
+// A finished segment of a unit: the output rows themselves when it is the whole unit, else a partial slot.
 template <int D, int NT>
-__device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, int row0, bool whole, float* slot,
-                                           int slot_rows, float* stage) {
+__device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs& a, const AttnEntry& en, int h, bool whole, float* slot,
+                                           float* stage) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -444,8 +346,8 @@ __device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs&
       l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
       l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
     }
-    const int row = row0 + 8 * n + 2 * t;
-    if (row0 + 8 * n >= en.rows) continue;   // warp-uniform
+    const int row = 8 * n + 2 * t;
+    if (8 * n >= en.rows) continue;   // warp-uniform
     if (whole) {
       const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};   // no token seen: the row is zero
       // Through shared memory, 64 dimensions at a time, and out in a loop: written out for every accumulator these lines
@@ -459,21 +361,23 @@ __device__ __forceinline__ void tile_store(TileState<D, NT>& st, const AttnArgs&
           for (int k = 0; k < 4; ++k)
             stage[(2 * t + (k & 1)) * STAGE_LD + 16 * d + 8 * (k >> 1) + g] = st.o[4 * half + d][n][k] * inv[k & 1];
         __syncwarp();
-        const int here = min(8, en.rows - (row0 + 8 * n));
+        const int here = min(8, en.rows - 8 * n);
 #pragma unroll 1
         for (int it = lane; it < here * 8; it += 32) {
-          const int r = it >> 3, c = (it & 7) * 8, rr = en.row0 + row0 + 8 * n + r, tk = div_group(a, rr);
+          const int r = it >> 3, c = (it & 7) * 8, rr = en.row0 + 8 * n + r, tk = div_group(a, rr);
           const size_t tok = en.first + tk;
           const int col = (h * a.group + rr - tk * a.group) * D + 64 * half + c;
-          store8(a, tok, col, stage + r * STAGE_LD + c);
+          const float4 lo = *reinterpret_cast<const float4*>(stage + r * STAGE_LD + c), hi = *reinterpret_cast<const float4*>(stage + r * STAGE_LD + c + 4);
+          float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          store8(a, tok, col, x);
         }
       }
     } else {
       if (g == 0) {
         *reinterpret_cast<float2*>(slot + row) = make_float2(st.mx[n][0], st.mx[n][1]);
-        *reinterpret_cast<float2*>(slot + slot_rows + row) = make_float2(l[0], l[1]);
+        *reinterpret_cast<float2*>(slot + 8 * NT + row) = make_float2(l[0], l[1]);
       }
-      float4* o = reinterpret_cast<float4*>(slot + 2 * slot_rows) + static_cast<size_t>(row0 / 8 + n) * (D / 16) * 32 + lane;
+      float4* o = reinterpret_cast<float4*>(slot + 2 * 8 * NT) + static_cast<size_t>(n) * (D / 16) * 32 + lane;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[d * 32] = make_float4(st.o[d][n][0], st.o[d][n][1], st.o[d][n][2], st.o[d][n][3]);
     }
@@ -521,31 +425,27 @@ __device__ __forceinline__ void merge_slots(const float* slots, int stride, floa
   }
 }
 
-// SHARED: the CTA is one worker, all its warps on the same pages, 8 NT rows each; else every warp is a worker of 8 NT rows.
-template <int D, int NT, bool SHARED>
+// Every warp is a worker of 8 NT rows.
+template <int D, int NT>
 __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int WARP_ROWS = 8 * NT, TILE = SHARED ? WARP_ROWS * ATTN_WARPS : WARP_ROWS;
-  constexpr int SLOTS = SHARED ? attn_slots(D) * ATTN_WARPS : attn_slots(D);   // ring slots of one worker
+  constexpr int TILE = 8 * NT;
+  constexpr int SLOTS = attn_slots(D);   // ring slots of a warp
   constexpr uint32_t SLOT_BYTES = ATTN_PAGE * D;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bar_full[attn_slots(D) * ATTN_WARPS], bar_empty[attn_slots(D) * ATTN_WARPS];
+  __shared__ __align__(8) uint64_t bar_full[attn_slots(D) * ATTN_WARPS];
   __shared__ long long s_sum[ATTN_WARPS];
   __shared__ int s_entry[ATTN_WARPS];
   __shared__ long long s_start[ATTN_WARPS];
   __shared__ __align__(16) float s_stage[ATTN_WARPS][8 * STAGE_LD];   // rows on their way out
   __shared__ int2 s_rec[ATTN_WARPS][64];   // looked-up pages: tile index in the pool, exponents (k | v << 8)
-  __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.hq / a.hk, entries = a.batch * a.tiles;
-  uint64_t* const full = bar_full + (SHARED ? 0 : warp * attn_slots(D));
-  uint64_t* const empty = bar_empty + (SHARED ? 0 : warp * attn_slots(D));
-  const uint32_t ring_base = smem_u32(smem) + static_cast<uint32_t>(SHARED ? 0 : warp) * attn_slots(D) * SLOT_BYTES;
+  uint64_t* const full = bar_full + warp * attn_slots(D);
+  const uint32_t ring_base = smem_u32(smem) + static_cast<uint32_t>(warp) * attn_slots(D) * SLOT_BYTES;
   if (tid < attn_slots(D) * ATTN_WARPS) {
     mbar_init(smem_u32(&bar_full[tid]), 1);
-    mbar_init(smem_u32(&bar_empty[tid]), ATTN_WARPS);   // used by the shared ring only
     fence_mbar_init();
   }
-  if (tid == 0) s_abort = 0;
   griddep_wait();
   // Only now: the kernel that adds up, when it comes in, may then take what was ready before this one as ready.
   griddep_launch_dependents();
@@ -558,15 +458,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   auto items_of = [&](int e) { return static_cast<long long>(attn_items(attn_entry_of(a, e, group, TILE))) * a.hk; };
   for (int e = e0; e < e1; ++e) {
     mine += items_of(e);
-    if (blockIdx.x == 0) {
-      const int b = e / a.tiles, len = __ldcg(a.seq_lens + b);
-      bool bad = len < 0 || len > a.width * ATTN_PAGE;
-      if (a.cu_q) {
-        const int c0 = __ldcg(a.cu_q + b), c1 = __ldcg(a.cu_q + b + 1);
-        bad |= c0 < 0 || c1 < c0 || c1 > a.m || c1 - c0 > a.max_q;
-      }
-      if (bad) atomicOr(a.status, ST_BAD_LENGTH);
-    }
+    if (blockIdx.x == 0) attn_report_bad(a, e);
   }
   long long incl = mine;
 #pragma unroll
@@ -582,13 +474,13 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     total += s_sum[w];
   }
   const long long begin = base + incl - mine, end = base + incl;   // this thread's share of the list
-  const AttnDeal deal = attn_deal(total, static_cast<int>(SHARED ? gridDim.x : gridDim.x * ATTN_WARPS));
+  const AttnDeal deal = attn_deal(total, static_cast<int>(gridDim.x * ATTN_WARPS));
   // Neighbouring workers are a CTA's warps, so that sums of a long unit meet on chip; a list with few items is spread over
   // the SMs instead.
-  const bool spread = !SHARED && total <= attn_spread_below(static_cast<int>(gridDim.x));
-  auto worker_of = [&](int w) { return static_cast<int>(SHARED ? blockIdx.x : spread ? w * gridDim.x + blockIdx.x : blockIdx.x * ATTN_WARPS + w); };
+  const bool spread = total <= attn_spread_below(static_cast<int>(gridDim.x));
+  auto worker_of = [&](int w) { return static_cast<int>(spread ? w * gridDim.x + blockIdx.x : blockIdx.x * ATTN_WARPS + w); };
   if (total > 0) {
-    for (int w = 0; w < (SHARED ? 1 : ATTN_WARPS); ++w) {
+    for (int w = 0; w < ATTN_WARPS; ++w) {
       if (worker_of(w) >= deal.workers) break;
       const long long f = attn_range(deal, worker_of(w));
       if (f >= begin && f < end) {
@@ -614,7 +506,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   if (blockIdx.x == 0 && tid == 0) a.prefix[entries] = total;
   __syncthreads();
   const int worker = worker_of(warp);
-  if (worker >= deal.workers) return;   // SHARED: CTA-uniform; else this warp has no item, and no warp waits for it (a merging CTA's have)
+  if (worker >= deal.workers) return;   // no item, and no warp waits for this one (a merging CTA's all have some)
   const long long f0 = attn_range(deal, worker);
   const int items = static_cast<int>(attn_range(deal, worker + 1) - f0);
 
@@ -623,13 +515,12 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   Cursor rd, fill;   // where the warp computes, and up to where it has looked up pages
   long long unit0;   // first item of the unit that rd stands in
   {
-    const int w = SHARED ? 0 : warp;
-    fill.e = s_entry[w];
+    fill.e = s_entry[warp];
     fill.en = attn_entry_cached(a, fill_cache, fill.e, entries, group, TILE);
-    const int off = static_cast<int>(f0 - s_start[w]), per_unit = attn_items(fill.en);
+    const int off = static_cast<int>(f0 - s_start[warp]), per_unit = attn_items(fill.en);
     fill.h = off / per_unit;
     fill.i = off % per_unit - ATTN_HEAD;
-    unit0 = s_start[w] + static_cast<long long>(fill.h) * per_unit;
+    unit0 = s_start[warp] + static_cast<long long>(fill.h) * per_unit;
     rd_cache = fill_cache;
     rd = fill;
   }
@@ -688,15 +579,9 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   look_up();
 
   int issued = 0, used = 0;               // halves (K, then V of a page) requested and consumed by this worker
-  const bool issuer = !SHARED || warp == 0;
-  // Requests the next half; every lane of the issuing warp runs it.
+  // Requests the next half.
   auto request = [&]() {
-    const int slot = issued % SLOTS, turn = issued / SLOTS;
-    if (SHARED && turn > 0 && !mbar_wait(smem_u32(&empty[slot]), (turn - 1) & 1)) {
-      if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
-      s_abort = 1;
-      return;
-    }
+    const int slot = issued % SLOTS;
     if (lane == 0) {
       const uint32_t bar = smem_u32(&full[slot]);
       const int tile = s_rec[warp][(issued >> 1) & 63].x;
@@ -712,13 +597,10 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   // The warp has read a half: its slot may be filled again.
   auto release = [&]() {
     __syncwarp();
-    if (SHARED && lane == 0) mbar_arrive(smem_u32(&empty[used % SLOTS]));
     ++used;
-    if (issuer)
-      while (issued < used + SLOTS && (issued >> 1) < filled && !(SHARED && s_abort)) request();
+    while (issued < used + SLOTS && (issued >> 1) < filled) request();
   };
-  if (issuer)
-    while (issued < SLOTS && (issued >> 1) < filled) request();
+  while (issued < SLOTS && (issued >> 1) < filled) request();
   look_up_exponents();
 
   TileState<D, NT> st;
@@ -726,11 +608,10 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   float qs[NT][2];
   RowInfo<NT> ri;
   float* const stage = s_stage[warp];
-  const int wrow = SHARED ? warp * WARP_ROWS : 0;   // this warp's first row in the worker's tile
   // All eight warps inside one unit: their sums meet in shared memory, and one slot leaves the CTA.
   const int w_first = worker - warp;
-  const bool merge = !SHARED && !spread && attn_merged(deal, w_first, ATTN_WARPS, unit0 + ATTN_HEAD, unit0 + attn_items(rd.en));   // CTA-uniform
-  bool fresh = true;
+  const bool merge = !spread && attn_merged(deal, w_first, ATTN_WARPS, unit0 + ATTN_HEAD, unit0 + attn_items(rd.en));   // CTA-uniform
+  bool fresh = true, gave_up = false;
   int seg_first = 0, left = items, n = 0;           // first page of the segment; items to go; pages done
   while (left > 0) {
     if (rd.i < 0) {   // the unit's head items
@@ -738,10 +619,10 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       --left;
       continue;
     }
-    const int my_rows = max(0, min(WARP_ROWS, rd.en.rows - wrow));
+    const int my_rows = rd.en.rows;
     if (fresh) {
       tile_reset(st);
-      const int r0 = rd.en.row0 + wrow, t = lane & 3;
+      const int r0 = rd.en.row0, t = lane & 3;
       load_q<D, NT>(a, rd.en, rd.h, r0, my_rows, qf, qs);
       if (a.gate && (lane & 3) == 0 && (lane >> 2) < my_rows) {   // on its way to L2 while the pages are worked on
 #pragma unroll
@@ -769,7 +650,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       look_up_exponents();
     }
     const int2 rec = s_rec[warp][n & 63];
-    const bool live = rec.x >= 0 && my_rows > 0;
+    const bool live = rec.x >= 0;
     const int p0 = (rd.en.page0 + rd.i) * ATTN_PAGE;
     // some row does not see some token of the page (positions grow with the row)
     const bool edge = ri.first < p0 + ATTN_PAGE - 1 || (a.window > 0 && ri.last - a.window + 1 > p0);
@@ -781,9 +662,8 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     release();
     if (ok && live) page_softmax<D, NT>(st, s, p, al, moved, qs, exp2_byte(rec.y & 255), ri, p0, a.window, edge);
     ok = ok && mbar_wait(smem_u32(&full[vsl]), vt & 1);
-    if (!ok || (SHARED && s_abort)) {
-      if (lane == 0 && !ok) atomicOr(a.status, ST_ATTN_TIMEOUT);
-      s_abort = 1;
+    if (!ok) {
+      gave_up = true;
       break;
     }
     if (live) {
@@ -802,7 +682,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       // (a warp's ring is idle by now when it merges: its range ends with this segment)
       float* slot = merge ? reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * attn_slots(D) * SLOT_BYTES / 4
                           : a.part + static_cast<size_t>(attn_slot_of(deal, worker, unit0 + ATTN_HEAD)) * attn_slot_floats(D, TILE);
-      tile_store<D, NT>(st, a, rd.en, rd.h, wrow, whole && !merge, slot, TILE, stage);
+      tile_store<D, NT>(st, a, rd.en, rd.h, whole && !merge, slot, stage);
       fresh = true;
     }
     if (left > 0) {
@@ -814,16 +694,14 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       }
     }
   }
-  if constexpr (!SHARED) {
-    if (merge) {
-      __syncthreads();   // every warp of the CTA comes here, also one that gave up
-      merge_slots<D, NT>(reinterpret_cast<const float*>(smem), attn_slots(D) * SLOT_BYTES / 4, a.part + static_cast<size_t>(2 * w_first) * attn_slot_floats(D, TILE));
-    }
-  }
-  if (s_abort) {
+  if (gave_up) {
+    if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
     // leave no copy in flight behind: each slot's last request is waited for (bounded)
-    if (issuer)
-      for (int i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(smem_u32(&full[i % SLOTS]), (i / SLOTS) & 1);
+    for (int i = issued > SLOTS ? issued - SLOTS : 0; i < issued; ++i) mbar_wait(smem_u32(&full[i % SLOTS]), (i / SLOTS) & 1);
+  }
+  if (merge) {
+    __syncthreads();   // every warp of the CTA comes here, also one that gave up
+    merge_slots<D, NT>(reinterpret_cast<const float*>(smem), attn_slots(D) * SLOT_BYTES / 4, a.part + static_cast<size_t>(2 * w_first) * attn_slot_floats(D, TILE));
   }
 }
 
@@ -833,8 +711,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
 template <int D, int TILE, bool DEEP>
 __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(const __grid_constant__ AttnArgs a, int workers, int spread_below) {
   constexpr int STEP = DEEP ? 8 : 1, FLOATS = attn_slot_floats(D, TILE);
-  __shared__ float s_m[STEP][8], s_l[STEP][8];
-  __shared__ float4 s_o[STEP][32];
+  __shared__ float4 s_ml[STEP][32], s_o[STEP][32];
   const int entries = a.batch * a.tiles, group = a.group;
   const int e = static_cast<int>(blockIdx.x) / a.hk, h = static_cast<int>(blockIdx.x) % a.hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -849,7 +726,12 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   const long long u0 = start + static_cast<long long>(h) * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;   // one worker had all of the unit's pages and has written it
   const AttnParts ps = attn_parts(deal, TILE > 16 || total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
-  const int row = r0 + 2 * t;
+  // The lane's two rows and where its quad of sums lies in a part. Tiles of 128 rows are kept by rows: a quad is then four
+  // neighbouring dimensions of one row.
+  constexpr bool BY_ROW = TILE > 16;
+  const int row = BY_ROW ? r0 + (DEEP ? lane / 4 : static_cast<int>(threadIdx.x) / (D / 4)) : r0 + 2 * t;
+  const int dim = DEEP ? 16 * d + 4 * (lane % 4) : 4 * (static_cast<int>(threadIdx.x) % (D / 4));   // BY_ROW: first of four
+  const size_t quad_at = 2 * TILE + (BY_ROW ? static_cast<size_t>(row) * D + dim : (static_cast<size_t>(r0 / 8) * (D / 16) + d) * 128 + lane * 4);
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](const float2& pm, const float2& pl, const float4& po) {   // one more part, or a warp's sums
     const float m0 = fmaxf(m[0], pm.x), m1 = fmaxf(m[1], pm.y);
@@ -873,9 +755,14 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
       const int j = i + k * STEP;
       if (j < ps.parts) {
         const float* s = a.part + static_cast<size_t>(attn_part_slot(ps, j)) * FLOATS;
-        pm[k] = __ldcg(reinterpret_cast<const float2*>(s + row));
-        pl[k] = __ldcg(reinterpret_cast<const float2*>(s + TILE + row));
-        po[k] = __ldcg(reinterpret_cast<const float4*>(s + 2 * TILE) + static_cast<size_t>((r0 / 8) * (D / 16) + d) * 32 + lane);
+        if constexpr (BY_ROW) {
+          pm[k].x = pm[k].y = __ldcg(s + row);
+          pl[k].x = pl[k].y = __ldcg(s + TILE + row);
+        } else {
+          pm[k] = __ldcg(reinterpret_cast<const float2*>(s + row));
+          pl[k] = __ldcg(reinterpret_cast<const float2*>(s + TILE + row));
+        }
+        po[k] = __ldcg(reinterpret_cast<const float4*>(s + quad_at));
       }
     }
 #pragma unroll
@@ -883,24 +770,35 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
       if (i + k * STEP < ps.parts) add(pm[k], pl[k], po[k]);
   }
   if constexpr (DEEP) {
-    if (g == 0) {
-      s_m[warp][2 * t] = m[0]; s_m[warp][2 * t + 1] = m[1];
-      s_l[warp][2 * t] = l[0]; s_l[warp][2 * t + 1] = l[1];
-    }
+    s_ml[warp][lane] = make_float4(m[0], m[1], l[0], l[1]);
     s_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
     __syncthreads();
     if (warp > 0) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w)
-      add(make_float2(s_m[w][2 * t], s_m[w][2 * t + 1]), make_float2(s_l[w][2 * t], s_l[w][2 * t + 1]), s_o[w][lane]);
+    for (int w = 1; w < 8; ++w) {
+      const float4 x = s_ml[w][lane];
+      add(make_float2(x.x, x.y), make_float2(x.z, x.w), s_o[w][lane]);
+    }
   }
   const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
-  const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
-  store_quads<1>(a, en, h, row, 16 * d + g, quad, inv, D);
+  if constexpr (BY_ROW) {
+    if (row >= en.rows) return;
+    const int rr = en.row0 + row, tk = div_group(a, rr), col = (h * a.group + rr - tk * a.group) * D + dim;
+    const size_t tok = en.first + tk;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = o[i] * inv[0];
+      if (a.gate) x *= sigmoid_f32(bf16lo_f32(__ldcg(reinterpret_cast<const unsigned short*>(a.gate + tok * a.ld_gate + col + i))));
+      a.out[tok * a.ld_out + col + i] = __float2bfloat16_rn(x);
+    }
+  } else {
+    const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
+    store_quads<1>(a, en, h, row, 16 * d + g, quad, inv, D);
+  }
 }
 
 // ---------------------------------------------------------------- host side
-// The form a call takes goes by the rows a KV head has at most: 8 or 16 per warp, or 128 per CTA.
+// The form a call takes goes by the rows a KV head has at most: 8 or 16 per warp, or (cache_attn_tc.cu) 128 per CTA.
 struct AttnForm {
   bool shared;
   int tile, tiles;
@@ -910,7 +808,7 @@ static AttnForm attn_form(int max_q, int hq, int hk) {
   const long long rows = static_cast<long long>(max_q) * (hq / hk);
   AttnForm f;
   f.shared = rows > 16;
-  f.tile = f.shared ? 16 * ATTN_WARPS : rows > 8 ? 16 : 8;
+  f.tile = f.shared ? 128 : rows > 8 ? 16 : 8;
   f.tiles = static_cast<int>((rows + f.tile - 1) / f.tile);
   return f;
 }
@@ -922,24 +820,32 @@ long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
   return 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile) * 4 + (static_cast<long long>(batch) * f.tiles + 1) * 8;
 }
 
-template <int D, int NT, bool SHARED>
-static cudaError_t attn_launch(const AttnArgs& a, const AttnForm& f, int sms, cudaStream_t stream) {
+template <int D, int NT>
+static cudaError_t attn_launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   const size_t smem = attn_ring_bytes(D);
   static DeviceOnce once;
   cudaError_t e = cudaSuccess;
-  if (once.first()) e = cudaFuncSetAttribute(cache_attn_kernel<D, NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (once.first()) e = cudaFuncSetAttribute(cache_attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   once.done();
-  e = launch_dependent(cache_attn_kernel<D, NT, SHARED>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
-  if (e != cudaSuccess) return e;
-  const int all = a.max_q * (a.hq / a.hk), rows = all < f.tile ? all : f.tile;
-  const unsigned units = static_cast<unsigned>(a.batch) * a.tiles * a.hk;
-  constexpr int TILE = SHARED ? 16 * ATTN_WARPS : 8 * NT;
-  const unsigned groups = (rows + 7) / 8;
+  return launch_dependent(cache_attn_kernel<D, NT>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
+}
+
+template <int D, int TILE>
+static cudaError_t join_launch(const AttnArgs& a, const AttnForm& f, int sms, cudaStream_t stream) {
+  const int all = a.max_q * a.group, rows = all < f.tile ? all : f.tile;
+  const unsigned units = static_cast<unsigned>(a.batch) * a.tiles * a.hk, groups = (rows + 7) / 8;
   // Few units may have many parts each; many units have few (there are two partial segments per worker in all).
   if (static_cast<long long>(units) * groups < 2ll * sms)
     return launch_dependent(cache_attn_join_kernel<D, TILE, true>, dim3(units, groups, D / 16), dim3(256), 0, stream, a, f.workers(sms), attn_spread_below(sms));
   return launch_dependent(cache_attn_join_kernel<D, TILE, false>, dim3(units, groups), dim3(D * 2), 0, stream, a, f.workers(sms), attn_spread_below(sms));
+}
+
+template <int D>
+static cudaError_t both_launch(const AttnArgs& a, const AttnForm& f, int sms, cudaStream_t stream) {
+  cudaError_t e = f.shared ? cache_attn_tc_launch(a, D, sms, stream) : f.tile == 16 ? attn_launch<D, 2>(a, sms, stream) : attn_launch<D, 1>(a, sms, stream);
+  if (e != cudaSuccess) return e;
+  return f.shared ? join_launch<D, 128>(a, f, sms, stream) : f.tile == 16 ? join_launch<D, 16>(a, f, sms, stream) : join_launch<D, 8>(a, f, sms, stream);
 }
 
 int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
@@ -963,11 +869,7 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
   a.part = static_cast<float*>(ws);
   a.prefix = reinterpret_cast<long long*>(a.part + 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile));
-  cudaError_t e;
-  if (dim == 128)
-    e = f.shared ? attn_launch<128, 2, true>(a, f, sms, stream) : f.tile == 16 ? attn_launch<128, 2, false>(a, f, sms, stream) : attn_launch<128, 1, false>(a, f, sms, stream);
-  else
-    e = f.shared ? attn_launch<64, 2, true>(a, f, sms, stream) : f.tile == 16 ? attn_launch<64, 2, false>(a, f, sms, stream) : attn_launch<64, 1, false>(a, f, sms, stream);
+  const cudaError_t e = dim == 128 ? both_launch<128>(a, f, sms, stream) : both_launch<64>(a, f, sms, stream);
   return static_cast<int>(e);
 }
 

@@ -1,0 +1,650 @@
+// The attention of cache_attn.cu for many query rows per KV head (chunks of prompts, long drafts under large groups):
+// tiles of 128 rows on tcgen05. At these sizes a page's codes are used for 128 rows at once and arithmetic bounds it:
+// 2 x 128 x 64 x D products, 128 x 64 exponentials (one SM makes 16 a clock: 512 clocks, as long as the products) and
+// the conversion of 128 D codes per page.
+//
+// The page list, its cut into ranges and the joining of split units are those of cache_attn.cu, a CTA being a worker. Per
+// page: K and V codes come in by bulk copies; two warps convert them to FP16 (exact) in the 128-byte-swizzled layout of the
+// MMA's B operand (K [token][dim], V [dim][token]: both K-major as the cache keeps them); S = Q K^T with Q in tensor
+// memory as the A operand; a thread per row turns its 64 scores into weights, which go back to tensor memory as the A
+// operand of O' = P V; another thread per row adds O' to its sums in registers, scaled in FP32 by the page's exponent and
+// by what the row's maximum has moved. S, P and O' are double-buffered in tensor memory (64 + 2 x 64 + 2 x 32 + 2 x 128
+// columns at D = 128), so the products of one page run under the exponentials of another.
+//
+// Roles: warp 0 looks pages up and copies, warp 1 issues MMAs, warps 2 and 3 convert, warps 4..7 softmax, warps 8..11
+// sums and output. All waits are bounded.
+#include "cache_attn.cuh"
+
+namespace muse {
+
+constexpr int TC_ROWS = 128;
+constexpr int TC_THREADS = 384;
+constexpr int TC_RAW = 8;              // ring slots of raw codes (K and V of a page are one each)
+constexpr int TC_UNITS = 16;           // ring of unit records: no role is that many pages behind another
+constexpr int TC_PAGES = 64;           // ring of page records
+__host__ __device__ constexpr int tc_raw_bytes(int D) { return ATTN_PAGE * D; }
+__host__ __device__ constexpr int tc_f16_bytes(int D) { return ATTN_PAGE * D * 2; }
+__host__ __device__ constexpr int tc_smem_bytes(int D) { return 4 * tc_f16_bytes(D) + TC_RAW * tc_raw_bytes(D) + 1024; }
+constexpr int TC_MIN_SMEM = 120 * 1024;   // one CTA per SM: it takes all of tensor memory
+
+// The last page of a unit's share of the range, of the range; some row does not see some token; there is a page at all.
+enum : int { PAGE_SEG_LAST = 1, PAGE_RANGE_LAST = 2, PAGE_EDGE = 4, PAGE_LIVE = 8 };
+struct PageRec {
+  int tile;      // index in the pool (page * hk + head)
+  int bits;      // exponents k | v << 8, PAGE_* << 16
+  int p0;        // position of the page's first token
+  int seen;      // first | last << 8: the page's tokens that some row of the tile sees
+};
+struct UnitRec {
+  int first, row0, rows, pos;   // as in AttnEntry
+  int h, whole;
+  int slot;
+};
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// FP16 x FP16 -> FP32, both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr uint32_t RAW = ATTN_PAGE * D, F16 = ATTN_PAGE * D * 2;
+  // tensor memory columns
+  constexpr uint32_t COL_Q = 0, COL_S = D / 2, COL_P = COL_S + 2 * ATTN_PAGE, COL_O = COL_P + ATTN_PAGE;
+  static_assert(COL_O + 2 * D <= 512, "tensor memory");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t raw_full[TC_RAW], raw_empty[TC_RAW], unit_full[TC_UNITS], kf_full[2], vf_full[2], qk_done[2], pv_done[2], s_empty[2],
+      p_full[2], o_empty[2], q_full, fin_full[8];
+  __shared__ __align__(16) PageRec s_page[TC_PAGES];
+  __shared__ UnitRec s_unit[TC_UNITS];
+  __shared__ float s_alpha[4][TC_ROWS], s_fin[8][2][TC_ROWS];
+  __shared__ __align__(8) unsigned short s_nan[4][D][4];      // edge pages: the tokens of each dimension that hold NaN
+  __shared__ int s_has_nan[4][2];
+  __shared__ long long s_sum[TC_THREADS / 32];
+  __shared__ int s_entry;
+  __shared__ long long s_start;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.group, entries = a.batch * a.tiles;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t k16 = smem_base, v16 = k16 + 2 * F16, raw = v16 + 2 * F16;
+
+  if (tid == 0) {
+    for (int i = 0; i < TC_RAW; ++i) {
+      mbar_init(smem_u32(&raw_full[i]), 1);
+      mbar_init(smem_u32(&raw_empty[i]), 2);
+    }
+    for (int i = 0; i < TC_UNITS; ++i) mbar_init(smem_u32(&unit_full[i]), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&kf_full[i]), 2);
+      mbar_init(smem_u32(&vf_full[i]), 2);
+      mbar_init(smem_u32(&qk_done[i]), 1);
+      mbar_init(smem_u32(&pv_done[i]), 1);
+      mbar_init(smem_u32(&s_empty[i]), 4);
+      mbar_init(smem_u32(&p_full[i]), 4);
+      mbar_init(smem_u32(&o_empty[i]), 4);
+    }
+    mbar_init(smem_u32(&q_full), 4);
+    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&fin_full[i]), 4);
+    fence_mbar_init();
+    s_abort = 0;
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // The list of items, as in cache_attn_kernel.
+  const int per = (entries + TC_THREADS - 1) / TC_THREADS;
+  const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
+  auto items_of = [&](int e) { return static_cast<long long>(attn_items(attn_entry_of(a, e, group, TC_ROWS))) * a.hk; };
+  long long mine = 0;
+  for (int e = e0; e < e1; ++e) {
+    mine += items_of(e);
+    if (blockIdx.x == 0) attn_report_bad(a, e);
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, s);
+    if (lane >= s) incl += up;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  long long base = 0, total = 0;
+  for (int w = 0; w < TC_THREADS / 32; ++w) {
+    if (w < warp) base += s_sum[w];
+    total += s_sum[w];
+  }
+  const long long begin = base + incl - mine, end = base + incl;
+  const AttnDeal deal = attn_deal(total, static_cast<int>(gridDim.x));
+  const int worker = blockIdx.x;
+  const long long f0 = worker < deal.workers ? attn_range(deal, worker) : 0;
+  const int items = worker < deal.workers ? static_cast<int>(attn_range(deal, worker + 1) - f0) : 0;
+  if (items > 0 && f0 >= begin && f0 < end) {
+    long long at = begin;
+    int e = e0;
+    for (; e + 1 < e1; ++e) {
+      const long long next = at + items_of(e);
+      if (f0 < next) break;
+      at = next;
+    }
+    s_entry = e;
+    s_start = at;
+  }
+  if (blockIdx.x == 0) {
+    long long at = begin;
+    for (int e = e0; e < e1; ++e) {
+      a.prefix[e] = at;
+      if (e + 1 < e1) at += items_of(e);
+    }
+    if (tid == 0) a.prefix[entries] = total;
+  }
+  __syncthreads();
+
+  if (items > 0 && warp == 0) {
+    // ---- looks pages up, describes them, and copies their codes
+    EntryCache cache;
+    cache.base = -64;
+    Cursor c;
+    c.e = s_entry;
+    c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
+    const int off0 = static_cast<int>(f0 - s_start), per_unit = attn_items(c.en);
+    c.h = off0 / per_unit;
+    c.i = off0 % per_unit - ATTN_HEAD;
+    long long unit0 = s_start + static_cast<long long>(c.h) * per_unit;
+    int left = items, n = 0, unit = 0, issued = 0;
+    bool ok = true, in_unit = false;
+    // how many pages of the range lie in the unit that c stands in, and whether any page follows
+    while (left > 0 && ok) {
+      if (c.i < 0) {
+        const int skip = min(-c.i, left);
+        c.i += skip;
+        left -= skip;
+        continue;
+      }
+      // pages of this unit in the range, up to 32 at a time, one per lane
+      const int in_range = min(c.en.pages - c.i, left), take = min(in_range, 32);
+      if (!in_unit) {
+        in_unit = true;
+        if (lane == 0) {
+          UnitRec& u = s_unit[unit & (TC_UNITS - 1)];
+          u.first = c.en.first; u.row0 = c.en.row0; u.rows = c.en.rows; u.pos = c.en.pos;
+          u.h = c.h;
+          u.whole = c.i == 0 && in_range == c.en.pages;
+          u.slot = attn_slot_of(deal, worker, unit0 + ATTN_HEAD);
+          mbar_arrive(smem_u32(&unit_full[unit & (TC_UNITS - 1)]));   // releases the record
+        }
+        ++unit;
+      }
+      int tile = -1, exps = 127 | 127 << 8;
+      if (lane < take && c.en.last >= 0) {
+        const int b = a.tiles == 1 ? c.e : c.e / a.tiles;
+        const int p = __ldcg(a.page_table + static_cast<size_t>(b) * a.width + c.en.page0 + c.i + lane);
+        if (p >= 0 && p < a.pages) {
+          tile = p * a.hk + c.h;
+          exps = __ldcg(a.k_exp + tile) | __ldcg(a.v_exp + tile) << 8;
+        } else {
+          atomicOr(a.status, ST_BAD_PAGE);
+        }
+      }
+      const int p_first = c.en.pos + div_group(a, c.en.row0), p_last = c.en.pos + div_group(a, c.en.row0 + c.en.rows - 1);
+      const bool follows = [&] {   // does a page follow this unit's share of the range?
+        int rest = left - in_range;
+        if (rest <= 0) return false;
+        return rest > ATTN_HEAD;   // the next unit's head items come first
+      }();
+      for (int j = 0; j < take && ok; ++j) {
+        const int t = __shfl_sync(0xffffffffu, tile, j), ex = __shfl_sync(0xffffffffu, exps, j);
+        const int p0 = (c.en.page0 + c.i + j) * ATTN_PAGE;
+        const bool seg_last = j + 1 == take && take == in_range;
+        // K, then V; the record is written ahead of the K slot's arrival
+        for (int half = 0; half < 2 && ok; ++half) {
+          const int slot = issued % TC_RAW, turn = issued / TC_RAW;
+          if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_empty[slot]), (turn - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            if (half == 0) {
+              PageRec r;
+              r.tile = t;
+              const bool edge = p_first < p0 + ATTN_PAGE - 1 || (a.window > 0 && p_last - a.window + 1 > p0);
+              r.bits = ex | ((seg_last ? PAGE_SEG_LAST : 0) | (seg_last && !follows ? PAGE_RANGE_LAST : 0) |
+                             (edge ? PAGE_EDGE : 0) | (t >= 0 ? PAGE_LIVE : 0)) << 16;
+              r.p0 = p0;
+              const int lo = a.window > 0 ? max(p_first - a.window + 1 - p0, 0) : 0, hi = min(p_last - p0, ATTN_PAGE - 1);
+              r.seen = (lo > 63 ? 63 : lo) | max(hi, 0) << 8;
+              s_page[n & (TC_PAGES - 1)] = r;
+            }
+            const uint32_t bar = smem_u32(&raw_full[slot]);
+            if (t >= 0) {
+              mbar_expect_tx(bar, RAW);
+              bulk_load_1d(raw + static_cast<uint32_t>(slot) * RAW, (half ? a.v : a.k) + static_cast<size_t>(t) * RAW, RAW, bar);
+            } else {
+              mbar_arrive(bar);
+            }
+          }
+          __syncwarp();
+          ++issued;
+        }
+        ++n;
+      }
+      c.i += take;
+      left -= take;
+      if (take == in_range) {
+        in_unit = false;
+        if (left > 0) {
+          unit0 += attn_items(c.en);
+          c.i = -ATTN_HEAD;
+          if (++c.h == a.hk) {
+            c.h = 0;
+            do {
+              if (++c.e >= entries) {
+                left = 0;
+                break;
+              }
+              c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
+            } while (c.en.pages == 0);
+          }
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
+      s_abort = 1;
+      for (int i = issued > TC_RAW ? issued - TC_RAW : 0; i < issued; ++i) mbar_wait(smem_u32(&raw_full[i % TC_RAW]), (i / TC_RAW) & 1);
+    }
+  } else if (items > 0 && items > ATTN_HEAD - static_cast<int>((f0 - s_start) % attn_items(attn_entry_of(a, s_entry, group, TC_ROWS)))) {
+    // (a range of head items alone has no page: these roles have nothing to wait for)
+    bool ok = true;
+    // A wait of the whole warp: all lanes come back with the same answer, and together.
+    auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity)) != 0; };
+    if (warp == 1) {
+      // ---- MMA
+      if (lane == 0) {
+        constexpr uint32_t id_s = umma_idesc_f16(TC_ROWS, ATTN_PAGE), id_o = umma_idesc_f16(TC_ROWS, D);
+        auto qk = [&](int n) {
+          const int b = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
+          ok = ok && mbar_wait(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait(smem_u32(&s_empty[b]), ph ^ 1u));
+          if (!ok) return;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16_ts(tmem + COL_S + b * ATTN_PAGE, tmem + COL_Q + 8 * k, umma_desc_k_sw128(k16 + b * F16 + (k / 4) * (ATTN_PAGE * 128)) + 2 * (k % 4), id_s,
+                        k > 0 ? 1u : 0u);
+          umma_commit(smem_u32(&qk_done[b]));
+        };
+        auto pv = [&](int n) {
+          const int b = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
+          ok = ok && mbar_wait(smem_u32(&p_full[b]), ph) && mbar_wait(smem_u32(&vf_full[b]), ph) && (n < 2 || mbar_wait(smem_u32(&o_empty[b]), ph ^ 1u));
+          if (!ok) return;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < ATTN_PAGE / 16; ++k)
+            umma_f16_ts(tmem + COL_O + b * D, tmem + COL_P + b * (ATTN_PAGE / 2) + 8 * k, umma_desc_k_sw128(v16 + b * F16) + 2 * k, id_o, k > 0 ? 1u : 0u);
+          umma_commit(smem_u32(&pv_done[b]));
+        };
+        int unit = 0;
+        bool fresh = true, last = false;
+        for (int n = 0; ok && !last; ++n) {
+          const bool early = fresh && n > 0;   // while the next unit's q is on its way
+          if (early) pv(n - 1);
+          if (ok && fresh) {   // the unit's q is in tensor memory
+            ok = mbar_wait(smem_u32(&q_full), unit & 1);
+            ++unit;
+          }
+          if (ok) qk(n);
+          if (!ok) break;
+          const int bits = s_page[n & (TC_PAGES - 1)].bits >> 16;   // visible: kf_full was waited for
+          if (n > 0 && !early) pv(n - 1);
+          last = bits & PAGE_RANGE_LAST;
+          fresh = bits & PAGE_SEG_LAST;
+          if (last) pv(n);
+        }
+      }
+      __syncwarp();
+    } else if (warp < 4) {
+      // ---- codes to FP16, two warps: a thread takes 16 codes (32 bytes of FP16) at a time
+      const int ct = tid - 64;
+      bool last = false;
+      int used = 0;
+      for (int n = 0; ok && !last; ++n) {
+        const int b = n & 1;
+        const uint32_t ph = (n >> 1) & 1;
+        int slot = used % TC_RAW;
+        ok = warp_wait(raw_full[slot], (used / TC_RAW) & 1) && (n < 2 || warp_wait(qk_done[b], ph ^ 1u));
+        if (!ok) break;
+        const PageRec r = s_page[n & (TC_PAGES - 1)];
+        const int bits = r.bits >> 16;
+        last = bits & PAGE_RANGE_LAST;
+        const bool live = bits & PAGE_LIVE, edge = bits & PAGE_EDGE;
+        if (live) {
+          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW;
+          constexpr int PIECES = D / 16;   // 16-code pieces of a token
+#pragma unroll 4
+          for (int it = ct; it < ATTN_PAGE * PIECES; it += 64) {
+            const int piece = it % PIECES, tok = it / PIECES, half = piece / 4, j = (piece % 4) * 2;
+            const uint4 x = lds16(src + static_cast<uint32_t>(it) * 16);
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[2 * i] = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu));
+              o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
+            }
+            const uint32_t row = k16 + b * F16 + static_cast<uint32_t>(half) * (ATTN_PAGE * 128) + static_cast<uint32_t>(tok) * 128;
+            const uint32_t c0 = row + ((j ^ (tok & 7)) << 4), c1 = row + (((j + 1) ^ (tok & 7)) << 4);
+            if (half == 0) {   // the two halves' lanes write even and odd chunks in turn: no bank twice
+              sts16(c0, o[0], o[1], o[2], o[3]);
+              sts16(c1, o[4], o[5], o[6], o[7]);
+            } else {
+              sts16(c1, o[4], o[5], o[6], o[7]);
+              sts16(c0, o[0], o[1], o[2], o[3]);
+            }
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&raw_empty[slot]));
+          mbar_arrive(smem_u32(&kf_full[b]));
+        }
+        ++used;
+        slot = used % TC_RAW;
+        ok = warp_wait(raw_full[slot], (used / TC_RAW) & 1) && (n < 2 || warp_wait(pv_done[b], ph ^ 1u));
+        if (!ok) break;
+        {
+          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW;
+          const int lo = r.seen & 255, hi = r.seen >> 8;
+          uint32_t any = 0;
+#pragma unroll 4
+          for (int it = ct; it < D * 4; it += 64) {
+            const int piece = it & 3, dim = it >> 2;
+            uint4 x = live ? lds16(src + static_cast<uint32_t>(it) * 16) : make_uint4(0u, 0u, 0u, 0u);
+            uint32_t u[4] = {x.x, x.y, x.z, x.w};
+            if (edge) {
+              // Tokens that no row sees may hold anything: zero. NaN that only some rows see: zero here, and noted.
+              uint32_t noted = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int from = max(lo - (16 * piece + 4 * i), 0), to = min(hi - (16 * piece + 4 * i), 3);
+                u[i] &= from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
+                const uint32_t bad = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                u[i] &= ~((bad >> 7) * 0xffu);
+                noted |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
+              }
+              s_nan[n & 3][dim][piece] = static_cast<unsigned short>(noted);
+              any |= noted;
+            }
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[2 * i] = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu));
+              o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
+            }
+            const uint32_t row = v16 + b * F16 + static_cast<uint32_t>(dim) * 128;
+            sts16(row + (((2 * piece) ^ (dim & 7)) << 4), o[0], o[1], o[2], o[3]);
+            sts16(row + (((2 * piece + 1) ^ (dim & 7)) << 4), o[4], o[5], o[6], o[7]);
+          }
+          const int some = __any_sync(0xffffffffu, any != 0);
+          if (lane == 0) s_has_nan[n & 3][warp - 2] = some;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&raw_empty[slot]));
+          mbar_arrive(smem_u32(&vf_full[b]));
+        }
+        ++used;
+      }
+    } else if (warp < 8) {
+      // ---- softmax: a thread per row
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      bool last = false;
+      int unit = 0, n = 0;
+      while (ok && !last) {
+        const int us = unit & (TC_UNITS - 1);
+        ok = warp_wait(unit_full[us], (unit / TC_UNITS) & 1);
+        if (!ok) break;
+        const UnitRec u = s_unit[us];
+        const bool there = row < u.rows;
+        const int rr = u.row0 + row, tk = div_group(a, rr), pos = u.pos + tk;
+        float f_row;
+        {   // q to tensor memory: FP16 under a power of two, the row's largest value to [2^9, 2^10)
+          const __nv_bfloat16* src = a.q + static_cast<size_t>(u.first + tk) * a.ld_q + static_cast<size_t>(u.h * group + rr - tk * group) * D;
+          uint4 w[D / 8];
+          float amax = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) w[i] = there ? __ldcg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(finite_abs(bf16lo_f32(x[k])), finite_abs(bf16hi_f32(x[k]))));
+          }
+          const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 9, 100), -100);
+          const float down = exp2_byte(127 - e);
+          f_row = a.scale_log2 * exp2_byte(127 + e);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const uint4& v = w[4 * i + k / 4];
+              const uint32_t x = (k & 3) == 0 ? v.x : (k & 3) == 1 ? v.y : (k & 3) == 2 ? v.z : v.w;
+              p[k] = pack_half2(bf16lo_f32(x) * down, bf16hi_f32(x) * down);
+            }
+            tmem_st16(tmem + lanes + COL_Q + 16 * i, p);
+          }
+          tmem_store_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&q_full));
+        }
+        float mx = -INFINITY, l = 0.f;
+        bool seg_last = false;
+        for (; ok && !seg_last; ++n) {
+          const int b = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
+          ok = warp_wait(qk_done[b], ph);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const PageRec r = s_page[n & (TC_PAGES - 1)];
+          const int bits = r.bits >> 16;
+          seg_last = bits & PAGE_SEG_LAST;
+          last = bits & PAGE_RANGE_LAST;
+          uint32_t s[2][32];
+          tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE, s[0]);
+          tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + 32, s[1]);
+          tmem_ld_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&s_empty[b]));
+          const float f = f_row * exp2_byte(r.bits & 255);
+          if (!(bits & PAGE_LIVE)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) s[i >> 5][i & 31] = 0xff800000u;
+          } else if (bits & PAGE_EDGE) {
+            const int lim = there ? pos - r.p0 : -1, low = a.window > 0 ? pos - a.window + 1 - r.p0 : 0;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i > lim || i < low) s[i >> 5][i & 31] = 0xff800000u;
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i >> 5][i & 31]));
+          const float m_new = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f, mx);
+          const float base2 = m_new == -INFINITY ? 0.f : m_new, alpha = exp2_fast(mx - base2);
+          mx = m_new;
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            const float e0 = exp2_fast(fmaf(__uint_as_float(s[i >> 5][i & 31]), f, -base2)), e1 = exp2_fast(fmaf(__uint_as_float(s[i >> 5][(i + 1) & 31]), f, -base2));
+            l4[(i >> 1) & 3] += e0 + e1;
+            p[i >> 1] = pack_half2(e0, e1);
+          }
+          l = fmaf(l, alpha, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+          s_alpha[n & 3][row] = alpha;
+          if (n >= 2) ok = warp_wait(pv_done[b], ph ^ 1u);   // the P buffer's last reader
+          if (!ok) break;
+          tc_fence_after_sync();
+          tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2), p);
+          tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + 16, p + 16);
+          tmem_store_wait();
+          if (seg_last) {
+            s_fin[unit & 7][0][row] = mx;
+            s_fin[unit & 7][1][row] = l;
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (seg_last) mbar_arrive(smem_u32(&fin_full[unit & 7]));
+            mbar_arrive(smem_u32(&p_full[b]));
+          }
+        }
+        ++unit;
+      }
+    } else {
+      // ---- sums and output: a thread per row
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      bool last = false;
+      int unit = 0;
+      float o[D];
+#pragma unroll
+      for (int i = 0; i < D; ++i) o[i] = 0.f;
+      for (int n = 0; ok && !last; ++n) {
+        const int b = n & 1;
+        const uint32_t ph = (n >> 1) & 1;
+        ok = warp_wait(pv_done[b], ph);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const PageRec r = s_page[n & (TC_PAGES - 1)];
+        const int bits = r.bits >> 16;
+        last = bits & PAGE_RANGE_LAST;
+        const float alpha = s_alpha[n & 3][row], vs = exp2_byte(r.bits >> 8 & 255);
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < D; ++i) o[i] *= alpha;
+        }
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(tmem + lanes + COL_O + b * D + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c + i] = fmaf(__uint_as_float(v[i]), vs, o[c + i]);
+        }
+        if ((bits & PAGE_EDGE) && (s_has_nan[n & 3][0] | s_has_nan[n & 3][1])) {
+          // rows that see a token with NaN in a dimension have NaN there
+          const UnitRec& u = s_unit[unit & (TC_UNITS - 1)];
+          const int pos = u.pos + div_group(a, u.row0 + row), lim = min(pos - r.p0, ATTN_PAGE - 1), low = a.window > 0 ? max(pos - a.window + 1 - r.p0, 0) : 0;
+          unsigned long long sees = 0;
+          if (row < u.rows && lim >= low) sees = (~0ull >> (63 - lim)) & (~0ull << low);
+#pragma unroll
+          for (int i = 0; i < D; ++i) {
+            const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&s_nan[n & 3][i][0]);
+            if (bad & sees) o[i] = __uint_as_float(0x7fffffffu);
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&o_empty[b]));
+        if (!(bits & PAGE_SEG_LAST)) continue;
+        ok = warp_wait(fin_full[unit & 7], (unit >> 3) & 1);
+        if (!ok) break;
+        const UnitRec u = s_unit[unit & (TC_UNITS - 1)];
+        if (row < u.rows) {
+          const float m = s_fin[unit & 7][0][row], l = s_fin[unit & 7][1][row];
+          if (u.whole) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;   // no token seen: the row is zero
+            const int rr = u.row0 + row, tk = div_group(a, rr), col = (u.h * group + rr - tk * group) * D;
+#pragma unroll
+            for (int c = 0; c < D; c += 8) {
+              float x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = o[c + i] * inv;
+              store8(a, u.first + tk, col + c, x);
+            }
+          } else {
+            float* slot = a.part + static_cast<size_t>(u.slot) * attn_slot_floats(D, TC_ROWS);
+            slot[row] = m;
+            slot[TC_ROWS + row] = l;
+            float4* dst = reinterpret_cast<float4*>(slot + 2 * TC_ROWS + static_cast<size_t>(row) * D);
+#pragma unroll
+            for (int c = 0; c < D; c += 4) dst[c / 4] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < D; ++i) o[i] = 0.f;
+        ++unit;
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
+      s_abort = 1;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+template <int D>
+static cudaError_t tc_launch(const AttnArgs& a, int sms, cudaStream_t stream) {
+  const size_t smem = tc_smem_bytes(D) > TC_MIN_SMEM ? tc_smem_bytes(D) : TC_MIN_SMEM;
+  static DeviceOnce once;
+  cudaError_t e = cudaSuccess;
+  if (once.first()) e = cudaFuncSetAttribute(cache_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  once.done();
+  return launch_dependent(cache_attn_tc_kernel<D>, dim3(sms), dim3(TC_THREADS), smem, stream, a);
+}
+
+cudaError_t cache_attn_tc_launch(const AttnArgs& a, int dim, int sms, cudaStream_t stream) {
+  return dim == 128 ? tc_launch<128>(a, sms, stream) : tc_launch<64>(a, sms, stream);
+}
+
+}  // namespace muse
