@@ -61,32 +61,33 @@ __host__ __device__ inline AttnEntry attn_entry(int cu0, int cu1, int len, int m
 
 // `total` items dealt to `workers` in equal ranges: the first `rem` workers get one more. With fewer items than workers
 // only `total` workers take part, with one item each.
-struct AttnDeal {
-  long long total, base, rem;
+struct AttnDeal {   // (the host sees to it that a call's items fit 31 bits)
+  int total, base, rem;
   int workers;   // those that take part
 };
-__host__ __device__ inline AttnDeal attn_deal(long long total, int workers) {
+__host__ __device__ inline AttnDeal attn_deal(int total, int workers) {
   AttnDeal d;
   d.total = total;
-  d.workers = total < workers ? static_cast<int>(total) : workers;
-  d.base = d.workers > 0 ? total / d.workers : 0;
+  d.workers = total < workers ? total : workers;
+  d.base = d.workers > 0 ? static_cast<int>(static_cast<unsigned>(total) / static_cast<unsigned>(d.workers)) : 0;
   d.rem = total - d.base * d.workers;
   return d;
 }
 // First item of worker w's range (w = workers: the end).
-__host__ __device__ inline long long attn_range(const AttnDeal& d, int w) { return d.base * w + (w < d.rem ? w : d.rem); }
+__host__ __device__ inline int attn_range(const AttnDeal& d, int w) { return d.base * w + (w < d.rem ? w : d.rem); }
 // The worker whose range holds item f.
-__host__ __device__ inline int attn_worker(const AttnDeal& d, long long f) {
-  const long long big = d.rem * (d.base + 1);
-  return static_cast<int>(f < big ? f / (d.base + 1) : d.rem + (f - big) / d.base);
+__host__ __device__ inline int attn_worker(const AttnDeal& d, int f) {
+  const int big = d.rem * (d.base + 1);   // below total
+  const unsigned div = static_cast<unsigned>(f < big ? d.base + 1 : d.base), from = static_cast<unsigned>(f < big ? f : f - big);
+  return (f < big ? 0 : d.rem) + static_cast<int>(from / div);
 }
 // Where worker w left its partial sums of the unit whose first page is item u0 (the caller knows that w has some of its
 // pages, and not all): a worker has at most two partial segments, one of a unit whose first page lies at or before its
 // range (slot 0) and one of a unit that begins inside it (slot 1).
-__host__ __device__ inline int attn_slot_of(const AttnDeal& d, int w, long long u0) { return 2 * w + (attn_range(d, w) >= u0 ? 0 : 1); }
+__host__ __device__ inline int attn_slot_of(const AttnDeal& d, int w, int u0) { return 2 * w + (attn_range(d, w) >= u0 ? 0 : 1); }
 // Workers that are the warps of a CTA, `per` of them from w on (a multiple of per), add their sums up on chip when
 // nothing but this one unit's pages [u0, u1) is theirs; the sums are then in the first one's slot 0.
-__host__ __device__ inline bool attn_merged(const AttnDeal& d, int w, int per, long long u0, long long u1) {
+__host__ __device__ inline bool attn_merged(const AttnDeal& d, int w, int per, int u0, int u1) {
   return per > 1 && w + per <= d.workers && attn_range(d, w) >= u0 && attn_range(d, w + per) <= u1;
 }
 // The partial sums of a split unit, in page order: slot(i) for i = 0 .. parts - 1. Workers w0 .. w1 have the unit's
@@ -96,7 +97,7 @@ struct AttnParts {
   int head, groups, parts;   // single workers in front, groups behind them; the rest is single again
   int first_slot;
 };
-__host__ __device__ inline AttnParts attn_parts(const AttnDeal& d, int per, long long u0, int pages) {
+__host__ __device__ inline AttnParts attn_parts(const AttnDeal& d, int per, int u0, int pages) {
   AttnParts p;
   p.per = per;
   p.w0 = attn_worker(d, u0);

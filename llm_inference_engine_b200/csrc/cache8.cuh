@@ -39,7 +39,7 @@ struct AttnArgs {
   const __nv_bfloat16* gate;   // [m, hq D], ld_gate elements between tokens, or null
   __nv_bfloat16* out;          // [m, hq D], ld_out elements between tokens
   float* part;                 // partial sums: 2 slots per worker
-  long long* prefix;           // [entries + 1] first page of each entry in the list (per head: pages)
+  int* prefix;                 // [entries + 1] first item of each entry in the list, and their number
   int* status;
   long long ld_q, ld_gate, ld_out;
   float scale_log2;            // softmax scale * log2(e)

@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   constexpr uint32_t SLOT_BYTES = ATTN_PAGE * D;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bar_full[attn_slots(D) * ATTN_WARPS];
-  __shared__ long long s_sum[ATTN_WARPS];
+  __shared__ int s_sum[ATTN_WARPS];
   __shared__ int s_entry[ATTN_WARPS];
-  __shared__ long long s_start[ATTN_WARPS];
+  __shared__ int s_start[ATTN_WARPS];
   __shared__ __align__(16) float s_stage[ATTN_WARPS][8 * STAGE_LD];   // rows on their way out
   __shared__ int2 s_rec[ATTN_WARPS][64];   // looked-up pages: tile index in the pool, exponents (k | v << 8)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -454,26 +454,26 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   // each share begins; the thread whose share holds a worker's first item finds the entry.
   const int per = (entries + ATTN_THREADS - 1) / ATTN_THREADS;
   const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
-  long long mine = 0;
-  auto items_of = [&](int e) { return static_cast<long long>(attn_items(attn_entry_of(a, e, group, TILE))) * a.hk; };
+  int mine = 0;
+  auto items_of = [&](int e) { return attn_items(attn_entry_of(a, e, group, TILE)) * a.hk; };
   for (int e = e0; e < e1; ++e) {
     mine += items_of(e);
     if (blockIdx.x == 0) attn_report_bad(a, e);
   }
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, s);
+    const int up = __shfl_up_sync(0xffffffffu, incl, s);
     if (lane >= s) incl += up;
   }
   if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  long long base = 0, total = 0;
+  int base = 0, total = 0;
   for (int w = 0; w < ATTN_WARPS; ++w) {
     if (w < warp) base += s_sum[w];
     total += s_sum[w];
   }
-  const long long begin = base + incl - mine, end = base + incl;   // this thread's share of the list
+  const int begin = base + incl - mine, end = base + incl;   // this thread's share of the list
   const AttnDeal deal = attn_deal(total, static_cast<int>(gridDim.x * ATTN_WARPS));
   // Neighbouring workers are a CTA's warps, so that sums of a long unit meet on chip; a list with few items is spread over
   // the SMs instead.
@@ -482,12 +482,12 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   if (total > 0) {
     for (int w = 0; w < ATTN_WARPS; ++w) {
       if (worker_of(w) >= deal.workers) break;
-      const long long f = attn_range(deal, worker_of(w));
+      const int f = attn_range(deal, worker_of(w));
       if (f >= begin && f < end) {
-        long long at = begin;
+        int at = begin;
         int e = e0;
         for (; e + 1 < e1; ++e) {
-          const long long next = at + items_of(e);
+          const int next = at + items_of(e);
           if (f < next) break;
           at = next;
         }
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       }
     }
     if (blockIdx.x == 0) {   // for the kernel that adds up the partial sums
-      long long at = begin;
+      int at = begin;
       for (int e = e0; e < e1; ++e) {
         a.prefix[e] = at;
         if (e + 1 < e1) at += items_of(e);
@@ -507,20 +507,19 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
   __syncthreads();
   const int worker = worker_of(warp);
   if (worker >= deal.workers) return;   // no item, and no warp waits for this one (a merging CTA's all have some)
-  const long long f0 = attn_range(deal, worker);
-  const int items = static_cast<int>(attn_range(deal, worker + 1) - f0);
+  const int f0 = attn_range(deal, worker), items = attn_range(deal, worker + 1) - f0;
 
   EntryCache rd_cache, fill_cache;
   rd_cache.base = fill_cache.base = -64;
   Cursor rd, fill;   // where the warp computes, and up to where it has looked up pages
-  long long unit0;   // first item of the unit that rd stands in
+  int unit0;         // first item of the unit that rd stands in
   {
     fill.e = s_entry[warp];
     fill.en = attn_entry_cached(a, fill_cache, fill.e, entries, group, TILE);
-    const int off = static_cast<int>(f0 - s_start[warp]), per_unit = attn_items(fill.en);
+    const int off = f0 - s_start[warp], per_unit = attn_items(fill.en);
     fill.h = off / per_unit;
     fill.i = off % per_unit - ATTN_HEAD;
-    unit0 = s_start[warp] + static_cast<long long>(fill.h) * per_unit;
+    unit0 = s_start[warp] + fill.h * per_unit;
     rd_cache = fill_cache;
     rd = fill;
   }
@@ -576,7 +575,6 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     if (pend_tile > -2) s_rec[warp][pend_at & 63].y = e;
     __syncwarp();
   };
-  look_up();
 
   int issued = 0, used = 0;               // halves (K, then V of a page) requested and consumed by this worker
   // Requests the next half.
@@ -594,14 +592,10 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     }
     ++issued;
   };
-  // The warp has read a half: its slot may be filled again.
-  auto release = [&]() {
-    __syncwarp();
-    ++used;
+  // Fills the slots that are free.
+  auto pump = [&]() {
     while (issued < used + SLOTS && (issued >> 1) < filled) request();
   };
-  while (issued < SLOTS && (issued >> 1) < filled) request();
-  look_up_exponents();
 
   TileState<D, NT> st;
   uint32_t qf[NT][D / 16][2];
@@ -620,6 +614,12 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       continue;
     }
     const int my_rows = rd.en.rows;
+    // Pages are looked up 32 at a time, while the records of those under way stay (the ring of records holds 64); their
+    // copies are asked for before their exponents.
+    const bool look = fill_left > 0 && filled - n <= SLOTS / 2 + 2;
+    if (look) look_up();
+    pump();
+    if (look) look_up_exponents();
     if (fresh) {
       tile_reset(st);
       const int r0 = rd.en.row0, t = lane & 3;
@@ -644,24 +644,21 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       fresh = false;
       seg_first = rd.i;
     }
-    // records: looked up 32 at a time, while those of the pages under way stay (the ring of records holds 64)
-    if (fill_left > 0 && filled - n <= SLOTS / 2 + 2) {
-      look_up();
-      look_up_exponents();
-    }
     const int2 rec = s_rec[warp][n & 63];
     const bool live = rec.x >= 0;
     const int p0 = (rd.en.page0 + rd.i) * ATTN_PAGE;
     // some row does not see some token of the page (positions grow with the row)
     const bool edge = ri.first < p0 + ATTN_PAGE - 1 || (a.window > 0 && ri.last - a.window + 1 > p0);
     const int ks = used % SLOTS, vsl = (used + 1) % SLOTS, vt = (used + 1) / SLOTS;
-    bool ok = mbar_wait(smem_u32(&full[ks]), (used / SLOTS) & 1), moved = false;
+    bool ok = mbar_wait_short(smem_u32(&full[ks]), (used / SLOTS) & 1), moved = false;
     float s[4][NT][4], al[NT][2];
     uint32_t p[4][NT][2];
     if (ok && live) page_scores<D, NT>(s, qf, ring_base + static_cast<uint32_t>(ks) * SLOT_BYTES);
-    release();
+    __syncwarp();
+    ++used;   // the K slot may be filled again
+    pump();
     if (ok && live) page_softmax<D, NT>(st, s, p, al, moved, qs, exp2_byte(rec.y & 255), ri, p0, a.window, edge);
-    ok = ok && mbar_wait(smem_u32(&full[vsl]), vt & 1);
+    ok = ok && mbar_wait_short(smem_u32(&full[vsl]), vt & 1);
     if (!ok) {
       gave_up = true;
       break;
@@ -672,7 +669,8 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
       if (page_pv<D, NT>(st, p, vs, al, moved, vscale, edge, a.window > 0 ? ri.first - a.window + 1 - p0 : 0, ri.last - p0))
         page_nan<D, NT>(st, vs, ri, p0, a.window);
     }
-    release();
+    __syncwarp();
+    ++used;
     ++n;
     --left;
     // end of the unit or of the range: the segment [seg_first, rd.i] is done
@@ -720,10 +718,10 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   const AttnEntry en = attn_entry_of(a, e, group, TILE);
   griddep_launch_dependents();
   griddep_wait();
-  const long long total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
+  const int total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
   if (r0 >= en.rows) return;
   const AttnDeal deal = attn_deal(total, workers);
-  const long long u0 = start + static_cast<long long>(h) * attn_items(en) + ATTN_HEAD;
+  const int u0 = start + h * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;   // one worker had all of the unit's pages and has written it
   const AttnParts ps = attn_parts(deal, TILE > 16 || total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
   // The lane's two rows and where its quad of sums lies in a part. Tiles of 128 rows are kept by rows: a quad is then four
@@ -817,7 +815,7 @@ long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim) {
   const int sms = device_sms();
   if (batch < 1 || max_q < 1 || hk < 1 || hq < hk || hq % hk || (dim != 64 && dim != 128) || sms < 1) return -1;
   const AttnForm f = attn_form(max_q, hq, hk);
-  return 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile) * 4 + (static_cast<long long>(batch) * f.tiles + 1) * 8;
+  return 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile) * 4 + (static_cast<long long>(batch) * f.tiles + 1) * 4;
 }
 
 template <int D, int NT>
@@ -866,9 +864,10 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   a.vec_out = a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   a.group_magic = static_cast<uint32_t>((1ull << 32) / static_cast<unsigned>(a.group) + 1);
   if (static_cast<long long>(f.tiles) * f.tile * a.group >= 1ll << 32) return -3;
-  if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
+  // items of the list, at most; and indices of the pool's tiles
+  if (static_cast<long long>(a.batch) * a.tiles * a.hk > 0x7fffffffll / (a.width + ATTN_HEAD) || static_cast<long long>(a.pages) * a.hk > 0x7fffffffll) return -3;
   a.part = static_cast<float*>(ws);
-  a.prefix = reinterpret_cast<long long*>(a.part + 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile));
+  a.prefix = reinterpret_cast<int*>(a.part + 2ll * f.workers(sms) * attn_slot_floats(dim, f.tile));
   const cudaError_t e = dim == 128 ? both_launch<128>(a, f, sms, stream) : both_launch<64>(a, f, sms, stream);
   return static_cast<int>(e);
 }
@@ -878,7 +877,7 @@ namespace {
 struct HostPlan {
   AttnForm form;
   int group, entries;
-  long long total;
+  int total;
   bool ok;
 };
 }  // namespace
@@ -890,6 +889,7 @@ static HostPlan host_plan(const int* seq_lens, int m, int batch, int width, int 
   p.form = attn_form(max_q, hq, hk);
   p.group = hq / hk;
   p.entries = batch * p.form.tiles;
+  p.ok = static_cast<long long>(p.entries) * hk <= 0x7fffffffll / (width + ATTN_HEAD);
   return p;
 }
 static AttnEntry host_entry(const HostPlan& p, const int* seq_lens, const int* cu_q, int m, int width, int max_q, int window, int e) {
@@ -901,28 +901,29 @@ long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch
                           int* segments, long long capacity) {
   HostPlan p = host_plan(seq_lens, m, batch, width, max_q, hq, hk, window, sms);
   if (!p.ok || !segments) return -1;
-  for (int e = 0; e < p.entries; ++e) p.total += static_cast<long long>(attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e))) * hk;
+  for (int e = 0; e < p.entries; ++e) p.total += attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e)) * hk;
   if (p.total == 0) return 0;
   const AttnDeal deal = attn_deal(p.total, p.form.workers(sms));
-  long long count = 0, start = 0;
+  long long count = 0;
+  int start = 0;
   int e = 0;
   AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, 0);
   for (int w = 0; w < deal.workers; ++w) {
-    for (long long f = attn_range(deal, w), f1 = attn_range(deal, w + 1); f < f1;) {
-      while (f >= start + static_cast<long long>(attn_items(en)) * hk) {
-        start += static_cast<long long>(attn_items(en)) * hk;
+    for (int f = attn_range(deal, w), f1 = attn_range(deal, w + 1); f < f1;) {
+      while (f >= start + attn_items(en) * hk) {
+        start += attn_items(en) * hk;
         en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, ++e);
       }
-      const int off = static_cast<int>(f - start), h = off / attn_items(en), i = off % attn_items(en) - ATTN_HEAD;
+      const int off = f - start, h = off / attn_items(en), i = off % attn_items(en) - ATTN_HEAD;
       if (i < 0) {
         ++f;
         continue;
       }
-      const int n = static_cast<int>(f1 - f < en.pages - i ? f1 - f : en.pages - i);
+      const int n = f1 - f < en.pages - i ? f1 - f : en.pages - i;
       if (count < capacity) {
         int* s = segments + 6 * count;
         s[0] = w; s[1] = e; s[2] = h; s[3] = en.page0 + i; s[4] = n;
-        const long long u0 = start + static_cast<long long>(h) * attn_items(en) + ATTN_HEAD;
+        const int u0 = start + h * attn_items(en) + ATTN_HEAD;
         const int per = p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, first = w - w % per;
         s[5] = n == en.pages ? -1 : attn_merged(deal, first, per, u0, u0 + en.pages) ? 2 * first : attn_slot_of(deal, w, u0);
       }
@@ -937,15 +938,15 @@ long long cache_attn_join(const int* seq_lens, const int* cu_q, int m, int batch
                           int entry, int head, int* slots, long long capacity) {
   HostPlan p = host_plan(seq_lens, m, batch, width, max_q, hq, hk, window, sms);
   if (!p.ok || !slots || entry < 0 || entry >= p.entries || head < 0 || head >= hk) return -1;
-  long long before = 0;
+  int before = 0;
   for (int e = 0; e < p.entries; ++e) {
     if (e == entry) before = p.total;
-    p.total += static_cast<long long>(attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e))) * hk;
+    p.total += attn_items(host_entry(p, seq_lens, cu_q, m, width, max_q, window, e)) * hk;
   }
   const AttnEntry en = host_entry(p, seq_lens, cu_q, m, width, max_q, window, entry);
   if (en.rows == 0) return 0;
   const AttnDeal deal = attn_deal(p.total, p.form.workers(sms));
-  const long long u0 = before + static_cast<long long>(head) * attn_items(en) + ATTN_HEAD;
+  const int u0 = before + head * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return 0;
   const AttnParts ps = attn_parts(deal, p.form.shared || p.total <= attn_spread_below(sms) ? 1 : ATTN_WARPS, u0, en.pages);
   for (int i = 0; i < ps.parts && i < capacity; ++i) slots[i] = attn_part_slot(ps, i);

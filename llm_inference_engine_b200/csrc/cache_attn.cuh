@@ -71,7 +71,7 @@ __device__ __forceinline__ void attn_report_bad(const AttnArgs& a, int e) {
   if (bad) atomicOr(a.status, ST_BAD_LENGTH);
 }
 
-__device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid_f32(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }   // 1 + e^-x beyond 2^126: 0, as it should be
 
 // Eight neighbouring output values, gated.
 __device__ __forceinline__ void store8(const AttnArgs& a, size_t tok, int col, float (&x)[8]) {
@@ -106,6 +106,11 @@ __device__ __forceinline__ void store8(const AttnArgs& a, size_t tok, int col, f
     for (int i = 0; i < 8; ++i) o[i] = __float2bfloat16_rn(x[i]);
   }
 }
+
+// A wait that usually finds its phase complete: only the first look is inline (the instruction cache is what these kernels
+// are short of).
+static __noinline__ __device__ bool mbar_wait_on(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity); }
+__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || mbar_wait_on(bar, parity); }
 
 cudaError_t cache_attn_tc_launch(const AttnArgs& a, int dim, int sms, cudaStream_t stream);   // cache_attn_tc.cu
 

@@ -76,6 +76,13 @@ __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// store8 as a call: written out for every eight of a row's dimensions it would be most of the kernel's code.
+static __noinline__ __device__ void store8_call(const AttnArgs& a, size_t tok, int col, float x0, float x1, float x2, float x3, float x4, float x5, float x6,
+                                                float x7) {
+  float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+  store8(a, tok, col, x);
+}
+
 template <int D>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
   constexpr uint32_t RAW = ATTN_PAGE * D, F16 = ATTN_PAGE * D * 2;
@@ -90,9 +97,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   __shared__ float s_alpha[4][TC_ROWS], s_fin[8][2][TC_ROWS];
   __shared__ __align__(8) unsigned short s_nan[4][D][4];      // edge pages: the tokens of each dimension that hold NaN
   __shared__ int s_has_nan[4][2];
-  __shared__ long long s_sum[TC_THREADS / 32];
+  __shared__ int s_sum[TC_THREADS / 32];
   __shared__ int s_entry;
-  __shared__ long long s_start;
+  __shared__ int s_start;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -130,16 +137,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   // The list of items, as in cache_attn_kernel.
   const int per = (entries + TC_THREADS - 1) / TC_THREADS;
   const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
-  auto items_of = [&](int e) { return static_cast<long long>(attn_items(attn_entry_of(a, e, group, TC_ROWS))) * a.hk; };
-  long long mine = 0;
+  auto items_of = [&](int e) { return attn_items(attn_entry_of(a, e, group, TC_ROWS)) * a.hk; };
+  int mine = 0;
   for (int e = e0; e < e1; ++e) {
     mine += items_of(e);
     if (blockIdx.x == 0) attn_report_bad(a, e);
   }
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, s);
+    const int up = __shfl_up_sync(0xffffffffu, incl, s);
     if (lane >= s) incl += up;
   }
   if (lane == 31) s_sum[warp] = incl;
@@ -147,21 +154,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  long long base = 0, total = 0;
+  int base = 0, total = 0;
   for (int w = 0; w < TC_THREADS / 32; ++w) {
     if (w < warp) base += s_sum[w];
     total += s_sum[w];
   }
-  const long long begin = base + incl - mine, end = base + incl;
+  const int begin = base + incl - mine, end = base + incl;
   const AttnDeal deal = attn_deal(total, static_cast<int>(gridDim.x));
   const int worker = blockIdx.x;
-  const long long f0 = worker < deal.workers ? attn_range(deal, worker) : 0;
-  const int items = worker < deal.workers ? static_cast<int>(attn_range(deal, worker + 1) - f0) : 0;
+  const int f0 = worker < deal.workers ? attn_range(deal, worker) : 0;
+  const int items = worker < deal.workers ? attn_range(deal, worker + 1) - f0 : 0;
   if (items > 0 && f0 >= begin && f0 < end) {
-    long long at = begin;
+    int at = begin;
     int e = e0;
     for (; e + 1 < e1; ++e) {
-      const long long next = at + items_of(e);
+      const int next = at + items_of(e);
       if (f0 < next) break;
       at = next;
     }
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
     s_start = at;
   }
   if (blockIdx.x == 0) {
-    long long at = begin;
+    int at = begin;
     for (int e = e0; e < e1; ++e) {
       a.prefix[e] = at;
       if (e + 1 < e1) at += items_of(e);
@@ -185,10 +192,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
     Cursor c;
     c.e = s_entry;
     c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
-    const int off0 = static_cast<int>(f0 - s_start), per_unit = attn_items(c.en);
+    const int off0 = f0 - s_start, per_unit = attn_items(c.en);
     c.h = off0 / per_unit;
     c.i = off0 % per_unit - ATTN_HEAD;
-    long long unit0 = s_start + static_cast<long long>(c.h) * per_unit;
+    int unit0 = s_start + c.h * per_unit;
     int left = items, n = 0, unit = 0, issued = 0;
     bool ok = true, in_unit = false;
     // how many pages of the range lie in the unit that c stands in, and whether any page follows
@@ -291,11 +298,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
       s_abort = 1;
       for (int i = issued > TC_RAW ? issued - TC_RAW : 0; i < issued; ++i) mbar_wait(smem_u32(&raw_full[i % TC_RAW]), (i / TC_RAW) & 1);
     }
-  } else if (items > 0 && items > ATTN_HEAD - static_cast<int>((f0 - s_start) % attn_items(attn_entry_of(a, s_entry, group, TC_ROWS)))) {
+  } else if (items > 0 && items > ATTN_HEAD - (f0 - s_start) % attn_items(attn_entry_of(a, s_entry, group, TC_ROWS))) {
     // (a range of head items alone has no page: these roles have nothing to wait for)
     bool ok = true;
     // A wait of the whole warp: all lanes come back with the same answer, and together.
-    auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity)) != 0; };
+    auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_short(smem_u32(&bar), parity)) != 0; };
     if (warp == 1) {
       // ---- MMA
       if (lane == 0) {
@@ -303,7 +310,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         auto qk = [&](int n) {
           const int b = n & 1;
           const uint32_t ph = (n >> 1) & 1;
-          ok = ok && mbar_wait(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait(smem_u32(&s_empty[b]), ph ^ 1u));
+          ok = ok && mbar_wait_short(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&s_empty[b]), ph ^ 1u));
           if (!ok) return;
           tc_fence_after_sync();
 #pragma unroll
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         auto pv = [&](int n) {
           const int b = n & 1;
           const uint32_t ph = (n >> 1) & 1;
-          ok = ok && mbar_wait(smem_u32(&p_full[b]), ph) && mbar_wait(smem_u32(&vf_full[b]), ph) && (n < 2 || mbar_wait(smem_u32(&o_empty[b]), ph ^ 1u));
+          ok = ok && mbar_wait_short(smem_u32(&p_full[b]), ph) && mbar_wait_short(smem_u32(&vf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&o_empty[b]), ph ^ 1u));
           if (!ok) return;
           tc_fence_after_sync();
 #pragma unroll
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           const bool early = fresh && n > 0;   // while the next unit's q is on its way
           if (early) pv(n - 1);
           if (ok && fresh) {   // the unit's q is in tensor memory
-            ok = mbar_wait(smem_u32(&q_full), unit & 1);
+            ok = mbar_wait_short(smem_u32(&q_full), unit & 1);
             ++unit;
           }
           if (ok) qk(n);
@@ -583,9 +590,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           unsigned long long sees = 0;
           if (row < u.rows && lim >= low) sees = (~0ull >> (63 - lim)) & (~0ull << low);
 #pragma unroll
-          for (int i = 0; i < D; ++i) {
-            const unsigned long long bad = *reinterpret_cast<const unsigned long long*>(&s_nan[n & 3][i][0]);
-            if (bad & sees) o[i] = __uint_as_float(0x7fffffffu);
+          for (int c = 0; c < D; c += 32) {
+            uint32_t bad = 0;
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i)
+              bad |= (*reinterpret_cast<const unsigned long long*>(&s_nan[n & 3][c + i][0]) & sees) ? 1u << i : 0u;
+            if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (bad >> i & 1u) o[c + i] = __uint_as_float(0x7fffffffu);
+            }
           }
         }
         tc_fence_before_sync();
@@ -602,10 +616,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
             const int rr = u.row0 + row, tk = div_group(a, rr), col = (u.h * group + rr - tk * group) * D;
 #pragma unroll
             for (int c = 0; c < D; c += 8) {
-              float x[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = o[c + i] * inv;
-              store8(a, u.first + tk, col + c, x);
+              store8_call(a, u.first + tk, col + c, o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv, o[c + 4] * inv, o[c + 5] * inv, o[c + 6] * inv,
+                          o[c + 7] * inv);
             }
           } else {
             float* slot = a.part + static_cast<size_t>(u.slot) * attn_slot_floats(D, TC_ROWS);
