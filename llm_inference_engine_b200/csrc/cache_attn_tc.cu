@@ -11,6 +11,10 @@
 // by what the row's maximum has moved. S, P and O' are double-buffered in tensor memory (64 + 2 x 64 + 2 x 32 + 2 x 128
 // columns at D = 128), so the products of one page run under the exponentials of another.
 //
+// What this kernel is short of is the instruction cache: its first form, every loop written out, was 183 KB of code, missed
+// on 4 of 10 fetches and took 349 us where this one takes less than a third (chunk of 2 x 512 tokens against 4096, 32 query and 8 KV
+// heads). So the loops over a row's scores and over the MMAs stay loops, and what runs once per unit is out of line.
+//
 // Roles: warp 0 looks pages up and copies, warp 1 issues MMAs, warps 2 and 3 convert, warps 4..7 softmax, warps 8..11
 // sums and output. All waits are bounded.
 #include "cache_attn.cuh"
@@ -81,6 +85,36 @@ static __noinline__ __device__ void store8_call(const AttnArgs& a, size_t tok, i
                                                 float x7) {
   float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
   store8(a, tok, col, x);
+}
+
+// Scores whose bit is not set become -infinity.
+__device__ __forceinline__ void mask32(uint32_t (&v)[32], uint32_t keep) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(keep >> i & 1u)) v[i] = 0xff800000u;
+}
+// Sixteen codes to FP16.
+__device__ __forceinline__ void to_half16(const uint4& x, uint32_t (&o)[8]) {
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu));
+    o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
+  }
+}
+// Of sixteen codes, those outside [lo, hi] and those that stand for NaN become zero; returns a bit for each NaN inside.
+__device__ __forceinline__ uint32_t tame16(uint4& x, int lo, int hi) {
+  uint32_t u[4] = {x.x, x.y, x.z, x.w}, noted = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int from = max(lo - 4 * i, 0), to = min(hi - 4 * i, 3);
+    u[i] &= from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
+    const uint32_t bad = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    u[i] &= ~((bad >> 7) * 0xffu);
+    noted |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
+  }
+  x = make_uint4(u[0], u[1], u[2], u[3]);
+  return noted;
 }
 
 template <int D>
@@ -307,51 +341,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
       // ---- MMA
       if (lane == 0) {
         constexpr uint32_t id_s = umma_idesc_f16(TC_ROWS, ATTN_PAGE), id_o = umma_idesc_f16(TC_ROWS, D);
-        auto qk = [&](int n) {
-          const int b = n & 1;
-          const uint32_t ph = (n >> 1) & 1;
-          ok = ok && mbar_wait_short(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&s_empty[b]), ph ^ 1u));
-          if (!ok) return;
-          tc_fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16_ts(tmem + COL_S + b * ATTN_PAGE, tmem + COL_Q + 8 * k, umma_desc_k_sw128(k16 + b * F16 + (k / 4) * (ATTN_PAGE * 128)) + 2 * (k % 4), id_s,
-                        k > 0 ? 1u : 0u);
-          umma_commit(smem_u32(&qk_done[b]));
-        };
-        auto pv = [&](int n) {
-          const int b = n & 1;
-          const uint32_t ph = (n >> 1) & 1;
-          ok = ok && mbar_wait_short(smem_u32(&p_full[b]), ph) && mbar_wait_short(smem_u32(&vf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&o_empty[b]), ph ^ 1u));
-          if (!ok) return;
-          tc_fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < ATTN_PAGE / 16; ++k)
-            umma_f16_ts(tmem + COL_O + b * D, tmem + COL_P + b * (ATTN_PAGE / 2) + 8 * k, umma_desc_k_sw128(v16 + b * F16) + 2 * k, id_o, k > 0 ? 1u : 0u);
-          umma_commit(smem_u32(&pv_done[b]));
-        };
         int unit = 0;
         bool fresh = true, last = false;
-        for (int n = 0; ok && !last; ++n) {
-          const bool early = fresh && n > 0;   // while the next unit's q is on its way
-          if (early) pv(n - 1);
-          if (ok && fresh) {   // the unit's q is in tensor memory
-            ok = mbar_wait_short(smem_u32(&q_full), unit & 1);
-            ++unit;
+        // S of page n, then O' of page n - 1, whose weights were made meanwhile
+        for (int n = 0; ok; ++n) {
+          const int b = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
+          const bool done = last;
+          if (!done) {
+            if (fresh) ok = mbar_wait_short(smem_u32(&q_full), unit++ & 1);   // the unit's q is in tensor memory
+            ok = ok && mbar_wait_short(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&s_empty[b]), ph ^ 1u));
+            if (!ok) break;
+            tc_fence_after_sync();
+            uint64_t kd = umma_desc_k_sw128(k16 + b * F16);
+#pragma unroll 1
+            for (int k = 0; k < D / 16; ++k) {
+              umma_f16_ts(tmem + COL_S + b * ATTN_PAGE, tmem + COL_Q + 8 * k, kd, id_s, k > 0 ? 1u : 0u);
+              kd += (k & 3) == 3 ? (ATTN_PAGE * 128 / 16) - 6 : 2;   // 16 dimensions on; the next 64 are an atom of their own
+            }
+            umma_commit(smem_u32(&qk_done[b]));
+            const int bits = s_page[n & (TC_PAGES - 1)].bits >> 16;   // visible: kf_full was waited for
+            last = bits & PAGE_RANGE_LAST;
+            fresh = bits & PAGE_SEG_LAST;
           }
-          if (ok) qk(n);
-          if (!ok) break;
-          const int bits = s_page[n & (TC_PAGES - 1)].bits >> 16;   // visible: kf_full was waited for
-          if (n > 0 && !early) pv(n - 1);
-          last = bits & PAGE_RANGE_LAST;
-          fresh = bits & PAGE_SEG_LAST;
-          if (last) pv(n);
+          if (n > 0) {
+            const int b1 = b ^ 1;
+            const uint32_t ph1 = ((n - 1) >> 1) & 1;
+            ok = mbar_wait_short(smem_u32(&p_full[b1]), ph1) && mbar_wait_short(smem_u32(&vf_full[b1]), ph1) &&
+                 (n < 3 || mbar_wait_short(smem_u32(&o_empty[b1]), ph1 ^ 1u));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint64_t vd = umma_desc_k_sw128(v16 + b1 * F16);
+#pragma unroll 1
+            for (int k = 0; k < ATTN_PAGE / 16; ++k)
+              umma_f16_ts(tmem + COL_O + b1 * D, tmem + COL_P + b1 * (ATTN_PAGE / 2) + 8 * k, vd + 2 * k, id_o, k > 0 ? 1u : 0u);
+            umma_commit(smem_u32(&pv_done[b1]));
+          }
+          if (done) break;
         }
       }
       __syncwarp();
     } else if (warp < 4) {
       // ---- codes to FP16, two warps: a thread takes 16 codes (32 bytes of FP16) at a time
       const int ct = tid - 64;
+      constexpr int PIECES = D / 16;   // 16-code pieces of a token
+      // Where the thread's piece of a token's K row goes: chunks j and j + 1 of its half's 128 bytes, swizzled. The lanes of the
+      // second half write theirs in the other order: no bank twice.
+      const int piece = ct % PIECES, tok0 = ct / PIECES;
+      const bool k_swap = piece >= 4;
+      const uint32_t k_at = static_cast<uint32_t>(piece / 4) * (ATTN_PAGE * 128) + static_cast<uint32_t>(tok0) * 128 +
+                            ((((piece % 4) * 2 + (k_swap ? 1 : 0)) ^ (tok0 & 7)) << 4);
+      // and 16 tokens of a V row (a dimension)
+      const int vp = ct & 3, dim0 = ct >> 2;
+      const uint32_t v_at = static_cast<uint32_t>(dim0) * 128 + (((2 * vp) ^ (dim0 & 7)) << 4);
       bool last = false;
       int used = 0;
       for (int n = 0; ok && !last; ++n) {
@@ -365,28 +407,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         last = bits & PAGE_RANGE_LAST;
         const bool live = bits & PAGE_LIVE, edge = bits & PAGE_EDGE;
         if (live) {
-          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW;
-          constexpr int PIECES = D / 16;   // 16-code pieces of a token
-#pragma unroll 4
-          for (int it = ct; it < ATTN_PAGE * PIECES; it += 64) {
-            const int piece = it % PIECES, tok = it / PIECES, half = piece / 4, j = (piece % 4) * 2;
-            const uint4 x = lds16(src + static_cast<uint32_t>(it) * 16);
-            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-            uint32_t o[8];
+          // A thread's pieces are 64 / PIECES tokens apart, a multiple of 8: the same place in the swizzle, a fixed stride.
+          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW + static_cast<uint32_t>(ct) * 16;
+          const uint32_t dst = k16 + b * F16 + k_at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[2 * i] = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu));
-              o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
+          for (int k = 0; k < ATTN_PAGE * PIECES / 64; ++k) {
+            const uint4 x = lds16(src + k * 1024);
+            uint32_t o[8];
+            to_half16(x, o);
+            // the two halves' lanes write even and odd chunks in turn: no bank twice
+            if (k_swap) {   // (registers cannot be indexed: a select each)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t t = o[i];
+                o[i] = o[i + 4];
+                o[i + 4] = t;
+              }
             }
-            const uint32_t row = k16 + b * F16 + static_cast<uint32_t>(half) * (ATTN_PAGE * 128) + static_cast<uint32_t>(tok) * 128;
-            const uint32_t c0 = row + ((j ^ (tok & 7)) << 4), c1 = row + (((j + 1) ^ (tok & 7)) << 4);
-            if (half == 0) {   // the two halves' lanes write even and odd chunks in turn: no bank twice
-              sts16(c0, o[0], o[1], o[2], o[3]);
-              sts16(c1, o[4], o[5], o[6], o[7]);
-            } else {
-              sts16(c1, o[4], o[5], o[6], o[7]);
-              sts16(c0, o[0], o[1], o[2], o[3]);
-            }
+            sts16(dst + k * (64 / PIECES) * 128, o[0], o[1], o[2], o[3]);
+            sts16((dst + k * (64 / PIECES) * 128) ^ 16u, o[4], o[5], o[6], o[7]);
           }
         }
         fence_proxy_async();
@@ -403,34 +442,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW;
           const int lo = r.seen & 255, hi = r.seen >> 8;
           uint32_t any = 0;
-#pragma unroll 4
-          for (int it = ct; it < D * 4; it += 64) {
-            const int piece = it & 3, dim = it >> 2;
-            uint4 x = live ? lds16(src + static_cast<uint32_t>(it) * 16) : make_uint4(0u, 0u, 0u, 0u);
-            uint32_t u[4] = {x.x, x.y, x.z, x.w};
+          const uint32_t dst = v16 + b * F16 + v_at;
+#pragma unroll 2
+          for (int k = 0; k < D / 16; ++k) {
+            uint4 x = live ? lds16(src + static_cast<uint32_t>(ct) * 16 + k * 1024) : make_uint4(0u, 0u, 0u, 0u);
             if (edge) {
               // Tokens that no row sees may hold anything: zero. NaN that only some rows see: zero here, and noted.
-              uint32_t noted = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int from = max(lo - (16 * piece + 4 * i), 0), to = min(hi - (16 * piece + 4 * i), 3);
-                u[i] &= from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
-                const uint32_t bad = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                u[i] &= ~((bad >> 7) * 0xffu);
-                noted |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
-              }
-              s_nan[n & 3][dim][piece] = static_cast<unsigned short>(noted);
+              const uint32_t noted = tame16(x, lo - 16 * vp, hi - 16 * vp);
+              s_nan[n & 3][dim0 + 16 * k][vp] = static_cast<unsigned short>(noted);
               any |= noted;
             }
             uint32_t o[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[2 * i] = fp8_to_half2(static_cast<uint16_t>(u[i] & 0xffffu));
-              o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
-            }
-            const uint32_t row = v16 + b * F16 + static_cast<uint32_t>(dim) * 128;
-            sts16(row + (((2 * piece) ^ (dim & 7)) << 4), o[0], o[1], o[2], o[3]);
-            sts16(row + (((2 * piece + 1) ^ (dim & 7)) << 4), o[4], o[5], o[6], o[7]);
+            to_half16(x, o);
+            sts16(dst + k * 2048, o[0], o[1], o[2], o[3]);
+            sts16((dst + k * 2048) ^ 16u, o[4], o[5], o[6], o[7]);
           }
           const int some = __any_sync(0xffffffffu, any != 0);
           if (lane == 0) s_has_nan[n & 3][warp - 2] = some;
@@ -500,45 +525,57 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           const int bits = r.bits >> 16;
           seg_last = bits & PAGE_SEG_LAST;
           last = bits & PAGE_RANGE_LAST;
-          uint32_t s[2][32];
-          tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE, s[0]);
-          tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + 32, s[1]);
-          tmem_ld_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&s_empty[b]));
           const float f = f_row * exp2_byte(r.bits & 255);
-          if (!(bits & PAGE_LIVE)) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) s[i >> 5][i & 31] = 0xff800000u;
-          } else if (bits & PAGE_EDGE) {
-            const int lim = there ? pos - r.p0 : -1, low = a.window > 0 ? pos - a.window + 1 - r.p0 : 0;
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i > lim || i < low) s[i >> 5][i & 31] = 0xff800000u;
+          // what the row sees of the page, a bit per token
+          unsigned long long sees = ~0ull;
+          const bool masked = !(bits & PAGE_LIVE) || (bits & PAGE_EDGE);
+          if (masked) {
+            const int lim = there && (bits & PAGE_LIVE) ? min(pos - r.p0, ATTN_PAGE - 1) : -1, low = a.window > 0 ? max(pos - a.window + 1 - r.p0, 0) : 0;
+            sees = lim >= low ? (~0ull >> (63 - lim)) & (~0ull << low) : 0ull;
           }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto scores = [&](int c, uint32_t (&v)[32]) {   // tokens 32 c .. of the row, those it does not see at -infinity
+            tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + 32 * c, v);
+            tmem_ld_wait();
+            if (masked) mask32(v, static_cast<uint32_t>(sees >> (32 * c)));
+          };
+          float m_page = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            scores(c, v);
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[i >> 5][i & 31]));
-          const float m_new = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f, mx);
-          const float base2 = m_new == -INFINITY ? 0.f : m_new, alpha = exp2_fast(mx - base2);
-          mx = m_new;
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t p[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const float e0 = exp2_fast(fmaf(__uint_as_float(s[i >> 5][i & 31]), f, -base2)), e1 = exp2_fast(fmaf(__uint_as_float(s[i >> 5][(i + 1) & 31]), f, -base2));
-            l4[(i >> 1) & 3] += e0 + e1;
-            p[i >> 1] = pack_half2(e0, e1);
+            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
+            m_page = fmaxf(m_page, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
           }
-          l = fmaf(l, alpha, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+          // The reference of the weights follows the maximum only when that has grown by more than 2^8 (the weights stay below
+          // 2^8, far inside FP16): the sums are then hardly ever to be scaled.
+          const float m_new = m_page * f, grown = m_new > mx + 8.f || (mx == -INFINITY && m_new > mx) ? m_new : mx;
+          const float base2 = grown == -INFINITY ? 0.f : grown, alpha = grown == mx ? 1.f : exp2_fast(mx - base2);
+          mx = grown;
           s_alpha[n & 3][row] = alpha;
           if (n >= 2) ok = warp_wait(pv_done[b], ph ^ 1u);   // the P buffer's last reader
           if (!ok) break;
           tc_fence_after_sync();
-          tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2), p);
-          tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + 16, p + 16);
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[32], p[16];
+            scores(c, v);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float e0 = exp2_fast(fmaf(__uint_as_float(v[i]), f, -base2)), e1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), f, -base2));
+              l4[i & 3] += e0;
+              l4[(i & 3) + 1] += e1;
+              p[i >> 1] = pack_half2(e0, e1);
+            }
+            tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + 16 * c, p);
+          }
           tmem_store_wait();
+          l = fmaf(l, alpha, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&s_empty[b]));
           if (seg_last) {
             s_fin[unit & 7][0][row] = mx;
             s_fin[unit & 7][1][row] = l;
