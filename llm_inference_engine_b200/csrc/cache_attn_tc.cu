@@ -338,49 +338,51 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
     // A wait of the whole warp: all lanes come back with the same answer, and together.
     auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_short(smem_u32(&bar), parity)) != 0; };
     if (warp == 1) {
-      // ---- MMA
-      if (lane == 0) {
-        constexpr uint32_t id_s = umma_idesc_f16(TC_ROWS, ATTN_PAGE), id_o = umma_idesc_f16(TC_ROWS, D);
-        int unit = 0;
-        bool fresh = true, last = false;
-        // S of page n, then O' of page n - 1, whose weights were made meanwhile
-        for (int n = 0; ok; ++n) {
-          const int b = n & 1;
-          const uint32_t ph = (n >> 1) & 1;
-          const bool done = last;
-          if (!done) {
-            if (fresh) ok = mbar_wait_short(smem_u32(&q_full), unit++ & 1);   // the unit's q is in tensor memory
-            ok = ok && mbar_wait_short(smem_u32(&kf_full[b]), ph) && (n < 2 || mbar_wait_short(smem_u32(&s_empty[b]), ph ^ 1u));
-            if (!ok) break;
-            tc_fence_after_sync();
-            uint64_t kd = umma_desc_k_sw128(k16 + b * F16);
-#pragma unroll 1
-            for (int k = 0; k < D / 16; ++k) {
-              umma_f16_ts(tmem + COL_S + b * ATTN_PAGE, tmem + COL_Q + 8 * k, kd, id_s, k > 0 ? 1u : 0u);
-              kd += (k & 3) == 3 ? (ATTN_PAGE * 128 / 16) - 6 : 2;   // 16 dimensions on; the next 64 are an atom of their own
-            }
+      // ---- MMA. The whole warp walks along and one elected lane issues: what is the same in all lanes is then known to be
+      // (an MMA's operands are uniform registers; out of a branch of one lane each would be moved there first, which
+      // took three times as long as the MMA itself).
+      constexpr uint32_t id_s = umma_idesc_f16(TC_ROWS, ATTN_PAGE), id_o = umma_idesc_f16(TC_ROWS, D);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      int unit = 0;
+      bool fresh = true, last = false;
+      // S of page n, then O' of page n - 1, whose weights were made meanwhile
+      for (int n = 0; ok; ++n) {
+        const uint32_t b = n & 1, ph = (n >> 1) & 1;
+        const bool done = last;
+        if (!done) {
+          if (fresh) ok = warp_wait(q_full, unit++ & 1);   // the unit's q is in tensor memory
+          ok = ok && warp_wait(kf_full[b], ph) && (n < 2 || warp_wait(s_empty[b], ph ^ 1u));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t kd = umma_desc_k_sw128(k16 + b * F16);
+          const uint32_t ds = tm + COL_S + b * ATTN_PAGE;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)   // the next 64 dimensions are a swizzle atom of their own
+              umma_f16_ts(ds, tm + COL_Q + 8 * k, kd + (k / 4) * (ATTN_PAGE * 128 / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
             umma_commit(smem_u32(&qk_done[b]));
-            const int bits = s_page[n & (TC_PAGES - 1)].bits >> 16;   // visible: kf_full was waited for
-            last = bits & PAGE_RANGE_LAST;
-            fresh = bits & PAGE_SEG_LAST;
           }
-          if (n > 0) {
-            const int b1 = b ^ 1;
-            const uint32_t ph1 = ((n - 1) >> 1) & 1;
-            ok = mbar_wait_short(smem_u32(&p_full[b1]), ph1) && mbar_wait_short(smem_u32(&vf_full[b1]), ph1) &&
-                 (n < 3 || mbar_wait_short(smem_u32(&o_empty[b1]), ph1 ^ 1u));
-            if (!ok) break;
-            tc_fence_after_sync();
-            const uint64_t vd = umma_desc_k_sw128(v16 + b1 * F16);
-#pragma unroll 1
-            for (int k = 0; k < ATTN_PAGE / 16; ++k)
-              umma_f16_ts(tmem + COL_O + b1 * D, tmem + COL_P + b1 * (ATTN_PAGE / 2) + 8 * k, vd + 2 * k, id_o, k > 0 ? 1u : 0u);
+          __syncwarp();
+          const int bits = __shfl_sync(0xffffffffu, s_page[n & (TC_PAGES - 1)].bits >> 16, 0);   // visible: kf_full was waited for
+          last = bits & PAGE_RANGE_LAST;
+          fresh = bits & PAGE_SEG_LAST;
+        }
+        if (n > 0) {
+          const uint32_t b1 = b ^ 1u, ph1 = ((n - 1) >> 1) & 1;
+          ok = warp_wait(p_full[b1], ph1) && warp_wait(vf_full[b1], ph1) && (n < 3 || warp_wait(o_empty[b1], ph1 ^ 1u));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t vd = umma_desc_k_sw128(v16 + b1 * F16);
+          const uint32_t dd = tm + COL_O + b1 * D, da = tm + COL_P + b1 * (ATTN_PAGE / 2);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < ATTN_PAGE / 16; ++k) umma_f16_ts(dd, da + 8 * k, vd + 2 * k, id_o, k > 0 ? 1u : 0u);
             umma_commit(smem_u32(&pv_done[b1]));
           }
-          if (done) break;
+          __syncwarp();
         }
+        if (done) break;
       }
-      __syncwarp();
     } else if (warp < 4) {
       // ---- codes to FP16, two warps: a thread takes 16 codes (32 bytes of FP16) at a time
       const int ct = tid - 64;
@@ -410,11 +412,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           // A thread's pieces are 64 / PIECES tokens apart, a multiple of 8: the same place in the swizzle, a fixed stride.
           const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW + static_cast<uint32_t>(ct) * 16;
           const uint32_t dst = k16 + b * F16 + k_at;
+          constexpr int N = ATTN_PAGE * PIECES / 64;
+          uint4 x[N];
 #pragma unroll
-          for (int k = 0; k < ATTN_PAGE * PIECES / 64; ++k) {
-            const uint4 x = lds16(src + k * 1024);
+          for (int k = 0; k < N; ++k) x[k] = lds16(src + k * 1024);   // all in flight
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
             uint32_t o[8];
-            to_half16(x, o);
+            to_half16(x[k], o);
             // the two halves' lanes write even and odd chunks in turn: no bank twice
             if (k_swap) {   // (registers cannot be indexed: a select each)
 #pragma unroll
@@ -443,17 +448,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           const int lo = r.seen & 255, hi = r.seen >> 8;
           uint32_t any = 0;
           const uint32_t dst = v16 + b * F16 + v_at;
-#pragma unroll 2
-          for (int k = 0; k < D / 16; ++k) {
-            uint4 x = live ? lds16(src + static_cast<uint32_t>(ct) * 16 + k * 1024) : make_uint4(0u, 0u, 0u, 0u);
-            if (edge) {
-              // Tokens that no row sees may hold anything: zero. NaN that only some rows see: zero here, and noted.
-              const uint32_t noted = tame16(x, lo - 16 * vp, hi - 16 * vp);
+          uint4 x[D / 16];
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) x[k] = live ? lds16(src + static_cast<uint32_t>(ct) * 16 + k * 1024) : make_uint4(0u, 0u, 0u, 0u);
+          if (edge) {
+            // Tokens that no row sees may hold anything: zero. NaN that only some rows see: zero here, and noted.
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t noted = tame16(x[k], lo - 16 * vp, hi - 16 * vp);
               s_nan[n & 3][dim0 + 16 * k][vp] = static_cast<unsigned short>(noted);
               any |= noted;
             }
+          }
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
             uint32_t o[8];
-            to_half16(x, o);
+            to_half16(x[k], o);
             sts16(dst + k * 2048, o[0], o[1], o[2], o[3]);
             sts16((dst + k * 2048) ^ 16u, o[4], o[5], o[6], o[7]);
           }
@@ -613,12 +623,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           for (int i = 0; i < D; ++i) o[i] *= alpha;
         }
 #pragma unroll
-        for (int c = 0; c < D; c += 16) {
-          uint32_t v[16];
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[16], w[16];
           tmem_ld16(tmem + lanes + COL_O + b * D + c, v);
+          tmem_ld16(tmem + lanes + COL_O + b * D + c + 16, w);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[c + i] = fmaf(__uint_as_float(v[i]), vs, o[c + i]);
+          for (int i = 0; i < 16; ++i) {
+            o[c + i] = fmaf(__uint_as_float(v[i]), vs, o[c + i]);
+            o[c + 16 + i] = fmaf(__uint_as_float(w[i]), vs, o[c + 16 + i]);
+          }
         }
         if ((bits & PAGE_EDGE) && (s_has_nan[n & 3][0] | s_has_nan[n & 3][1])) {
           // rows that see a token with NaN in a dimension have NaN there

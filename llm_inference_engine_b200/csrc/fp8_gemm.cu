@@ -156,52 +156,59 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int s = 0, sf = 0;
-      uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        int tok, row, kb0, kb1;
-        slice(t, tok, row, kb0, kb1);
-        // the accumulators are free once the epilogue has read the tile before
-        if (t != static_cast<int>(blockIdx.x) && !mbar_wait(smem_u32(&bar_acc_empty), acc_phase ^ 1u)) ok = false;
+    // The whole warp walks along and one elected lane issues: an MMA's operands are uniform registers, and what is the
+    // same in all lanes is then known to be.
+    int s = 0, sf = 0;
+    uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity)) != 0; };
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tok, row, kb0, kb1;
+      slice(t, tok, row, kb0, kb1);
+      // the accumulators are free once the epilogue has read the tile before
+      if (t != static_cast<int>(blockIdx.x) && !wait(bar_acc_empty, acc_phase ^ 1u)) ok = false;
+      tc_fence_after_sync();
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        const int j = (kb - kb0) & 3;
+        if (j == 0 && !wait(bar_sf_full[sf], sf_phase)) ok = false;
+        if (ok && !wait(bar_full[s], phase)) ok = false;
+        if (!ok) break;
         tc_fence_after_sync();
-        for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          const int j = (kb - kb0) & 3;
-          if (j == 0 && !mbar_wait(smem_u32(&bar_sf_full[sf]), sf_phase)) ok = false;
-          if (ok && !mbar_wait(smem_u32(&bar_full[s]), phase)) ok = false;
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
-          const uint64_t bd = umma_desc_k_sw128(at + MT * a_tile);
-          const uint32_t sfa = tmem + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE, sfb = sfa + 4 * MT;
-          const uint32_t idesc = g8_idesc(a.nt, j);
+        const uint32_t at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
+        const uint64_t ad = umma_desc_k_sw128(at), bd = umma_desc_k_sw128(at + MT * a_tile);
+        const uint32_t sfa = tm + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE, sfb = sfa + 4 * MT;
+        const uint32_t idesc = g8_idesc(a.nt, j), more = kb > kb0 ? 1u : 0u;
+        const bool sf_last = j == 3 || kb + 1 == kb1;
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < FP8_BLOCK / 32; ++k)   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
 #pragma unroll
             for (int h = 0; h < MT; ++h)
-              umma_mxf8(tmem + static_cast<uint32_t>(h * a.nt), umma_desc_k_sw128(at + static_cast<uint32_t>(h) * a_tile) + 2 * k, bd + 2 * k, idesc,
-                        sfa + 4u * static_cast<uint32_t>(h), sfb, (kb > kb0 || k > 0) ? 1u : 0u);
+              umma_mxf8(tm + static_cast<uint32_t>(h * a.nt), ad + h * (a_tile >> 4) + 2 * k, bd + 2 * k, idesc, sfa + 4u * static_cast<uint32_t>(h), sfb,
+                        k > 0 ? 1u : more);
           umma_commit(smem_u32(&bar_empty[s]));
-          if (j == 3 || kb + 1 == kb1) {
-            umma_commit(smem_u32(&bar_sf_empty[sf]));
-            if (++sf == 2) {
-              sf = 0;
-              sf_phase ^= 1u;
-            }
-          }
-          if (++s == a.stages) {
-            s = 0;
-            phase ^= 1u;
-          }
+          if (sf_last) umma_commit(smem_u32(&bar_sf_empty[sf]));
+          if (kb + 1 == kb1) umma_commit(smem_u32(&bar_acc_full));
         }
-        umma_commit(smem_u32(&bar_acc_full));   // also on the way out, so that the epilogue is released
-        acc_phase ^= 1u;
+        __syncwarp();
+        if (sf_last && ++sf == 2) {
+          sf = 0;
+          sf_phase ^= 1u;
+        }
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1u;
+        }
       }
-      if (!ok) {
+      acc_phase ^= 1u;
+    }
+    if (!ok) {
+      if (lane == 0) {
         atomicOr(a.status, ST_MMA_TIMEOUT);
-        s_abort = 1;
+        umma_commit(smem_u32(&bar_acc_full));   // on the way out, so that the epilogue is released
       }
+      s_abort = 1;
     }
     __syncwarp();
   } else {
