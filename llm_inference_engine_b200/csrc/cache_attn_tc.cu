@@ -87,12 +87,6 @@ static __noinline__ __device__ void store8_call(const AttnArgs& a, size_t tok, i
   store8(a, tok, col, x);
 }
 
-// Scores whose bit is not set become -infinity.
-__device__ __forceinline__ void mask32(uint32_t (&v)[32], uint32_t keep) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (!(keep >> i & 1u)) v[i] = 0xff800000u;
-}
 // Sixteen codes to FP16.
 __device__ __forceinline__ void to_half16(const uint4& x, uint32_t (&o)[8]) {
   const uint32_t u[4] = {x.x, x.y, x.z, x.w};
@@ -102,19 +96,81 @@ __device__ __forceinline__ void to_half16(const uint4& x, uint32_t (&o)[8]) {
     o[2 * i + 1] = fp8_to_half2(static_cast<uint16_t>(u[i] >> 16));
   }
 }
-// Of sixteen codes, those outside [lo, hi] and those that stand for NaN become zero; returns a bit for each NaN inside.
-__device__ __forceinline__ uint32_t tame16(uint4& x, int lo, int hi) {
-  uint32_t u[4] = {x.x, x.y, x.z, x.w}, noted = 0;
+// A page's V for one thread of the converters when some row does not see some token (or there is no page): of the thread's
+// sixteen tokens those outside [lo, hi], which no row sees and which may hold anything, become zero, and so do NaN that only
+// some rows see; those are noted, a bit per token, in `nan` (of dimensions 16 apart), and whether there are any comes back.
+template <int D>
+static __noinline__ __device__ int convert_v_edge(uint32_t src, uint32_t dst, bool live, int lo, int hi, unsigned short* nan) {
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int k = 0; k < D / 16; ++k) {
+    const uint4 x = live ? lds16(src + k * 1024) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t u[4] = {x.x, x.y, x.z, x.w}, noted = 0, o[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int from = max(lo - 4 * i, 0), to = min(hi - 4 * i, 3);
-    u[i] &= from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
-    const uint32_t bad = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-    u[i] &= ~((bad >> 7) * 0xffu);
-    noted |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
+    for (int i = 0; i < 4; ++i) {
+      const int from = max(lo - 4 * i, 0), to = min(hi - 4 * i, 3);
+      u[i] &= from > 3 || to < from ? 0u : (0xffffffffu << (8 * from)) & (0xffffffffu >> (8 * (3 - to)));
+      const uint32_t bad = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+      u[i] &= ~((bad >> 7) * 0xffu);
+      noted |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
+    }
+    nan[k * 16 * 4] = static_cast<unsigned short>(noted);
+    any |= noted;
+    to_half16(make_uint4(u[0], u[1], u[2], u[3]), o);
+    sts16(dst + k * 2048, o[0], o[1], o[2], o[3]);
+    sts16((dst + k * 2048) ^ 16u, o[4], o[5], o[6], o[7]);
   }
-  x = make_uint4(u[0], u[1], u[2], u[3]);
-  return noted;
+  return __any_sync(0xffffffffu, any != 0);
+}
+
+// The two passes over a row's scores of a page (64 columns of tensor memory from `ts`), with the tokens whose bit is not
+// set in `sees` at -infinity: the largest raw score, and the weights 2^(f s - base) to `tp`, whose sum comes back. MASKED
+// pages are few: their passes are a call.
+template <bool MASKED>
+__device__ __forceinline__ void row_scores(uint32_t ts, int c, unsigned long long sees, uint32_t (&v)[32]) {
+  tmem_ld32(ts + 32 * c, v);
+  tmem_ld_wait();
+  if (MASKED) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (!(sees >> (32 * c + i) & 1ull)) v[i] = 0xff800000u;
+  }
+}
+template <bool MASKED>
+__device__ __forceinline__ float row_max(uint32_t ts, unsigned long long sees) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    uint32_t v[32];
+    row_scores<MASKED>(ts, c, sees, v);
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
+    m = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+  }
+  return m;
+}
+template <bool MASKED>
+__device__ __forceinline__ float row_weights(uint32_t ts, uint32_t tp, unsigned long long sees, float f, float base) {
+  float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    uint32_t v[32], p[16];
+    row_scores<MASKED>(ts, c, sees, v);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float e0 = exp2_fast(fmaf(__uint_as_float(v[i]), f, -base)), e1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), f, -base));
+      l4[i & 2] += e0;
+      l4[(i & 2) + 1] += e1;
+      p[i >> 1] = pack_half2(e0, e1);
+    }
+    tmem_st16(tp + 16 * c, p);
+  }
+  return (l4[0] + l4[1]) + (l4[2] + l4[3]);
+}
+static __noinline__ __device__ float row_max_masked(uint32_t ts, unsigned long long sees) { return row_max<true>(ts, sees); }
+static __noinline__ __device__ float row_weights_masked(uint32_t ts, uint32_t tp, unsigned long long sees, float f, float base) {
+  return row_weights<true>(ts, tp, sees, f, base);
 }
 
 template <int D>
@@ -387,12 +443,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
       // ---- codes to FP16, two warps: a thread takes 16 codes (32 bytes of FP16) at a time
       const int ct = tid - 64;
       constexpr int PIECES = D / 16;   // 16-code pieces of a token
-      // Where the thread's piece of a token's K row goes: chunks j and j + 1 of its half's 128 bytes, swizzled. The lanes of the
-      // second half write theirs in the other order: no bank twice.
+      // Where the thread's piece of a token's K row goes: chunks j and j + 1 of its half's 128 bytes, swizzled.
       const int piece = ct % PIECES, tok0 = ct / PIECES;
-      const bool k_swap = piece >= 4;
       const uint32_t k_at = static_cast<uint32_t>(piece / 4) * (ATTN_PAGE * 128) + static_cast<uint32_t>(tok0) * 128 +
-                            ((((piece % 4) * 2 + (k_swap ? 1 : 0)) ^ (tok0 & 7)) << 4);
+                            ((((piece % 4) * 2) ^ (tok0 & 7)) << 4);
       // and 16 tokens of a V row (a dimension)
       const int vp = ct & 3, dim0 = ct >> 2;
       const uint32_t v_at = static_cast<uint32_t>(dim0) * 128 + (((2 * vp) ^ (dim0 & 7)) << 4);
@@ -421,14 +475,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
             uint32_t o[8];
             to_half16(x[k], o);
             // the two halves' lanes write even and odd chunks in turn: no bank twice
-            if (k_swap) {   // (registers cannot be indexed: a select each)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t t = o[i];
-                o[i] = o[i + 4];
-                o[i + 4] = t;
-              }
-            }
             sts16(dst + k * (64 / PIECES) * 128, o[0], o[1], o[2], o[3]);
             sts16((dst + k * (64 / PIECES) * 128) ^ 16u, o[4], o[5], o[6], o[7]);
           }
@@ -444,30 +490,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         ok = warp_wait(raw_full[slot], (used / TC_RAW) & 1) && (n < 2 || warp_wait(pv_done[b], ph ^ 1u));
         if (!ok) break;
         {
-          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW;
-          const int lo = r.seen & 255, hi = r.seen >> 8;
-          uint32_t any = 0;
-          const uint32_t dst = v16 + b * F16 + v_at;
-          uint4 x[D / 16];
+          const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW + static_cast<uint32_t>(ct) * 16, dst = v16 + b * F16 + v_at;
+          int some = 0;
+          if (edge || !live) {
+            some = convert_v_edge<D>(src, dst, live, (r.seen & 255) - 16 * vp, (r.seen >> 8) - 16 * vp, &s_nan[n & 3][dim0][vp]);
+          } else {
+            uint4 x[D / 16];
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) x[k] = live ? lds16(src + static_cast<uint32_t>(ct) * 16 + k * 1024) : make_uint4(0u, 0u, 0u, 0u);
-          if (edge) {
-            // Tokens that no row sees may hold anything: zero. NaN that only some rows see: zero here, and noted.
+            for (int k = 0; k < D / 16; ++k) x[k] = lds16(src + k * 1024);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint32_t noted = tame16(x[k], lo - 16 * vp, hi - 16 * vp);
-              s_nan[n & 3][dim0 + 16 * k][vp] = static_cast<unsigned short>(noted);
-              any |= noted;
+              uint32_t o[8];
+              to_half16(x[k], o);
+              sts16(dst + k * 2048, o[0], o[1], o[2], o[3]);
+              sts16((dst + k * 2048) ^ 16u, o[4], o[5], o[6], o[7]);
             }
           }
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t o[8];
-            to_half16(x[k], o);
-            sts16(dst + k * 2048, o[0], o[1], o[2], o[3]);
-            sts16((dst + k * 2048) ^ 16u, o[4], o[5], o[6], o[7]);
-          }
-          const int some = __any_sync(0xffffffffu, any != 0);
           if (lane == 0) s_has_nan[n & 3][warp - 2] = some;
         }
         fence_proxy_async();
@@ -543,21 +581,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
             const int lim = there && (bits & PAGE_LIVE) ? min(pos - r.p0, ATTN_PAGE - 1) : -1, low = a.window > 0 ? max(pos - a.window + 1 - r.p0, 0) : 0;
             sees = lim >= low ? (~0ull >> (63 - lim)) & (~0ull << low) : 0ull;
           }
-          auto scores = [&](int c, uint32_t (&v)[32]) {   // tokens 32 c .. of the row, those it does not see at -infinity
-            tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + 32 * c, v);
-            tmem_ld_wait();
-            if (masked) mask32(v, static_cast<uint32_t>(sees >> (32 * c)));
-          };
-          float m_page = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t v[32];
-            scores(c, v);
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
-            m_page = fmaxf(m_page, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-          }
+          const uint32_t ts = tmem + lanes + COL_S + b * ATTN_PAGE;
+          const float m_page = masked ? row_max_masked(ts, sees) : row_max<false>(ts, sees);
           // The reference of the weights follows the maximum only when that has grown by more than 2^8 (the weights stay below
           // 2^8, far inside FP16): the sums are then hardly ever to be scaled.
           const float m_new = m_page * f, grown = m_new > mx + 8.f || (mx == -INFINITY && m_new > mx) ? m_new : mx;
@@ -567,22 +592,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           if (n >= 2) ok = warp_wait(pv_done[b], ph ^ 1u);   // the P buffer's last reader
           if (!ok) break;
           tc_fence_after_sync();
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t v[32], p[16];
-            scores(c, v);
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float e0 = exp2_fast(fmaf(__uint_as_float(v[i]), f, -base2)), e1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), f, -base2));
-              l4[i & 3] += e0;
-              l4[(i & 3) + 1] += e1;
-              p[i >> 1] = pack_half2(e0, e1);
-            }
-            tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + 16 * c, p);
-          }
+          const uint32_t tp = tmem + lanes + COL_P + b * (ATTN_PAGE / 2);
+          const float l_page = masked ? row_weights_masked(ts, tp, sees, f, base2) : row_weights<false>(ts, tp, sees, f, base2);
           tmem_store_wait();
-          l = fmaf(l, alpha, (l4[0] + l4[1]) + (l4[2] + l4[3]));
+          l = fmaf(l, alpha, l_page);
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&s_empty[b]));
