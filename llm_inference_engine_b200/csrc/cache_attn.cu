@@ -723,13 +723,10 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
   const AttnDeal deal = attn_deal(total, workers);
   const int u0 = start + h * attn_items(en) + ATTN_HEAD;
   if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;   // one worker had all of the unit's pages and has written it
-  const AttnParts ps = attn_parts(deal, TILE > 16 || total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
-  // The lane's two rows and where its quad of sums lies in a part. Tiles of 128 rows are kept by rows: a quad is then four
-  // neighbouring dimensions of one row.
-  constexpr bool BY_ROW = TILE > 16;
-  const int row = BY_ROW ? r0 + (DEEP ? lane / 4 : static_cast<int>(threadIdx.x) / (D / 4)) : r0 + 2 * t;
-  const int dim = DEEP ? 16 * d + 4 * (lane % 4) : 4 * (static_cast<int>(threadIdx.x) % (D / 4));   // BY_ROW: first of four
-  const size_t quad_at = 2 * TILE + (BY_ROW ? static_cast<size_t>(row) * D + dim : (static_cast<size_t>(r0 / 8) * (D / 16) + d) * 128 + lane * 4);
+  const AttnParts ps = attn_parts(deal, total <= spread_below ? 1 : ATTN_WARPS, u0, en.pages);
+  // The lane's two rows and where its quad of sums lies in a part.
+  const int row = r0 + 2 * t;
+  const size_t quad_at = 2 * TILE + (static_cast<size_t>(r0 / 8) * (D / 16) + d) * 128 + lane * 4;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](const float2& pm, const float2& pl, const float4& po) {   // one more part, or a warp's sums
     const float m0 = fmaxf(m[0], pm.x), m1 = fmaxf(m[1], pm.y);
@@ -753,13 +750,8 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
       const int j = i + k * STEP;
       if (j < ps.parts) {
         const float* s = a.part + static_cast<size_t>(attn_part_slot(ps, j)) * FLOATS;
-        if constexpr (BY_ROW) {
-          pm[k].x = pm[k].y = __ldcg(s + row);
-          pl[k].x = pl[k].y = __ldcg(s + TILE + row);
-        } else {
-          pm[k] = __ldcg(reinterpret_cast<const float2*>(s + row));
-          pl[k] = __ldcg(reinterpret_cast<const float2*>(s + TILE + row));
-        }
+        pm[k] = __ldcg(reinterpret_cast<const float2*>(s + row));
+        pl[k] = __ldcg(reinterpret_cast<const float2*>(s + TILE + row));
         po[k] = __ldcg(reinterpret_cast<const float4*>(s + quad_at));
       }
     }
@@ -779,19 +771,84 @@ __global__ void __launch_bounds__(DEEP ? 256 : D * 2) cache_attn_join_kernel(con
     }
   }
   const float inv[2] = {l[0] == 0.f ? 0.f : 1.f / l[0], l[1] == 0.f ? 0.f : 1.f / l[1]};
-  if constexpr (BY_ROW) {
-    if (row >= en.rows) return;
-    const int rr = en.row0 + row, tk = div_group(a, rr), col = (h * a.group + rr - tk * a.group) * D + dim;
+  const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
+  store_quads<1>(a, en, h, row, 16 * d + g, quad, inv, D);
+}
+
+// The same for tiles of 128 rows, which are kept by rows: a thread has four neighbouring dimensions of GROUPS rows, 8 apart.
+// Where most units are split (a chunk of 2 x 512 tokens: 147 of 256), GROUPS = 4 is what gets the latency of a CTA's
+// chain of loads paid once for 32 rows.
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(D * 2) cache_attn_join_rows_kernel(const __grid_constant__ AttnArgs a, int workers) {
+  constexpr int TILE = 128, FLOATS = attn_slot_floats(D, TILE);
+  const int entries = a.batch * a.tiles, group = a.group;
+  const int e = static_cast<int>(blockIdx.x) / a.hk, h = static_cast<int>(blockIdx.x) % a.hk;
+  const int row = static_cast<int>(blockIdx.y) * 8 * GROUPS + static_cast<int>(threadIdx.x) / (D / 4), dim = 4 * (static_cast<int>(threadIdx.x) % (D / 4));
+  const AttnEntry en = attn_entry_of(a, e, group, TILE);
+  griddep_launch_dependents();
+  griddep_wait();
+  const int total = __ldcg(a.prefix + entries), start = __ldcg(a.prefix + e);
+  if (row >= en.rows) return;
+  const AttnDeal deal = attn_deal(total, workers);
+  const int u0 = start + h * attn_items(en) + ATTN_HEAD;
+  if (attn_worker(deal, u0) == attn_worker(deal, u0 + en.pages - 1)) return;
+  const AttnParts ps = attn_parts(deal, 1, u0, en.pages);
+  float m[GROUPS], l[GROUPS], o[GROUPS][4];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    m[g] = -INFINITY;
+    l[g] = o[g][0] = o[g][1] = o[g][2] = o[g][3] = 0.f;
+  }
+  constexpr int AHEAD = GROUPS > 1 ? 2 : 4;
+  for (int i = 0; i < ps.parts; i += AHEAD) {
+    float pm[AHEAD][GROUPS], pl[AHEAD][GROUPS];
+    float4 po[AHEAD][GROUPS];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (i + k >= ps.parts) break;
+      const float* s = a.part + static_cast<size_t>(attn_part_slot(ps, i + k)) * FLOATS;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {   // (a slot has all 128 rows: those behind the tile's last hold what was there)
+        pm[k][g] = __ldcg(s + row + 8 * g);
+        pl[k][g] = __ldcg(s + TILE + row + 8 * g);
+        po[k][g] = __ldcg(reinterpret_cast<const float4*>(s + 2 * TILE + static_cast<size_t>(row + 8 * g) * D + dim));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (i + k >= ps.parts) break;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const float top = fmaxf(m[g], pm[k][g]), base = top == -INFINITY ? 0.f : top, f = exp2_fast(m[g] - base), p = exp2_fast(pm[k][g] - base);
+        m[g] = top;
+        l[g] = fmaf(l[g], f, pl[k][g] * p);
+        o[g][0] = fmaf(o[g][0], f, po[k][g].x * p);
+        o[g][1] = fmaf(o[g][1], f, po[k][g].y * p);
+        o[g][2] = fmaf(o[g][2], f, po[k][g].z * p);
+        o[g][3] = fmaf(o[g][3], f, po[k][g].w * p);
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    if (row + 8 * g >= en.rows) break;
+    const float inv = l[g] == 0.f ? 0.f : 1.f / l[g];
+    const int rr = en.row0 + row + 8 * g, tk = div_group(a, rr), col = (h * group + rr - tk * group) * D + dim;
     const size_t tok = en.first + tk;
+    __nv_bfloat16* out = a.out + tok * a.ld_out + col;
+    float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float x = o[i] * inv[0];
-      if (a.gate) x *= sigmoid_f32(bf16lo_f32(__ldcg(reinterpret_cast<const unsigned short*>(a.gate + tok * a.ld_gate + col + i))));
-      a.out[tok * a.ld_out + col + i] = __float2bfloat16_rn(x);
+      x[i] = o[g][i] * inv;
+      if (a.gate) x[i] *= sigmoid_f32(bf16lo_f32(__ldcg(reinterpret_cast<const unsigned short*>(a.gate + tok * a.ld_gate + col + i))));
     }
-  } else {
-    const float quad[1][4] = {{o[0], o[1], o[2], o[3]}};
-    store_quads<1>(a, en, h, row, 16 * d + g, quad, inv, D);
+    if (a.vec_out) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+      *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] = __float2bfloat16_rn(x[i]);
+    }
   }
 }
 
@@ -834,9 +891,14 @@ static cudaError_t join_launch(const AttnArgs& a, const AttnForm& f, int sms, cu
   const int all = a.max_q * a.group, rows = all < f.tile ? all : f.tile;
   const unsigned units = static_cast<unsigned>(a.batch) * a.tiles * a.hk, groups = (rows + 7) / 8;
   // Few units may have many parts each; many units have few (there are two partial segments per worker in all).
-  if (static_cast<long long>(units) * groups < 2ll * sms)
-    return launch_dependent(cache_attn_join_kernel<D, TILE, true>, dim3(units, groups, D / 16), dim3(256), 0, stream, a, f.workers(sms), attn_spread_below(sms));
-  return launch_dependent(cache_attn_join_kernel<D, TILE, false>, dim3(units, groups), dim3(D * 2), 0, stream, a, f.workers(sms), attn_spread_below(sms));
+  const bool few = static_cast<long long>(units) * groups < 2ll * sms;
+  if constexpr (TILE == 128) {
+    return few ? launch_dependent(cache_attn_join_rows_kernel<D, 1>, dim3(units, groups), dim3(D * 2), 0, stream, a, f.workers(sms))
+               : launch_dependent(cache_attn_join_rows_kernel<D, 4>, dim3(units, (groups + 3) / 4), dim3(D * 2), 0, stream, a, f.workers(sms));
+  } else {
+    return few ? launch_dependent(cache_attn_join_kernel<D, TILE, true>, dim3(units, groups, D / 16), dim3(256), 0, stream, a, f.workers(sms), attn_spread_below(sms))
+               : launch_dependent(cache_attn_join_kernel<D, TILE, false>, dim3(units, groups), dim3(D * 2), 0, stream, a, f.workers(sms), attn_spread_below(sms));
+  }
 }
 
 template <int D>

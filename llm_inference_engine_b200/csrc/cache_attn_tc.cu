@@ -22,7 +22,7 @@
 namespace muse {
 
 constexpr int TC_ROWS = 128;
-constexpr int TC_THREADS = 384;
+constexpr int TC_THREADS = 512;
 constexpr int TC_RAW = 8;              // ring slots of raw codes (K and V of a page are one each)
 constexpr int TC_UNITS = 16;           // ring of unit records: no role is that many pages behind another
 constexpr int TC_PAGES = 64;           // ring of page records
@@ -68,6 +68,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
@@ -80,11 +86,27 @@ __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// store8 as a call: written out for every eight of a row's dimensions it would be most of the kernel's code.
-static __noinline__ __device__ void store8_call(const AttnArgs& a, size_t tok, int col, float x0, float x1, float x2, float x3, float x4, float x5, float x6,
-                                                float x7) {
-  float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
-  store8(a, tok, col, x);
+// Two FP32 operations in one instruction: issue slots are what the softmax and the sums are short of.
+__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(unsigned long long x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // Sixteen codes to FP16.
@@ -100,7 +122,7 @@ __device__ __forceinline__ void to_half16(const uint4& x, uint32_t (&o)[8]) {
 // sixteen tokens those outside [lo, hi], which no row sees and which may hold anything, become zero, and so do NaN that only
 // some rows see; those are noted, a bit per token, in `nan` (of dimensions 16 apart), and whether there are any comes back.
 template <int D>
-static __noinline__ __device__ int convert_v_edge(uint32_t src, uint32_t dst, bool live, int lo, int hi, unsigned short* nan) {
+__device__ __forceinline__ int convert_v_edge(uint32_t src, uint32_t dst, bool live, int lo, int hi, unsigned short* nan) {
   uint32_t any = 0;
 #pragma unroll 1
   for (int k = 0; k < D / 16; ++k) {
@@ -123,55 +145,11 @@ static __noinline__ __device__ int convert_v_edge(uint32_t src, uint32_t dst, bo
   return __any_sync(0xffffffffu, any != 0);
 }
 
-// The two passes over a row's scores of a page (64 columns of tensor memory from `ts`), with the tokens whose bit is not
-// set in `sees` at -infinity: the largest raw score, and the weights 2^(f s - base) to `tp`, whose sum comes back. MASKED
-// pages are few: their passes are a call.
-template <bool MASKED>
-__device__ __forceinline__ void row_scores(uint32_t ts, int c, unsigned long long sees, uint32_t (&v)[32]) {
-  tmem_ld32(ts + 32 * c, v);
-  tmem_ld_wait();
-  if (MASKED) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (!(sees >> (32 * c + i) & 1ull)) v[i] = 0xff800000u;
-  }
-}
-template <bool MASKED>
-__device__ __forceinline__ float row_max(uint32_t ts, unsigned long long sees) {
-  float m = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
-    uint32_t v[32];
-    row_scores<MASKED>(ts, c, sees, v);
-    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
-    m = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-  }
-  return m;
-}
-template <bool MASKED>
-__device__ __forceinline__ float row_weights(uint32_t ts, uint32_t tp, unsigned long long sees, float f, float base) {
-  float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
-    uint32_t v[32], p[16];
-    row_scores<MASKED>(ts, c, sees, v);
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float e0 = exp2_fast(fmaf(__uint_as_float(v[i]), f, -base)), e1 = exp2_fast(fmaf(__uint_as_float(v[i + 1]), f, -base));
-      l4[i & 2] += e0;
-      l4[(i & 2) + 1] += e1;
-      p[i >> 1] = pack_half2(e0, e1);
-    }
-    tmem_st16(tp + 16 * c, p);
-  }
-  return (l4[0] + l4[1]) + (l4[2] + l4[3]);
-}
-static __noinline__ __device__ float row_max_masked(uint32_t ts, unsigned long long sees) { return row_max<true>(ts, sees); }
-static __noinline__ __device__ float row_weights_masked(uint32_t ts, uint32_t tp, unsigned long long sees, float f, float base) {
-  return row_weights<true>(ts, tp, sees, f, base);
-}
+// More registers for the sums, fewer for the others: 96 + 2 x 112 + 192 = 512 is what the launch has, 128 each.
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D>
 __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
@@ -181,17 +159,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   static_assert(COL_O + 2 * D <= 512, "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t raw_full[TC_RAW], raw_empty[TC_RAW], unit_full[TC_UNITS], kf_full[2], vf_full[2], qk_done[2], pv_done[2], s_empty[2],
-      p_full[2], o_empty[2], q_full, fin_full[8];
+      p_full[2], o_empty[2], q_full, fin_full[8], pair_full[4];
   __shared__ __align__(16) PageRec s_page[TC_PAGES];
   __shared__ UnitRec s_unit[TC_UNITS];
-  __shared__ float s_alpha[4][TC_ROWS], s_fin[8][2][TC_ROWS];
+  __shared__ float s_alpha[4][TC_ROWS], s_fin[8][3][TC_ROWS], s_max[2][2][TC_ROWS];
   __shared__ __align__(8) unsigned short s_nan[4][D][4];      // edge pages: the tokens of each dimension that hold NaN
   __shared__ int s_has_nan[4][2];
   __shared__ int s_sum[TC_THREADS / 32];
   __shared__ int s_entry;
   __shared__ int s_start;
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.group, entries = a.batch * a.tiles;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -208,14 +185,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
       mbar_init(smem_u32(&vf_full[i]), 2);
       mbar_init(smem_u32(&qk_done[i]), 1);
       mbar_init(smem_u32(&pv_done[i]), 1);
-      mbar_init(smem_u32(&s_empty[i]), 4);
-      mbar_init(smem_u32(&p_full[i]), 4);
+      mbar_init(smem_u32(&s_empty[i]), 8);
+      mbar_init(smem_u32(&p_full[i]), 8);
       mbar_init(smem_u32(&o_empty[i]), 4);
     }
-    mbar_init(smem_u32(&q_full), 4);
-    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&fin_full[i]), 4);
+    mbar_init(smem_u32(&q_full), 8);
+    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&fin_full[i]), 8);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&pair_full[i]), 2);
     fence_mbar_init();
-    s_abort = 0;
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -275,125 +252,138 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   }
   __syncthreads();
 
-  if (items > 0 && warp == 0) {
-    // ---- looks pages up, describes them, and copies their codes
-    EntryCache cache;
-    cache.base = -64;
-    Cursor c;
-    c.e = s_entry;
-    c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
-    const int off0 = f0 - s_start, per_unit = attn_items(c.en);
-    c.h = off0 / per_unit;
-    c.i = off0 % per_unit - ATTN_HEAD;
-    int unit0 = s_start + c.h * per_unit;
-    int left = items, n = 0, unit = 0, issued = 0;
-    bool ok = true, in_unit = false;
-    // how many pages of the range lie in the unit that c stands in, and whether any page follows
-    while (left > 0 && ok) {
-      if (c.i < 0) {
-        const int skip = min(-c.i, left);
-        c.i += skip;
-        left -= skip;
-        continue;
-      }
-      // pages of this unit in the range, up to 32 at a time, one per lane
-      const int in_range = min(c.en.pages - c.i, left), take = min(in_range, 32);
-      if (!in_unit) {
-        in_unit = true;
-        if (lane == 0) {
-          UnitRec& u = s_unit[unit & (TC_UNITS - 1)];
-          u.first = c.en.first; u.row0 = c.en.row0; u.rows = c.en.rows; u.pos = c.en.pos;
-          u.h = c.h;
-          u.whole = c.i == 0 && in_range == c.en.pages;
-          u.slot = attn_slot_of(deal, worker, unit0 + ATTN_HEAD);
-          mbar_arrive(smem_u32(&unit_full[unit & (TC_UNITS - 1)]));   // releases the record
+  // (A range of head items alone has no page: beside the first, no role has anything to wait for.)
+  const bool pages = items > 0 && items > ATTN_HEAD - (f0 - s_start) % attn_items(attn_entry_of(a, s_entry, group, TC_ROWS));
+  bool ok = true;
+  // (A barrier of which no phase is complete yet lets a wait for the parity before the first pass: that is how the two
+  // buffers' first uses find them free.)
+  // A wait of the whole warp: all lanes come back with the same answer, and together.
+  // (Several at once: their first looks are in flight together, a look takes a hundred clocks or two.)
+  auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity)) != 0; };
+  auto warp_wait2 = [&](uint64_t& bar0, uint32_t p0, uint64_t& bar1, uint32_t p1) {
+    const bool r0 = mbar_try_wait(smem_u32(&bar0), p0), r1 = mbar_try_wait(smem_u32(&bar1), p1);
+    if (__all_sync(0xffffffffu, r0 && r1)) return true;
+    return warp_wait(bar0, p0) && warp_wait(bar1, p1);
+  };
+  auto warp_wait3 = [&](uint64_t& bar0, uint32_t p0, uint64_t& bar1, uint32_t p1, uint64_t& bar2, uint32_t p2) {
+    const bool r0 = mbar_try_wait(smem_u32(&bar0), p0), r1 = mbar_try_wait(smem_u32(&bar1), p1), r2 = mbar_try_wait(smem_u32(&bar2), p2);
+    if (__all_sync(0xffffffffu, r0 && r1 && r2)) return true;
+    return warp_wait(bar0, p0) && warp_wait(bar1, p1) && warp_wait(bar2, p2);
+  };
+  if (warp < 4) {
+    regs_down<96>();
+    if (warp == 0 && items > 0) {
+      // ---- looks pages up, describes them, and copies their codes
+      EntryCache cache;
+      cache.base = -64;
+      Cursor c;
+      c.e = s_entry;
+      c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
+      const int off0 = f0 - s_start, per_unit = attn_items(c.en);
+      c.h = off0 / per_unit;
+      c.i = off0 % per_unit - ATTN_HEAD;
+      int unit0 = s_start + c.h * per_unit;
+      int left = items, n = 0, unit = 0, issued = 0;
+      bool in_unit = false;
+      // how many pages of the range lie in the unit that c stands in, and whether any page follows
+      while (left > 0 && ok) {
+        if (c.i < 0) {
+          const int skip = min(-c.i, left);
+          c.i += skip;
+          left -= skip;
+          continue;
         }
-        ++unit;
-      }
-      int tile = -1, exps = 127 | 127 << 8;
-      if (lane < take && c.en.last >= 0) {
-        const int b = a.tiles == 1 ? c.e : c.e / a.tiles;
-        const int p = __ldcg(a.page_table + static_cast<size_t>(b) * a.width + c.en.page0 + c.i + lane);
-        if (p >= 0 && p < a.pages) {
-          tile = p * a.hk + c.h;
-          exps = __ldcg(a.k_exp + tile) | __ldcg(a.v_exp + tile) << 8;
-        } else {
-          atomicOr(a.status, ST_BAD_PAGE);
-        }
-      }
-      const int p_first = c.en.pos + div_group(a, c.en.row0), p_last = c.en.pos + div_group(a, c.en.row0 + c.en.rows - 1);
-      const bool follows = [&] {   // does a page follow this unit's share of the range?
-        int rest = left - in_range;
-        if (rest <= 0) return false;
-        return rest > ATTN_HEAD;   // the next unit's head items come first
-      }();
-      for (int j = 0; j < take && ok; ++j) {
-        const int t = __shfl_sync(0xffffffffu, tile, j), ex = __shfl_sync(0xffffffffu, exps, j);
-        const int p0 = (c.en.page0 + c.i + j) * ATTN_PAGE;
-        const bool seg_last = j + 1 == take && take == in_range;
-        // K, then V; the record is written ahead of the K slot's arrival
-        for (int half = 0; half < 2 && ok; ++half) {
-          const int slot = issued % TC_RAW, turn = issued / TC_RAW;
-          if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_empty[slot]), (turn - 1) & 1))) {
-            ok = false;
-            break;
-          }
+        // pages of this unit in the range, up to 32 at a time, one per lane
+        const int in_range = min(c.en.pages - c.i, left), take = min(in_range, 32);
+        if (!in_unit) {
+          in_unit = true;
           if (lane == 0) {
-            if (half == 0) {
-              PageRec r;
-              r.tile = t;
-              const bool edge = p_first < p0 + ATTN_PAGE - 1 || (a.window > 0 && p_last - a.window + 1 > p0);
-              r.bits = ex | ((seg_last ? PAGE_SEG_LAST : 0) | (seg_last && !follows ? PAGE_RANGE_LAST : 0) |
-                             (edge ? PAGE_EDGE : 0) | (t >= 0 ? PAGE_LIVE : 0)) << 16;
-              r.p0 = p0;
-              const int lo = a.window > 0 ? max(p_first - a.window + 1 - p0, 0) : 0, hi = min(p_last - p0, ATTN_PAGE - 1);
-              r.seen = (lo > 63 ? 63 : lo) | max(hi, 0) << 8;
-              s_page[n & (TC_PAGES - 1)] = r;
-            }
-            const uint32_t bar = smem_u32(&raw_full[slot]);
-            if (t >= 0) {
-              mbar_expect_tx(bar, RAW);
-              bulk_load_1d(raw + static_cast<uint32_t>(slot) * RAW, (half ? a.v : a.k) + static_cast<size_t>(t) * RAW, RAW, bar);
-            } else {
-              mbar_arrive(bar);
-            }
+            UnitRec& u = s_unit[unit & (TC_UNITS - 1)];
+            u.first = c.en.first; u.row0 = c.en.row0; u.rows = c.en.rows; u.pos = c.en.pos;
+            u.h = c.h;
+            u.whole = c.i == 0 && in_range == c.en.pages;
+            u.slot = attn_slot_of(deal, worker, unit0 + ATTN_HEAD);
+            mbar_arrive(smem_u32(&unit_full[unit & (TC_UNITS - 1)]));   // releases the record
           }
-          __syncwarp();
-          ++issued;
+          ++unit;
         }
-        ++n;
-      }
-      c.i += take;
-      left -= take;
-      if (take == in_range) {
-        in_unit = false;
-        if (left > 0) {
-          unit0 += attn_items(c.en);
-          c.i = -ATTN_HEAD;
-          if (++c.h == a.hk) {
-            c.h = 0;
-            do {
-              if (++c.e >= entries) {
-                left = 0;
-                break;
+        int tile = -1, exps = 127 | 127 << 8;
+        if (lane < take && c.en.last >= 0) {
+          const int b = a.tiles == 1 ? c.e : c.e / a.tiles;
+          const int p = __ldcg(a.page_table + static_cast<size_t>(b) * a.width + c.en.page0 + c.i + lane);
+          if (p >= 0 && p < a.pages) {
+            tile = p * a.hk + c.h;
+            exps = __ldcg(a.k_exp + tile) | __ldcg(a.v_exp + tile) << 8;
+          } else {
+            atomicOr(a.status, ST_BAD_PAGE);
+          }
+        }
+        const int p_first = c.en.pos + div_group(a, c.en.row0), p_last = c.en.pos + div_group(a, c.en.row0 + c.en.rows - 1);
+        const bool follows = [&] {   // does a page follow this unit's share of the range?
+          int rest = left - in_range;
+          if (rest <= 0) return false;
+          return rest > ATTN_HEAD;   // the next unit's head items come first
+        }();
+        for (int j = 0; j < take && ok; ++j) {
+          const int t = __shfl_sync(0xffffffffu, tile, j), ex = __shfl_sync(0xffffffffu, exps, j);
+          const int p0 = (c.en.page0 + c.i + j) * ATTN_PAGE;
+          const bool seg_last = j + 1 == take && take == in_range;
+          // K, then V; the record is written ahead of the K slot's arrival
+          for (int half = 0; half < 2 && ok; ++half) {
+            const int slot = issued % TC_RAW, turn = issued / TC_RAW;
+            if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_empty[slot]), (turn - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) {
+              if (half == 0) {
+                PageRec r;
+                r.tile = t;
+                const bool edge = p_first < p0 + ATTN_PAGE - 1 || (a.window > 0 && p_last - a.window + 1 > p0);
+                r.bits = ex | ((seg_last ? PAGE_SEG_LAST : 0) | (seg_last && !follows ? PAGE_RANGE_LAST : 0) |
+                               (edge ? PAGE_EDGE : 0) | (t >= 0 ? PAGE_LIVE : 0)) << 16;
+                r.p0 = p0;
+                const int lo = a.window > 0 ? max(p_first - a.window + 1 - p0, 0) : 0, hi = min(p_last - p0, ATTN_PAGE - 1);
+                r.seen = (lo > 63 ? 63 : lo) | max(hi, 0) << 8;
+                s_page[n & (TC_PAGES - 1)] = r;
               }
-              c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
-            } while (c.en.pages == 0);
+              const uint32_t bar = smem_u32(&raw_full[slot]);
+              if (t >= 0) {
+                mbar_expect_tx(bar, RAW);
+                bulk_load_1d(raw + static_cast<uint32_t>(slot) * RAW, (half ? a.v : a.k) + static_cast<size_t>(t) * RAW, RAW, bar);
+              } else {
+                mbar_arrive(bar);
+              }
+            }
+            __syncwarp();
+            ++issued;
+          }
+          ++n;
+        }
+        c.i += take;
+        left -= take;
+        if (take == in_range) {
+          in_unit = false;
+          if (left > 0) {
+            unit0 += attn_items(c.en);
+            c.i = -ATTN_HEAD;
+            if (++c.h == a.hk) {
+              c.h = 0;
+              do {
+                if (++c.e >= entries) {
+                  left = 0;
+                  break;
+                }
+                c.en = attn_entry_cached(a, cache, c.e, entries, group, TC_ROWS);
+              } while (c.en.pages == 0);
+            }
           }
         }
       }
-    }
-    if (!ok) {
-      if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
-      s_abort = 1;
-      for (int i = issued > TC_RAW ? issued - TC_RAW : 0; i < issued; ++i) mbar_wait(smem_u32(&raw_full[i % TC_RAW]), (i / TC_RAW) & 1);
-    }
-  } else if (items > 0 && items > ATTN_HEAD - (f0 - s_start) % attn_items(attn_entry_of(a, s_entry, group, TC_ROWS))) {
-    // (a range of head items alone has no page: these roles have nothing to wait for)
-    bool ok = true;
-    // A wait of the whole warp: all lanes come back with the same answer, and together.
-    auto warp_wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_short(smem_u32(&bar), parity)) != 0; };
-    if (warp == 1) {
+      if (!ok) {
+        for (int i = issued > TC_RAW ? issued - TC_RAW : 0; i < issued; ++i) mbar_wait(smem_u32(&raw_full[i % TC_RAW]), (i / TC_RAW) & 1);
+      }
+    } else if (warp == 1 && pages) {
       // ---- MMA. The whole warp walks along and one elected lane issues: what is the same in all lanes is then known to be
       // (an MMA's operands are uniform registers; out of a branch of one lane each would be moved there first, which
       // took three times as long as the MMA itself).
@@ -407,7 +397,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         const bool done = last;
         if (!done) {
           if (fresh) ok = warp_wait(q_full, unit++ & 1);   // the unit's q is in tensor memory
-          ok = ok && warp_wait(kf_full[b], ph) && (n < 2 || warp_wait(s_empty[b], ph ^ 1u));
+          ok = ok && warp_wait2(kf_full[b], ph, s_empty[b], ph ^ 1u);
           if (!ok) break;
           tc_fence_after_sync();
           const uint64_t kd = umma_desc_k_sw128(k16 + b * F16);
@@ -425,7 +415,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         if (n > 0) {
           const uint32_t b1 = b ^ 1u, ph1 = ((n - 1) >> 1) & 1;
-          ok = warp_wait(p_full[b1], ph1) && warp_wait(vf_full[b1], ph1) && (n < 3 || warp_wait(o_empty[b1], ph1 ^ 1u));
+          ok = warp_wait3(p_full[b1], ph1, vf_full[b1], ph1, o_empty[b1], ph1 ^ 1u);
           if (!ok) break;
           tc_fence_after_sync();
           const uint64_t vd = umma_desc_k_sw128(v16 + b1 * F16);
@@ -439,7 +429,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         if (done) break;
       }
-    } else if (warp < 4) {
+    } else if (warp >= 2 && pages) {
       // ---- codes to FP16, two warps: a thread takes 16 codes (32 bytes of FP16) at a time
       const int ct = tid - 64;
       constexpr int PIECES = D / 16;   // 16-code pieces of a token
@@ -456,7 +446,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         const int b = n & 1;
         const uint32_t ph = (n >> 1) & 1;
         int slot = used % TC_RAW;
-        ok = warp_wait(raw_full[slot], (used / TC_RAW) & 1) && (n < 2 || warp_wait(qk_done[b], ph ^ 1u));
+        ok = warp_wait2(raw_full[slot], (used / TC_RAW) & 1, qk_done[b], ph ^ 1u);
         if (!ok) break;
         const PageRec r = s_page[n & (TC_PAGES - 1)];
         const int bits = r.bits >> 16;
@@ -487,7 +477,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         ++used;
         slot = used % TC_RAW;
-        ok = warp_wait(raw_full[slot], (used / TC_RAW) & 1) && (n < 2 || warp_wait(pv_done[b], ph ^ 1u));
+        ok = warp_wait2(raw_full[slot], (used / TC_RAW) & 1, pv_done[b], ph ^ 1u);
         if (!ok) break;
         {
           const uint32_t src = raw + static_cast<uint32_t>(slot) * RAW + static_cast<uint32_t>(ct) * 16, dst = v16 + b * F16 + v_at;
@@ -516,8 +506,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         ++used;
       }
-    } else if (warp < 8) {
-      // ---- softmax: a thread per row
+    }
+  } else if (warp < 12) {
+    regs_down<112>();
+    if (pages) {
+      // ---- softmax: two threads per row, 32 tokens of a page each; warps w and w + 4 share their rows
+      const int half = warp >= 8, other = half ^ 1;
       const int row = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       bool last = false;
@@ -547,6 +541,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           f_row = a.scale_log2 * exp2_byte(127 + e);
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
+            if (i / (D / 64) != half) continue;   // half the row each
             uint32_t p[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -574,35 +569,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           seg_last = bits & PAGE_SEG_LAST;
           last = bits & PAGE_RANGE_LAST;
           const float f = f_row * exp2_byte(r.bits & 255);
-          // what the row sees of the page, a bit per token
-          unsigned long long sees = ~0ull;
-          const bool masked = !(bits & PAGE_LIVE) || (bits & PAGE_EDGE);
-          if (masked) {
-            const int lim = there && (bits & PAGE_LIVE) ? min(pos - r.p0, ATTN_PAGE - 1) : -1, low = a.window > 0 ? max(pos - a.window + 1 - r.p0, 0) : 0;
-            sees = lim >= low ? (~0ull >> (63 - lim)) & (~0ull << low) : 0ull;
-          }
-          const uint32_t ts = tmem + lanes + COL_S + b * ATTN_PAGE;
-          const float m_page = masked ? row_max_masked(ts, sees) : row_max<false>(ts, sees);
-          // The reference of the weights follows the maximum only when that has grown by more than 2^8 (the weights stay below
-          // 2^8, far inside FP16): the sums are then hardly ever to be scaled.
-          const float m_new = m_page * f, grown = m_new > mx + 8.f || (mx == -INFINITY && m_new > mx) ? m_new : mx;
-          const float base2 = grown == -INFINITY ? 0.f : grown, alpha = grown == mx ? 1.f : exp2_fast(mx - base2);
-          mx = grown;
-          s_alpha[n & 3][row] = alpha;
-          if (n >= 2) ok = warp_wait(pv_done[b], ph ^ 1u);   // the P buffer's last reader
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t tp = tmem + lanes + COL_P + b * (ATTN_PAGE / 2);
-          const float l_page = masked ? row_weights_masked(ts, tp, sees, f, base2) : row_weights<false>(ts, tp, sees, f, base2);
-          tmem_store_wait();
-          l = fmaf(l, alpha, l_page);
+          // The thread's scores stay in registers; what the row does not see of them becomes -infinity.
+          uint32_t v[32];
+          tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + half * 32, v);
+          tmem_ld_wait();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&s_empty[b]));
-          if (seg_last) {
-            s_fin[unit & 7][0][row] = mx;
-            s_fin[unit & 7][1][row] = l;
+          if (!(bits & PAGE_LIVE) || (bits & PAGE_EDGE)) {
+            const int lim = there && (bits & PAGE_LIVE) ? min(pos - r.p0, ATTN_PAGE - 1) : -1, low = a.window > 0 ? max(pos - a.window + 1 - r.p0, 0) : 0;
+            const unsigned long long all = lim >= low ? (~0ull >> (63 - lim)) & (~0ull << low) : 0ull;
+            const uint32_t sees = static_cast<uint32_t>(all >> (32 * half));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(sees >> i & 1u)) v[i] = 0xff800000u;
           }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) m4[i / 2 & 3] = max3(m4[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          const float m_half = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          s_max[b][half][row] = m_half;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&pair_full[warp & 3]));
+          // (the second: the P buffer's last reader)
+          ok = warp_wait2(pair_full[warp & 3], n & 1, pv_done[b], ph ^ 1u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          // The reference of the weights follows the maximum only when that has grown by more than 2^8 (the weights stay below
+          // 2^8, far inside FP16): the sums are then hardly ever to be scaled.
+          const float m_new = fmaxf(m_half, s_max[b][other][row]) * f, grown = m_new > mx + 8.f || (mx == -INFINITY && m_new > mx) ? m_new : mx;
+          const float base2 = grown == -INFINITY ? 0.f : grown, alpha = grown == mx ? 1.f : exp2_fast(mx - base2);
+          mx = grown;
+          if (half == 0) s_alpha[n & 3][row] = alpha;
+          const unsigned long long ff = pack2(f, f), bb = pack2(-base2, -base2);
+          unsigned long long l2[2] = {0ull, 0ull};
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float e0, e1;
+            unpack2(fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), ff, bb), e0, e1);
+            e0 = exp2_fast(e0);
+            e1 = exp2_fast(e1);
+            l2[i / 2 & 1] = add2(l2[i / 2 & 1], pack2(e0, e1));
+            p[i >> 1] = pack_half2(e0, e1);
+          }
+          float l_lo, l_hi;
+          unpack2(add2(l2[0], l2[1]), l_lo, l_hi);
+          tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + half * 16, p);
+          l = fmaf(l, alpha, l_lo + l_hi);
+          if (seg_last) {
+            if (half == 0) s_fin[unit & 7][2][row] = mx;
+            s_fin[unit & 7][half][row] = l;
+          }
+          tmem_store_wait();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) {
@@ -612,15 +631,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         }
         ++unit;
       }
-    } else {
+    }
+  } else {
+    regs_up<192>();
+    if (pages) {
       // ---- sums and output: a thread per row
       const int row = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       bool last = false;
       int unit = 0;
-      float o[D];
+      unsigned long long o[D / 2];   // two dimensions each
 #pragma unroll
-      for (int i = 0; i < D; ++i) o[i] = 0.f;
+      for (int i = 0; i < D / 2; ++i) o[i] = 0ull;
       for (int n = 0; ok && !last; ++n) {
         const int b = n & 1;
         const uint32_t ph = (n >> 1) & 1;
@@ -631,9 +653,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         const int bits = r.bits >> 16;
         last = bits & PAGE_RANGE_LAST;
         const float alpha = s_alpha[n & 3][row], vs = exp2_byte(r.bits >> 8 & 255);
+        const unsigned long long vs2 = pack2(vs, vs);
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < D; ++i) o[i] *= alpha;
+          for (int i = 0; i < D / 2; ++i) o[i] = fma2(o[i], pack2(alpha, alpha), 0ull);
         }
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -643,8 +666,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            o[c + i] = fmaf(__uint_as_float(v[i]), vs, o[c + i]);
-            o[c + 16 + i] = fmaf(__uint_as_float(w[i]), vs, o[c + 16 + i]);
+            if (i & 1) continue;
+            o[(c + i) / 2] = fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), vs2, o[(c + i) / 2]);
+            o[(c + 16 + i) / 2] = fma2(pack2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), vs2, o[(c + 16 + i) / 2]);
           }
         }
         if ((bits & PAGE_EDGE) && (s_has_nan[n & 3][0] | s_has_nan[n & 3][1])) {
@@ -662,46 +686,65 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
             if (__any_sync(0xffffffffu, bad != 0)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (bad >> i & 1u) o[c + i] = __uint_as_float(0x7fffffffu);
+                if (bad >> i & 1u) o[(c + i) / 2] |= 0x7fffffffull << (32 * (i & 1));
             }
           }
+        }
+        if (!(bits & PAGE_SEG_LAST)) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&o_empty[b]));
+          continue;
+        }
+        // The unit's end. The sums go through the page's O' once more: read back from there, the loop over a row's dimensions
+        // can stay one.
+        const uint32_t to = tmem + lanes + COL_O + b * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = static_cast<uint32_t>(o[(c + i) / 2] >> (32 * (i & 1)));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[c / 2 + i] = 0ull;
+          tmem_st16(to + c, v);
+        }
+        tmem_store_wait();
+        ok = warp_wait(fin_full[unit & 7], (unit >> 3) & 1);
+        if (!ok) break;
+        const UnitRec u = s_unit[unit & (TC_UNITS - 1)];
+        const bool there = row < u.rows;
+        const float m = s_fin[unit & 7][2][row], l = s_fin[unit & 7][0][row] + s_fin[unit & 7][1][row];
+        const float inv = !u.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;   // no token seen: the row is zero
+        const int rr = u.row0 + row, tk = div_group(a, rr), col = (u.h * group + rr - tk * group) * D;
+        float* part = a.part + static_cast<size_t>(u.slot) * attn_slot_floats(D, TC_ROWS);
+        if (there && !u.whole) {
+          part[row] = m;
+          part[TC_ROWS + row] = l;
+        }
+        part += 2 * TC_ROWS + static_cast<size_t>(row) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 8) {
+          uint32_t v[8];
+          tmem_ld8(to + c, v);
+          tmem_ld_wait();
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[i]) * inv;
+          if (there && u.whole) store8(a, u.first + tk, col + c, x);
+          if (there && !u.whole) {
+            *reinterpret_cast<float4*>(part + c) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(part + c + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          }
+          __syncwarp();
         }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&o_empty[b]));
-        if (!(bits & PAGE_SEG_LAST)) continue;
-        ok = warp_wait(fin_full[unit & 7], (unit >> 3) & 1);
-        if (!ok) break;
-        const UnitRec u = s_unit[unit & (TC_UNITS - 1)];
-        if (row < u.rows) {
-          const float m = s_fin[unit & 7][0][row], l = s_fin[unit & 7][1][row];
-          if (u.whole) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;   // no token seen: the row is zero
-            const int rr = u.row0 + row, tk = div_group(a, rr), col = (u.h * group + rr - tk * group) * D;
-#pragma unroll
-            for (int c = 0; c < D; c += 8) {
-              store8_call(a, u.first + tk, col + c, o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv, o[c + 4] * inv, o[c + 5] * inv, o[c + 6] * inv,
-                          o[c + 7] * inv);
-            }
-          } else {
-            float* slot = a.part + static_cast<size_t>(u.slot) * attn_slot_floats(D, TC_ROWS);
-            slot[row] = m;
-            slot[TC_ROWS + row] = l;
-            float4* dst = reinterpret_cast<float4*>(slot + 2 * TC_ROWS + static_cast<size_t>(row) * D);
-#pragma unroll
-            for (int c = 0; c < D; c += 4) dst[c / 4] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < D; ++i) o[i] = 0.f;
         ++unit;
       }
     }
-    if (!ok) {
-      if (lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
-      s_abort = 1;
-    }
   }
+  if (!ok && lane == 0) atomicOr(a.status, ST_ATTN_TIMEOUT);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
