@@ -6,16 +6,19 @@
 // The page list, its cut into ranges and the joining of split units are those of cache_attn.cu, a CTA being a worker. Per
 // page: K and V codes come in by bulk copies; two warps convert them to FP16 (exact) in the 128-byte-swizzled layout of the
 // MMA's B operand (K [token][dim], V [dim][token]: both K-major as the cache keeps them); S = Q K^T with Q in tensor
-// memory as the A operand; a thread per row turns its 64 scores into weights, which go back to tensor memory as the A
-// operand of O' = P V; another thread per row adds O' to its sums in registers, scaled in FP32 by the page's exponent and
-// by what the row's maximum has moved. S, P and O' are double-buffered in tensor memory (64 + 2 x 64 + 2 x 32 + 2 x 128
+// memory as the A operand; two threads per row turn 32 of its scores each into weights, which go back to tensor memory as
+// the A operand of O' = P V; another thread per row adds O' to its sums in registers, scaled in FP32 by the page's exponent
+// and by what the row's reference has moved. S, P and O' are double-buffered in tensor memory (64 + 2 x 64 + 2 x 32 + 2 x 128
 // columns at D = 128), so the products of one page run under the exponentials of another.
 //
-// What this kernel is short of is the instruction cache: its first form, every loop written out, was 183 KB of code, missed
-// on 4 of 10 fetches and took 349 us where this one takes less than a third (chunk of 2 x 512 tokens against 4096, 32 query and 8 KV
-// heads). So the loops over a row's scores and over the MMAs stay loops, and what runs once per unit is out of line.
+// Measured (chunk of 2 x 512 tokens against 4096, 32 query and 8 KV heads, D = 128; with the join): 138 us, 466
+// TFLOP/s; a page takes a CTA about 2000 clocks. What it is short of is instructions: some 3500 per page on four schedulers,
+// and their fetching. With every loop written out the kernel was 183 KB of code, missed the instruction cache on 4 of 10
+// fetches and took 349 us; loops over MMAs kept as loops and masks out of the way 220 and 176; FP32 operations two at a time
+// and a row split over two threads (so that its scores stay in registers) 138. Tried and slower: four warps that convert
+// (20 warps, 145 us), one for K and one for V (213), even and odd pages on different softmax warps (180).
 //
-// Roles: warp 0 looks pages up and copies, warp 1 issues MMAs, warps 2 and 3 convert, warps 4..7 softmax, warps 8..11
+// Roles: warp 0 looks pages up and copies, warp 1 issues MMAs, warps 2 and 3 convert, warps 4..11 softmax, warps 12..15
 // sums and output. All waits are bounded.
 #include "cache_attn.cuh"
 
