@@ -29,6 +29,7 @@ from . import _capi
 
 PAGE = 64
 HEAD_DIMS = (64, 128)
+_INT_MAX = 0x7fffffff
 
 
 class Cache8(NamedTuple):
@@ -115,7 +116,7 @@ def _refuse_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int,
             raise ValueError(f"without cu_q there is one new token per sequence: {m} rows for {batch} sequences, max_q={max_q}")
     elif cu_q.shape != (batch + 1,):
         raise ValueError(f"cu_q must be [batch + 1] = [{batch + 1}], got {tuple(cu_q.shape)}")
-    raise ValueError(f"max_q={max_q} must be positive and q_heads={q_heads} a multiple of the cache's {heads}")
+    raise ValueError(f"max_q={max_q} must be positive (and less than 2^31) and q_heads={q_heads} a multiple of the cache's {heads}")
 
 
 def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, q_heads: int):
@@ -133,7 +134,7 @@ def _check_batch(cache: Cache8, page_table, seq_lens, cu_q, max_q: int, m: int, 
                 and v.get_device() == index and ke.get_device() == index and ve.get_device() == index
                 and batch and width and seq_lens.shape == (batch,) and page_table.dtype is _I32 and seq_lens.dtype is _I32
                 and page_table.is_contiguous() and seq_lens.is_contiguous() and page_table.get_device() == index
-                and seq_lens.get_device() == index and max_q >= 1 and q_heads >= heads and not q_heads % heads):
+                and seq_lens.get_device() == index and 1 <= max_q <= _INT_MAX and q_heads >= heads and not q_heads % heads):
             if cu_q is None:
                 if m == batch and max_q == 1:
                     return index, kp, vp, ke.data_ptr(), ve.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), None, pages, heads, dim, batch, width
@@ -184,7 +185,7 @@ def rope_append(qkv: torch.Tensor, cache: Cache8, cos_sin: torch.Tensor, page_ta
             kvp, vvp = k_val.data_ptr(), v_val.data_ptr()
         rc = _capi.load().muse_rope_append(qkv.data_ptr(), cos_sin.data_ptr(), tp, lp, cp, kp, vp, kep, vep, q.data_ptr(), kvp, vvp,
                                            _capi.status_ptr(index), ld if m > 1 else cols, m, batch, width, pages, max_q, q_heads, heads, dim,
-                                           rot, 1 if interleaved else 0, positions, _capi.raw_stream(index))
+                                           rot, 1 if interleaved else 0, min(positions, _INT_MAX), _capi.raw_stream(index))
     if rc:
         _capi.check(rc, f"muse_rope_append(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
     return (q, k_val, v_val) if values else q
@@ -241,7 +242,7 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
         ws = _capi.new_tensor((_ws_bytes(index, batch, max_q, q_heads, heads, dim),), (1,), _U8, dev)
         rc = _capi.load().muse_cache_attention(q.data_ptr(), kp, vp, kep, vep, tp, lp, cp, gp, out.data_ptr(), ws.data_ptr(), _capi.status_ptr(index),
                                                ld_q if m > 1 else cols, ld_gate if m > 1 else cols, ld_out if m > 1 else cols, scale, m, batch,
-                                               width, pages, max_q, q_heads, heads, dim, window, _capi.raw_stream(index))
+                                               width, pages, max_q, q_heads, heads, dim, min(window, _INT_MAX), _capi.raw_stream(index))
     if rc:
         _capi.check(rc, f"muse_cache_attention(m={m}, batch={batch}, q_heads={q_heads}, heads={heads}, dim={dim})")
     return out

@@ -49,7 +49,7 @@ struct AttnArgs {
   uint32_t group_magic;        // 2^32 / group + 1: a row's token without a division
 };
 
-int rope_append_dispatch(const RopeArgs& a, int dim, cudaStream_t stream);
+int rope_append_dispatch(RopeArgs a, int dim, cudaStream_t stream);
 int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream);
 long long cache_attn_ws_bytes(int batch, int max_q, int hq, int hk, int dim);
 long long cache_attn_plan(const int* seq_lens, const int* cu_q, int m, int batch, int width, int max_q, int hq, int hk, int window, int sms,

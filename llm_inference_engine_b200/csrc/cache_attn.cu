@@ -916,7 +916,8 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   if (a.gate && a.ld_gate < static_cast<long long>(a.hq) * dim) return -4;
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(ws)) & 15) return -5;
   if ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 1) return -5;
-  if (!a.cu_q && a.max_q != 1) return -6;
+  if (!a.cu_q && (a.max_q != 1 || a.m != a.batch)) return -6;
+  if (!(a.scale_log2 > 0.f && a.scale_log2 < INFINITY)) return -6;
   const int sms = device_sms();
   if (sms < 1) return -7;
   const AttnForm f = attn_form(a.max_q, a.hq, a.hk);

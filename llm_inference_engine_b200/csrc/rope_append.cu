@@ -333,16 +333,18 @@ static cudaError_t rope_launch(const RopeArgs& a, cudaStream_t stream) {
                           static_cast<int>(kv), reach, static_cast<int>(per));
 }
 
-int rope_append_dispatch(const RopeArgs& a, int dim, cudaStream_t stream) {
+int rope_append_dispatch(RopeArgs a, int dim, cudaStream_t stream) {
   if (!a.qkv || !a.cos_sin || !a.page_table || !a.seq_lens || !a.k || !a.v || !a.k_exp || !a.v_exp || !a.q_out || !a.status) return -1;
   if ((a.k_val == nullptr) != (a.v_val == nullptr)) return -1;
   if (a.m < 1 || a.batch < 1 || a.width < 1 || a.pages < 1 || a.max_q < 1 || a.hq < 1 || a.hk < 1 || (dim != 64 && dim != 128)) return -2;
   if (a.rot < 16 || a.rot > dim || a.rot % 16 || a.width > 0x7fffffff / PAGE_TOKENS || a.table_rows < a.width * PAGE_TOKENS) return -3;
-  if (a.ld_qkv % 8 || a.ld_qkv < static_cast<long long>(a.hq + 2 * a.hk) * dim) return -4;
+  if (a.ld_qkv % 8 || a.ld_qkv < (a.hq + 2ll * a.hk) * dim) return -4;
   if ((reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.cos_sin) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
        reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_val) | reinterpret_cast<uintptr_t>(a.v_val)) & 15)
     return -5;
-  if (!a.cu_q && a.max_q != 1) return -6;
+  if (!a.cu_q && (a.max_q != 1 || a.m != a.batch)) return -6;
+  if (a.max_q > a.m) a.max_q = a.m;   // no sequence has more new tokens than the batch has rows
+  if (a.max_q > 0x7fffffff - PAGE_TOKENS) return -3;
   cudaError_t e;
   // A page's new tokens have to fit a CTA's registers: up to 16 tokens take 64 threads, a whole page 256.
   if (dim == 128) e = a.max_q <= 16 ? rope_launch<128, 64, 2>(a, stream) : rope_launch<128, 256, 2>(a, stream);

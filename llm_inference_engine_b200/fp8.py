@@ -20,6 +20,7 @@ from . import _capi
 
 BLOCK = 128
 E_MIN = -64
+_INT_MAX = 0x7fffffff
 WALK_MAX_TOKENS = 16   # csrc/fp8_linear.cu; more tokens or a longer K take csrc/fp8_gemm.cu
 WALK_MAX_K = 8192
 
@@ -62,8 +63,8 @@ def dequantize_weight(w8: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor
 
 
 def _rows(x: torch.Tensor, m: int, k: int) -> torch.Tensor:
-    """x itself where its rows can be read in 16-byte vectors, else a copy."""
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
+    """x itself where its rows can be read in 16-byte vectors (and their distance is an int), else a copy."""
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (m > 1 and (x.stride(0) % 8 or not k <= x.stride(0) <= _INT_MAX)):
         return x.contiguous().clone()
     return x
 
@@ -123,8 +124,8 @@ def _refuse_linear(x, w8, w_exp, out):
     if w_exp.shape != (-(-n // BLOCK), -(-k // BLOCK)) or not w8.is_contiguous() or not w_exp.is_contiguous() or w8.data_ptr() % 16:
         raise ValueError(f"w8 {tuple(w8.shape)} and w_exp {tuple(w_exp.shape)} must be contiguous, one exponent per 128 x 128 block")
     if out is not None and (out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n or out.stride(1) != 1
-                            or (m > 1 and out.stride(0) < n)):
-        raise ValueError("out must be BF16 [m, >= N] with unit column stride")
+                            or (m > 1 and not n <= out.stride(0) <= _INT_MAX)):
+        raise ValueError("out must be BF16 [m, >= N] with unit column stride and rows less than 2^31 elements apart that do not overlap")
     raise ValueError("x, w8, w_exp and out must be on the same CUDA device")
 
 
@@ -159,7 +160,7 @@ def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = 
     ld_out = n
     if out is not None:
         if (out.dtype is not _BF16 or out.dim() != 2 or out.shape[0] != m or out.shape[1] < n or out.get_device() != index or out.stride(1) != 1
-                or (m > 1 and out.stride(0) < n)):
+                or (m > 1 and not n <= out.stride(0) <= _INT_MAX)):
             _refuse_linear(x, w8, w_exp, out)
         if m > 1:
             ld_out = out.stride(0)
