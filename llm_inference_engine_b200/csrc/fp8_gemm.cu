@@ -24,6 +24,7 @@ constexpr int G8_TOK = 128;             // rows of one MMA
 constexpr int G8_MAX_STAGES = 12;
 constexpr int G8_SF_COL = 448;          // first tensor-memory column of the scales
 constexpr int G8_SF_STRIDE = 16;        // columns of one group of scales: 4 per token tile, 8 for W's rows
+constexpr int G8_SF_BUFS = 4;           // groups of scales in tensor memory: 64 columns
 constexpr int G8_THREADS = 192;
 constexpr int G8_MIN_SMEM = 116 * 1024;  // one CTA per SM: it takes all of tensor memory
 
@@ -36,6 +37,7 @@ struct G8Args {
   int m, n, k, kblocks, ld_out;
   int nt, a_rows;      // rows of W per tile; token rows a TMA box brings
   int row_tiles, tok_tiles, split, stages;
+  int at_once;         // blocks of K that the MMA warp takes at a time: 1, 2 or 4, at most half of the stages
 };
 
 __device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
@@ -61,12 +63,45 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Sixteen sums of a token: BF16 to out, or FP32 to slice s of the workspace.
+__device__ __forceinline__ void put16(const G8Args& a, const uint32_t (&v)[16], int token, int n0, int s, bool vec) {
+  if (a.split > 1) {
+    float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
+    if ((a.n & 3) == 0 && n0 + 16 <= a.n) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n0 + i < a.n) o[i] = __uint_as_float(v[i]);
+    }
+  } else {
+    __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
+    if (vec && n0 + 16 <= a.n) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 8) {
+        uint32_t p[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[i + 2 * q]), __uint_as_float(v[i + 2 * q + 1]));
+          p[q] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(o + i) = make_uint4(p[0], p[1], p[2], p[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n0 + i < a.n) o[i] = __float2bfloat16_rn(__uint_as_float(v[i]));
+    }
+  }
+}
+
 template <int MT>
 __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                                                                  const __grid_constant__ G8Args a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[G8_MAX_STAGES], bar_empty[G8_MAX_STAGES];
-  __shared__ __align__(8) uint64_t bar_sf_full[2], bar_sf_empty[2], bar_acc_full, bar_acc_empty;
+  __shared__ __align__(8) uint64_t bar_sf_full[G8_SF_BUFS], bar_sf_empty[G8_SF_BUFS], bar_acc_full, bar_acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -81,17 +116,19 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     tok = t % a.tok_tiles;
     row = t / a.tok_tiles % a.row_tiles;
     const int s = t / (a.tok_tiles * a.row_tiles);
-    kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * s / a.split);
-    kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (s + 1) / a.split);
+    kb0 = a.kblocks * s / a.split;   // kblocks < 2^24, split <= 16
+    kb1 = a.kblocks * (s + 1) / a.split;
     return s;
   };
 
   if (tid == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
     for (int s = 0; s < a.stages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < G8_SF_BUFS; ++i) {
       mbar_init(smem_u32(&bar_sf_full[i]), 4);
       mbar_init(smem_u32(&bar_sf_empty[i]), 1);
     }
@@ -169,37 +206,56 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       // the accumulators are free once the epilogue has read the tile before
       if (t != static_cast<int>(blockIdx.x) && !wait(bar_acc_empty, acc_phase ^ 1u)) ok = false;
       tc_fence_after_sync();
-      for (int kb = kb0; kb < kb1 && ok; ++kb) {
-        const int j = (kb - kb0) & 3;
-        if (j == 0 && !wait(bar_sf_full[sf], sf_phase)) ok = false;
-        if (ok && !wait(bar_full[s], phase)) ok = false;
-        if (!ok) break;
+      for (int kb = kb0; kb < kb1 && ok;) {
+        // `take` blocks of one group of scales at once: a look at a barrier, the election and what follows a commit take
+        // 600 clocks, as long as the MMAs of a small block, and so are paid once for up to four.
+        const int j0 = (kb - kb0) & 3, take = min(a.at_once, kb1 - kb);
+        const int ends = s + take;
+        bool there[5];   // the looks are in flight together
+        there[4] = j0 > 0 || mbar_try_wait(smem_u32(&bar_sf_full[sf]), sf_phase);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int st = s + i;
+          there[i] = i >= take || mbar_try_wait(smem_u32(&bar_full[st < a.stages ? st : st - a.stages]), st < a.stages ? phase : phase ^ 1u);
+        }
+        if (!__all_sync(0xffffffffu, there[0] && there[1] && there[2] && there[3] && there[4])) {
+          if (j0 == 0 && !wait(bar_sf_full[sf], sf_phase)) ok = false;
+          for (int i = s; i < ends && ok; ++i) ok = wait(bar_full[i < a.stages ? i : i - a.stages], i < a.stages ? phase : phase ^ 1u);
+          if (!ok) break;
+        }
         tc_fence_after_sync();
-        const uint32_t at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
-        const uint64_t ad = umma_desc_k_sw128(at), bd = umma_desc_k_sw128(at + MT * a_tile);
         const uint32_t sfa = tm + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE, sfb = sfa + 4 * MT;
-        const uint32_t idesc = g8_idesc(a.nt, j), more = kb > kb0 ? 1u : 0u;
-        const bool sf_last = j == 3 || kb + 1 == kb1;
+        const bool sf_last = j0 + take == 4 || kb + take == kb1;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < FP8_BLOCK / 32; ++k)   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
+          for (int i = 0; i < 4; ++i) {
+            if (i >= take) break;
+            const int st = s + i < a.stages ? s + i : s + i - a.stages;
+            const uint32_t at = smem_base + static_cast<uint32_t>(st) * stage_bytes;
+            const uint64_t ad = umma_desc_k_sw128(at), bd = umma_desc_k_sw128(at + MT * a_tile);
+            const uint32_t idesc = g8_idesc(a.nt, j0 + i), more = kb + i > kb0 ? 1u : 0u;
 #pragma unroll
-            for (int h = 0; h < MT; ++h)
-              umma_mxf8(tm + static_cast<uint32_t>(h * a.nt), ad + h * (a_tile >> 4) + 2 * k, bd + 2 * k, idesc, sfa + 4u * static_cast<uint32_t>(h), sfb,
-                        k > 0 ? 1u : more);
-          umma_commit(smem_u32(&bar_empty[s]));
+            for (int k = 0; k < FP8_BLOCK / 32; ++k)   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
+#pragma unroll
+              for (int h = 0; h < MT; ++h)
+                umma_mxf8(tm + static_cast<uint32_t>(h * a.nt), ad + h * (a_tile >> 4) + 2 * k, bd + 2 * k, idesc, sfa + 4u * static_cast<uint32_t>(h), sfb,
+                          k > 0 ? 1u : more);
+            umma_commit(smem_u32(&bar_empty[st]));
+          }
           if (sf_last) umma_commit(smem_u32(&bar_sf_empty[sf]));
-          if (kb + 1 == kb1) umma_commit(smem_u32(&bar_acc_full));
+          if (kb + take == kb1) umma_commit(smem_u32(&bar_acc_full));
         }
         __syncwarp();
-        if (sf_last && ++sf == 2) {
+        if (sf_last && ++sf == G8_SF_BUFS) {
           sf = 0;
           sf_phase ^= 1u;
         }
-        if (++s == a.stages) {
-          s = 0;
+        s = ends;
+        if (s >= a.stages) {
+          s -= a.stages;
           phase ^= 1u;
         }
+        kb += take;
       }
       acc_phase ^= 1u;
     }
@@ -218,56 +274,73 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     int sf = 0;
     uint32_t sf_phase = 0, acc_phase = 0, groups = 0;
     bool ok = true;
-    griddep_wait();   // x's exponents come from the kernel ahead, and out may still be being read
-    auto word = [&](const uint8_t* row, int kb, int kb1) {   // four successive exponents of a row
-      uint32_t w = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (kb + i < kb1) w |= static_cast<uint32_t>(__ldcg(row + kb + i)) << (8 * i);
-      return w;
+    // Four successive exponents of a row, wherever they start: the one or two words that they lie in, put together when
+    // they are used (that must not wait for the loads here).
+    auto get = [&](const uint8_t* row, int kb, int kb1, uint32_t (&w)[2]) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(row + kb);
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+      w[0] = __ldcg(p);
+      w[1] = static_cast<int>(at & 3) + min(kb1 - kb, 4) > 4 ? __ldcg(p + 1) : 0u;
     };
-    const bool words = (a.kblocks & 3) == 0 && (reinterpret_cast<uintptr_t>(a.xe) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.we) & 3) == 0;
+    auto joined = [&](const uint32_t (&w)[2], const uint8_t* row, int kb) {
+      return __funnelshift_r(w[0], w[1], 8 * static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + kb) & 3));
+    };
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       int tok, row, kb0, kb1;
       const int s = slice(t, tok, row, kb0, kb1);
-      const bool fast = words && (kb0 & 3) == 0;
-      auto fetch = [&](int kb, uint32_t (&wa)[MT][4], uint32_t (&wb)[8]) {
-        auto get = [&](const uint8_t* r) { return fast && kb + 4 <= kb1 ? __ldcg(reinterpret_cast<const uint32_t*>(r + kb)) : word(r, kb, kb1); };
+      auto x_row = [&](int h, int c) { return a.xe + static_cast<size_t>((tok * MT + h) * G8_TOK + 32 * c + lane) * a.kblocks; };
+      auto w_row = [&](int c) { return a.we + static_cast<size_t>((row * a.nt + 32 * c + lane) >> 7) * a.kblocks; };
+      auto fetch_x = [&](int kb, uint32_t (&wa)[MT][4][2]) {
 #pragma unroll
         for (int h = 0; h < MT; ++h)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int r = (tok * MT + h) * G8_TOK + 32 * c + lane;
-            wa[h][c] = r < a.m ? get(a.xe + static_cast<size_t>(r) * a.kblocks) : 0u;
+            wa[h][c][0] = wa[h][c][1] = 0u;
+            if ((tok * MT + h) * G8_TOK + 32 * c + lane < a.m) get(x_row(h, c), kb, kb1, wa[h][c]);
           }
+      };
+      auto fetch_w = [&](int kb, uint32_t (&wb)[8][2]) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const int r = row * a.nt + 32 * c + lane;
-          wb[c] = 32 * c < a.nt && r < a.n ? get(a.we + static_cast<size_t>(r >> 7) * a.kblocks) : 0u;
+          wb[c][0] = wb[c][1] = 0u;
+          if (32 * c < a.nt && row * a.nt + 32 * c + lane < a.n) get(w_row(c), kb, kb1, wb[c]);
         }
       };
-      uint32_t wa[MT][4], wb[8];
-      fetch(kb0, wa, wb);
+      uint32_t wa[MT][4][2], wb[8][2];
+      fetch_w(kb0, wb);
+      if (t == static_cast<int>(blockIdx.x)) griddep_wait();   // x's exponents come from the kernel ahead, and out may still be being read
+      fetch_x(kb0, wa);
       for (int kb = kb0; kb < kb1 && ok; kb += 4) {
-        if (groups >= 2 && !mbar_wait(smem_u32(&bar_sf_empty[sf]), sf_phase ^ 1u)) {
+        if (groups >= G8_SF_BUFS && !mbar_wait(smem_u32(&bar_sf_empty[sf]), sf_phase ^ 1u)) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
         const uint32_t at = tmem + lanes + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE;
 #pragma unroll
-        for (int h = 0; h < MT; ++h) tmem_st4(at + 4u * static_cast<uint32_t>(h), wa[h]);
-        tmem_st8(at + 4 * MT, wb);
+        for (int h = 0; h < MT; ++h) {
+          uint32_t v[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = joined(wa[h][c], x_row(h, c), kb);
+          tmem_st4(at + 4u * static_cast<uint32_t>(h), v);
+        }
+        uint32_t v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = joined(wb[c], w_row(c), kb);
+        tmem_st8(at + 4 * MT, v);
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_sf_full[sf]));
         ++groups;
-        if (++sf == 2) {
+        if (++sf == G8_SF_BUFS) {
           sf = 0;
           sf_phase ^= 1u;
         }
-        if (kb + 4 < kb1) fetch(kb + 4, wa, wb);
+        if (kb + 4 < kb1) {
+          fetch_w(kb + 4, wb);
+          fetch_x(kb + 4, wa);
+        }
       }
       if (ok && !mbar_wait(smem_u32(&bar_acc_full), acc_phase)) ok = false;
       if (!ok || s_abort) {
@@ -282,41 +355,16 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       for (int h = 0; h < MT; ++h) {
         const int token = (tok * MT + h) * G8_TOK + quarter * 32 + lane;
 #pragma unroll 1
-        for (int c = 0; c < a.nt; c += 16) {
-          uint32_t v[16];
-          tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c), v);
+        for (int c = 0; c < a.nt; c += 32) {
+          uint32_t v[2][16];
+          __syncwarp();
+          tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c), v[0]);
+          if (c + 16 < a.nt) tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c + 16), v[1]);
           tmem_ld_wait();
-          const int n0 = row * a.nt + c;
-          if (token >= a.m || n0 >= a.n) continue;
-          if (a.split > 1) {
-            float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
-            if ((a.n & 3) == 0 && n0 + 16 <= a.n) {
 #pragma unroll
-              for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (n0 + i < a.n) o[i] = __uint_as_float(v[i]);
-            }
-          } else {
-            __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
-            if (vec && n0 + 16 <= a.n) {
-#pragma unroll
-              for (int i = 0; i < 16; i += 8) {
-                uint32_t p[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[i + 2 * q]), __uint_as_float(v[i + 2 * q + 1]));
-                  p[q] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-                *reinterpret_cast<uint4*>(o + i) = make_uint4(p[0], p[1], p[2], p[3]);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (n0 + i < a.n) o[i] = __float2bfloat16_rn(__uint_as_float(v[i]));
-            }
+          for (int half = 0; half < 2; ++half) {
+            const int n0 = row * a.nt + c + 16 * half;
+            if (token < a.m && n0 < a.n && c + 16 * half < a.nt) put16(a, v[half], token, n0, s, vec);
           }
         }
       }
@@ -448,6 +496,7 @@ int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void*
   a.row_tiles = (n + p.nt - 1) / p.nt;
   a.split = p.split;
   a.stages = p.stages;
+  a.at_once = p.stages >= 8 ? 4 : p.stages >= 4 ? 2 : 1;
   CUtensorMap tx, tw;
   int r = encode_2d_u8(&tx, xq, m, k, a.a_rows);
   if (r == 0) r = encode_2d_u8(&tw, W, n, k, p.nt);

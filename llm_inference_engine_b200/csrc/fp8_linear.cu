@@ -9,6 +9,7 @@
 //                     blocks, so its x fragments, quantised in registers from BF16 (the four lanes of a token share
 //                     the block: two shuffles give its largest magnitude), and their scales never change.
 //   fp8_quantize_kernel   x to codes and exponents, for the many-token kernel (fp8_gemm.cu) and for callers.
+#include "../../include/muse_proj.h"
 #include "fp8.cuh"
 
 namespace muse {
@@ -56,6 +57,10 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
   __shared__ __align__(16) float red[2][NW][OUTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  const int tok0 = static_cast<int>(blockIdx.y) * 16;
+  x += static_cast<size_t>(tok0) * ld_x;
+  out += static_cast<size_t>(tok0) * ld_out;
+  m = min(m - tok0, 16);
   const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   const int ks = warp & (wk - 1), rs = warp / wk, rslots = NW / wk;   // this warp's K slice and row slot
   const int groups = (N + 7) >> 3;
@@ -180,13 +185,14 @@ static cudaError_t fp8_walk_launch(const void* W, const void* we, const void* x,
   int wk = 1;
   while (wk < NW && wk < kblocks) wk *= 2;
   const int sets = ((N + 7) / 8 + NW / wk - 1) / (NW / wk);
-  return launch_dependent(fp8_walk_kernel<NW, BPW, D, HI>, dim3(sets < sms ? sets : sms), dim3(NW * 32), 0, stream,
+  const int tokens = (m + 15) / 16, share = sms / tokens;
+  return launch_dependent(fp8_walk_kernel<NW, BPW, D, HI>, dim3(sets < share ? sets : share, tokens), dim3(NW * 32), 0, stream,
                           static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(we), static_cast<const __nv_bfloat16*>(x),
                           static_cast<__nv_bfloat16*>(out), m, N, K, ld_x, ld_out, wk);
 }
 
 int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, cudaStream_t stream) {
-  if (!W || !we || !x || !out || m < 1 || m > 16 || N < 1 || K < 16 || K % 16 || K > 8192) return -1;
+  if (!W || !we || !x || !out || m < 1 || m > MUSE_FP8_WALK_TOKENS || N < 1 || K < 16 || K % 16 || K > MUSE_FP8_WALK_K) return -1;
   if (ld_x < K || ld_x % 8 || ld_out < N || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
   const int sms = device_sms();
   if (sms < 1) return -4;
