@@ -12,8 +12,8 @@
 // products with MT = 2, hence the widest tile that tensor memory holds beside the scales (2 x 224 + 2 x 16 columns);
 // at 17..256 tokens it is the weight's own bytes, for which K is cut so that all SMs load.
 //
-// Roles: warp 0 TMA, warp 1 tensor memory and MMA issue, warps 2..5 scales (registers one group ahead) and epilogue, a
-// warp per quarter of the lanes. The grid is persistent: a CTA walks tiles of (K slice, row tile, token tile), and the
+// Roles: warps 0 and 6 TMA (W and x), warp 1 tensor memory and MMA issue, warps 2..5 scales (registers one group ahead)
+// and epilogue, a warp per quarter of the lanes. The grid is persistent: a CTA walks tiles of (K slice, row tile, token tile), and the
 // loads of its next tile start while the epilogue drains the accumulators. K slices leave FP32 sums in a workspace that a
 // second kernel adds up in slice order (same bits in every run).
 #include "fp8.cuh"
@@ -25,7 +25,8 @@ constexpr int G8_MAX_STAGES = 12;
 constexpr int G8_SF_COL = 448;          // first tensor-memory column of the scales
 constexpr int G8_SF_STRIDE = 16;        // columns of one group of scales: 4 per token tile, 8 for W's rows
 constexpr int G8_SF_BUFS = 4;           // groups of scales in tensor memory: 64 columns
-constexpr int G8_THREADS = 192;
+constexpr int G8_THREADS = 224;
+constexpr int G8_SMEM = 207 * 1024;     // beside the epilogue's staging rows
 constexpr int G8_MIN_SMEM = 116 * 1024;  // one CTA per SM: it takes all of tensor memory
 
 struct G8Args {
@@ -63,37 +64,23 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Sixteen sums of a token: BF16 to out, or FP32 to slice s of the workspace.
-__device__ __forceinline__ void put16(const G8Args& a, const uint32_t (&v)[16], int token, int n0, int s, bool vec) {
-  if (a.split > 1) {
-    float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
-    if ((a.n & 3) == 0 && n0 + 16 <= a.n) {
+// A warp's 32 rows of 32 values, one row per lane (WORDS words), to global memory through shared memory, so that a store
+// covers whole pieces of few rows: a row per lane would touch 32 lines with each store (the epilogue of 128 x 32 values
+// took 900 clocks that way). `first` is the first row's address, of which `rows` exist.
+template <int WORDS, int BYTES>
+__device__ __forceinline__ void put_rows(uint8_t* stage, const uint32_t (&v)[WORDS], uint8_t* first, size_t ld_bytes, int rows, int lane) {
+  constexpr int PIECES = WORDS / 4, STRIDE = 32 * BYTES + 16, STEP = 32 / PIECES;
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
+  for (int i = 0; i < PIECES; ++i)
+    *reinterpret_cast<uint4*>(stage + lane * STRIDE + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  const int piece = lane % PIECES;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n0 + i < a.n) o[i] = __uint_as_float(v[i]);
-    }
-  } else {
-    __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
-    if (vec && n0 + 16 <= a.n) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        uint32_t p[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[i + 2 * q]), __uint_as_float(v[i + 2 * q + 1]));
-          p[q] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(o + i) = make_uint4(p[0], p[1], p[2], p[3]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n0 + i < a.n) o[i] = __float2bfloat16_rn(__uint_as_float(v[i]));
-    }
+  for (int r0 = 0; r0 < 32; r0 += STEP) {
+    const int r = r0 + lane / PIECES;
+    if (r < rows) *reinterpret_cast<uint4*>(first + static_cast<size_t>(r) * ld_bytes + 16 * piece) = *reinterpret_cast<const uint4*>(stage + r * STRIDE + 16 * piece);
   }
+  __syncwarp();
 }
 
 template <int MT>
@@ -104,12 +91,12 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   __shared__ __align__(8) uint64_t bar_sf_full[G8_SF_BUFS], bar_sf_empty[G8_SF_BUFS], bar_acc_full, bar_acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_abort;
+  __shared__ __align__(16) uint8_t s_rows[4][32 * (32 * 4 + 16)];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // the 128-byte swizzle repeats every 1024 bytes
   const uint32_t a_tile = G8_TOK * FP8_BLOCK;                          // a token tile's place in a stage (its box may be shorter)
   const uint32_t b_bytes = static_cast<uint32_t>(a.nt) * FP8_BLOCK;
   const uint32_t stage_bytes = MT * a_tile + b_bytes;
-  const uint32_t tx_bytes = MT * static_cast<uint32_t>(a.a_rows) * FP8_BLOCK + b_bytes;
   const int tiles = a.row_tiles * a.tok_tiles * a.split;
   // Tile t: token tiles innermost (neighbouring CTAs share W's rows through L2), then row tiles, then K slices.
   auto slice = [&](int t, int& tok, int& row, int& kb0, int& kb1) {
@@ -125,7 +112,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_x);
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_full[s]), 2);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
     for (int i = 0; i < G8_SF_BUFS; ++i) {
@@ -147,20 +134,20 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   const uint32_t tmem = tmem_slot;
   griddep_launch_dependents();
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 6) {
+    // ---- loads, W by one warp and x by another: W's do not wait for the kernel ahead, and one thread issues a copy
+    // every 400 clocks or so
     if (lane == 0) {
       const uint64_t pol = l2_policy_evict_last();
+      const bool is_x = warp == 6;
+      const uint32_t bytes = is_x ? MT * static_cast<uint32_t>(a.a_rows) * FP8_BLOCK : b_bytes;
       int s = 0;
       uint32_t phase = 0, issued = 0;
-      bool ok = true, waited = false;
-      auto load_x = [&](int st, int kb, int tok) {
-        const uint32_t bar = smem_u32(&bar_full[st]), at = smem_base + static_cast<uint32_t>(st) * stage_bytes;
-        for (int h = 0; h < MT; ++h) tma_load_2d(at + static_cast<uint32_t>(h) * a_tile, &tm_x, kb * FP8_BLOCK, (tok * MT + h) * G8_TOK, bar, pol);
-      };
+      bool ok = true;
+      if (is_x) griddep_wait();
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         int tok, row, kb0, kb1;
         slice(t, tok, row, kb0, kb1);
-        int held = 0;   // stages whose weights are under way while x may still be being written by the kernel ahead
         for (int kb = kb0; kb < kb1; ++kb) {
           if (issued >= static_cast<uint32_t>(a.stages) && !mbar_wait(smem_u32(&bar_empty[s]), phase ^ 1u)) {
             atomicOr(a.status, ST_PRODUCER_TIMEOUT);
@@ -169,23 +156,20 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
             break;
           }
           const uint32_t bar = smem_u32(&bar_full[s]), at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
-          mbar_expect_tx(bar, tx_bytes);
-          tma_load_2d(at + MT * a_tile, &tm_w, kb * FP8_BLOCK, row * a.nt, bar, pol);
-          ++issued;
-          if (waited) {
-            load_x(s, kb, tok);
-          } else if (++held == a.stages || kb + 1 == kb1) {
-            griddep_wait();
-            waited = true;
-            for (int i = 0; i < held; ++i) load_x(i, kb0 + i, tok);
+          mbar_expect_tx(bar, bytes);
+          if (is_x) {
+            for (int h = 0; h < MT; ++h) tma_load_2d(at + static_cast<uint32_t>(h) * a_tile, &tm_x, kb * FP8_BLOCK, (tok * MT + h) * G8_TOK, bar, pol);
+          } else {
+            tma_load_2d(at + MT * a_tile, &tm_w, kb * FP8_BLOCK, row * a.nt, bar, pol);
           }
+          ++issued;
           if (++s == a.stages) {
             s = 0;
             phase ^= 1u;
           }
         }
       }
-      if (!ok)   // leave no copy in flight: the stages issued last (bounded)
+      if (!ok)   // leave no copy in flight: the stages issued last (bounded; a stage that the other loader has not reached is waited for in vain)
         for (int i = 0; i < a.stages && i < static_cast<int>(issued); ++i) {
           const uint32_t j = issued - 1 - static_cast<uint32_t>(i);
           if (!mbar_wait(smem_u32(&bar_full[j % static_cast<uint32_t>(a.stages)]), (j / static_cast<uint32_t>(a.stages)) & 1u)) atomicOr(a.status, ST_DRAIN_TIMEOUT);
@@ -350,21 +334,52 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       }
       acc_phase ^= 1u;
       tc_fence_after_sync();
-      const bool vec = (a.ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.nt & 7) == 0;
+      const bool vec = (a.ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.nt & 7) == 0, vec_ws = (a.n & 3) == 0;
+      uint8_t* stage = s_rows[quarter];
 #pragma unroll 1
       for (int h = 0; h < MT; ++h) {
         const int token = (tok * MT + h) * G8_TOK + quarter * 32 + lane;
 #pragma unroll 1
         for (int c = 0; c < a.nt; c += 32) {
-          uint32_t v[2][16];
+          uint32_t v[32];
           __syncwarp();
-          tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c), v[0]);
-          if (c + 16 < a.nt) tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c + 16), v[1]);
+          tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c), reinterpret_cast<uint32_t(&)[16]>(v[0]));
+          if (c + 16 < a.nt) tmem_ld16(tmem + lanes + static_cast<uint32_t>(h * a.nt + c + 16), reinterpret_cast<uint32_t(&)[16]>(v[16]));
           tmem_ld_wait();
+          const int n0 = row * a.nt + c, cols = min(min(32, a.nt - c), a.n - n0);
+          if (cols <= 0) continue;   // (the same in all lanes)
+          const int rows = min(32, a.m - (token - lane));
+          if (a.split > 1) {
+            float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
+            if (vec_ws && cols == 32) {
+              put_rows<32, 4>(stage, v, reinterpret_cast<uint8_t*>(o - static_cast<size_t>(lane) * a.n), static_cast<size_t>(a.n) * 4, rows, lane);
+            } else if (lane < rows && vec_ws) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int n0 = row * a.nt + c + 16 * half;
-            if (token < a.m && n0 < a.n && c + 16 * half < a.nt) put16(a, v[half], token, n0, s, vec);
+              for (int i = 0; i < 32; i += 4)
+                if (i < cols) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else if (lane < rows) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < cols) o[i] = __uint_as_float(v[i]);
+            }
+          } else {
+            __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              p[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            if (vec && cols == 32) {
+              put_rows<16, 2>(stage, p, reinterpret_cast<uint8_t*>(o - static_cast<size_t>(lane) * a.ld_out), static_cast<size_t>(a.ld_out) * 2, rows, lane);
+            } else if (lane < rows && vec && cols == 16) {   // a tile's last columns, where nt is not a multiple of 32
+              *reinterpret_cast<uint4*>(o) = make_uint4(p[0], p[1], p[2], p[3]);
+              *reinterpret_cast<uint4*>(o + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+            } else if (lane < rows) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < cols) reinterpret_cast<unsigned short*>(o)[i] = static_cast<unsigned short>(p[i / 2] >> (16 * (i & 1)));
+            }
           }
         }
       }
@@ -436,7 +451,7 @@ static G8Plan g8_search(int m, int n, int k, int sms) {
     }
   }
   const int stage = best.mt * G8_TOK * FP8_BLOCK + best.nt * FP8_BLOCK;
-  best.stages = (225 * 1024 - 1024) / stage;
+  best.stages = (G8_SMEM - 1024) / stage;
   if (best.stages > G8_MAX_STAGES) best.stages = G8_MAX_STAGES;
   return best;
 }
@@ -465,7 +480,7 @@ template <int MT>
 static cudaError_t g8_launch(const CUtensorMap& tx, const CUtensorMap& tw, const G8Args& a, int grid, size_t smem, cudaStream_t stream) {
   static DeviceOnce once;   // the largest any plan asks for, once
   cudaError_t e = cudaSuccess;
-  if (once.first()) e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+  if (once.first()) e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_SMEM);
   if (e != cudaSuccess) return e;
   once.done();
   return launch_dependent(fp8_gemm_kernel<MT>, dim3(grid), dim3(G8_THREADS), smem, stream, tx, tw, a);
