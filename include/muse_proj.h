@@ -354,13 +354,16 @@ int muse_skinny_tc_noalloc(const void* tmap_w, const void* tmap_w_lo, const void
  * in the reference, whose weights are BF16. */
 /* x BF16 [m, K] (ld_x elements between rows, ld_x % 8 == 0) to codes xq [m, K] and exponent bytes xe. */
 int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x, void* stream);
-#define MUSE_FP8_WALK_TOKENS 16
+#define MUSE_FP8_WALK_TOKENS 8
 #define MUSE_FP8_WALK_K 8192
 /* 1 .. MUSE_FP8_WALK_TOKENS tokens, K <= MUSE_FP8_WALK_K: x in BF16, quantised on the way; one launch. */
 int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream);
 
-/* Any number of tokens, x already in 8 bits: TMA and block-scaled tcgen05 MMAs. ws: muse_fp8_gemm_ws_bytes bytes (0: may be NULL), 16-byte aligned,
- * contents irrelevant; it belongs to the call until it completes. status: as for muse_gemm_tc. */
+/* Any number of tokens, x already in 8 bits: TMA and block-scaled tcgen05 MMAs. Where the walk is allowed too it is the faster
+ * one up to weights of MUSE_FP8_WALK_BYTES (us per call on a B200, walk / quantize + gemm, 8 tokens: 256 x 4096 3.8 / 7.1, 4096 x
+ * 4096 7.7 / 9.4, 4096 x 8192 12.8 / 14.0, 12288 x 4096 15.5 / 14.0; the gemm with 9 tokens 9.6 where a walk of twice the
+ * tokens took 11.1). ws: muse_fp8_gemm_ws_bytes bytes (0: may be NULL), 16-byte aligned, contents irrelevant; it belongs to the call until it completes. status: as for muse_gemm_tc. */
+#define MUSE_FP8_WALK_BYTES (40ll << 20)
 long long muse_fp8_gemm_ws_bytes(int m, int N, int K);
 int muse_fp8_gemm(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int N, int K,
                   int ld_out, void* stream);

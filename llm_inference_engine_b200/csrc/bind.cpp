@@ -70,7 +70,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {   // x, 
     Py_RETURN_NONE;
   const int64_t ld = m > 1 ? x->stride(0) : k;
   if (ld > INT32_MAX) Py_RETURN_NONE;
-  const bool walk = m <= MUSE_FP8_WALK_TOKENS && k <= MUSE_FP8_WALK_K;
+  const bool walk = m <= MUSE_FP8_WALK_TOKENS && k <= MUSE_FP8_WALK_K && n * k <= MUSE_FP8_WALK_BYTES;
   if (!walk && !status_of[index]) Py_RETURN_NONE;
   void* stream = stream_of(index);
   at::Tensor out = at::empty({m, n}, x->options());

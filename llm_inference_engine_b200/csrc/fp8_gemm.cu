@@ -9,8 +9,13 @@
 // selects; so one store serves 512 columns of K.
 //
 // What bounds it at many tokens is traffic from L2 into shared memory, (256 + nt) x 128 bytes per 256 x nt x 128
-// products with MT = 2, hence the widest tile that tensor memory holds beside the scales (2 x 224 + 2 x 16 columns);
-// at 17..256 tokens it is the weight's own bytes, for which K is cut so that all SMs load.
+// products with MT = 2, hence the widest tile that tensor memory holds beside the scales (2 x 224 + 4 x 16 columns);
+// at fewer it is the weight's own bytes from memory, and below 20 MB of them the start (4 us to the first MMA behind the
+// quantizing kernel: set-up, x's exponents, one block's way through) and the end. K is cut where that lets all SMs load.
+// Measured with the quantizing kernel (us; TB/s of W or TFLOP/s): 27 x 4093 x 2064 8.8; 27 x 12288 x 4096 14.8 (3.4 TB/s);
+// 256 x 12288 x 4096 18.6 (1390 TFLOP/s); 4096 x 12288 x 4096 190 (2170 TFLOP/s). What gave the most: a warp that waits, issues
+// and commits for several blocks of K at once (a block alone costs 730 clocks of latency, four cost 1330), uniform issue,
+// exponents that are joined from whole words when used instead of byte by byte when loaded, results through shared memory.
 //
 // Roles: warps 0 and 6 TMA (W and x), warp 1 tensor memory and MMA issue, warps 2..5 scales (registers one group ahead)
 // and epilogue, a warp per quarter of the lanes. The grid is persistent: a CTA walks tiles of (K slice, row tile, token tile), and the
@@ -35,7 +40,7 @@ struct G8Args {
   __nv_bfloat16* out;
   float* ws;           // [split, m, N] when split > 1
   int* status;
-  int m, n, k, kblocks, ld_out;
+  int m, n, kblocks, ld_out;
   int nt, a_rows;      // rows of W per tile; token rows a TMA box brings
   int row_tiles, tok_tiles, split, stages;
   int at_once;         // blocks of K that the MMA warp takes at a time: 1, 2 or 4, at most half of the stages
@@ -65,20 +70,30 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A warp's 32 rows of 32 values, one row per lane (WORDS words), to global memory through shared memory, so that a store
-// covers whole pieces of few rows: a row per lane would touch 32 lines with each store (the epilogue of 128 x 32 values
-// took 900 clocks that way). `first` is the first row's address, of which `rows` exist.
+// covers pieces of few rows: a row per lane would touch 32 lines with each store (the epilogue of 128 x 32 values
+// took 900 clocks that way, now 550). `first` is the first row's address; `rows` rows and `cols` values of each exist; `vec`:
+// rows start on 16 bytes.
 template <int WORDS, int BYTES>
-__device__ __forceinline__ void put_rows(uint8_t* stage, const uint32_t (&v)[WORDS], uint8_t* first, size_t ld_bytes, int rows, int lane) {
+__device__ __forceinline__ void put_rows(uint8_t* stage, const uint32_t (&v)[WORDS], uint8_t* first, size_t ld_bytes, int rows, int cols, bool vec, int lane) {
   constexpr int PIECES = WORDS / 4, STRIDE = 32 * BYTES + 16, STEP = 32 / PIECES;
 #pragma unroll
   for (int i = 0; i < PIECES; ++i)
     *reinterpret_cast<uint4*>(stage + lane * STRIDE + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   __syncwarp();
-  const int piece = lane % PIECES;
+  if (vec && (cols * BYTES) % 16 == 0) {
+    const int piece = lane % PIECES;
 #pragma unroll
-  for (int r0 = 0; r0 < 32; r0 += STEP) {
-    const int r = r0 + lane / PIECES;
-    if (r < rows) *reinterpret_cast<uint4*>(first + static_cast<size_t>(r) * ld_bytes + 16 * piece) = *reinterpret_cast<const uint4*>(stage + r * STRIDE + 16 * piece);
+    for (int r0 = 0; r0 < 32; r0 += STEP) {
+      const int r = r0 + lane / PIECES;
+      if (r < rows && piece * 16 < cols * BYTES)
+        *reinterpret_cast<uint4*>(first + static_cast<size_t>(r) * ld_bytes + 16 * piece) = *reinterpret_cast<const uint4*>(stage + r * STRIDE + 16 * piece);
+    }
+  } else if (lane < cols) {
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(first + static_cast<size_t>(r) * ld_bytes + 4 * lane) = *reinterpret_cast<const uint32_t*>(stage + r * STRIDE + 4 * lane);
+      else *reinterpret_cast<unsigned short*>(first + static_cast<size_t>(r) * ld_bytes + 2 * lane) = *reinterpret_cast<const unsigned short*>(stage + r * STRIDE + 2 * lane);
+    }
   }
   __syncwarp();
 }
@@ -135,45 +150,50 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
   griddep_launch_dependents();
 
   if (warp == 0 || warp == 6) {
-    // ---- loads, W by one warp and x by another: W's do not wait for the kernel ahead, and one thread issues a copy
-    // every 400 clocks or so
-    if (lane == 0) {
-      const uint64_t pol = l2_policy_evict_last();
-      const bool is_x = warp == 6;
-      const uint32_t bytes = is_x ? MT * static_cast<uint32_t>(a.a_rows) * FP8_BLOCK : b_bytes;
-      int s = 0;
-      uint32_t phase = 0, issued = 0;
-      bool ok = true;
-      if (is_x) griddep_wait();
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        int tok, row, kb0, kb1;
-        slice(t, tok, row, kb0, kb1);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (issued >= static_cast<uint32_t>(a.stages) && !mbar_wait(smem_u32(&bar_empty[s]), phase ^ 1u)) {
-            atomicOr(a.status, ST_PRODUCER_TIMEOUT);
-            s_abort = 1;
-            ok = false;
-            break;
-          }
-          const uint32_t bar = smem_u32(&bar_full[s]), at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
+    // ---- loads, W by one warp and x by another (W's do not wait for the kernel ahead). The whole warps walk along and one
+    // elected lane issues, as for the MMAs.
+    const uint64_t pol = l2_policy_evict_last();
+    const bool is_x = warp == 6;
+    const uint32_t bytes = is_x ? MT * static_cast<uint32_t>(a.a_rows) * FP8_BLOCK : b_bytes;
+    int s = 0;
+    uint32_t phase = 0, issued = 0;
+    bool ok = true;
+    if (is_x) griddep_wait();
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tok, row, kb0, kb1;
+      slice(t, tok, row, kb0, kb1);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (issued >= static_cast<uint32_t>(a.stages) && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_empty[s]), phase ^ 1u))) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = smem_u32(&bar_full[s]), at = smem_base + static_cast<uint32_t>(s) * stage_bytes;
+        if (elect_one()) {
           mbar_expect_tx(bar, bytes);
           if (is_x) {
+#pragma unroll
             for (int h = 0; h < MT; ++h) tma_load_2d(at + static_cast<uint32_t>(h) * a_tile, &tm_x, kb * FP8_BLOCK, (tok * MT + h) * G8_TOK, bar, pol);
           } else {
             tma_load_2d(at + MT * a_tile, &tm_w, kb * FP8_BLOCK, row * a.nt, bar, pol);
           }
-          ++issued;
-          if (++s == a.stages) {
-            s = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == a.stages) {
+          s = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok)   // leave no copy in flight: the stages issued last (bounded; a stage that the other loader has not reached is waited for in vain)
-        for (int i = 0; i < a.stages && i < static_cast<int>(issued); ++i) {
-          const uint32_t j = issued - 1 - static_cast<uint32_t>(i);
-          if (!mbar_wait(smem_u32(&bar_full[j % static_cast<uint32_t>(a.stages)]), (j / static_cast<uint32_t>(a.stages)) & 1u)) atomicOr(a.status, ST_DRAIN_TIMEOUT);
-        }
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(a.status, ST_PRODUCER_TIMEOUT);
+      s_abort = 1;
+      // leave no copy in flight: the stages issued last (bounded; a stage that the other loader has not reached is waited for in vain)
+      for (int i = 0; i < a.stages && i < static_cast<int>(issued); ++i) {
+        const uint32_t j = issued - 1 - static_cast<uint32_t>(i);
+        if (!mbar_wait(smem_u32(&bar_full[j % static_cast<uint32_t>(a.stages)]), (j / static_cast<uint32_t>(a.stages)) & 1u) && lane == 0)
+          atomicOr(a.status, ST_DRAIN_TIMEOUT);
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -334,7 +354,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       }
       acc_phase ^= 1u;
       tc_fence_after_sync();
-      const bool vec = (a.ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.nt & 7) == 0, vec_ws = (a.n & 3) == 0;
+      const bool vec = (a.ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.nt & 7) == 0;
       uint8_t* stage = s_rows[quarter];
 #pragma unroll 1
       for (int h = 0; h < MT; ++h) {
@@ -350,36 +370,17 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
           if (cols <= 0) continue;   // (the same in all lanes)
           const int rows = min(32, a.m - (token - lane));
           if (a.split > 1) {
-            float* o = a.ws + (static_cast<size_t>(s) * a.m + token) * a.n + n0;
-            if (vec_ws && cols == 32) {
-              put_rows<32, 4>(stage, v, reinterpret_cast<uint8_t*>(o - static_cast<size_t>(lane) * a.n), static_cast<size_t>(a.n) * 4, rows, lane);
-            } else if (lane < rows && vec_ws) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                if (i < cols) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            } else if (lane < rows) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < cols) o[i] = __uint_as_float(v[i]);
-            }
+            put_rows<32, 4>(stage, v, reinterpret_cast<uint8_t*>(a.ws + (static_cast<size_t>(s) * a.m + (token - lane)) * a.n + n0),
+                            static_cast<size_t>(a.n) * 4, rows, cols, (a.n & 3) == 0, lane);
           } else {
-            __nv_bfloat16* o = a.out + static_cast<size_t>(token) * a.ld_out + n0;
             uint32_t p[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
               p[i] = *reinterpret_cast<const uint32_t*>(&b);
             }
-            if (vec && cols == 32) {
-              put_rows<16, 2>(stage, p, reinterpret_cast<uint8_t*>(o - static_cast<size_t>(lane) * a.ld_out), static_cast<size_t>(a.ld_out) * 2, rows, lane);
-            } else if (lane < rows && vec && cols == 16) {   // a tile's last columns, where nt is not a multiple of 32
-              *reinterpret_cast<uint4*>(o) = make_uint4(p[0], p[1], p[2], p[3]);
-              *reinterpret_cast<uint4*>(o + 8) = make_uint4(p[4], p[5], p[6], p[7]);
-            } else if (lane < rows) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < cols) reinterpret_cast<unsigned short*>(o)[i] = static_cast<unsigned short>(p[i / 2] >> (16 * (i & 1)));
-            }
+            put_rows<16, 2>(stage, p, reinterpret_cast<uint8_t*>(a.out + static_cast<size_t>(token - lane) * a.ld_out + n0), static_cast<size_t>(a.ld_out) * 2,
+                            rows, cols, vec, lane);
           }
         }
       }
@@ -424,10 +425,19 @@ struct G8Plan {
   int mt, nt, split, stages;
 };
 
-// The tile and the K slices that make the longest CTA's traffic smallest: bytes it brings into shared memory, at
-// about 60 bytes per ns, against its MMAs, plus what a tile and a join cost.
+// Stages of the ring, and blocks of K that the MMA warp takes at once.
+static int g8_stages(int mt, int nt) {
+  const int fit = (G8_SMEM - 1024) / ((mt * G8_TOK + nt) * FP8_BLOCK);
+  return fit < G8_MAX_STAGES ? fit : G8_MAX_STAGES;
+}
+static int g8_at_once(int stages) { return stages >= 8 ? 4 : stages >= 4 ? 2 : 1; }
+
+// The tile and the K slices with the shortest time by what was measured, in ns: a block of K costs a CTA the bytes that it
+// brings into shared memory (140 a ns), its MMAs, or the issuing of them (385, 250 or 185 for 1, 2 or 4 blocks at once),
+// whichever is longest, and all CTAs together W's bytes from memory (6000 a ns); 290 per 32 columns of the epilogue; slices cost a second launch and the sums' way through L2.
 static G8Plan g8_search(int m, int n, int k, int sms) {
   const int kblocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
+  const double from_memory = static_cast<double>(n) * k / 6000.0;
   G8Plan best = {};
   double best_ns = 1e30;
   for (int mt = 1; mt <= 2; ++mt) {
@@ -435,24 +445,24 @@ static G8Plan g8_search(int m, int n, int k, int sms) {
     const int tok_tiles = (m + mt * G8_TOK - 1) / (mt * G8_TOK);
     const double a_rows = mt == 1 && m < G8_TOK ? (m + 7) / 8 * 8 : mt * G8_TOK;
     for (int nt = 32; nt <= (mt == 2 ? 224 : 256); nt += 16) {
-      const int row_tiles = (n + nt - 1) / nt;
+      const int row_tiles = (n + nt - 1) / nt, at_once = g8_at_once(g8_stages(mt, nt));
+      const double issue = at_once == 4 ? 185.0 : at_once == 2 ? 250.0 : 385.0, load = (a_rows + nt) * FP8_BLOCK / 140.0, mma = 1.05 * mt * nt;
+      const double block = load > mma ? (load > issue ? load : issue) : mma > issue ? mma : issue;
       for (int split = 1; split <= 16 && split <= kblocks; ++split) {
         const long long tiles = static_cast<long long>(tok_tiles) * row_tiles * split;
         const long long waves = (tiles + sms - 1) / sms;
         const int kb = (kblocks + split - 1) / split;
-        const double load = kb * (a_rows + nt) * FP8_BLOCK / 60.0, mma = kb * 4.0 * mt * nt / 2.0 / 1.8;
-        double ns = waves * ((load > mma ? load : mma) + 1500.0 + 8.0 * mt * nt / 2) + 3000.0;
-        if (split > 1) ns += 2000.0 + static_cast<double>(m) * n * split * 8 / 5000.0;
+        double body = static_cast<double>(waves) * kb * block;
+        if (body < from_memory) body = from_memory;
+        double ns = body + waves * (290.0 * mt * ((nt + 31) / 32) + 300.0);
+        if (split > 1) ns += 2200.0 + static_cast<double>(m) * n * split * 8 / 4000.0;
         if (ns < best_ns) {
           best_ns = ns;
-          best = {mt, nt, split, 0};
+          best = {mt, nt, split, g8_stages(mt, nt)};
         }
       }
     }
   }
-  const int stage = best.mt * G8_TOK * FP8_BLOCK + best.nt * FP8_BLOCK;
-  best.stages = (G8_SMEM - 1024) / stage;
-  if (best.stages > G8_MAX_STAGES) best.stages = G8_MAX_STAGES;
   return best;
 }
 
@@ -502,7 +512,7 @@ int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void*
   a.out = static_cast<__nv_bfloat16*>(out);
   a.ws = static_cast<float*>(ws);
   a.status = status;
-  a.m = m; a.n = n; a.k = k;
+  a.m = m; a.n = n;
   a.kblocks = (k + FP8_BLOCK - 1) / FP8_BLOCK;
   a.ld_out = ld_out;
   a.nt = p.nt;
@@ -511,7 +521,7 @@ int fp8_gemm_dispatch(const void* W, const void* we, const void* xq, const void*
   a.row_tiles = (n + p.nt - 1) / p.nt;
   a.split = p.split;
   a.stages = p.stages;
-  a.at_once = p.stages >= 8 ? 4 : p.stages >= 4 ? 2 : 1;
+  a.at_once = g8_at_once(p.stages);
   CUtensorMap tx, tw;
   int r = encode_2d_u8(&tx, xq, m, k, a.a_rows);
   if (r == 0) r = encode_2d_u8(&tw, W, n, k, p.nt);

@@ -3,8 +3,8 @@
 // BF16 out; x comes in BF16 and is quantised here (one exponent per token and 128 columns), W as codes and exponent
 // bytes. The products of codes are exact in FP32 and so is the scaling; the sums are FP32.
 //
-//   fp8_walk_kernel       up to 16 tokens: the persistent walk of fewtok_mma.cu over half the bytes. Tokens are the MMA's
-//                     M = 16, 8 weight rows its N; a lane loads 16-byte pieces of W straight into the B fragments of
+//   fp8_walk_kernel       up to 8 tokens: the persistent walk of fewtok_mma.cu over half the bytes. Tokens are half of the
+//                     MMA's M = 16, 8 weight rows its N; a lane loads 16-byte pieces of W straight into the B fragments of
 //                     two m16n8k32 MMAs (the k slots are a permutation that x follows). A warp owns whole 128-column
 //                     blocks, so its x fragments, quantised in registers from BF16 (the four lanes of a token share
 //                     the block: two shuffles give its largest magnitude), and their scales never change.
@@ -46,21 +46,17 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const __nv_bfloat16* 
   if (lane == 0) xe[static_cast<size_t>(t) * kblocks + b] = static_cast<uint8_t>(e);
 }
 
-// ---------------------------------------------------------------- up to 16 tokens
-// NW warps; BPW blocks of K per warp (K <= 128 * NW * BPW); D row groups in flight per warp; HI: tokens 8..15 exist.
+// ---------------------------------------------------------------- up to 8 tokens
+// NW warps; BPW blocks of K per warp (K <= 128 * NW * BPW); D row groups in flight per warp.
 // The warps are wk (a power of two) slices of K times NW / wk neighbouring row groups.
-template <int NW, int BPW, int D, bool HI>
+template <int NW, int BPW, int D>
 __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ we,
                                                            const __nv_bfloat16* __restrict__ x, __nv_bfloat16* __restrict__ out, int m,
                                                            int N, int K, int ld_x, int ld_out, int wk) {
-  constexpr int OUTS = HI ? 128 : 64;   // 8 or 16 tokens x 8 rows
+  constexpr int OUTS = 64;   // 8 tokens x 8 rows
   __shared__ __align__(16) float red[2][NW][OUTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int tok0 = static_cast<int>(blockIdx.y) * 16;
-  x += static_cast<size_t>(tok0) * ld_x;
-  out += static_cast<size_t>(tok0) * ld_out;
-  m = min(m - tok0, 16);
   const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   const int ks = warp & (wk - 1), rs = warp / wk, rslots = NW / wk;   // this warp's K slice and row slot
   const int groups = (N + 7) >> 3;
@@ -90,9 +86,9 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
   griddep_launch_dependents();
   griddep_wait();   // x and out belong to the stream: only the weights were touched so far
 
-  // x fragments: the lane's 32 columns of each of its blocks, for token g (and g + 8), in BF16 -> codes in registers.
-  uint32_t xa[BPW][8], xb[HI ? BPW : 1][8];
-  float sa[BPW], sb[HI ? BPW : 1];
+  // x fragments: the lane's 32 columns of each of its blocks, for token g, in BF16 -> codes in registers.
+  uint32_t xa[BPW][8];
+  float sa[BPW];
   auto quantise = [&](int tok, int kb, uint32_t (&q)[8], float& scale) {
     uint4 v[4];
 #pragma unroll
@@ -121,38 +117,30 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
     }
   };
 #pragma unroll
-  for (int j = 0; j < BPW; ++j) {
-    quantise(g, ks + j * wk, xa[j], sa[j]);
-    if constexpr (HI) quantise(g + 8, ks + j * wk, xb[j], sb[j]);
-  }
+  for (int j = 0; j < BPW; ++j) quantise(g, ks + j * wk, xa[j], sa[j]);
 
   for (int i0 = 0; i0 < my_sets; i0 += D) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int i = i0 + d;
       if (i < my_sets) {   // CTA-uniform
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float acc[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < BPW; ++j) {
           float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const uint4 u = w[d][j][p];
-            mma_e4m3_16832(c, xa[j][4 * p], HI ? xb[HI ? j : 0][4 * p] : 0u, xa[j][4 * p + 1], HI ? xb[HI ? j : 0][4 * p + 1] : 0u, u.x, u.y);
-            mma_e4m3_16832(c, xa[j][4 * p + 2], HI ? xb[HI ? j : 0][4 * p + 2] : 0u, xa[j][4 * p + 3], HI ? xb[HI ? j : 0][4 * p + 3] : 0u, u.z, u.w);
+            mma_e4m3_16832(c, xa[j][4 * p], 0u, xa[j][4 * p + 1], 0u, u.x, u.y);
+            mma_e4m3_16832(c, xa[j][4 * p + 2], 0u, xa[j][4 * p + 3], 0u, u.z, u.w);
           }
           const float s = exp2_byte(static_cast<int>(se[d][j]));
           acc[0] = fmaf(c[0], s * sa[j], acc[0]);
           acc[1] = fmaf(c[1], s * sa[j], acc[1]);
-          if constexpr (HI) {
-            acc[2] = fmaf(c[2], s * sb[j], acc[2]);
-            acc[3] = fmaf(c[3], s * sb[j], acc[3]);
-          }
         }
         if (i + D < my_sets) load(w[d], se[d], i + D);   // into the registers just read: in flight across the reduction
         float* mine = red[i & 1][warp];
         *reinterpret_cast<float2*>(mine + g * 8 + 2 * t) = make_float2(acc[0], acc[1]);
-        if constexpr (HI) *reinterpret_cast<float2*>(mine + (g + 8) * 8 + 2 * t) = make_float2(acc[2], acc[3]);
         __syncthreads();   // the buffer written two steps ago is free again once every warp passed this
         for (int o = threadIdx.x; o < rslots * OUTS; o += NW * 32) {
           const int slot = o / OUTS, v = o % OUTS;
@@ -178,15 +166,14 @@ int fp8_quantize_dispatch(const void* x, void* xq, void* xe, int m, int K, int l
                                            static_cast<const __nv_bfloat16*>(x), static_cast<uint8_t*>(xq), static_cast<uint8_t*>(xe), m, K, ld_x, kblocks));
 }
 
-template <int NW, int BPW, int D, bool HI>
+template <int NW, int BPW, int D>
 static cudaError_t fp8_walk_launch(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out,
                                    int sms, cudaStream_t stream) {
   const int kblocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   int wk = 1;
   while (wk < NW && wk < kblocks) wk *= 2;
   const int sets = ((N + 7) / 8 + NW / wk - 1) / (NW / wk);
-  const int tokens = (m + 15) / 16, share = sms / tokens;
-  return launch_dependent(fp8_walk_kernel<NW, BPW, D, HI>, dim3(sets < share ? sets : share, tokens), dim3(NW * 32), 0, stream,
+  return launch_dependent(fp8_walk_kernel<NW, BPW, D>, dim3(sets < sms ? sets : sms), dim3(NW * 32), 0, stream,
                           static_cast<const uint8_t*>(W), static_cast<const uint8_t*>(we), static_cast<const __nv_bfloat16*>(x),
                           static_cast<__nv_bfloat16*>(out), m, N, K, ld_x, ld_out, wk);
 }
@@ -196,16 +183,9 @@ int fp8_walk_dispatch(const void* W, const void* we, const void* x, void* out, i
   if (ld_x < K || ld_x % 8 || ld_out < N || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W)) & 15)) return -2;
   const int sms = device_sms();
   if (sms < 1) return -4;
-  cudaError_t e;
-  // 32 warps of 64 registers hold 16 bytes x 4 of W and up to 16 words of x per lane; longer rows of more tokens
-  // take 16 warps of 128.
-  if (K <= 4096)
-    e = m <= 8 ? fp8_walk_launch<32, 1, 2, false>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
-               : fp8_walk_launch<32, 1, 2, true>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream);
-  else
-    e = m <= 8 ? fp8_walk_launch<32, 2, 1, false>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
-               : fp8_walk_launch<16, 4, 1, true>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream);
-  return static_cast<int>(e);
+  // 32 warps of 64 registers hold two row groups of one block of K in flight, or one of two blocks.
+  return static_cast<int>(K <= 4096 ? fp8_walk_launch<32, 1, 2>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream)
+                                    : fp8_walk_launch<32, 2, 1>(W, we, x, out, m, N, K, ld_x, ld_out, sms, stream));
 }
 
 }  // namespace muse

@@ -21,8 +21,10 @@ from . import _capi
 BLOCK = 128
 E_MIN = -64
 _INT_MAX = 0x7fffffff
-WALK_MAX_TOKENS = 16   # csrc/fp8_linear.cu; more tokens or a longer K take csrc/fp8_gemm.cu
+# What csrc/fp8_linear.cu takes in one launch; the rest csrc/fp8_gemm.cu (include/muse_proj.h has both sides' times).
+WALK_MAX_TOKENS = 8
 WALK_MAX_K = 8192
+WALK_MAX_BYTES = 40 << 20
 
 
 def _require(t: torch.Tensor, what: str, dtype: torch.dtype, dims: int) -> None:
@@ -170,7 +172,7 @@ def linear(x, w8: torch.Tensor, w_exp: torch.Tensor, out: torch.Tensor | None = 
             out = _capi.new_tensor((m, n), (n, 1), _BF16, dev)
         if not pair:
             x = _rows(x, m, k)
-            if m <= WALK_MAX_TOKENS and k <= WALK_MAX_K:
+            if m <= WALK_MAX_TOKENS and k <= WALK_MAX_K and n * k <= WALK_MAX_BYTES:
                 rc = lib.muse_fp8_walk(w8.data_ptr(), w_exp.data_ptr(), x.data_ptr(), out.data_ptr(), m, n, k, x.stride(0) if m > 1 else k, ld_out,
                                        _capi.raw_stream(index))
                 if rc:

@@ -106,7 +106,7 @@ ATTEND = dict(q=P, k=P, v=P, k_exp=P, v_exp=P, page_table=P, seq_lens=P, cu_q=P,
 REFUSED = (
     [("muse_fp8_quantize", QUANTIZE, dict(bad)) for bad in ([("x", None)], [("xq", None)], [("xe", None)], [("m", 0)], [("K", 120)], [("K", 0)], [("ld_x", 120)],
                                                             [("ld_x", 132)], [("x", ODD)], [("xq", ODD)])]
-    + [("muse_fp8_walk", WALK, dict(bad)) for bad in ([("W", None)], [("we", None)], [("x", None)], [("out", None)], [("m", 17)], [("m", 0)], [("N", 0)], [("K", 24)],
+    + [("muse_fp8_walk", WALK, dict(bad)) for bad in ([("W", None)], [("we", None)], [("x", None)], [("out", None)], [("m", 9)], [("m", 0)], [("N", 0)], [("K", 24)],
                                                       [("K", 8208), ("ld_x", 8208)], [("ld_x", 64)], [("ld_x", 130)], [("ld_out", 64)], [("W", ODD)], [("x", ODD)])]
     + [("muse_fp8_gemm", GEMM, dict(bad)) for bad in ([("W", None)], [("we", None)], [("xq", None)], [("xe", None)], [("out", None)], [("status", None)], [("m", 0)],
                                                       [("N", 0)], [("K", 100)], [("ld_out", 127)], [("W", ODD)], [("xq", ODD)])]
