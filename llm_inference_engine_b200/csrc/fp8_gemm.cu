@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
       if (t == static_cast<int>(blockIdx.x)) griddep_wait();   // x's exponents come from the kernel ahead, and out may still be being read
       fetch_x(kb0, wa);
       for (int kb = kb0; kb < kb1 && ok; kb += 4) {
-        if (groups >= G8_SF_BUFS && !mbar_wait(smem_u32(&bar_sf_empty[sf]), sf_phase ^ 1u)) {
+        if (groups >= G8_SF_BUFS && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_sf_empty[sf]), sf_phase ^ 1u))) {
           ok = false;
           break;
         }
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
           fetch_x(kb + 4, wa);
         }
       }
-      if (ok && !mbar_wait(smem_u32(&bar_acc_full), acc_phase)) ok = false;
-      if (!ok || s_abort) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_acc_full), acc_phase))) ok = false;
+      if (__any_sync(0xffffffffu, !ok || s_abort)) {
         if (!ok && lane == 0) atomicOr(a.status, ST_EPILOGUE_TIMEOUT);
         s_abort = 1;
         break;
