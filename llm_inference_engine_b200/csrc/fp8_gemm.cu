@@ -13,9 +13,12 @@
 // at fewer it is the weight's own bytes from memory, and below 20 MB of them the start (4 us to the first MMA behind the
 // quantizing kernel: set-up, x's exponents, one block's way through) and the end. K is cut where that lets all SMs load.
 // Measured with the quantizing kernel (us; TB/s of W or TFLOP/s): 27 x 4093 x 2064 8.8; 27 x 12288 x 4096 14.8 (3.4 TB/s);
-// 256 x 12288 x 4096 18.6 (1390 TFLOP/s); 4096 x 12288 x 4096 190 (2170 TFLOP/s). What gave the most: a warp that waits, issues
+// 256 x 12288 x 4096 18.6 (1390 TFLOP/s); 4096 x 12288 x 4096 183 (2250 TFLOP/s). What gave the most: a warp that waits, issues
 // and commits for several blocks of K at once (a block alone costs 730 clocks of latency, four cost 1330), uniform issue,
 // exponents that are joined from whole words when used instead of byte by byte when loaded, results through shared memory.
+// At 4096 tokens a block of K takes 960 clocks, 896 of them MMAs at the tensor core's rate; a fifth of a tile's time is the epilogue,
+// under which nothing runs (the accumulators take all of tensor memory; twice the warps for it gained 1%). Tiles of other
+// widths are slower: 192 199 us, 128 224, one token tile of 256 217.
 //
 // Roles: warps 0 and 6 TMA (W and x), warp 1 tensor memory and MMA issue, warps 2..5 scales (registers one group ahead)
 // and epilogue, a warp per quarter of the lanes. The grid is persistent: a CTA walks tiles of (K slice, row tile, token tile), and the
@@ -58,6 +61,18 @@ __device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t a, uint64_t b, ui
 __host__ __device__ constexpr uint32_t g8_idesc(int N, int sf_byte) {
   return (static_cast<uint32_t>(sf_byte) << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(G8_TOK >> 7) << 27) |
          (static_cast<uint32_t>(sf_byte) << 29);
+}
+// A look that never waits.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return r != 0;
 }
 __device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
@@ -201,7 +216,7 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
     // same in all lanes is then known to be.
     int s = 0, sf = 0;
     uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-    bool ok = true;
+    bool ok = true, looked = false;   // looked: the next block was seen to be there while this one's MMAs were issued
     auto wait = [&](uint64_t& bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), parity)) != 0; };
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -215,14 +230,17 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         // 600 clocks, as long as the MMAs of a small block, and so are paid once for up to four.
         const int j0 = (kb - kb0) & 3, take = min(a.at_once, kb1 - kb);
         const int ends = s + take;
-        bool there[5];   // the looks are in flight together
-        there[4] = j0 > 0 || mbar_try_wait(smem_u32(&bar_sf_full[sf]), sf_phase);
+        if (!looked) {
+          bool there[5];   // the looks are in flight together
+          there[4] = j0 > 0 || mbar_try_wait(smem_u32(&bar_sf_full[sf]), sf_phase);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int st = s + i;
-          there[i] = i >= take || mbar_try_wait(smem_u32(&bar_full[st < a.stages ? st : st - a.stages]), st < a.stages ? phase : phase ^ 1u);
+          for (int i = 0; i < 4; ++i) {
+            const int st = s + i;
+            there[i] = i >= take || mbar_try_wait(smem_u32(&bar_full[st < a.stages ? st : st - a.stages]), st < a.stages ? phase : phase ^ 1u);
+          }
+          looked = __all_sync(0xffffffffu, there[0] && there[1] && there[2] && there[3] && there[4]);
         }
-        if (!__all_sync(0xffffffffu, there[0] && there[1] && there[2] && there[3] && there[4])) {
+        if (!looked) {
           if (j0 == 0 && !wait(bar_sf_full[sf], sf_phase)) ok = false;
           for (int i = s; i < ends && ok; ++i) ok = wait(bar_full[i < a.stages ? i : i - a.stages], i < a.stages ? phase : phase ^ 1u);
           if (!ok) break;
@@ -230,6 +248,9 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
         tc_fence_after_sync();
         const uint32_t sfa = tm + G8_SF_COL + static_cast<uint32_t>(sf) * G8_SF_STRIDE, sfb = sfa + 4 * MT;
         const bool sf_last = j0 + take == 4 || kb + take == kb1;
+        // One block at a time is a large one: the queue of MMAs is full while its last are issued, which hides a look.
+        const bool look = a.at_once == 1 && kb + 1 < kb1;
+        bool seen = false;
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -239,17 +260,22 @@ __global__ void __launch_bounds__(G8_THREADS, 1) fp8_gemm_kernel(const __grid_co
             const uint64_t ad = umma_desc_k_sw128(at), bd = umma_desc_k_sw128(at + MT * a_tile);
             const uint32_t idesc = g8_idesc(a.nt, j0 + i), more = kb + i > kb0 ? 1u : 0u;
 #pragma unroll
-            for (int k = 0; k < FP8_BLOCK / 32; ++k)   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
+            for (int k = 0; k < FP8_BLOCK / 32; ++k) {   // 32 bytes further along K inside the swizzle span: +2 in 16-byte units
+              if (i == 0 && k == FP8_BLOCK / 32 - 1 && look) {
+                seen = mbar_test_wait(smem_u32(&bar_full[s + 1 < a.stages ? s + 1 : 0]), s + 1 < a.stages ? phase : phase ^ 1u);
+                if (sf_last) seen &= mbar_test_wait(smem_u32(&bar_sf_full[sf + 1 < G8_SF_BUFS ? sf + 1 : 0]), sf + 1 < G8_SF_BUFS ? sf_phase : sf_phase ^ 1u);
+              }
 #pragma unroll
               for (int h = 0; h < MT; ++h)
                 umma_mxf8(tm + static_cast<uint32_t>(h * a.nt), ad + h * (a_tile >> 4) + 2 * k, bd + 2 * k, idesc, sfa + 4u * static_cast<uint32_t>(h), sfb,
                           k > 0 ? 1u : more);
+            }
             umma_commit(smem_u32(&bar_empty[st]));
           }
           if (sf_last) umma_commit(smem_u32(&bar_sf_empty[sf]));
           if (kb + take == kb1) umma_commit(smem_u32(&bar_acc_full));
         }
-        __syncwarp();
+        looked = __any_sync(0xffffffffu, seen) != 0;
         if (sf_last && ++sf == G8_SF_BUFS) {
           sf = 0;
           sf_phase ^= 1u;
