@@ -928,6 +928,7 @@ int cache_attn_dispatch(AttnArgs a, int dim, void* ws, cudaStream_t stream) {
   const int sms = device_sms();
   if (sms < 1) return -7;
   const AttnForm f = attn_form(a.max_q, a.hq, a.hk);
+  if (a.window >= a.width * ATTN_PAGE) a.window = 0;   // wider than any sequence
   a.tiles = f.tiles;
   a.group = a.hq / a.hk;
   a.vec_gate = a.ld_gate % 8 == 0 && (reinterpret_cast<uintptr_t>(a.gate) & 15) == 0;
