@@ -36,8 +36,7 @@ constexpr int TC_MIN_SMEM = 120 * 1024;   // one CTA per SM: it takes all of ten
 
 // The last page of a unit's share of the range, of the range; some row does not see some token; there is a page at all.
 enum : int { PAGE_SEG_LAST = 1, PAGE_RANGE_LAST = 2, PAGE_EDGE = 4, PAGE_LIVE = 8 };
-struct PageRec {
-  int tile;      // index in the pool (page * hk + head)
+struct __align__(16) PageRec {
   int bits;      // exponents k | v << 8, PAGE_* << 16
   int p0;        // position of the page's first token
   int seen;      // first | last << 8: the page's tokens that some row of the tile sees
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t raw_full[TC_RAW], raw_empty[TC_RAW], unit_full[TC_UNITS], kf_full[2], vf_full[2], qk_done[2], pv_done[2], s_empty[2],
       p_full[2], o_empty[2], q_full, fin_full[8], pair_full[4];
-  __shared__ __align__(16) PageRec s_page[TC_PAGES];
+  __shared__ PageRec s_page[TC_PAGES];
   __shared__ UnitRec s_unit[TC_UNITS];
   __shared__ float s_alpha[4][TC_ROWS], s_fin[8][3][TC_ROWS], s_max[2][2][TC_ROWS];
   __shared__ __align__(8) unsigned short s_nan[4][D][4];      // edge pages: the tokens of each dimension that hold NaN
@@ -202,7 +201,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
     tmem_relinquish();
   }
   griddep_wait();
-  griddep_launch_dependents();
 
   // The list of items, as in cache_attn_kernel.
   const int per = (entries + TC_THREADS - 1) / TC_THREADS;
@@ -223,6 +221,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  griddep_launch_dependents();   // behind the wait, as in cache_attn_kernel, and behind the allocation: who comes in may want tensor memory
   const uint32_t tmem = tmem_slot;
   int base = 0, total = 0;
   for (int w = 0; w < TC_THREADS / 32; ++w) {
@@ -341,7 +340,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
             if (lane == 0) {
               if (half == 0) {
                 PageRec r;
-                r.tile = t;
                 const bool edge = p_first < p0 + ATTN_PAGE - 1 || (a.window > 0 && p_last - a.window + 1 > p0);
                 r.bits = ex | ((seg_last ? PAGE_SEG_LAST : 0) | (seg_last && !follows ? PAGE_RANGE_LAST : 0) |
                                (edge ? PAGE_EDGE : 0) | (t >= 0 ? PAGE_LIVE : 0)) << 16;
