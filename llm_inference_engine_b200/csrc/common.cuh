@@ -201,7 +201,8 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
 // kernel ever writes -- the weights -- so its first weight loads, its launch latency and its set-up run under the
 // previous kernel's tail; activations, outputs, workspaces, counters and the status word come after the wait, which
 // returns once every kernel ahead in the stream has completed and its writes are visible. A kernel says with
-// griddep_launch_dependents() that the next one may be brought in; without it that happens when the kernel ends.
+// griddep_launch_dependents() that the next one may be brought in; without it that happens when the kernel ends. A kernel
+// that uses tensor memory says so only once it has allocated it: who comes in may want all of it.
 // Both are no-ops for a kernel launched the ordinary way. One more rule follows from the overlap: anything another
 // kernel writes (activations, residual streams) is read with L2-coherent loads (__ldcg, TMA, bulk copies), never
 // through the non-coherent path (__ldg / ld.global.nc): that path is for data that is read-only for the kernel's

@@ -164,7 +164,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     // (a launch allowed to start under the previous kernel's tail touches only weights until then).
     const int pre = min(stages, nchunks);
     for (int i = 0; i < pre; ++i) issue_w(i, i);
-    griddep_launch_dependents();
     griddep_wait();
     for (int i = 0; i < pre; ++i) issue_x(i, i);
     s_abort = 0;
@@ -178,6 +177,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   if (warp == 2) {
     tmem_alloc(smem_u32(&tmem_slot), static_cast<uint32_t>(tmem_cols));
     tmem_relinquish();
+    // Only now: the next kernel may want all of tensor memory, and would hold it while it waits for this one to end.
+    griddep_launch_dependents();
   }
   griddep_wait();   // every thread, before the first barrier: what follows reads and writes more than weights
   tc_fence_before_sync();

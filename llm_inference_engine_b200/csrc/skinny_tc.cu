@@ -200,7 +200,6 @@ skinny_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
     // (a launch allowed to start under the previous kernel's tail touches only weights until then).
     const int pre = min(stages, nchunks);
     for (int i = 0; i < pre; ++i) issue_w(i, i);
-    griddep_launch_dependents();
     griddep_wait();
     for (int i = 0; i < pre; ++i) issue_x(i, i);
     s_abort = 0;
@@ -234,6 +233,8 @@ skinny_tc_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant
   if (warp == 2) {
     tmem_alloc(smem_u32(&tmem_slot), Cfg::TMEM_COLS);
     tmem_relinquish();
+    // Only now: the next kernel may want all of tensor memory, and would hold it while it waits for this one to end.
+    griddep_launch_dependents();
     if (lane == 0) MUSE_STAMP(12);
   }
   griddep_wait();   // every thread, before the first barrier: what follows reads and writes more than weights
