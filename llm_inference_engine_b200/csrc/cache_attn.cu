@@ -103,8 +103,8 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const AttnEntry& en, i
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // largest value to [2^9, 2^10): FP16's smallest step, 2^-24, is then 2^-34 of it
-    const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 9, 100), -100);
+    // FP16's smallest step, 2^-24, is then 2^-34 of the largest value
+    const int e = q_exponent(amax);
     const float down = exp2_byte(127 - e), up = a.scale_log2 * exp2_byte(127 + e);
     qs[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
     qs[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
@@ -152,7 +152,7 @@ __device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4]
   bool same = true;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float f[2] = {qs[n][0] * kscale, qs[n][1] * kscale};
+    const float f[2] = {score_factor(qs[n][0], kscale), score_factor(qs[n][1], kscale)};
     if (edge) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {

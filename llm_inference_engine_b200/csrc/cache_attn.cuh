@@ -27,6 +27,13 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
   return r;
 }
 
+// A row's power of two under which q is FP16: the largest value to [2^9, 2^10). Between the powers whose inverses are normal.
+__device__ __forceinline__ int q_exponent(float amax) { return max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 9, 118), -100); }
+// The factor of a page's scores (the row's power, the softmax scale, the page's power) stays positive and finite: the product of
+// a zero row's smallest power and a zero page's would be 0 and a masked score, -inf, times 0 NaN. Where the border counts,
+// scores lie below 2^-90, or above what FP32 holds.
+__device__ __forceinline__ float score_factor(float row, float page) { return fminf(fmaxf(row * page, 1.17549435e-38f), 3.402823466e38f); }
+
 // Row to token: n / group, for n * group < 2^32 (the host sees to it).
 __device__ __forceinline__ int div_group(const AttnArgs& a, int n) { return a.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), a.group_magic)); }
 

@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
 #pragma unroll
             for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(finite_abs(bf16lo_f32(x[k])), finite_abs(bf16hi_f32(x[k]))));
           }
-          const int e = max(min(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 9, 100), -100);
+          const int e = q_exponent(amax);
           const float down = exp2_byte(127 - e);
           f_row = a.scale_log2 * exp2_byte(127 + e);
 #pragma unroll
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           const int bits = r.bits >> 16;
           seg_last = bits & PAGE_SEG_LAST;
           last = bits & PAGE_RANGE_LAST;
-          const float f = f_row * exp2_byte(r.bits & 255);
+          const float f = score_factor(f_row, exp2_byte(r.bits & 255));
           // The thread's scores stay in registers; what the row does not see of them becomes -infinity.
           uint32_t v[32];
           tmem_ld32(tmem + lanes + COL_S + b * ATTN_PAGE + half * 32, v);
