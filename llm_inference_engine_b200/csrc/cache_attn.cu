@@ -17,8 +17,8 @@
 // long as q follows it. O^T[dim][row] += V^T[dim][token] P^T[token][row]: V is kept [dim, token], so a lane's 16 bytes are
 // tokens 16 t .. 16 t + 15 of a dimension, and the token order of the score tiles is chosen so that, after one 8 x 8
 // transpose in registers (movmatrix), the lane holds the same tokens' weights. Neither operand passes through
-// shared memory a second time. The weights are rounded to FP16 (2^-11, values below 2^-14 of the running maximum to 2^-25
-// of it), a page's sum is scaled by its V exponent in FP32.
+// shared memory a second time. The weights are rounded to FP16, lifted by 2^14 (2^-11 of a weight; those below 2^-28 of the
+// running maximum to 2^-39 of it), a page's sum is scaled by its V exponent, and back, in FP32.
 //
 // Measured with the kernel that adds up split units (us, and the cache's bytes against 6.46 TB/s of copying): 64 sequences of up to
 // 4000 tokens, 32 query and 16 KV heads 116 (5.06 TB/s, 0.78); 2 of 100,000, 32 and 4 heads, 45 (4.5 TB/s, 0.70); 21 with drafts of
@@ -144,15 +144,17 @@ __device__ __forceinline__ void page_scores(float (&s)[4][NT][4], const uint32_t
 }
 
 // Scores to weights: p[i][n] = the weights of the lane's two tokens of tile i, packed over rows (2 t, 2 t + 1), before the
-// transpose; `a`: what the rows' sums so far are to be scaled by (`moved`: not all of the warp's are 1).
+// transpose, lifted: times `unlift` (the same for all of the warp's rows) they are the weights. `a`: what the rows' sums so
+// far are to be scaled by (`moved`: not all of the warp's are 1).
+constexpr float ATTN_LIFT = 14.f, ATTN_UNLIFT = 1.f / 16384.f;   // FP16 then holds weights down to 2^-38 of the row's largest
 template <int D, int NT>
-__device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4][NT][4], uint32_t (&p)[4][NT][2], float (&a)[NT][2], bool& moved,
+__device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4][NT][4], uint32_t (&p)[4][NT][2], float (&a)[NT][2], bool& moved, float& unlift,
                                              const float (&qs)[NT][2], float kscale, const RowInfo<NT>& ri, int p0, int window, bool edge) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
-  bool same = true;
+  bool same = true, loud = false;
+  float f[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float f[2] = {score_factor(qs[n][0], kscale), score_factor(qs[n][1], kscale)};
     if (edge) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -168,27 +170,39 @@ __device__ __forceinline__ void page_softmax(TileState<D, NT>& st, float (&s)[4]
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      f[n][c] = score_factor(qs[n][c], kscale);
       float m = s[0][n][c];
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(s[i][n][c], s[i][n][2 + c]));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      m = fmaxf(m * f[c], st.mx[n][c]);                  // the factor is positive
+      m = fmaxf(m * f[n][c], st.mx[n][c]);               // the factor is positive
       const float b = m == -INFINITY ? 0.f : m;          // nothing seen yet: every weight is 2^-inf = 0
       a[n][c] = exp2_fast(st.mx[n][c] - b);
       same &= st.mx[n][c] == m;
+      loud |= too_loud_to_lift(m);
       st.mx[n][c] = m;
+    }
+  }
+  loud = __any_sync(0xffffffffu, loud);
+  const float lift = loud ? 0.f : ATTN_LIFT;
+  unlift = loud ? 1.f : ATTN_UNLIFT;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float b = st.mx[n][c] == -INFINITY ? lift : lift - st.mx[n][c];
       float l = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float e = exp2_fast(fmaf(s[i][n][2 * x + c], f[c], -b));
+          const float e = exp2_fast(fmaf(s[i][n][2 * x + c], f[n][c], b));
           s[i][n][2 * x + c] = e;
           l += e;
         }
-      st.l[n][c] = fmaf(st.l[n][c], a[n][c], l);
+      st.l[n][c] = fmaf(st.l[n][c], a[n][c], l * unlift);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -658,13 +672,13 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     const bool edge = ri.first < p0 + ATTN_PAGE - 1 || (a.window > 0 && ri.last - a.window + 1 > p0);
     const int ks = used % SLOTS, vsl = (used + 1) % SLOTS, vt = (used + 1) / SLOTS;
     bool ok = mbar_wait_short(smem_u32(&full[ks]), (used / SLOTS) & 1), moved = false;
-    float s[4][NT][4], al[NT][2];
+    float s[4][NT][4], al[NT][2], unlift = 1.f;
     uint32_t p[4][NT][2];
     if (ok && live) page_scores<D, NT>(s, qf, ring_base + static_cast<uint32_t>(ks) * SLOT_BYTES);
     __syncwarp();
     ++used;   // the K slot may be filled again
     pump();
-    if (ok && live) page_softmax<D, NT>(st, s, p, al, moved, qs, exp2_byte(rec.y & 255), ri, p0, a.window, edge);
+    if (ok && live) page_softmax<D, NT>(st, s, p, al, moved, unlift, qs, exp2_byte(rec.y & 255), ri, p0, a.window, edge);
     ok = ok && mbar_wait_short(smem_u32(&full[vsl]), vt & 1);
     if (!ok) {
       gave_up = true;
@@ -672,7 +686,7 @@ __global__ void __launch_bounds__(ATTN_THREADS, 1) cache_attn_kernel(const __gri
     }
     if (live) {
       const uint32_t vs = ring_base + static_cast<uint32_t>(vsl) * SLOT_BYTES;
-      const float vscale = exp2_byte(rec.y >> 8);
+      const float vscale = exp2_byte(rec.y >> 8) * unlift;
       if (page_pv<D, NT>(st, p, vs, al, moved, vscale, edge, a.window > 0 ? ri.first - a.window + 1 - p0 : 0, ri.last - p0))
         page_nan<D, NT>(st, vs, ri, p0, a.window);
     }

@@ -34,6 +34,12 @@ __device__ __forceinline__ int q_exponent(float amax) { return max(min(static_ca
 // scores lie below 2^-90, or above what FP32 holds.
 __device__ __forceinline__ float score_factor(float row, float page) { return fminf(fmaxf(row * page, 1.17549435e-38f), 3.402823466e38f); }
 
+// The weights enter the products with V lifted by 2^lift, and their sums are scaled back in FP32. FP16's smallest step is 2^-24: not
+// lifted, weights below 2^-25 of the largest would be missing from the products (but not from the row's sum), and a long
+// cache holds many of them (400,000 of 2^-25.5 are 0.8 % of the result). A maximum of 2^20 and more is itself rounded by
+// enough to take a lifted weight past FP16's largest value: no lift then.
+__device__ __forceinline__ bool too_loud_to_lift(float mx) { return fabsf(mx) >= 1048576.f && mx > -INFINITY; }
+
 // Row to token: n / group, for n * group < 2^32 (the host sees to it).
 __device__ __forceinline__ int div_group(const AttnArgs& a, int n) { return a.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), a.group_magic)); }
 

@@ -29,6 +29,7 @@ constexpr int TC_THREADS = 512;
 constexpr int TC_RAW = 8;              // ring slots of raw codes (K and V of a page are one each)
 constexpr int TC_UNITS = 16;           // ring of unit records: no role is that many pages behind another
 constexpr int TC_PAGES = 64;           // ring of page records
+constexpr float TC_LIFT = 7.f, TC_UNLIFT = 0.0078125f;   // the lift of weights up to 2^8 (their reference lags behind): FP16 holds them down to 2^-31 of it
 __host__ __device__ constexpr int tc_raw_bytes(int D) { return ATTN_PAGE * D; }
 __host__ __device__ constexpr int tc_f16_bytes(int D) { return ATTN_PAGE * D * 2; }
 __host__ __device__ constexpr int tc_smem_bytes(int D) { return 4 * tc_f16_bytes(D) + TC_RAW * tc_raw_bytes(D) + 1024; }
@@ -164,7 +165,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
       p_full[2], o_empty[2], q_full, fin_full[8], pair_full[4];
   __shared__ PageRec s_page[TC_PAGES];
   __shared__ UnitRec s_unit[TC_UNITS];
-  __shared__ float s_alpha[4][TC_ROWS], s_fin[8][3][TC_ROWS], s_max[2][2][TC_ROWS];
+  __shared__ float2 s_alpha[4][TC_ROWS];   // what a row's sums so far are scaled by, and what its page's sum is
+  __shared__ float s_fin[8][3][TC_ROWS], s_max[2][2][TC_ROWS];
   __shared__ __align__(8) unsigned short s_nan[4][D][4];      // edge pages: the tokens of each dimension that hold NaN
   __shared__ int s_has_nan[4][2];
   __shared__ int s_sum[TC_THREADS / 32];
@@ -597,12 +599,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           if (!ok) break;
           tc_fence_after_sync();
           // The reference of the weights follows the maximum only when that has grown by more than 2^8 (the weights stay below
-          // 2^8, far inside FP16): the sums are then hardly ever to be scaled.
+          // 2^8, and lifted inside FP16): the sums are then hardly ever to be scaled.
           const float m_new = fmaxf(m_half, s_max[b][other][row]) * f, grown = m_new > mx + 8.f || (mx == -INFINITY && m_new > mx) ? m_new : mx;
           const float base2 = grown == -INFINITY ? 0.f : grown, alpha = grown == mx ? 1.f : exp2_fast(mx - base2);
           mx = grown;
-          if (half == 0) s_alpha[n & 3][row] = alpha;
-          const unsigned long long ff = pack2(f, f), bb = pack2(-base2, -base2);
+          const bool loud = too_loud_to_lift(mx);
+          const float lift = loud ? 0.f : TC_LIFT, unlift = loud ? 1.f : TC_UNLIFT;
+          if (half == 0) s_alpha[n & 3][row] = make_float2(alpha, unlift);
+          const unsigned long long ff = pack2(f, f), bb = pack2(lift - base2, lift - base2);
           unsigned long long l2[2] = {0ull, 0ull};
           uint32_t p[16];
 #pragma unroll
@@ -617,7 +621,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
           float l_lo, l_hi;
           unpack2(add2(l2[0], l2[1]), l_lo, l_hi);
           tmem_st16(tmem + lanes + COL_P + b * (ATTN_PAGE / 2) + half * 16, p);
-          l = fmaf(l, alpha, l_lo + l_hi);
+          l = fmaf(l, alpha, (l_lo + l_hi) * unlift);
           if (seg_last) {
             if (half == 0) s_fin[unit & 7][2][row] = mx;
             s_fin[unit & 7][half][row] = l;
@@ -653,7 +657,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) cache_attn_tc_kernel(const __gr
         const PageRec r = s_page[n & (TC_PAGES - 1)];
         const int bits = r.bits >> 16;
         last = bits & PAGE_RANGE_LAST;
-        const float alpha = s_alpha[n & 3][row], vs = exp2_byte(r.bits >> 8 & 255);
+        const float2 scale = s_alpha[n & 3][row];
+        const float alpha = scale.x, vs = exp2_byte(r.bits >> 8 & 255) * scale.y;
         const unsigned long long vs2 = pack2(vs, vs);
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll

@@ -78,3 +78,59 @@ def test_zero_rows_through_append_and_attention(c8, new, rows):
     out = c8.attention(q, cache, table, lens, cu_q=cu, max_q=new)
     c8.check_status(DEV)
     assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("new,rows", [(1, 8), (1, 16), (3, 24)])
+@pytest.mark.parametrize("last", [False, True])
+def test_many_small_weights_add_up(c8, new, rows, last):
+    """One token that takes most, 400,000 others with 2^-25.5 of its weight each: together 0.8 % of the result. As many sequences
+    as there are workers, so that each walks a whole sequence alone. Tolerance: the result's rounding (2^-8); each weight's
+    rounding to FP16, at most half its smallest step, 2^-39 of the largest weight (2^-32 with 128-row tiles); FP32 sums of a
+    term per page after one another, and 100 steps for what happens inside a page and the exponential."""
+    n, dim, hq = 400000, 64, rows // new
+    pages, batch = n // PAGE, torch.cuda.get_device_properties(DEV).multi_processor_count * (8 if rows <= 16 else 1)
+    cache = c8.new_cache(2, 1, dim, DEV)   # all pages are page 1 but the one that holds the loud token
+    one = 0x38   # 1.0
+    cache.k.view(torch.uint8)[0, 0, 5, 0] = one
+    cache.v.view(torch.uint8).fill_(one)
+    cache.v.view(torch.uint8)[0, 0, dim // 2 :, 5] = 0
+    q = torch.zeros((batch * new, hq, dim), device=DEV, dtype=torch.bfloat16)
+    q[:, :, 0] = 1.0
+    table = torch.ones((batch, pages), dtype=torch.int32, device=DEV)
+    table[:, pages - 2 if last else 0] = 0
+    lens, cu = torch.full((batch,), n, dtype=torch.int32, device=DEV), torch.arange(batch + 1, dtype=torch.int32, device=DEV) * new
+    got = c8.attention(q, cache, table, lens, cu_q=cu, max_q=new, scale=25.5 * math.log(2.0)).double().view(batch, new, hq, dim)
+    c8.check_status(DEV)
+    weights = n * (2.0**-32 if rows > 16 else 2.0**-39) + (pages + 100) * 2.0**-24
+    for j in range(new):
+        rest = (n - new + j) * 2.0**-25.5
+        for part, want in ((got[:, j, :, : dim // 2], 1.0), (got[:, j, :, dim // 2 :], rest / (1.0 + rest))):
+            assert float((part - want).abs().max()) <= 2.0**-8 * want + weights, (j, want, float(part.min()), float(part.max()))
+
+
+@pytest.mark.parametrize("new,rows", HEADS)
+def test_scores_far_beyond_the_others(c8, new, rows):
+    """Scores of 2^20 to 2^24, where a maximum's own rounding is worth powers of two, in rows beside zero rows: one token has
+    all of a loud row's weight (the next is 2^19 and more below), a zero row is the mean of what it sees."""
+    hk, dim, n = 2, 64, 150
+    hq = hk * rows // new
+    cache = filled_cache(c8, 3, hk, dim, 41)
+    cache.k.view(torch.uint8).zero_()
+    cache.k_exp.fill_(127)
+    table = i32([[2, 0, 1]])
+    for p, code in ((3, 0x34), (70, 0x38), (140, 0x36)):   # 0.75, 1, 0.875
+        cache.k.view(torch.uint8)[int(table[0, p // PAGE]), :, p % PAGE, 0] = code
+    q = torch.zeros((new, hq, dim), device=DEV, dtype=torch.bfloat16)
+    q[:, 1::2, 0] = torch.exp2(torch.arange(hq // 2, device=DEV) % 4 + 12.0).bfloat16()
+    got = c8.attention(q, cache, table, i32([n]), cu_q=i32([0, new]), max_q=new, scale=1023.0)
+    c8.check_status(DEV)
+    want, room = attention64(q, cache, table, [n], [0, new], scale=1023.0)
+    top = values64_v(cache, table, 70).repeat_interleave(hq // hk, 0)[1::2]
+    assert torch.equal(want.view(new, hq, dim)[:, 1::2], top.expand(new, -1, -1))
+    assert bool(((got.double() - want).view(new, hq, dim)[:, 1::2].abs() <= 2.0**-8 * top.abs()).all())
+    assert bool(((got.double() - want).abs() <= room).view(new, hq, dim)[:, ::2].all())
+
+
+def values64_v(cache, table, p):
+    page = int(table[0, p // PAGE])
+    return cache.v[page, :, :, p % PAGE].double() * torch.exp2(cache.v_exp[page].double() - 127.0)[:, None]
