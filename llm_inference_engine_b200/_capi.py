@@ -7,6 +7,7 @@ does every call that needs it. There is no PyTorch or CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from pathlib import Path
 
 import torch
@@ -171,6 +172,7 @@ def new_tensor(shape, strides, dtype, device) -> torch.Tensor:
 
 
 _STATUS: dict[int, torch.Tensor] = {}
+_STATUS_LOCK = threading.Lock()
 STATUS_TEXT = ((128, "a page index outside the pool"), (256, "lengths or row bounds that do not fit"))
 
 
@@ -181,17 +183,28 @@ def status_ptr(index: int) -> int:
     if word is None:
         if torch.cuda.is_current_stream_capturing():   # it must outlive the graph
             raise MuseError("the first call of the 8-bit operators on a device makes their status word: make it outside stream capture")
-        word = _STATUS[index] = torch.zeros(1, device=torch.device("cuda", index), dtype=torch.int32)
-        bind().set_status(index, word.data_ptr())
+        with _STATUS_LOCK:   # one word per device, whoever comes first
+            word = _STATUS.get(index)
+            if word is None:
+                word = torch.zeros(1, device=torch.device("cuda", index), dtype=torch.int32)
+                torch.cuda.synchronize(word.device)   # a report from another stream must not meet the filling with zero
+                _STATUS[index] = word
+                bind().set_status(index, word.data_ptr())
     return word.data_ptr()
 
 
 def check_status_word(device) -> None:
+    """Waits for the whole device, whatever stream the calls ran on, and raises what they have reported; takes away the bits it
+    raises and no others."""
     device = torch.device(device)
-    word = _STATUS.get(torch.cuda.current_device() if device.index is None else device.index)
-    bits = 0 if word is None else int(word.item())
+    index = torch.cuda.current_device() if device.index is None else device.index
+    word = _STATUS.get(index)
+    if word is None:
+        return
+    torch.cuda.synchronize(torch.device("cuda", index))
+    bits = int(word.item())
     if bits:
-        word.zero_()
+        word.bitwise_and_(~bits)
         what = [text for bit, text in STATUS_TEXT if bits & bit] + (["a timed-out wait"] if bits & ~384 else [])
         raise MuseError(f"the 8-bit operators reported: {', '.join(what)} (status bits {bits:#x}, see MUSE_ST_* in muse_proj.h)")
 

@@ -79,9 +79,10 @@ def rotary_table(rot: int, positions: int, device, base: float = 10000.0, scalin
 
 
 def check_status(device) -> None:
-    """Synchronise and raise if a call since the last check met a page index outside the pool (the page was neither
-    read nor written), lengths or row bounds that do not fit the table, the batch or max_q (they were clamped), or gave up
-    on a bounded wait. Not for use inside a stream capture. (One word per device for the 8-bit operators, fp8's among them.)"""
+    """Wait for the device (all its streams) and raise if a call since the last check met a page index outside the pool (the
+    page was neither read nor written), lengths or row bounds that do not fit the table, the batch or max_q (they were
+    clamped), or gave up on a bounded wait. Not for use inside a stream capture. One word per device for the 8-bit operators,
+    fp8's and all threads' among them: a check takes what any of them reported."""
     _capi.check_status_word(device)
 
 

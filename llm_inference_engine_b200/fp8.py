@@ -81,8 +81,9 @@ def _ws_bytes(index: int, m: int, n: int, k: int) -> int:
 
 
 def check_status(device) -> None:
-    """Synchronise and raise if a kernel since the last check gave up on one of its bounded waits. Not for use inside a
-    stream capture. (One word per device for the 8-bit operators, cache8's among them.)"""
+    """Wait for the device (all its streams) and raise if a kernel since the last check gave up on one of its bounded waits. Not
+    for use inside a stream capture. One word per device for the 8-bit operators, cache8's and all threads' among them: a
+    check takes what any of them reported."""
     _capi.check_status_word(device)
 
 
