@@ -900,10 +900,8 @@ template <int D, int NT>
 static cudaError_t attn_launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   const size_t smem = attn_ring_bytes(D);
   static DeviceOnce once;
-  cudaError_t e = cudaSuccess;
-  if (once.first()) e = cudaFuncSetAttribute(cache_attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(cache_attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)); });
   if (e != cudaSuccess) return e;
-  once.done();
   return launch_dependent(cache_attn_kernel<D, NT>, dim3(sms), dim3(ATTN_THREADS), smem, stream, a);
 }
 

@@ -761,10 +761,8 @@ template <int D>
 static cudaError_t tc_launch(const AttnArgs& a, int sms, cudaStream_t stream) {
   const size_t smem = tc_smem_bytes(D) > TC_MIN_SMEM ? tc_smem_bytes(D) : TC_MIN_SMEM;
   static DeviceOnce once;
-  cudaError_t e = cudaSuccess;
-  if (once.first()) e = cudaFuncSetAttribute(cache_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(cache_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)); });
   if (e != cudaSuccess) return e;
-  once.done();
   return launch_dependent(cache_attn_tc_kernel<D>, dim3(sms), dim3(TC_THREADS), smem, stream, a);
 }
 

@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "device_once.cuh"
+
 namespace muse {
 
 // Status codes a kernel may OR into its status word (0 = clean).
@@ -227,29 +229,6 @@ inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block,
   cfg.numAttrs = g_programmatic_launch ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
-
-// Device facts that a launch needs, asked once per device (a small call's host time counts). As everywhere in this
-// library the first call of a variant on a device is made from one thread.
-constexpr int MAX_DEVICES = 64;
-inline int device_sms() {
-  static int sms[MAX_DEVICES];
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
-  if (sms[dev] == 0) {
-    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    sms[dev] = v;
-  }
-  return sms[dev];
-}
-// What is done once per device: `if (once.first()) ...; once.done();`.
-struct DeviceOnce {
-  bool was[MAX_DEVICES] = {};
-  int dev = 0;
-  bool first() { return cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES || !was[dev]; }
-  void done() {
-    if (dev >= 0 && dev < MAX_DEVICES) was[dev] = true;
-  }
-};
 
 // ---------------------------------------------------------------- plain memory helpers
 __device__ __forceinline__ uint4 ldg_stream16(const void* p) {

@@ -515,10 +515,8 @@ long long fp8_gemm_ws_bytes(int m, int n, int k) {
 template <int MT>
 static cudaError_t g8_launch(const CUtensorMap& tx, const CUtensorMap& tw, const G8Args& a, int grid, size_t smem, cudaStream_t stream) {
   static DeviceOnce once;   // the largest any plan asks for, once
-  cudaError_t e = cudaSuccess;
-  if (once.first()) e = cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_SMEM);
+  const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(fp8_gemm_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G8_SMEM); });
   if (e != cudaSuccess) return e;
-  once.done();
   return launch_dependent(fp8_gemm_kernel<MT>, dim3(grid), dim3(G8_THREADS), smem, stream, tx, tw, a);
 }
 
