@@ -143,9 +143,10 @@ def check(rc: int, what: str) -> None:
 
 
 # Small calls are bound by what the host does for them: the two helpers below are torch.cuda.current_stream(i).cuda_stream
-# and torch.cuda.device(i) without the objects those build (2 us and 1 us a call).
-raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# and torch.cuda.device(i) without the objects those build (2 us and 1 us a call). A torch without CUDA has neither; the host
+# side of the package works with it all the same.
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class on_device:
