@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import threading
+import warnings
 from pathlib import Path
 
 import torch
@@ -114,16 +115,29 @@ def load(build_if_missing: bool = True):
 _BIND = None
 
 
+class _NoBinding:
+    """In the binding's place where it cannot be built: no call is an ordinary one."""
+
+    linear = rope_append = attention = staticmethod(lambda *args: None)
+    set_status = staticmethod(lambda index, address: None)
+
+
 def bind():
     """The torch-side binding of the 8-bit operators (csrc/bind.cpp): their ordinary calls in one step. Built with the
-    library; like it, loading raises where it is missing and cannot be built."""
+    library. Where it is missing and cannot be built, every call takes the way through Python to the same entry points (10 us
+    of host time more), and a warning says so once."""
     global _BIND
     if _BIND is None:
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_loader
 
         lib = load()
-        path = str(_build.build_bind() if not _build.BIND_PATH.exists() else _build.BIND_PATH)
+        try:
+            path = str(_build.build_bind() if not _build.BIND_PATH.exists() else _build.BIND_PATH)
+        except Exception as e:
+            warnings.warn(f"the torch-side binding cannot be built ({e}): calls of the 8-bit operators go through Python", RuntimeWarning, stacklevel=2)
+            _BIND = _NoBinding
+            return _BIND
         loader = ExtensionFileLoader("_bind", path)
         module = module_from_spec(spec_from_loader("_bind", loader))
         loader.exec_module(module)

@@ -72,10 +72,19 @@ def build_bind(force: bool = False) -> Path:
     return BIND_PATH
 
 
+def _bind_or_say(make) -> None:
+    """The binding is a shorter way to the library, not a part of it: where it cannot be built, calls go through Python."""
+    try:
+        make()
+    except Exception as e:
+        sys.stderr.write(f"the torch-side binding was not built ({e}): calls of the 8-bit operators go through Python\n")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library and the binding where they are missing or older than their sources; return the library's path."""
+    """Compile the library and the binding where they are missing or older than their sources; return the library's path. A
+    binding that cannot be built (no g++, no headers of Python or torch) is said, and the library built all the same."""
     if not force and not _stale():
-        build_bind()
+        _bind_or_say(build_bind)
         return LIB_PATH
     nvcc = _nvcc()
     compile_flags = ([f for f in NVCC_FLAGS if f != "--shared"] + (["-Xptxas", "-v"] if verbose else [])
@@ -91,7 +100,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as pool:   # one nvcc per translation unit, side by side
         bind = pool.submit(build_bind, force)
         results = list(pool.map(compile_one, zip(SOURCES, objs)))
-    bind.result()
     for src, proc in zip(SOURCES, results):
         if verbose or proc.returncode != 0:
             sys.stderr.write(proc.stdout + proc.stderr)
@@ -102,6 +110,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if link.returncode != 0:
         sys.stderr.write(link.stdout + link.stderr)
         raise RuntimeError(f"link failed ({link.returncode})")
+    _bind_or_say(bind.result)
     return LIB_PATH
 
 
