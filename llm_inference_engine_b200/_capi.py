@@ -133,7 +133,8 @@ def bind():
 
         lib = load()
         try:
-            path = str(_build.build_bind() if not _build.BIND_PATH.exists() else _build.BIND_PATH)
+            path = _build.bind_path()
+            path = str(path if path.exists() else _build.build_bind())
         except Exception as e:
             warnings.warn(f"the torch-side binding cannot be built ({e}): calls of the 8-bit operators go through Python", RuntimeWarning, stacklevel=2)
             _BIND = _NoBinding

@@ -23,7 +23,6 @@ LIB_PATH = PKG_DIR / ("libmuse_proj_trace.so" if TRACE else "libmuse_proj.so")
 SOURCES = ["gemv1.cu", "fewtok_mma.cu", "fewtok_zip.cu", "ffn_boundary.cu", "skinny_tc.cu", "gemm_tc.cu", "fp8_linear.cu", "fp8_gemm.cu", "rope_append.cu", "cache_attn.cu", "cache_attn_tc.cu", "capi.cu"]
 # The torch-side binding of the 8-bit operators (a host-only extension module), beside the library.
 BIND_SOURCE = CSRC / "bind.cpp"
-BIND_PATH = PKG_DIR / "_bind.so"
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -46,15 +45,26 @@ def _stale() -> bool:
     return any(d.stat().st_mtime > built for d in deps)
 
 
-def _bind_stale() -> bool:
+def bind_path() -> Path:
+    """Where the binding lies. It holds torch's and Python's C++ interfaces, which differ between their versions: the name says
+    for which it was built, so that no other is ever loaded."""
+    import sysconfig
+
+    import torch
+
+    return PKG_DIR / f"_bind.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX') or '.so'}"
+
+
+def _bind_stale(path: Path) -> bool:
     deps = [BIND_SOURCE, PKG_DIR.parent / "include" / "muse_proj.h"]
-    return not BIND_PATH.exists() or any(d.stat().st_mtime > BIND_PATH.stat().st_mtime for d in deps)
+    return not path.exists() or any(d.stat().st_mtime > path.stat().st_mtime for d in deps)
 
 
 def build_bind(force: bool = False) -> Path:
     """Compile the binding if it is missing or older than its source; return its path."""
-    if not force and not _bind_stale():
-        return BIND_PATH
+    path = bind_path()
+    if not force and not _bind_stale(path):
+        return path
     import sysconfig
 
     import torch
@@ -63,13 +73,13 @@ def build_bind(force: bool = False) -> Path:
     nvcc = Path(_nvcc()).resolve()
     include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], nvcc.parent.parent / "include"]
     cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{p}" for p in include], str(BIND_SOURCE), "-o", str(BIND_PATH), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+           *[f"-I{p}" for p in include], str(BIND_SOURCE), "-o", str(path), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)
         raise RuntimeError(f"g++ failed ({proc.returncode}) on {BIND_SOURCE.name}")
-    return BIND_PATH
+    return path
 
 
 def _bind_or_say(make) -> None:

@@ -50,7 +50,7 @@ def test_the_library_is_built_without_the_binding(monkeypatch, tmp_path, capfd, 
     tools = Tools(missing)
     monkeypatch.setattr(build.subprocess, "run", tools)
     monkeypatch.setattr(build, "LIB_PATH", tmp_path / "lib.so")
-    monkeypatch.setattr(build, "BIND_PATH", tmp_path / "bind.so")
+    monkeypatch.setattr(build, "bind_path", lambda: tmp_path / "bind.so")
     assert build.build(force=force) == tmp_path / "lib.so"
     links = [cmd for cmd in tools.ran if str(tmp_path / "lib.so") in cmd]
     assert len(links) == 1 and sum("-c" in cmd for cmd in tools.ran) == len(build.SOURCES)
@@ -61,10 +61,26 @@ def test_calls_go_through_python_without_the_binding(monkeypatch, tmp_path):
     from llm_inference_engine_b200 import _capi, build, fp8
 
     monkeypatch.setattr(build.subprocess, "run", Tools(False))
-    monkeypatch.setattr(build, "BIND_PATH", tmp_path / "bind.so")
+    monkeypatch.setattr(build, "bind_path", lambda: tmp_path / "bind.so")
     monkeypatch.setattr(_capi, "_BIND", None)
     with pytest.warns(RuntimeWarning, match="go through Python"):
         assert _capi.bind().linear(None, None, None) is None
     w8, we = fp8.quantize_weight(torch.ones(16, 16))
     with pytest.raises(RuntimeError, match="no CPU fallback"):   # what the Python way says
         fp8.linear(torch.ones(1, 16, dtype=torch.bfloat16), w8, we)
+
+
+def test_a_binding_of_another_torch_is_not_taken(monkeypatch):
+    """What was built against one torch stays beside what is built against another, and neither is loaded for the other."""
+    from llm_inference_engine_b200 import _capi, build
+
+    here = build.build_bind()
+    assert here.exists() and here == build.bind_path()
+    monkeypatch.setattr(torch, "__version__", "9.9.9+other")
+    tools = Tools(False)
+    monkeypatch.setattr(build.subprocess, "run", tools)
+    assert build.bind_path() != here and not build.bind_path().exists()
+    monkeypatch.setattr(_capi, "_BIND", None)
+    with pytest.warns(RuntimeWarning):
+        _capi.bind()
+    assert len(tools.ran) == 1 and str(build.bind_path()) in tools.ran[0]   # it tried to build its own
