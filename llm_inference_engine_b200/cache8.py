@@ -263,8 +263,8 @@ def attention_half(data, state, cache: Cache8, cos_sin: torch.Tensor, page_table
     """The attention half of the decode layer: the qkv_gate projection, rope_append, attention, the `o` projection; its
     result is what muse_bf16_proj.attn_boundary takes as attn_out. data = {"x": BF16 [m, K]}; `state` as
     muse_bf16_proj.prepare made it, with "qkv_gate" (rows q | k | v | gate; without the gate rows when gated is False)
-    and "o". eight_bit: both projections through kernel_fn_fp8 (prepare_fp8 made their 8-bit forms). The rest as in
-    rope_append and attention."""
+    and "o". eight_bit: both projections through kernel_fn_fp8 (prepare_fp8 made their 8-bit forms; the BF16 weights are not
+    looked at). The rest as in rope_append and attention."""
     from . import muse_bf16_proj as proj
 
     project = proj.kernel_fn_fp8 if eight_bit else proj.kernel_fn
@@ -272,11 +272,12 @@ def attention_half(data, state, cache: Cache8, cos_sin: torch.Tensor, page_table
     m = x.shape[0]
     heads, dim = cache.k.shape[1], cache.k.shape[3]
     qkv, cols = (q_heads + 2 * heads) * dim, q_heads * dim
-    n, k = state["qkv_gate"].shape
-    if n != qkv + (cols if gated else 0) or state["o"].shape[1] != cols:
-        raise ValueError(f"qkv_gate {tuple(state['qkv_gate'].shape)} and o {tuple(state['o'].shape)} do not fit {q_heads} query heads and "
+    in_proj, out_proj = (proj.fp8_form(state, name)[0].shape if eight_bit else state[name].shape for name in ("qkv_gate", "o"))
+    n, k = in_proj
+    if n != qkv + (cols if gated else 0) or out_proj[1] != cols:
+        raise ValueError(f"qkv_gate {tuple(in_proj)} and o {tuple(out_proj)} do not fit {q_heads} query heads and "
                          f"{heads} KV heads of {dim}, {'gated' if gated else 'not gated'}")
     rows = project({"x": x, "config": {"layer": "qkv_gate", "m": m, "n": n, "k": k}}, state)
     q = rope_append(rows, cache, cos_sin, page_table, seq_lens, q_heads=q_heads, cu_q=cu_q, max_q=max_q, interleaved=interleaved)
     a = attention(q, cache, page_table, seq_lens, cu_q=cu_q, max_q=max_q, window=window, gate=rows[:, qkv:] if gated else None)
-    return project({"x": a, "config": {"layer": "o", "m": m, "n": state["o"].shape[0], "k": cols}}, state)
+    return project({"x": a, "config": {"layer": "o", "m": m, "n": out_proj[0], "k": cols}}, state)

@@ -546,7 +546,8 @@ def kernel_fn_zip12(data, state) -> torch.Tensor:
 def prepare_fp8(state, layers=None) -> None:
     """The 8-bit form (fp8.quantize_weight: e4m3 codes, a power-of-two scale per 128 x 128 block) of the BF16 weights
     named in `layers` (default: all of them), kept in `state` beside the weights for kernel_fn_fp8(). K must be a multiple
-    of 16. The router stays in FP32: its logits decide between experts."""
+    of 16. The router stays in FP32: its logits decide between experts. What runs in 8 bits reads these forms only: a BF16
+    weight that nothing else uses may be deleted from `state` afterwards."""
     from . import fp8
 
     for name in (layers if layers is not None else [k for k in state if not k.startswith("_") and k not in FP32_LAYERS]):
@@ -561,6 +562,14 @@ def prepare_fp8(state, layers=None) -> None:
         torch.cuda.synchronize(w.device)   # codes are weights: complete before the first call
 
 
+def fp8_form(state, layer: str):
+    """The codes and exponent bytes that prepare_fp8() made of a layer."""
+    form = state.get("_fp8", _EMPTY).get(layer)
+    if form is None:
+        raise KeyError(f"{layer}: prepare_fp8() has not made an 8-bit form of this layer")
+    return form
+
+
 def kernel_fn_fp8(data: Inputs, state, out: torch.Tensor | None = None) -> torch.Tensor:
     """kernel_fn with both operands in 8 bits (fp8.linear): x is quantised per token and 128 columns on the way, the
     weight's codes are those of prepare_fp8(). Same arguments, same slice rule, BF16 result; half the weight bytes. The
@@ -569,10 +578,7 @@ def kernel_fn_fp8(data: Inputs, state, out: torch.Tensor | None = None) -> torch
 
     x, cfg = data["x"], data["config"]
     layer, n = cfg["layer"], int(cfg["n"])
-    form = state.get("_fp8", _EMPTY).get(layer)
-    if form is None:
-        raise KeyError(f"{layer}: prepare_fp8() has not made an 8-bit form of this layer")
-    w8, w_exp = form
+    w8, w_exp = fp8_form(state, layer)
     if not 0 < n <= w8.shape[0]:
         raise ValueError(f"{layer}: n={n} does not fit W {tuple(w8.shape)}")
     return fp8.linear(x, w8[:n], w_exp[: -(-n // fp8.BLOCK)], out)

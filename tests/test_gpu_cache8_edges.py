@@ -134,3 +134,27 @@ def test_scores_far_beyond_the_others(c8, new, rows):
 def values64_v(cache, table, p):
     page = int(table[0, p // PAGE])
     return cache.v[page, :, :, p % PAGE].double() * torch.exp2(cache.v_exp[page].double() - 127.0)[:, None]
+
+
+def test_attention_half_in_8_bits_needs_no_bf16_weights(c8):
+    """The BF16 weights may go once their 8-bit forms are made; without a form the call says so."""
+    from llm_inference_engine_b200 import muse_bf16_proj as proj
+
+    hq, hk, d, k = 4, 2, 64, 256
+    g = torch.Generator(device=DEV).manual_seed(3)
+    weights = {"qkv_gate": (0.05 * torch.randn(((2 * hq + 2 * hk) * d, k), generator=g, device=DEV)).bfloat16(),
+               "o": (0.05 * torch.randn((k, hq * d), generator=g, device=DEV)).bfloat16()}
+    state = proj.prepare(weights, warmup=False)
+    cos_sin, table, lens = c8.rotary_table(64, PAGE, DEV), i32([[1], [0]]), i32([1, 1])
+    x = torch.randn((2, k), generator=g, device=DEV).bfloat16()
+    step = lambda: c8.attention_half({"x": x}, state, c8.new_cache(2, hk, d, DEV), cos_sin, table, lens, q_heads=hq, eight_bit=True)
+    with pytest.raises(KeyError, match="prepare_fp8"):
+        step()
+    proj.prepare_fp8(state)
+    before = step()
+    del state["qkv_gate"], state["o"]
+    assert torch.equal(step(), before)
+    state["_fp8"]["o"] = tuple(t[:, :128] for t in state["_fp8"]["o"])
+    with pytest.raises(ValueError, match="do not fit"):
+        step()
+    c8.check_status(DEV)
