@@ -208,6 +208,7 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
         raise TypeError(f"q must be BF16 [m, heads, dim], got {q.dtype} {tuple(q.shape)}")
     m, q_heads, d = q.shape
     index, kp, vp, kep, vep, tp, lp, cp, pages, heads, dim, batch, width = _check_batch(cache, page_table, seq_lens, cu_q, max_q, m, q_heads)
+    max_q = min(max_q, m)   # no sequence has more new tokens than the batch has rows
     if d != dim or q.get_device() != index or window < 0:
         raise ValueError(f"q {tuple(q.shape)} on {q.device} does not fit the cache's heads of {dim}, or window={window} is negative")
     if scale is None:

@@ -180,6 +180,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t m = q->size(0), q_heads = q->size(1);
   Batch b;
   if (!batch_of(args[1], args[2], args[3], args[4], m, max_q, q_heads, &b) || q->get_device() != b.index || q->size(2) != b.dim) Py_RETURN_NONE;
+  if (max_q > m) max_q = m;   // no sequence has more new tokens than the batch has rows
   const int64_t cols = q_heads * b.dim;
   if (q->stride(2) != 1 || q->stride(1) != b.dim || addr(*q) % 16 || (m > 1 && (q->stride(0) % 8 || q->stride(0) < cols))) Py_RETURN_NONE;
   double scale = b.dim == 128 ? 0.08838834764831845 : 0.125;

@@ -158,3 +158,23 @@ def test_attention_half_in_8_bits_needs_no_bf16_weights(c8):
     with pytest.raises(ValueError, match="do not fit"):
         step()
     c8.check_status(DEV)
+
+
+@pytest.mark.parametrize("most", [2**31 - 1, 1 << 20, 4096])
+def test_max_q_may_be_any_bound(c8, most):
+    """max_q is a bound: one far above what the batch holds gives what the batch's own row count gives."""
+    hk, dim, hq = 2, 64, 8
+    lens, new = [150, 64, 70], [3, 1, 0]
+    cache = filled_cache(c8, 8, hk, dim, 77)
+    table = make_table(lens, 3, 8, 1)
+    x = torch.randn((4, (hq + 2 * hk) * dim), generator=torch.Generator(device=DEV).manual_seed(9), device=DEV).bfloat16()
+    cu, cos_sin = i32(bounds(new)), c8.rotary_table(dim, 3 * PAGE, DEV)
+    got = []
+    for bound in (most, 4):
+        held = type(cache)(*[t.clone() for t in cache])
+        q = c8.rope_append(x, held, cos_sin, table, i32(lens), q_heads=hq, cu_q=cu, max_q=bound)
+        got.append((c8.attention(q, held, table, i32(lens), cu_q=cu, max_q=bound), c8.attention(q, held, table, i32(lens), cu_q=cu, max_q=bound, out=torch.empty_like(q).flatten(1))))
+    c8.check_status(DEV)
+    assert all(torch.equal(t, got[1][0]) for pair in got for t in pair)
+    want, room = attention64(q, held, table, lens, bounds(new))
+    assert bool(((got[0][0].double() - want).abs() <= room).all())
