@@ -92,8 +92,8 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
 
   // x fragments: the lane's 32 columns of each of its blocks, for token g, in BF16 -> codes in registers.
   uint32_t xa[BPW][8];
-  float sa[BPW];
-  auto quantise = [&](int tok, int kb, uint32_t (&q)[8], float& scale) {
+  int sa[BPW];
+  auto quantise = [&](int tok, int kb, uint32_t (&q)[8], int& byte) {
     uint4 v[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -109,9 +109,8 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
     }
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const int e = fp8_exponent_byte(a);
-    const float inv = exp2_byte_inv(e);
-    scale = exp2_byte(e);
+    byte = fp8_exponent_byte(a);
+    const float inv = exp2_byte_inv(byte);
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const uint32_t u[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
@@ -138,9 +137,17 @@ __global__ void __launch_bounds__(NW * 32) fp8_walk_kernel(const uint8_t* __rest
             mma_e4m3_16832(c, xa[j][4 * p], 0u, xa[j][4 * p + 1], 0u, u.x, u.y);
             mma_e4m3_16832(c, xa[j][4 * p + 2], 0u, xa[j][4 * p + 3], 0u, u.z, u.w);
           }
-          const float s = exp2_byte(static_cast<int>(se[d][j]));
-          acc[0] = fmaf(c[0], s * sa[j], acc[0]);
-          acc[1] = fmaf(c[1], s * sa[j], acc[1]);
+          // Both powers in one, or, where their sum lies beyond FP32 (the scaled product need not), half of it at a time.
+          const int byte = static_cast<int>(se[d][j]) + sa[j] - 127;
+          float s2 = exp2_byte(byte);
+          if (static_cast<unsigned>(byte - 1) > 253u) {
+            const float s1 = exp2_byte((byte + 127) >> 1);
+            s2 = exp2_byte(byte + 127 - ((byte + 127) >> 1));
+            c[0] *= s1;
+            c[1] *= s1;
+          }
+          acc[0] = fmaf(c[0], s2, acc[0]);
+          acc[1] = fmaf(c[1], s2, acc[1]);
         }
         if (i + D < my_sets) load(w[d], se[d], i + D);   // into the registers just read: in flight across the reduction
         float* mine = red[i & 1][warp];

@@ -229,3 +229,27 @@ def test_refusals(fp8):
         fp8.quantize(x[:, :40].contiguous())
     with pytest.raises(RuntimeError, match="CUDA device only"):
         fp8.linear(x.cpu(), w8.cpu(), we.cpu())
+
+
+@pytest.mark.parametrize("m", [1, 8, 20, 200])
+def test_scales_whose_product_leaves_fp32(fp8, m):
+    """A block of x near 2^104 against a block of W near 2^46: the two exponents add up to 133, more than FP32's scale factors
+    reach, while products of its small codes, and zeros, are inside FP32. Rows beyond FP32 are infinite."""
+    x, w = inputs(m, 256, 272, 90 + m)
+    x[:, :128], w[:128, :128] = 0, 0
+    x[:, 0] = 2.0**104          # met by zeros of W, but in the last rows of its block
+    x[:, 1:9] = 2.0**87         # small codes of the same block
+    w[1:120, 9] = 2.0**46       # met by zeros of x
+    w[1:100, 1:9] = 2.0**29     # small codes of the same block
+    w[120:128, 0] = 2.0**46
+    w8, we = fp8.quantize_weight(w)
+    _, xe = fp8.quantize(x)
+    assert int(we[0, 0]) + int(xe[0, 0]) - 254 >= 128
+    values = fp8.dequantize_weight(w8, we).double()
+    want = quantised64(x)[0] @ values.T
+    out = fp8.linear(x, w8, we)
+    assert bool((want[:, 120:128] > 3.5e38).all()) and bool(out[:, 120:128].isinf().all())
+    assert bool((want[:, 1:100] > 1e34).all()) and bool((want[:, 1:120].abs() < 3e38).all())
+    rows = torch.cat([torch.arange(120), torch.arange(128, 256)]).to(DEV)
+    room = 2.0**-8 * want.abs() + 272 * 2.0**-23 * (quantised64(x)[0].abs() @ values.abs().T)
+    assert bool(((out.double() - want).abs() <= room)[:, rows].all()), (out[0, :4], want[0, :4])
