@@ -360,9 +360,11 @@ int muse_fp8_quantize(const void* x, void* xq, void* xe, int m, int K, int ld_x,
 int muse_fp8_walk(const void* W, const void* we, const void* x, void* out, int m, int N, int K, int ld_x, int ld_out, void* stream);
 
 /* Any number of tokens, x already in 8 bits: TMA and block-scaled tcgen05 MMAs. Where the walk is allowed too it is the faster
- * one up to weights of MUSE_FP8_WALK_BYTES (us per call on a B200, walk / quantize + gemm, 8 tokens: 256 x 4096 3.8 / 7.1, 4096 x
- * 4096 7.7 / 9.4, 4096 x 8192 12.8 / 14.0, 12288 x 4096 15.5 / 14.0; the gemm with 9 tokens 9.6 where a walk of twice the
- * tokens took 11.1). ws: muse_fp8_gemm_ws_bytes bytes (0: may be NULL), 16-byte aligned, contents irrelevant; it belongs to the call until it completes. status: as for muse_gemm_tc. */
+ * one up to weights of MUSE_FP8_WALK_BYTES (us per call in a replayed graph on a B200, weights not in cache, walk / quantize + gemm, at
+ * 1 token and at 8: 256 x 4096 3.5 / 6.4 and 3.7 / 7.1, 4096 x 4096 7.4 / 9.6 and 7.6 / 9.9, 4096 x 8192 12.1 / 12.5 and 12.4 /
+ * 14.3, 10240 x 4096 13.3 / 13.1 and 13.4 / 13.5, 12288 x 4096 15.2 / 13.5 and 15.3 / 13.9). ws: muse_fp8_gemm_ws_bytes bytes
+ * (0: may be NULL), 16-byte aligned, contents irrelevant; it belongs to the call until it completes. status: as for
+ * muse_gemm_tc. */
 #define MUSE_FP8_WALK_BYTES (40ll << 20)
 long long muse_fp8_gemm_ws_bytes(int m, int N, int K);
 int muse_fp8_gemm(const void* W, const void* we, const void* xq, const void* xe, void* out, void* ws, int* status, int m, int N, int K,

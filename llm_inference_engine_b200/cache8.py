@@ -58,7 +58,9 @@ def rotary_table(rot: int, positions: int, device, base: float = 10000.0, scalin
       "linear"  positions are divided by `factor`
       "ntk"     base * factor^(rot / (rot - 2)): the slowest pair is slowed by `factor`, the fastest not at all
       "yarn"    pairs that make more than 32 turns over `trained_positions` keep their frequency, those that make less
-                than one are slowed by `factor`, linearly between; cos and sin grow by 0.1 ln(factor) + 1"""
+                than one are slowed by `factor`, between them by a ramp that is linear in the number of turns; cos and sin
+                grow by 0.1 ln(factor) + 1. (Many published models were trained with a ramp that is linear in the pair's
+                index instead: their tables are to be made by the caller, in the same layout.)"""
     if rot < 2 or rot % 2 or positions < 1 or factor < 1.0:
         raise ValueError(f"rotary table of rot={rot} (even), positions={positions}, factor={factor} (at least 1)")
     i = torch.arange(rot // 2, dtype=torch.float64, device=device)
@@ -197,7 +199,10 @@ def attention(q: torch.Tensor, cache: Cache8, page_table: torch.Tensor, seq_lens
               out: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q K^T) V over the cached tokens up to each query token's own position (the last `window` of them
     when window > 0), times sigmoid(gate) when gate is given: BF16 [m, q_heads * dim], ready for the `o` projection. A row
-    that sees no token is zero; rows beyond the last sequence are left as they are. q: BF16 [m, q_heads, dim]; gate: BF16
+    that sees no token is zero; rows beyond the last sequence are left as they are. One call has one form, chosen by max_q times
+    the query heads per KV head: up to 16 rows the cache is read at memory speed, above that in tiles of 128 rows whatever
+    their filling, so sequences that decode single tokens are better not mixed with a prompt's chunk in one call (63 of 4000
+    tokens beside a chunk of 512: 396 us, as two calls 182). q: BF16 [m, q_heads, dim]; gate: BF16
     [m, q_heads * dim] (the gate columns of qkv_gate, any row stride); scale: positive, 1 / sqrt(dim) by default; out
     (optional): BF16 [m, q_heads * dim] with unit column stride. Two launches, the same bits in every run."""
     if out is None:

@@ -12,8 +12,8 @@
 //
 // The cache is the MMAs' M operand and the rows their N = 8 (or two such tiles): the work per page then follows the
 // rows there are, and a page's codes are converted once for all of them. Codes become FP16 in registers (exact, as e4m3
-// is a subset), q becomes FP16 under a power of two per row (exact down to 2^-34 of the row's largest value), the scores take
-// both powers in FP32. Scores S^T[token][row]: a lane's 16 bytes of k are 4 k-slots of 4 MMAs; the order of slots is free as
+// is a subset), q becomes FP16 under a power of two per row (rounded by at most 2^-34 of the row's largest value; BF16 values down
+// to 2^-27 of it are exact), the scores take both powers in FP32. Scores S^T[token][row]: a lane's 16 bytes of k are 4 k-slots of 4 MMAs; the order of slots is free as
 // long as q follows it. O^T[dim][row] += V^T[dim][token] P^T[token][row]: V is kept [dim, token], so a lane's 16 bytes are
 // tokens 16 t .. 16 t + 15 of a dimension, and the token order of the score tiles is chosen so that, after one 8 x 8
 // transpose in registers (movmatrix), the lane holds the same tokens' weights. Neither operand passes through
@@ -21,9 +21,10 @@
 // running maximum to 2^-39 of it), a page's sum is scaled by its V exponent, and back, in FP32.
 //
 // Measured with the kernel that adds up split units (us, and the cache's bytes against 6.46 TB/s of copying): 64 sequences of up to
-// 4000 tokens, 32 query and 16 KV heads 116 (5.06 TB/s, 0.78); 2 of 100,000, 32 and 4 heads, 45 (4.5 TB/s, 0.70); 21 with drafts of
-// up to 4 and a window of 1000, 16 and 4 heads of 64, 16.8; one of 300 tokens 10.5, where nothing is moved and the chain of the two launches is what is waited for (index
-// tensors, page table, one page's copy, its products, a partial sum, adding up). What made the difference on the way
+// 4000 tokens, 32 query and 16 KV heads 117 (5.02 TB/s, 0.78); 2 of 100,000, 32 and 4 heads, 46.5 (4.4 TB/s, 0.68); 21 with drafts of
+// up to 4 and a window of 1000, 16 and 4 heads of 64, 17.4; 32 of 4000 with 4 drafts, 32 and 8 heads, 73; one of 300 tokens 11.1,
+// where nothing is moved and the chain of the two launches is what is waited for (index tensors, page table, one page's copy,
+// its products, a partial sum, adding up). The form with 16 rows and D = 128 spills 60 bytes at 255 registers. What made the difference on the way
 // (64 sequences): a CTA per sequence and head with barriers 250; a ring per warp 213; equal ranges over one list 148;
 // page records and q for the next unit under way early 127; parts of one unit in one CTA met in shared memory, head items 116.
 #include "cache_attn.cuh"

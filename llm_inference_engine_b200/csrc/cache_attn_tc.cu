@@ -11,8 +11,9 @@
 // and by what the row's reference has moved. S, P and O' are double-buffered in tensor memory (64 + 2 x 64 + 2 x 32 + 2 x 128
 // columns at D = 128), so the products of one page run under the exponentials of another.
 //
-// Measured (chunk of 2 x 512 tokens against 4096, 32 query and 8 KV heads, D = 128; with the join): 138 us, 466
-// TFLOP/s; a page takes a CTA about 2000 clocks. What it is short of is instructions: some 3500 per page on four schedulers,
+// Measured (chunk of 2 x 512 tokens against 4096, 32 query and 8 KV heads, D = 128; with the join): 141 us, 458
+// TFLOP/s; a page takes a CTA about 2000 clocks, whatever the rows of a tile: 32 sequences of 4000 with 5 drafts (20 rows) take
+// 124 us, with 4 (16 rows, the other kernel) 73. At 128 registers the D = 128 form spills 138 bytes. What it is short of is instructions: some 3500 per page on four schedulers,
 // and their fetching. With every loop written out the kernel was 183 KB of code, missed the instruction cache on 4 of 10
 // fetches and took 349 us; loops over MMAs kept as loops and masks out of the way 220 and 176; FP32 operations two at a time
 // and a row split over two threads (so that its scores stay in registers) 138. Tried and slower: four warps that convert

@@ -12,8 +12,10 @@
 // products with MT = 2, hence the widest tile that tensor memory holds beside the scales (2 x 224 + 4 x 16 columns);
 // at fewer it is the weight's own bytes from memory, and below 20 MB of them the start (4 us to the first MMA behind the
 // quantizing kernel: set-up, x's exponents, one block's way through) and the end. K is cut where that lets all SMs load.
-// Measured with the quantizing kernel (us; TB/s of W or TFLOP/s): 27 x 4093 x 2064 8.8; 27 x 12288 x 4096 14.8 (3.4 TB/s);
-// 256 x 12288 x 4096 18.6 (1390 TFLOP/s); 4096 x 12288 x 4096 183 (2250 TFLOP/s). What gave the most: a warp that waits, issues
+// Measured with the quantizing kernel in a replayed graph of calls, each on a weight that is not in cache (us; TB/s of W or
+// TFLOP/s; in brackets the same weight every time): 27 x 4093 x 2064 8.9 (8.8); 16 x 4096 x 4096 10.4 (9.6); 27 x 12288 x
+// 4096 14.3, 3.5 TB/s (13.7); 256 x 12288 x 4096 18.3, 1410 TFLOP/s (17.3); 4096 x 12288 x 4096 184, 2240 TFLOP/s. Kept up for
+// long the last two take 20.5 and 205 to 217 (power). What gave the most: a warp that waits, issues
 // and commits for several blocks of K at once (a block alone costs 730 clocks of latency, four cost 1330), uniform issue,
 // exponents that are joined from whole words when used instead of byte by byte when loaded, results through shared memory.
 // At 4096 tokens a block of K takes 960 clocks, 896 of them MMAs at the tensor core's rate; a fifth of a tile's time is the epilogue,

@@ -10,9 +10,13 @@
 //                     the block: two shuffles give its largest magnitude), and their scales never change.
 //   fp8_quantize_kernel   x to codes and exponents, for the many-token kernel (fp8_gemm.cu) and for callers.
 //
-// Reading W bounds the walk (4096 x 4096, one token: 7.0 us, 2.4 TB/s; 4096 x 8192 12.2 us, 2.8 TB/s), below 10 MB its fixed
-// 3.7 us: launch, x's way to all SMs, the sum over the warps. With 9 to 16 tokens in the MMA's other half it took 2.8 us more for
-// any W (x read and quantised by every SM), where fp8_gemm.cu is as fast or faster, so it has no such form.
+// Measured in a replayed graph of calls, each on weights that are not in cache: 4096 x 4096 at 1 / 8 tokens 7.4 / 7.6 us (2.2 TB/s
+// of W), 4096 x 8192 12.1 / 12.4 (2.7 TB/s), 256 x 4096 3.5 / 3.7. It is not memory that bounds it (35 to 43 % of its rate) but the
+// chain of a call: x's way to all SMs and its rounding, a barrier and a sum over 32 warps for every 8 rows, 3.5 us of which
+// are there for any W. K above 4096 takes the form with two blocks of K per warp, which spills 28 bytes at 64 registers.
+// With 9 to 16 tokens in the MMA's other half it took 2.8 us more for any W (x read and quantised by every SM), where
+// fp8_gemm.cu is as fast or faster, so it has no such form. fp8_quantize_kernel: 4096 x 4096 22.0 us of 7.8 for its bytes
+// (bound by issue: 62 %), 256 x 4096 2.4.
 #include "../../include/muse_proj.h"
 #include "fp8.cuh"
 

@@ -12,7 +12,7 @@
 // (sequence, page that new tokens fall into, head) does k and v: the new tokens stay in registers between the search
 // for the largest magnitude and the rounding. The other CTAs rotate q, eight threads per head of 128.
 //
-// Measured: three prompts of up to 1500 tokens (32 query and 16 KV heads, with the values) 39 us, 3.6 TB/s of what has to move (61 us
+// Measured on the device: three prompts of up to 1500 tokens (32 query and 16 KV heads, with the values) 39 us, 3.6 TB/s of what has to move (61 us
 // while a CTA took the 64 tokens of a page in four rounds of 64 threads); 32 sequences of one token 3.7 us, 45 with drafts of
 // up to 5 4.6 us: those wait for a launch, three loads one after the other (lengths, page table, exponent) and the codes' way back.
 #include "cache8.cuh"
